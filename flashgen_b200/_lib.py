@@ -28,7 +28,8 @@ FG_ROW_GREEDY = 0x0200
 
 EXPORTED_SYMBOLS = ("fg_sample", "fg_sample_workspace_size", "fg_sample_candidates", "fg_sample_noalloc",
                     "fg_sample_set_split",
-                    "fg_apply_repetition_penalty", "fg_argmax", "fg_strerror", "fg_version")
+                    "fg_apply_repetition_penalty", "fg_argmax", "fg_token_logprobs", "fg_token_logprobs_grad",
+                    "fg_strerror", "fg_version")
 
 
 class FgSampleArgs(ctypes.Structure):
@@ -61,7 +62,53 @@ class FgSampleArgs(ctypes.Structure):
     ]
 
 
+class FgLogprobArgs(ctypes.Structure):
+    """Mirror of ``FgLogprobArgs``."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("top", ctypes.c_int32),
+        ("row_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("out_logprobs", ctypes.c_void_p),
+        ("out_entropy", ctypes.c_void_p),
+        ("out_max", ctypes.c_void_p),
+        ("out_logsum", ctypes.c_void_p),
+        ("out_rank", ctypes.c_void_p),
+        ("out_top_ids", ctypes.c_void_p),
+        ("out_top_logprobs", ctypes.c_void_p),
+        ("out_status", ctypes.c_void_p),
+    ]
+
+
+class FgLogprobGradArgs(ctypes.Structure):
+    """Mirror of ``FgLogprobGradArgs``."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("row_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("max", ctypes.c_void_p),
+        ("logsum", ctypes.c_void_p),
+        ("entropy", ctypes.c_void_p),
+        ("grad_logprobs", ctypes.c_void_p),
+        ("grad_entropy", ctypes.c_void_p),
+        ("out_grad", ctypes.c_void_p),
+        ("grad_stride", ctypes.c_int64),
+    ]
+
+
 FG_SAMPLE_WORKSPACE_MIN_BYTES = 256
+FG_LOGPROB_MAX_TOP = 32
 
 
 _lib = None
@@ -104,6 +151,10 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.fg_argmax.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                   ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]
         lib.fg_argmax.restype = ctypes.c_int
+        lib.fg_token_logprobs.argtypes = [ctypes.POINTER(FgLogprobArgs), ctypes.c_void_p]
+        lib.fg_token_logprobs.restype = ctypes.c_int
+        lib.fg_token_logprobs_grad.argtypes = [ctypes.POINTER(FgLogprobGradArgs), ctypes.c_void_p]
+        lib.fg_token_logprobs_grad.restype = ctypes.c_int
         lib.fg_strerror.argtypes = [ctypes.c_int]
         lib.fg_strerror.restype = ctypes.c_char_p
         lib.fg_version.argtypes = []

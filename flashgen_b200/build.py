@@ -23,7 +23,8 @@ LIBDIR = os.path.join(HERE, "lib")
 OBJDIR = os.path.join(LIBDIR, "obj")
 LIBNAME = "libflashgen_sampler.so"
 LIBPATH = os.path.join(LIBDIR, LIBNAME)
-SOURCES = [os.path.join(CSRC, f) for f in ("fg_abi.cu", "fg_host.cu", "fg_cluster.cu", "fg_stream.cu")]
+SOURCES = [os.path.join(CSRC, f) for f in ("fg_abi.cu", "fg_host.cu", "fg_cluster.cu", "fg_stream.cu",
+                                             "fg_logprobs.cu")]
 HEADERS = sorted(glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h"))) + [
     os.path.join(ROOT, "include", "flashgen_sampler.h")]
 DEPS = SOURCES + HEADERS

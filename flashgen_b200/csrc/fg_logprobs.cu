@@ -1,0 +1,94 @@
+// fg_logprobs.cu — C ABI entry points of the token log probabilities and their
+// gradient: argument checks and launches.
+#include <algorithm>
+
+#include "fg_internal.h"
+#include "fg_logprobs.cuh"
+
+namespace {
+
+using fg::host::elem_size;
+
+bool rows_ok(const void* p, int dtype, int64_t stride, int32_t vocab) {
+    return p != nullptr && stride >= vocab && reinterpret_cast<uintptr_t>(p) % elem_size(dtype) == 0;
+}
+
+constexpr int32_t kMaxRows = 1 << 30;
+
+template <int DT>
+int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
+    fg::lp::logprob_kernel<DT><<<batch, fg::lp::THREADS, 0, st>>>(P);
+    return cudaGetLastError() == cudaSuccess ? FG_OK : FG_ELAUNCH;
+}
+
+template <int DT>
+int launch_grad(const fg::lp::GradParams& P, int32_t batch, cudaStream_t st) {
+    const int per_row = std::max(1, std::min(8, P.vocab / 2048));
+    for (int32_t lo = 0; lo < batch; lo += 65535) {
+        fg::lp::GradParams Q = P;
+        const int32_t n = std::min<int32_t>(65535, batch - lo);
+        const int64_t esz = fg::Elem<DT>::SIZE;
+        Q.logits = reinterpret_cast<const char*>(P.logits) + lo * P.row_stride * esz;
+        Q.out_grad = reinterpret_cast<char*>(P.out_grad) + lo * P.grad_stride * esz;
+        if (P.tokens) Q.tokens = P.tokens + lo;
+        if (P.temperature) Q.temperature = P.temperature + lo;
+        Q.max = P.max + lo;
+        Q.logsum = P.logsum + lo;
+        if (P.entropy) Q.entropy = P.entropy + lo;
+        if (P.grad_logprobs) Q.grad_logprobs = P.grad_logprobs + lo;
+        if (P.grad_entropy) Q.grad_entropy = P.grad_entropy + lo;
+        fg::lp::logprob_grad_kernel<DT><<<dim3(per_row, n), fg::lp::THREADS, 0, st>>>(Q);
+    }
+    return cudaGetLastError() == cudaSuccess ? FG_OK : FG_ELAUNCH;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fg_token_logprobs(const FgLogprobArgs* a, void* stream) {
+    if (a == nullptr || elem_size(a->dtype) == 0 || a->batch < 0 || a->vocab < 1) return FG_EINVAL;
+    if (!rows_ok(a->logits, a->dtype, a->row_stride, a->vocab)) return FG_EINVAL;
+    if (a->top < 0 || a->top > FG_LOGPROB_MAX_TOP) return FG_EINVAL;
+    if (a->batch > kMaxRows || a->vocab > (1 << 28)) return FG_ENOTSUP;
+    if (a->batch == 0) return FG_OK;
+    fg::lp::Params P{};
+    P.logits = a->logits; P.row_stride = a->row_stride; P.vocab = a->vocab;
+    P.top = (a->out_top_ids || a->out_top_logprobs) ? a->top : 0;
+    P.tokens = a->tokens; P.temperature = a->temperature;
+    P.out_logprobs = a->out_logprobs; P.out_entropy = a->out_entropy; P.out_max = a->out_max;
+    P.out_logsum = a->out_logsum; P.out_rank = a->out_rank; P.out_top_ids = a->out_top_ids;
+    P.out_top_logprobs = a->out_top_logprobs; P.out_status = a->out_status;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    switch (a->dtype) {
+        case FG_DTYPE_F32: return launch_forward<FG_DTYPE_F32>(P, a->batch, st);
+        case FG_DTYPE_F16: return launch_forward<FG_DTYPE_F16>(P, a->batch, st);
+        default: return launch_forward<FG_DTYPE_BF16>(P, a->batch, st);
+    }
+}
+
+int fg_token_logprobs_grad(const FgLogprobGradArgs* a, void* stream) {
+    if (a == nullptr || elem_size(a->dtype) == 0 || a->batch < 0 || a->vocab < 1 || a->reserved != 0)
+        return FG_EINVAL;
+    if (!rows_ok(a->logits, a->dtype, a->row_stride, a->vocab) ||
+        !rows_ok(a->out_grad, a->dtype, a->grad_stride, a->vocab))
+        return FG_EINVAL;
+    if (a->out_grad == a->logits && a->grad_stride != a->row_stride) return FG_EINVAL;
+    if (a->max == nullptr || a->logsum == nullptr) return FG_EINVAL;
+    if (a->grad_entropy != nullptr && a->entropy == nullptr) return FG_EINVAL;
+    if (a->batch > kMaxRows || a->vocab > (1 << 28)) return FG_ENOTSUP;
+    if (a->batch == 0) return FG_OK;
+    fg::lp::GradParams P{};
+    P.logits = a->logits; P.row_stride = a->row_stride; P.vocab = a->vocab;
+    P.tokens = a->tokens; P.temperature = a->temperature; P.max = a->max; P.logsum = a->logsum;
+    P.entropy = a->entropy; P.grad_logprobs = a->grad_logprobs; P.grad_entropy = a->grad_entropy;
+    P.out_grad = a->out_grad; P.grad_stride = a->grad_stride;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    switch (a->dtype) {
+        case FG_DTYPE_F32: return launch_grad<FG_DTYPE_F32>(P, a->batch, st);
+        case FG_DTYPE_F16: return launch_grad<FG_DTYPE_F16>(P, a->batch, st);
+        default: return launch_grad<FG_DTYPE_BF16>(P, a->batch, st);
+    }
+}
+
+}  // extern "C"

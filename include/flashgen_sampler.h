@@ -233,6 +233,89 @@ int fg_apply_repetition_penalty(void* logits, int32_t dtype, int32_t batch,
 int fg_argmax(const void* logits, int32_t dtype, int32_t batch, int32_t vocab,
               int64_t row_stride, int64_t* out_ids, void* stream);
 
+/*
+ * Log probabilities of given tokens, one per row of [batch, vocab] logits, with
+ * the row's entropy, the token's rank and the row's `top` likeliest ids. With
+ * T = temperature[r] (NULL: 1), m = the row's largest logit and
+ * L = log sum_j exp((x_j - m) / T):
+ *
+ *   out_max, out_logsum     m and L: the row's log sum of exp(x / T) is m / T + L
+ *   out_logprobs            (x_t - m) / T - L for t = tokens[r]
+ *   out_entropy             -sum_j p_j log p_j, p_j = exp((x_j - m) / T - L)
+ *   out_rank                the number of ids ahead of t: larger logit, or the
+ *                           same logit and a smaller id
+ *   out_top_ids/_logprobs   the first `top` ids in that order, [batch, top]; past
+ *                           the vocabulary's end -1 and -inf
+ *
+ * Everything is accumulated in fp32 whatever the logits' type, in one pass over
+ * the logits. Every output may be NULL; tokens NULL or tokens[r] < 0 means that
+ * the row has no token: log probability 0 and rank -1, everything else as usual.
+ *
+ * Special rows (out_status bits): a row that is all -inf (FG_ROW_ALL_MASKED) has
+ * no distribution: every log probability is -inf, the entropy 0. A row with a
+ * NaN or +inf logit (FG_ROW_NAN, FG_ROW_POS_INF), or whose temperature is not a
+ * positive normal number or whose token is not below vocab (FG_ROW_BAD_PARAM),
+ * has NaN results (out_max stays the row's maximum), rank -1 and ids -1.
+ *
+ * Replaces the reference's per-token log probability that nothing fills
+ * (flashgen/outputs.py:25, CompletionOutput.cumulative_logprob).
+ */
+#define FG_LOGPROB_MAX_TOP 32   /* largest `top`                                */
+
+typedef struct FgLogprobArgs {
+    const void*    logits;
+    int32_t        dtype;               /* FG_DTYPE_*                              */
+    int32_t        batch;               /* B >= 0                                  */
+    int32_t        vocab;               /* V >= 1                                  */
+    int32_t        top;                 /* 0 .. FG_LOGPROB_MAX_TOP                 */
+    int64_t        row_stride;          /* elements between rows, >= vocab         */
+    const int64_t* tokens;              /* [B] or NULL                             */
+    const float*   temperature;         /* [B] or NULL                             */
+    float*         out_logprobs;        /* [B] or NULL                             */
+    float*         out_entropy;         /* [B] or NULL                             */
+    float*         out_max;             /* [B] or NULL                             */
+    float*         out_logsum;          /* [B] or NULL                             */
+    int32_t*       out_rank;            /* [B] or NULL                             */
+    int64_t*       out_top_ids;         /* [B, top] or NULL                        */
+    float*         out_top_logprobs;    /* [B, top] or NULL                        */
+    int32_t*       out_status;          /* [B] or NULL                             */
+} FgLogprobArgs;
+
+int fg_token_logprobs(const FgLogprobArgs* args, void* stream);
+
+/*
+ * Gradient of fg_token_logprobs with respect to the logits. With g =
+ * grad_logprobs[r] (0 where NULL or the row has no token) and h =
+ * grad_entropy[r] (0 where NULL):
+ *
+ *   out_grad_j = (g * (1[j == t] - p_j) - h * p_j * (log p_j + H)) / T
+ *
+ * computed in fp32 from the saved max, logsum and (with grad_entropy) entropy H
+ * and rounded once to the logits' type. out_grad may be the logits buffer
+ * itself (same pointer and stride): the gradient then replaces the logits. A
+ * row with g = h = 0 and a row that is all -inf have gradient 0; a row whose
+ * forward results are NaN has NaN.
+ */
+typedef struct FgLogprobGradArgs {
+    const void*    logits;
+    int32_t        dtype;               /* FG_DTYPE_* of logits and out_grad       */
+    int32_t        batch;               /* B >= 0                                  */
+    int32_t        vocab;               /* V >= 1                                  */
+    int32_t        reserved;            /* 0                                       */
+    int64_t        row_stride;          /* elements between logits rows, >= vocab  */
+    const int64_t* tokens;              /* [B] or NULL                             */
+    const float*   temperature;         /* [B] or NULL                             */
+    const float*   max;                 /* [B] out_max of the forward call         */
+    const float*   logsum;              /* [B] out_logsum of the forward call      */
+    const float*   entropy;             /* [B] out_entropy; NULL without grad_entropy */
+    const float*   grad_logprobs;       /* [B] or NULL                             */
+    const float*   grad_entropy;        /* [B] or NULL                             */
+    void*          out_grad;            /* [B, vocab]                              */
+    int64_t        grad_stride;         /* elements between gradient rows, >= vocab */
+} FgLogprobGradArgs;
+
+int fg_token_logprobs_grad(const FgLogprobGradArgs* args, void* stream);
+
 /* Human-readable name of a return code. */
 const char* fg_strerror(int code);
 

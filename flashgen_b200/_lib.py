@@ -29,7 +29,7 @@ FG_ROW_GREEDY = 0x0200
 EXPORTED_SYMBOLS = ("fg_sample", "fg_sample_workspace_size", "fg_sample_candidates", "fg_sample_noalloc",
                     "fg_sample_set_split",
                     "fg_apply_repetition_penalty", "fg_argmax", "fg_token_logprobs", "fg_token_logprobs_grad",
-                    "fg_strerror", "fg_version")
+                    "fg_adapter_logits", "fg_adapter_workspace_size", "fg_strerror", "fg_version")
 
 
 class FgSampleArgs(ctypes.Structure):
@@ -107,7 +107,37 @@ class FgLogprobGradArgs(ctypes.Structure):
     ]
 
 
+class FgAdapterArgs(ctypes.Structure):
+    """Mirror of ``FgAdapterArgs``."""
+
+    _fields_ = [
+        ("hidden", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("down", ctypes.c_void_p),
+        ("up", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("adapters", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_status", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("rank", ctypes.c_int32),
+        ("slots", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("hidden_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("down_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+    ]
+
+
 FG_SAMPLE_WORKSPACE_MIN_BYTES = 256
+FG_ADAPTER_MAX_RANK = 128
 FG_LOGPROB_MAX_TOP = 32
 
 
@@ -155,6 +185,10 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.fg_token_logprobs.restype = ctypes.c_int
         lib.fg_token_logprobs_grad.argtypes = [ctypes.POINTER(FgLogprobGradArgs), ctypes.c_void_p]
         lib.fg_token_logprobs_grad.restype = ctypes.c_int
+        lib.fg_adapter_logits.argtypes = [ctypes.POINTER(FgAdapterArgs), ctypes.c_void_p]
+        lib.fg_adapter_logits.restype = ctypes.c_int
+        lib.fg_adapter_workspace_size.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
+        lib.fg_adapter_workspace_size.restype = ctypes.c_size_t
         lib.fg_strerror.argtypes = [ctypes.c_int]
         lib.fg_strerror.restype = ctypes.c_char_p
         lib.fg_version.argtypes = []

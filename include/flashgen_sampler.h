@@ -316,6 +316,66 @@ typedef struct FgLogprobGradArgs {
 
 int fg_token_logprobs_grad(const FgLogprobGradArgs* args, void* stream);
 
+/*
+ * Logits of a batch of requests that share one LM head and have each their own
+ * low-rank adapter beside it: for row b with a = adapters[b],
+ *
+ *   out[b, v] = sum_k hidden[b, k] weight[v, k]
+ *             + scales[a] sum_i (sum_k hidden[b, k] down[a, i, k]) up[a, v, i]
+ *
+ * and without the second term where a < 0 or scales[a] == 0 (or adapters is NULL).
+ * Products of the
+ * 16-bit operands are summed in fp32, the inner sums of the second term stay in
+ * fp32, and out is rounded once. A row reads its own adapter only: NaN or inf in
+ * another row's adapter cannot reach it. An id >= slots marks the row's
+ * out_status FG_ROW_BAD_PARAM and leaves it without an adapter.
+ *
+ * Layout: weight [vocab, dim] with weight_stride, down [slots, rank, dim] with
+ * down_stride between the rows of one adapter and rank * down_stride between
+ * adapters, up [slots, vocab, rank] dense. All three 16-byte aligned, the
+ * strides multiples of 8 elements, rank a multiple of 16 up to
+ * FG_ADAPTER_MAX_RANK (an adapter of lower rank has zero rows of down or zero
+ * columns of up). hidden and out need only the alignment of their elements.
+ *
+ * Workspace: fg_adapter_workspace_size bytes, 256-byte aligned, written and read
+ * within the call (no initial value). Calls that may run concurrently need
+ * separate workspaces.
+ *
+ * Replaces the LM-head product in front of the reference's sampler
+ * (csrc/runtime/transformer.cu:384-389, cublasSgemm), which has no adapters.
+ */
+#define FG_ADAPTER_MAX_RANK 128
+
+typedef struct FgAdapterArgs {
+    const void*    hidden;              /* [B, dim]                                */
+    const void*    weight;              /* [V, dim]                                */
+    const void*    down;                /* [slots, rank, dim]; NULL if slots == 0  */
+    const void*    up;                  /* [slots, V, rank]; NULL if slots == 0    */
+    const float*   scales;              /* [slots]; NULL if slots == 0             */
+    const int32_t* adapters;            /* [B] or NULL                             */
+    void*          out;                 /* [B, V]                                  */
+    int32_t*       out_status;          /* [B] or NULL                             */
+    void*          workspace;
+    size_t         workspace_bytes;
+    int32_t        dtype;               /* FG_DTYPE_F16 or FG_DTYPE_BF16           */
+    int32_t        out_dtype;           /* dtype or FG_DTYPE_F32                   */
+    int32_t        batch;               /* B >= 0                                  */
+    int32_t        dim;                 /* >= 1                                    */
+    int32_t        vocab;               /* V >= 1                                  */
+    int32_t        rank;                /* 16 .. FG_ADAPTER_MAX_RANK, or any if slots == 0 */
+    int32_t        slots;               /* >= 0                                    */
+    int32_t        reserved;            /* 0                                       */
+    int64_t        hidden_stride;       /* elements between rows, >= dim           */
+    int64_t        weight_stride;
+    int64_t        down_stride;
+    int64_t        out_stride;          /* elements between rows, >= vocab         */
+} FgAdapterArgs;
+
+int fg_adapter_logits(const FgAdapterArgs* args, void* stream);
+
+/* Bytes of workspace of fg_adapter_logits; 0 for an invalid shape. Host-only. */
+size_t fg_adapter_workspace_size(int32_t batch, int32_t dim, int32_t rank, int32_t slots);
+
 /* Human-readable name of a return code. */
 const char* fg_strerror(int code);
 

@@ -1,23 +1,112 @@
 // fg_adapter.cu — C ABI entry points of the LM head with per-row adapters:
 // argument checks, workspace layout and launches.
 #include <algorithm>
+#include <atomic>
 
 #include "fg_adapter.cuh"
 #include "fg_internal.h"
 
 namespace {
 
+using fg::host::DevInfo;
 using fg::host::elem_size;
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's tensor-map encoder, through the runtime (the library links no libcuda).
+EncodeTiledFn encoder() {
+    static std::atomic<EncodeTiledFn> fn{nullptr};
+    EncodeTiledFn f = fn.load(std::memory_order_acquire);
+    if (f == nullptr) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) !=
+                cudaSuccess || q != cudaDriverEntryPointSuccess)
+            return nullptr;
+        f = reinterpret_cast<EncodeTiledFn>(p);
+        fn.store(f, std::memory_order_release);
+    }
+    return f;
+}
+
+// A [rows, dim] matrix read in boxes of box_rows x 64 elements; columns past dim
+// and rows past `rows` read as zero.
+bool encode(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t dim, int64_t stride, int box_rows) {
+    EncodeTiledFn f = encoder();
+    if (f == nullptr) return false;
+    const cuuint64_t extent[2] = {cuuint64_t(dim), cuuint64_t(rows)};
+    const cuuint64_t pitch[1] = {cuuint64_t(stride) * 2};
+    const cuuint32_t box[2] = {cuuint32_t(fg::adapt::TILE_K), cuuint32_t(box_rows)};
+    const cuuint32_t step[2] = {1, 1};
+    return f(map, dtype == FG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(base), extent, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DT, int ODT, int RC>
+int launch_project(const fg::adapt::Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, bool dependent,
+                   DevInfo* d, cudaStream_t st) {
+    auto kern = fg::adapt::project_kernel<DT, ODT, RC>;
+    static std::atomic<bool> attr_set[fg::host::kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return FG_EDEVICE;
+    const int room = d->smem_optin - int(sizeof(fg::adapt::Control)) - 256;
+    if (!attr_set[dev].load(std::memory_order_acquire)) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, room) != cudaSuccess)
+            return FG_EDEVICE;
+        attr_set[dev].store(true, std::memory_order_release);
+    }
+    fg::adapt::Params Q = P;
+    const int stage = fg::adapt::A_BYTES + P.nt * fg::adapt::TILE_K * 2;
+    Q.stages = std::min(fg::adapt::MAX_STAGES, (room - 1024) / stage);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(std::min(P.nvt * P.ntile, d->sms));
+    cfg.blockDim = dim3(fg::adapt::PROJ_THREADS);
+    cfg.dynamicSmemBytes = size_t(1024 + Q.stages * stage);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = dependent ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, wmap, xmap, Q) == cudaSuccess ? FG_OK : FG_ELAUNCH;
+}
+
 template <int DT, int ODT>
-int launch(const fg::adapt::Params& P, cudaStream_t st) {
-    if (P.slots > 0 || P.out_status) fg::adapt::down_kernel<DT><<<P.batch, fg::adapt::DOWN_THREADS, 0, st>>>(P);
-    const dim3 grid((P.vocab + fg::adapt::TILE - 1) / fg::adapt::TILE,
-                    (P.batch + fg::adapt::TILE - 1) / fg::adapt::TILE);
-    fg::adapt::project_kernel<DT, ODT><<<grid, 256, 0, st>>>(P);
-    return cudaGetLastError() == cudaSuccess ? FG_OK : FG_ELAUNCH;
+int launch(const fg::adapt::Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, DevInfo* d,
+           cudaStream_t st) {
+    const bool first = P.adapters || P.copy || P.out_status;
+    if (first) {
+        fg::adapt::down_kernel<DT><<<P.batch + P.ntile, fg::adapt::DOWN_THREADS, 0, st>>>(P);
+        if (cudaGetLastError() != cudaSuccess) return FG_ELAUNCH;
+    }
+    const int rc = P.adapters && P.slots > 0 ? P.rank / 16 : 0;
+    if (rc == 0) return launch_project<DT, ODT, 0>(P, wmap, xmap, first, d, st);
+    if (rc == 1) return launch_project<DT, ODT, 1>(P, wmap, xmap, first, d, st);
+    if (rc == 2) return launch_project<DT, ODT, 2>(P, wmap, xmap, first, d, st);
+    if (rc <= 4) return launch_project<DT, ODT, 4>(P, wmap, xmap, first, d, st);
+    return launch_project<DT, ODT, 8>(P, wmap, xmap, first, d, st);
+}
+
+// Workspace: U, the order of the rows, the aligned copy of the hidden rows.
+struct Layout {
+    size_t u, order, copy, total;
+    int64_t copy_stride;
+};
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+Layout layout(int64_t batch, int64_t dim, int64_t rank, int64_t slots) {
+    Layout L{};
+    L.copy_stride = (dim + 7) / 8 * 8;
+    L.u = 0;
+    L.order = round256(slots > 0 ? sizeof(float) * size_t(batch * rank) : 0);
+    L.copy = L.order + round256(sizeof(int32_t) * size_t(batch));
+    L.total = std::max<size_t>(256, L.copy + round256(2 * size_t(batch * L.copy_stride)));
+    return L;
 }
 
 constexpr int32_t kMaxRows = 1 << 20;
@@ -29,7 +118,7 @@ extern "C" {
 size_t fg_adapter_workspace_size(int32_t batch, int32_t dim, int32_t rank, int32_t slots) {
     if (batch < 0 || batch > kMaxRows || dim < 1 || slots < 0) return 0;
     if (slots > 0 && (rank < 16 || rank > FG_ADAPTER_MAX_RANK || rank % 16 != 0)) return 0;
-    return std::max<size_t>(256, slots > 0 ? sizeof(float) * size_t(batch) * rank : 0);
+    return layout(batch, dim, rank, slots).total;
 }
 
 int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
@@ -47,22 +136,49 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
         if (!aligned(a->down, 16) || !aligned(a->up, 16) || a->down_stride < a->dim || a->down_stride % 8 != 0)
             return FG_EINVAL;
     }
-    if (a->batch > kMaxRows || a->vocab > (1 << 28) || a->dim > (1 << 20)) return FG_ENOTSUP;
+    if (a->batch > kMaxRows || a->vocab > (1 << 28) || a->dim > (1 << 20) || a->slots > (1 << 20)) return FG_ENOTSUP;
     const size_t need = fg_adapter_workspace_size(a->batch, a->dim, a->rank, a->slots);
     if (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < need) return FG_EINVAL;
     if (a->batch == 0) return FG_OK;
+    DevInfo* d = nullptr;
+    const int rc = fg::host::device_info(&d);
+    if (rc != FG_OK) return rc;
+
+    const Layout L = layout(a->batch, a->dim, a->rank, a->slots);
+    char* ws = reinterpret_cast<char*>(a->workspace);
     fg::adapt::Params P{};
-    P.hidden = a->hidden; P.weight = a->weight; P.down = a->down; P.up = a->up; P.scales = a->scales;
+    P.raw_hidden = a->hidden; P.raw_stride = a->hidden_stride;
+    P.down = a->down; P.up = a->up; P.scales = a->scales;
     P.adapters = a->slots > 0 || a->out_status ? a->adapters : nullptr;
-    P.out = a->out; P.out_status = a->out_status; P.u = reinterpret_cast<float*>(a->workspace);
+    P.out = a->out; P.out_status = a->out_status;
+    P.u = reinterpret_cast<float*>(ws + L.u);
+    P.order = reinterpret_cast<int32_t*>(ws + L.order);
     P.batch = a->batch; P.dim = a->dim; P.vocab = a->vocab; P.rank = a->rank; P.slots = a->slots;
-    P.hidden_stride = a->hidden_stride; P.weight_stride = a->weight_stride; P.down_stride = a->down_stride;
-    P.out_stride = a->out_stride;
+    P.down_stride = a->down_stride; P.out_stride = a->out_stride; P.copy_stride = L.copy_stride;
+    // TMA reads rows that start on 16-byte boundaries: others are copied first
+    const bool copy = !aligned(a->hidden, 16) || (a->batch > 1 && a->hidden_stride % 8 != 0);
+    P.copy = copy ? ws + L.copy : nullptr;
+    P.hidden = copy ? P.copy : a->hidden;
+    P.hidden_stride = copy || a->batch == 1 ? L.copy_stride : a->hidden_stride;
+    // batch tiles of equal width, at most 256 columns
+    P.ntile = (a->batch + fg::adapt::MAX_NT - 1) / fg::adapt::MAX_NT;
+    P.nt = ((a->batch + P.ntile - 1) / P.ntile + 15) / 16 * 16;
+    P.ntile = (a->batch + P.nt - 1) / P.nt;
+    P.nvt = (a->vocab + fg::adapt::TILE_V - 1) / fg::adapt::TILE_V;
+    P.tmem_cols = 32;
+    while (P.tmem_cols < 2 * P.nt) P.tmem_cols *= 2;
+    if (int64_t(P.nvt) * P.ntile > (1 << 30)) return FG_ENOTSUP;
+    CUtensorMap wmap, xmap;
+    if (!encode(&wmap, a->dtype, a->weight, a->vocab, a->dim, a->weight_stride, fg::adapt::TILE_V) ||
+        !encode(&xmap, a->dtype, P.hidden, a->batch, a->dim, P.hidden_stride, P.nt))
+        return FG_EDEVICE;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const bool f32 = a->out_dtype == FG_DTYPE_F32;
     if (a->dtype == FG_DTYPE_F16)
-        return f32 ? launch<FG_DTYPE_F16, FG_DTYPE_F32>(P, st) : launch<FG_DTYPE_F16, FG_DTYPE_F16>(P, st);
-    return f32 ? launch<FG_DTYPE_BF16, FG_DTYPE_F32>(P, st) : launch<FG_DTYPE_BF16, FG_DTYPE_BF16>(P, st);
+        return f32 ? launch<FG_DTYPE_F16, FG_DTYPE_F32>(P, wmap, xmap, d, st)
+                   : launch<FG_DTYPE_F16, FG_DTYPE_F16>(P, wmap, xmap, d, st);
+    return f32 ? launch<FG_DTYPE_BF16, FG_DTYPE_F32>(P, wmap, xmap, d, st)
+               : launch<FG_DTYPE_BF16, FG_DTYPE_BF16>(P, wmap, xmap, d, st);
 }
 
 }  // extern "C"

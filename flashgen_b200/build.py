@@ -24,7 +24,8 @@ OBJDIR = os.path.join(LIBDIR, "obj")
 LIBNAME = "libflashgen_sampler.so"
 LIBPATH = os.path.join(LIBDIR, LIBNAME)
 SOURCES = [os.path.join(CSRC, f) for f in ("fg_abi.cu", "fg_host.cu", "fg_cluster.cu", "fg_stream.cu",
-                                             "fg_logprobs.cu", "fg_adapter.cu")]
+                                             "fg_logprobs.cu", "fg_adapter.cu", "fg_adapter_f16.cu",
+                                             "fg_adapter_f16_f32.cu", "fg_adapter_bf16.cu", "fg_adapter_bf16_f32.cu")]
 HEADERS = sorted(glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h"))) + [
     os.path.join(ROOT, "include", "flashgen_sampler.h")]
 DEPS = SOURCES + HEADERS

@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "fg_adapter.cuh"
+#include "fg_adapter.h"
 #include "fg_internal.h"
 
 namespace {
@@ -46,51 +46,6 @@ bool encode(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t
              const_cast<void*>(base), extent, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <int DT, int ODT, int RC>
-int launch_project(const fg::adapt::Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, bool dependent,
-                   DevInfo* d, cudaStream_t st) {
-    auto kern = fg::adapt::project_kernel<DT, ODT, RC>;
-    static std::atomic<bool> attr_set[fg::host::kMaxDevices] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return FG_EDEVICE;
-    const int room = d->smem_optin - int(sizeof(fg::adapt::Control)) - 256;
-    if (!attr_set[dev].load(std::memory_order_acquire)) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, room) != cudaSuccess)
-            return FG_EDEVICE;
-        attr_set[dev].store(true, std::memory_order_release);
-    }
-    fg::adapt::Params Q = P;
-    const int stage = fg::adapt::A_BYTES + P.nt * fg::adapt::TILE_K * 2;
-    Q.stages = std::min(fg::adapt::MAX_STAGES, (room - 1024) / stage);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(std::min(P.nvt * P.ntile, d->sms));
-    cfg.blockDim = dim3(fg::adapt::PROJ_THREADS);
-    cfg.dynamicSmemBytes = size_t(1024 + Q.stages * stage);
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = dependent ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, wmap, xmap, Q) == cudaSuccess ? FG_OK : FG_ELAUNCH;
-}
-
-template <int DT, int ODT>
-int launch(const fg::adapt::Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, DevInfo* d,
-           cudaStream_t st) {
-    const bool first = P.adapters || P.copy || P.out_status;
-    if (first) {
-        fg::adapt::down_kernel<DT><<<P.batch + P.ntile, fg::adapt::DOWN_THREADS, 0, st>>>(P);
-        if (cudaGetLastError() != cudaSuccess) return FG_ELAUNCH;
-    }
-    const int rc = P.adapters && P.slots > 0 ? P.rank / 16 : 0;
-    if (rc == 0) return launch_project<DT, ODT, 0>(P, wmap, xmap, first, d, st);
-    if (rc == 1) return launch_project<DT, ODT, 1>(P, wmap, xmap, first, d, st);
-    if (rc == 2) return launch_project<DT, ODT, 2>(P, wmap, xmap, first, d, st);
-    if (rc <= 4) return launch_project<DT, ODT, 4>(P, wmap, xmap, first, d, st);
-    return launch_project<DT, ODT, 8>(P, wmap, xmap, first, d, st);
 }
 
 // Workspace: U, the order of the rows, the aligned copy of the hidden rows.
@@ -164,21 +119,24 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
     P.ntile = (a->batch + fg::adapt::MAX_NT - 1) / fg::adapt::MAX_NT;
     P.nt = ((a->batch + P.ntile - 1) / P.ntile + 15) / 16 * 16;
     P.ntile = (a->batch + P.nt - 1) / P.nt;
-    P.nvt = (a->vocab + fg::adapt::TILE_V - 1) / fg::adapt::TILE_V;
+    const bool pair = P.nt > 128;
+    const int tile_v = fg::adapt::TILE_V * (pair ? 2 : 1);
+    P.nvt = (a->vocab + tile_v - 1) / tile_v;
+    P.kb = P.nt <= 64 ? 2 : 1;
     P.tmem_cols = 32;
     while (P.tmem_cols < 2 * P.nt) P.tmem_cols *= 2;
     if (int64_t(P.nvt) * P.ntile > (1 << 30)) return FG_ENOTSUP;
     CUtensorMap wmap, xmap;
     if (!encode(&wmap, a->dtype, a->weight, a->vocab, a->dim, a->weight_stride, fg::adapt::TILE_V) ||
-        !encode(&xmap, a->dtype, P.hidden, a->batch, a->dim, P.hidden_stride, P.nt))
+        !encode(&xmap, a->dtype, P.hidden, a->batch, a->dim, P.hidden_stride, pair ? P.nt / 2 : P.nt))
         return FG_EDEVICE;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const bool f32 = a->out_dtype == FG_DTYPE_F32;
     if (a->dtype == FG_DTYPE_F16)
-        return f32 ? launch<FG_DTYPE_F16, FG_DTYPE_F32>(P, wmap, xmap, d, st)
-                   : launch<FG_DTYPE_F16, FG_DTYPE_F16>(P, wmap, xmap, d, st);
-    return f32 ? launch<FG_DTYPE_BF16, FG_DTYPE_F32>(P, wmap, xmap, d, st)
-               : launch<FG_DTYPE_BF16, FG_DTYPE_BF16>(P, wmap, xmap, d, st);
+        return f32 ? fg::adapt::launch<FG_DTYPE_F16, FG_DTYPE_F32>(P, wmap, xmap, pair, d, st)
+                   : fg::adapt::launch<FG_DTYPE_F16, FG_DTYPE_F16>(P, wmap, xmap, pair, d, st);
+    return f32 ? fg::adapt::launch<FG_DTYPE_BF16, FG_DTYPE_F32>(P, wmap, xmap, pair, d, st)
+               : fg::adapt::launch<FG_DTYPE_BF16, FG_DTYPE_BF16>(P, wmap, xmap, pair, d, st);
 }
 
 }  // extern "C"

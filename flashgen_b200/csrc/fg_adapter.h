@@ -1,0 +1,46 @@
+// fg_adapter.h — what the entry points (fg_adapter.cu) and the launches
+// (fg_adapter_*.cu, one unit per operand and result type) share.
+#pragma once
+
+#include <cuda.h>
+
+#include "fg_internal.h"
+
+namespace fg {
+namespace adapt {
+
+constexpr int TILE_V = 128, TILE_K = 64;   // accumulator lanes; elements of a K step (128 bytes)
+constexpr int MAX_NT = 256;                // batch columns of a tile
+
+struct Params {
+    const void* hidden;       // rows for the products: the caller's, or the aligned copy
+    const void* raw_hidden;   // the caller's rows
+    int64_t hidden_stride, raw_stride;
+    const void* down;
+    const void* up;
+    const float* scales;
+    const int32_t* adapters;
+    void* out;
+    int32_t* out_status;
+    float* u;                 // [B, rank] in the sorted order (workspace)
+    int32_t* order;           // [B] per batch tile: (slot + 1) << 9 | column, sorted (workspace)
+    void* copy;               // [B, copy_stride] aligned hidden rows, or null (workspace)
+    int32_t batch, dim, vocab, rank, slots;
+    int64_t down_stride, out_stride, copy_stride;
+    int32_t ntile;            // batch tiles
+    int32_t nt;               // columns of a batch tile, a multiple of 16 up to 256
+    // project_kernel
+    int32_t nvt;              // vocabulary tiles of 128 (256 for a pair)
+    int32_t stages;           // of the operand ring
+    int32_t kb;               // 64-wide boxes of K in a stage
+    int32_t tmem_cols;
+};
+
+// Both launches of a call: operands of type DT, result of type ODT. `pair`: two
+// CTAs share each product (tiles of 256 vocabulary rows).
+template <int DT, int ODT>
+int launch(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, bool pair, host::DevInfo* d,
+           cudaStream_t st);
+
+}  // namespace adapt
+}  // namespace fg

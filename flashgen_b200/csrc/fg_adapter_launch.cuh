@@ -1,0 +1,75 @@
+// fg_adapter_launch.cuh — launches of the LM-head kernels; included by the units
+// that instantiate them.
+#pragma once
+
+#include <algorithm>
+#include <atomic>
+
+#include "fg_adapter.cuh"
+
+namespace fg {
+namespace adapt {
+
+template <int CG, int DT, int ODT, int RC>
+int launch_project(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, bool dependent,
+                   host::DevInfo* d, cudaStream_t st) {
+    auto kern = project_kernel<CG, DT, ODT, RC>;
+    static std::atomic<bool> attr_set[host::kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return FG_EDEVICE;
+    const int room = d->smem_optin - int(sizeof(Control)) - 256;
+    if (!attr_set[dev].load(std::memory_order_acquire)) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, room) != cudaSuccess)
+            return FG_EDEVICE;
+        attr_set[dev].store(true, std::memory_order_release);
+    }
+    Params Q = P;
+    const int stage = P.kb * (A_BYTES + P.nt / CG * TILE_K * 2);
+    const int ubytes = RC > 0 ? U_BYTES : 0;
+    Q.stages = std::min(MAX_STAGES, (room - 1024 - ubytes) / stage);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(std::min(P.nvt * P.ntile, d->sms / CG) * CG);
+    cfg.blockDim = dim3(PROJ_THREADS);
+    cfg.dynamicSmemBytes = size_t(1024 + Q.stages * stage + ubytes);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2] = {};
+    if (CG == 2) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = 2;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    if (dependent) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    cfg.attrs = attr;
+    return cudaLaunchKernelEx(&cfg, kern, wmap, xmap, Q) == cudaSuccess ? FG_OK : FG_ELAUNCH;
+}
+
+template <int DT, int ODT, int RC>
+int launch_rank(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, bool pair,
+                host::DevInfo* d, cudaStream_t st) {
+    const bool first = P.adapters || P.copy || P.out_status;
+    if (first) {
+        down_kernel<DT, RC ? RC : 1><<<P.batch, DOWN_THREADS, 0, st>>>(P);
+        if (cudaGetLastError() != cudaSuccess) return FG_ELAUNCH;
+    }
+    return pair ? launch_project<2, DT, ODT, RC>(P, wmap, xmap, first, d, st)
+                : launch_project<1, DT, ODT, RC>(P, wmap, xmap, first, d, st);
+}
+
+template <int DT, int ODT>
+int launch(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, bool pair, host::DevInfo* d,
+           cudaStream_t st) {
+    const int rc = P.adapters && P.slots > 0 ? P.rank / 16 : 0;
+    if (rc == 0) return launch_rank<DT, ODT, 0>(P, wmap, xmap, pair, d, st);
+    if (rc == 1) return launch_rank<DT, ODT, 1>(P, wmap, xmap, pair, d, st);
+    if (rc == 2) return launch_rank<DT, ODT, 2>(P, wmap, xmap, pair, d, st);
+    if (rc <= 4) return launch_rank<DT, ODT, 4>(P, wmap, xmap, pair, d, st);
+    return launch_rank<DT, ODT, 8>(P, wmap, xmap, pair, d, st);
+}
+
+}  // namespace adapt
+}  // namespace fg

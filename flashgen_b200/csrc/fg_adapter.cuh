@@ -3,18 +3,26 @@
 //   out[b, v] = X[b, :] . W[v, :] + U[b, :] . up[a_b, v, :],
 //   U[b, i]   = scales[a_b] * (X[b, :] . down[a_b, i, :])
 //
-// Two launches. down_kernel computes U (fp32, a CTA per row), sorts the rows of
-// each batch tile by adapter and, where the hidden rows are not 16-byte aligned,
-// copies them to aligned ones. project_kernel does the rest: the shared product
-// on the tensor cores with the vocabulary on the accumulator's 128 lanes and the
-// batch on its columns, so that a small batch wastes no tensor-core rows and a
-// warp's stores of one column are 32 neighbouring logits. The adapters' product
-// is added by the epilogue warps on the CUDA cores, in fp32, column by column in
-// the sorted order: a row touches no adapter but its own (a masked product would
-// let NaN from one request's adapter into the others), U needs no rounding to 16
-// bits, and each adapter's rows of `up` are read once per tile and kept in
-// registers.
+// Two launches. down_kernel computes U and sorts the rows of each batch tile by
+// adapter (it copies the hidden rows in that order, which also aligns them).
+// project_kernel does the rest: the shared product on the tensor cores with the
+// vocabulary on the accumulator's 128 lanes and the batch on its columns, so that a
+// small batch wastes no tensor-core rows. Its epilogue warps add the adapters'
+// product, eight columns at a time, with warp-level products whose fragments match
+// the layout in which they read the accumulator.
+//
+// A row must not see another row's adapter, not even as 0 * NaN. So a product of
+// one adapter with eight columns goes to registers of its own and each column takes
+// or leaves it; sorting keeps that to about one product per eight columns plus one
+// per adapter.
+//
+// U enters the tensor cores in its fp32 precision: a row of U is scaled by a power
+// of two to at most 1 and split into 16-bit parts (three of bf16 make 24 bits, two
+// of f16 make 22; two of bf16 where the result has 16 bits anyway), whose products
+// are summed in fp32; the power of two multiplies the sum.
 #pragma once
+
+#include <type_traits>
 
 #include "fg_adapter.h"
 #include "fg_tcgen05.cuh"
@@ -22,122 +30,175 @@
 namespace fg {
 namespace adapt {
 
-// The row's slot, or -1 without an adapter: none wanted, an id out of range, or
-// a slot with scale 0.
+// The slot a row names, or -1 without an adapter: none wanted, or an id out of range.
 __device__ __forceinline__ int row_slot(const Params& P, int b) {
     const int a = P.adapters ? P.adapters[b] : -1;
-    return (a >= 0 && a < P.slots && P.scales[a] != 0.0f) ? a : -1;
+    return (a >= 0 && a < P.slots) ? a : -1;
 }
 
 constexpr int DOWN_THREADS = 256;
-constexpr int DOWN_K = 4096;   // hidden elements staged at a time
 
-// One row per CTA: its position in the sorted order of its batch tile (rows with
-// the same adapter next to each other, ties in row order), and U, a warp per rank
-// index (2 * RC of them each, their 16-byte loads in flight together).
 template <int DT>
 __device__ __forceinline__ float from_bits(uint16_t b) {
     if constexpr (DT == FG_DTYPE_F16) return __half2float(__ushort_as_half(b));
     else return __uint_as_float(uint32_t(b) << 16);
 }
+template <int DT>
+__device__ __forceinline__ uint16_t to_bits(float x) {
+    if constexpr (DT == FG_DTYPE_F16) return __half_as_ushort(__float2half_rn(x));
+    else return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+}
 
+// Eight 16-bit elements from any element-aligned address.
+template <bool WIDE>
+__device__ __forceinline__ uint4 load8(const uint16_t* p) {
+    if constexpr (WIDE) return *reinterpret_cast<const uint4*>(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = uint32_t(p[2 * i]) | (uint32_t(p[2 * i + 1]) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// This thread's part of the row's products with the warp's rank indices.
+template <int DT, int RC, bool WIDE>
+__device__ __forceinline__ void down_dots(const Params& P, const uint16_t* src, const uint16_t* dn, int warp, int lane,
+                                          float (&acc)[2 * RC]) {
+    const int vec = P.dim / 8;
+#pragma unroll(RC == 1 ? 4 : RC == 2 ? 2 : 1)
+    for (int i = lane; i < vec; i += 32) {
+        uint4 q[2 * RC];
+#pragma unroll
+        for (int j = 0; j < 2 * RC; ++j)
+            if (warp + 8 * j < P.rank)
+                q[j] = __ldg(reinterpret_cast<const uint4*>(dn + (warp + 8 * j) * P.down_stride) + i);
+        float x[8];
+        Elem<DT>::unpack(load8<WIDE>(src + 8 * i), x);
+#pragma unroll
+        for (int j = 0; j < 2 * RC; ++j) {
+            if (warp + 8 * j >= P.rank) break;
+            float y[8];
+            Elem<DT>::unpack(q[j], y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[j] = fmaf(x[e], y[e], acc[j]);
+        }
+    }
+    const int k = vec * 8 + lane;
+    if (k < P.dim) {
+        const float x = from_bits<DT>(src[k]);
+#pragma unroll
+        for (int j = 0; j < 2 * RC; ++j)
+            if (warp + 8 * j < P.rank)
+                acc[j] = fmaf(x, from_bits<DT>(dn[(warp + 8 * j) * P.down_stride + k]), acc[j]);
+    }
+}
+
+// One row per CTA: its position in the sorted order of its batch tile (rows with
+// the same adapter next to each other, ties in row order), its copy there, and U, a
+// warp per rank index (2 * RC of them each, their 16-byte loads in flight together).
+// It stages nothing in shared memory: project_kernel's CTAs take nearly all of it
+// and start beside this kernel's.
 template <int DT, int RC>
 __global__ void __launch_bounds__(DOWN_THREADS) down_kernel(const Params P) {
-    __shared__ __align__(16) uint16_t xs[DOWN_K];
+    __shared__ float us[16 * RC];
     tc::launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = blockIdx.x;
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(P.raw_hidden) + int64_t(b) * P.raw_stride;
+    const bool wide = reinterpret_cast<uintptr_t>(src) % 16 == 0;
     const int b0 = b / P.nt * P.nt, n = min(P.nt, P.batch - b0);
+    // the row's slot is the only step on the way to its loads: the scale (0: no
+    // adapter), the order and the copy are worked out while those are under way
     const int slot = row_slot(P, b);
-    const int key = ((slot + 1) << 9) | (b - b0);
-    int ahead = 0;
-    if (tid < n) ahead = (((row_slot(P, b0 + tid) + 1) << 9) | tid) < key;
-    const int pos = b0 + __syncthreads_count(ahead);
+    const float scale = slot >= 0 ? P.scales[slot] : 0.0f;
+    float acc[2 * RC] = {};
+    if (slot >= 0) {
+        const uint16_t* dn = reinterpret_cast<const uint16_t*>(P.down) + int64_t(slot) * P.rank * P.down_stride;
+        if (wide) down_dots<DT, RC, true>(P, src, dn, warp, lane, acc);
+        else down_dots<DT, RC, false>(P, src, dn, warp, lane, acc);
+    }
+    int pos = b;
+    if (P.sorted) {
+        const int key = slot * MAX_NT + (b - b0);
+        const bool ahead = tid < n && row_slot(P, b0 + tid) * MAX_NT + tid < key;
+        pos = b0 + __syncthreads_count(ahead);
+    }
     if (tid == 0) {
-        P.order[pos] = key;
+        P.order[pos] = ((scale != 0.0f ? slot + 1 : 0) << 9) | (b - b0);
         if (P.out_status) P.out_status[b] = (P.adapters && P.adapters[b] >= P.slots) ? FG_ROW_BAD_PARAM : 0;
     }
-    if (slot < 0 && P.copy == nullptr) return;
-
-    const uint16_t* src = reinterpret_cast<const uint16_t*>(P.raw_hidden) + int64_t(b) * P.raw_stride;
-    const uint16_t* dn = reinterpret_cast<const uint16_t*>(P.down) + int64_t(max(slot, 0)) * P.rank * P.down_stride;
-    const bool wide = reinterpret_cast<uintptr_t>(src) % 16 == 0;
-    float acc[2 * RC] = {};
-    for (int k0 = 0; k0 < P.dim; k0 += DOWN_K) {
-        const int len = min(DOWN_K, P.dim - k0), vec = len / 8;
-        __syncthreads();
+    if (P.copy) {
+        uint16_t* dst = reinterpret_cast<uint16_t*>(P.copy) + int64_t(pos) * P.copy_stride;
+        const int vec = P.dim / 8;
         if (wide) {
-            for (int i = tid; i < vec; i += DOWN_THREADS)
-                reinterpret_cast<uint4*>(xs)[i] = reinterpret_cast<const uint4*>(src + k0)[i];
-            for (int k = vec * 8 + tid; k < len; k += DOWN_THREADS) xs[k] = src[k0 + k];
-        } else {
-#pragma unroll 4
-            for (int k = tid; k < len; k += DOWN_THREADS) xs[k] = src[k0 + k];
-        }
-        __syncthreads();
-        if (P.copy) {
-            uint16_t* dst = reinterpret_cast<uint16_t*>(P.copy) + int64_t(b) * P.copy_stride + k0;
-            for (int i = tid; i < vec; i += DOWN_THREADS)
-                reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<uint4*>(xs)[i];
-            for (int k = vec * 8 + tid; k < len; k += DOWN_THREADS) dst[k] = xs[k];
-        }
-        if (slot < 0) continue;
 #pragma unroll 2
-        for (int i = lane; i < vec; i += 32) {
-            float x[8];
-            Elem<DT>::unpack(reinterpret_cast<const uint4*>(xs)[i], x);
-            uint4 q[2 * RC];
-#pragma unroll
-            for (int j = 0; j < 2 * RC; ++j)
-                if (warp + 8 * j < P.rank)
-                    q[j] = __ldg(reinterpret_cast<const uint4*>(dn + (warp + 8 * j) * P.down_stride + k0) + i);
-#pragma unroll
-            for (int j = 0; j < 2 * RC; ++j) {
-                if (warp + 8 * j >= P.rank) break;
-                float y[8];
-                Elem<DT>::unpack(q[j], y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) acc[j] = fmaf(x[e], y[e], acc[j]);
-            }
+            for (int i = tid; i < vec; i += DOWN_THREADS)
+                reinterpret_cast<uint4*>(dst)[i] = load8<true>(src + 8 * i);
+        } else {
+#pragma unroll 2
+            for (int i = tid; i < vec; i += DOWN_THREADS)
+                reinterpret_cast<uint4*>(dst)[i] = load8<false>(src + 8 * i);
         }
-        const int k = vec * 8 + lane;
-        if (k < len) {
-            const float x = from_bits<DT>(xs[k]);
-#pragma unroll
-            for (int j = 0; j < 2 * RC; ++j)
-                if (warp + 8 * j < P.rank)
-                    acc[j] = fmaf(x, Elem<DT>::load(dn + (warp + 8 * j) * P.down_stride + k0, k), acc[j]);
-        }
+        for (int k = vec * 8 + tid; k < P.dim; k += DOWN_THREADS) dst[k] = src[k];
     }
-    if (slot < 0) return;
-    const float scale = P.scales[slot];
+    if (scale == 0.0f) return;
 #pragma unroll
     for (int j = 0; j < 2 * RC; ++j) {
-        float s = acc[j];
-        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if (lane == 0 && warp + 8 * j < P.rank) P.u[int64_t(pos) * P.rank + warp + 8 * j] = s * scale;
+        float v = acc[j];
+        for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+        if (lane == 0) us[warp + 8 * j] = v * scale;   // 0 past the rank
+    }
+    __syncthreads();
+    if (warp == 0) {
+        float top = 0.0f;
+        for (int i = lane; i < 16 * RC; i += 32) top = fmaxf(top, fabsf(us[i]));
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        // |U| 2^-e <= 1; outside [2^-100, 2^100] (and without a finite maximum) the row is left as it is
+        const bool plain = !(top >= 0x1p-100f && top <= 0x1p100f);
+        const int e = plain ? 0 : ilogbf(top) + 1;
+        const float down = ldexpf(1.0f, -e);
+        if (lane == 0) P.unit[pos] = ldexpf(1.0f, e);
+        uint16_t* dst = reinterpret_cast<uint16_t*>(P.u) + int64_t(pos) * (3 * 16 * RC);
+        for (int i = lane; i < 16 * RC; i += 32) {
+            float v = us[i] * down;
+#pragma unroll
+            for (int part = 0; part < 3; ++part) {
+                const uint16_t h = to_bits<DT>(v);
+                dst[part * 16 * RC + i] = h;
+                const float left = v - from_bits<DT>(h);
+                v = (left - left == 0.0f) ? left : 0.0f;   // inf and NaN live in the first part
+            }
+        }
     }
 }
 
 // ---------------------------------------------------------------------------
 // project_kernel: persistent, one CTA per SM (CG = 1) or one pair of CTAs per two
-// SMs (CG = 2). Warp 0 loads (TMA), warp 1 issues the products, warps 2..9 are the
-// epilogue (two per quarter of the accumulator's lanes). Two accumulators in
-// tensor memory: one tile's epilogue runs beside the next tile's products.
+// SMs (CG = 2). Warp 0 loads (TMA), warp 1 issues the products, the others are the
+// epilogue (two or four per quarter of the accumulator's lanes). Two to eight
+// accumulators in tensor memory: one tile's epilogue runs beside the next products.
 //
 // fp32 results: the tensor core truncates when it adds a product to the
 // accumulator, and over hundreds of steps that bias shows in 32 bits. So the sum
-// over K is taken in pieces of PIECE_K, alternating between the two accumulators,
-// and the epilogue warps add the pieces in registers with rounding. A 16-bit
+// over K is taken in pieces of PIECE_K, one accumulator each, and the epilogue warps
+// add the pieces in registers with rounding. A 16-bit
 // result does not see the difference and takes the whole sum in one piece.
 // ---------------------------------------------------------------------------
 constexpr int A_BYTES = TILE_V * TILE_K * 2;
 constexpr int MAX_STAGES = 12;
-constexpr int EPI_WARPS = 8;
-constexpr int PROJ_THREADS = 64 + 32 * EPI_WARPS;
-constexpr int U_FLOATS = 512;                      // U of a group of columns, per epilogue warp
-constexpr int U_BYTES = EPI_WARPS * U_FLOATS * 4;
+// Epilogue warps, and how many windows of its tile each works out before the
+// products arrive (the others' adapters are added as they are read). With fp32
+// results the registers go to the sums: next to the ring there is no L1 left, and a
+// spilled register would wait for L2.
+template <int ODT, int RC>
+struct Epilogue {
+    static constexpr bool PIECES = ODT == FG_DTYPE_F32;
+    static constexpr int WARPS = PIECES ? (RC <= 2 ? 16 : 8) : (RC <= 2 ? 12 : 8);
+    static constexpr int EARLY = RC == 0 || PIECES ? 0 : RC == 1 ? 3 : RC <= 4 ? 2 : 1;
+    static constexpr int THREADS = 64 + 32 * WARPS;            // of the CTA
+};
 constexpr int PIECE_K = 8;                         // 64-wide steps of K per piece of an fp32 sum
+
+constexpr int MAX_ACC = 8;   // accumulators in tensor memory
 
 // Barrier over `threads` threads that also tells all of them whether any had `p`.
 __device__ __forceinline__ bool named_any(int id, int threads, bool p) {
@@ -150,7 +211,7 @@ __device__ __forceinline__ bool named_any(int id, int threads, bool p) {
 
 struct Control {
     uint64_t full[MAX_STAGES], empty[MAX_STAGES];
-    uint64_t acc_full[2], acc_empty[2], drain;
+    uint64_t acc_full[MAX_ACC], acc_empty[MAX_ACC], drain;
     uint32_t tmem;
     int abort;
 };
@@ -163,154 +224,192 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return *reinterpret_cast<float2*>(&d);
 }
 
-// One vocabulary row of an adapter's `up`: 16 * RC elements (zero past the rank).
-template <int DT, int RC>
-struct UpRow {
-    uint4 q[2 * RC];
-    __device__ __forceinline__ void load(const Params& P, int slot, int v) {
-        const uint4* src = reinterpret_cast<const uint4*>(
-            reinterpret_cast<const uint16_t*>(P.up) + (int64_t(slot) * P.vocab + v) * P.rank);
+// D (16 x 8, fp32) += A (16 x 16) B (16 x 8) of 16-bit operands, on one warp.
+template <int DT>
+__device__ __forceinline__ void warp_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+    if constexpr (DT == FG_DTYPE_F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                     "{%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+
+// The A fragments of one adapter for the warp's 32 vocabulary rows: two tiles of 16
+// rows, RC steps of 16 ranks. A thread (g = lane / 4, t = lane % 4) holds ranks
+// 4t .. 4t + 3 of a step in rows g and g + 8 of a tile: eight bytes at a time, where
+// the instruction's own order would be two pairs (B is laid out alike, so the sum
+// does not change).
+template <int RC>
+struct UpTile {
+    uint2 q[RC][4];   // rows g, g + 8, g + 16, g + 24
+    __device__ __forceinline__ void load(const Params& P, int slot, int v0, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        const uint16_t* up = reinterpret_cast<const uint16_t*>(P.up) + int64_t(slot) * P.vocab * P.rank + 4 * t;
 #pragma unroll
-        for (int i = 0; i < 2 * RC; ++i) q[i] = (i * 8 < P.rank) ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-    }
-    __device__ __forceinline__ void unpack(float2 (&w)[8 * RC]) const {
+        for (int i = 0; i < 4; ++i) {
+            const uint16_t* row = up + int64_t(min(v0 + g + 8 * i, P.vocab - 1)) * P.rank;
 #pragma unroll
-        for (int i = 0; i < 2 * RC; ++i) {
-            float x[8];
-            Elem<DT>::unpack(q[i], x);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[4 * i + j] = make_float2(x[2 * j], x[2 * j + 1]);
+            for (int c = 0; c < RC; ++c)
+                q[c][i] = 16 * c + 4 * t < P.rank ? __ldg(reinterpret_cast<const uint2*>(row + 16 * c))
+                                                  : make_uint2(0, 0);
         }
     }
 };
 
-// x + U[row] . up[v]; `u` in shared memory, the same for the whole warp.
-template <int RC>
-__device__ __forceinline__ float add_adapter(float x, const float* u, const float2 (&w)[8 * RC], int rank) {
-    float2 s0 = make_float2(x, 0.0f), s1 = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int c = 0; c < RC; ++c) {
-        if (c > 0 && c * 16 >= rank) break;
-#pragma unroll
-        for (int q = 4 * c; q < 4 * c + 4; ++q) {
-            const float4 f = reinterpret_cast<const float4*>(u)[q];
-            s0 = fma2(make_float2(f.x, f.y), w[2 * q], s0);
-            s1 = fma2(make_float2(f.z, f.w), w[2 * q + 1], s1);
-        }
-    }
-    return (s0.x + s0.y) + (s1.x + s1.y);
-}
-
-// The epilogue of one warp over positions [p, p1) of the tile's sorted order.
-// `base`: the warp's lanes of the accumulator; v: this lane's vocabulary id (in:
-// below vocab). Columns go eight at a time where they share an adapter and one at
-// a time around the changes; the next adapter's row is on its way meanwhile.
+// What one epilogue warp keeps while it goes over windows of eight columns: the
+// fragments of the adapter used last. A window's other adapters come BATCH at a
+// time, their loads in flight together.
 template <int DT, int ODT, int RC>
-__device__ __forceinline__ void finish_columns(const Params& P, uint32_t base, int b0, int p, int p1, int v, bool in,
-                                               float* ubuf, int lane) {
-    constexpr int R = RC > 0 ? RC : 1;
-    if constexpr (RC == 0) {
-        for (; p < p1; p += 8) {
-            float x[8];
+struct Windows {
+    static constexpr int PARTS = (DT == FG_DTYPE_BF16 && ODT == FG_DTYPE_F32) ? 3 : 2;
+    static constexpr int BATCH = RC == 1 && ODT != FG_DTYPE_F32 ? 3 : 1;
+    static constexpr uint32_t ALL = 0xffffffffu;
+    UpTile<RC> up;
+    int cur = -1;
+
+    // This lane's column (lane % 8) of window w: (slot + 1) << 9 | row of the tile,
+    // or -1 past the rows.
+    __device__ __forceinline__ static int entry(const Params& P, int b0, int rows, int w, int lane) {
+        const int p = 8 * w + (lane & 7);
+        return p < rows ? P.order[b0 + p] : -1;
+    }
+
+    // One adapter's product with the window; the columns in `match` take it, no other does.
+    __device__ __forceinline__ static void apply(float (&x)[2][4], const UpTile<RC>& tile, const uint2 (&u)[RC][PARTS],
+                                                 float unit0, float unit1, uint32_t match, int t) {
+        float d[2][4] = {};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) tc::tmem_ld1(x[i], base + min(p + i, p1 - 1));
-            tc::tmem_wait_ld(x);
+        for (int i = PARTS - 1; i >= 0; --i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (p + i < p1 && in) Elem<ODT>::store(P.out, int64_t(b0 + p + i) * P.out_stride + v, x[i]);
+            for (int c = 0; c < RC; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    warp_mma<DT>(d[h], tile.q[c][2 * h].x, tile.q[c][2 * h + 1].x, tile.q[c][2 * h].y,
+                                 tile.q[c][2 * h + 1].y, u[c][i]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (match >> (2 * t) & (i & 1 ? 2 : 1)) x[h][i] = d[h][i] * (i & 1 ? unit1 : unit0);
+    }
+
+    // The adapters' share of window w, eight columns by 32 vocabulary rows from v0 on:
+    // columns 2t, 2t + 1 of rows g + 8 i.
+    __device__ __forceinline__ void adapters(float (&x)[2][4], const Params& P, int b0, int rows, int w, int v0,
+                                             int ent, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        const int slots = ent < 0 ? -1 : (ent >> 9) - 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[0][i] = x[1][i] = 0.0f;
+        uint32_t left = __ballot_sync(ALL, slots >= 0) & 0xffu;   // columns still without their adapter
+        if (left == 0) return;
+        // B fragments: parts of U for column g
+        uint2 u[RC][PARTS];
+        const uint2* src = reinterpret_cast<const uint2*>(P.u) + int64_t(b0 + min(8 * w + g, rows - 1)) * (12 * RC) + t;
+#pragma unroll
+        for (int c = 0; c < RC; ++c)
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) u[c][i] = src[i * 4 * RC + c * 4];
+        const int p = 8 * w + 2 * t;
+        const float unit0 = p < rows ? P.unit[b0 + p] : 0.0f, unit1 = p + 1 < rows ? P.unit[b0 + p + 1] : 0.0f;
+        const uint32_t held = __ballot_sync(ALL, slots == cur) & left;
+        if (held) {
+            left &= ~held;
+            apply(x, up, u, unit0, unit1, held, t);
         }
-    } else {
-        constexpr int GROUP = R == 1 ? 32 : U_FLOATS / (16 * R);
-        constexpr int STEP = GROUP < 8 ? GROUP : 8;
-        constexpr bool AHEAD = R <= 4;   // registers for a second row
-        const int rank = P.rank;
-        const int vrow = in ? v : P.vocab - 1;
-        float2 w[8 * R];
-        UpRow<DT, R> next;
-        int cur = -1, next_slot = -1;
-        int entry = (lane < GROUP && p + lane < p1) ? P.order[b0 + p + lane] : 0;
-        float4 un[4];
-        auto fetch_u = [&](int at) {
-            const int total = min(GROUP, p1 - at) * rank / 4;
-            const float4* src = reinterpret_cast<const float4*>(P.u + int64_t(b0 + at) * rank);
+        while (left) {
+            // all but the last go through registers of their own; the last stays
+            UpTile<RC> tile[BATCH > 1 ? BATCH - 1 : 1];
+            uint32_t match[BATCH];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (lane + 32 * i < total) un[i] = src[lane + 32 * i];
-        };
-        if (p < p1) fetch_u(p);
-        while (p < p1) {
-            const int cnt = min(GROUP, p1 - p);
-            const int ent = entry;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (lane + 32 * i < cnt * rank / 4) reinterpret_cast<float4*>(ubuf)[lane + 32 * i] = un[i];
-            __syncwarp();
-            const int pn = p + cnt;
-            entry = (lane < GROUP && pn + lane < p1) ? P.order[b0 + pn + lane] : 0;
-            if (pn < p1) fetch_u(pn);
-            const int slots = (ent >> 9) - 1;   // this lane's column's
-            for (int j = 0; j < cnt;) {
-                const int slot = __shfl_sync(0xffffffffu, slots, j);
-                if (slot != cur) {
-                    cur = slot;
-                    if (slot >= 0) {
-                        if (!AHEAD || slot != next_slot) next.load(P, slot, vrow);
-                        next.unpack(w);
-                    }
-                    if (AHEAD) {
-                        uint32_t m = __ballot_sync(0xffffffffu, lane > j && lane < cnt && slots != slot);
-                        next_slot = -1;
-                        if (m) {
-                            next_slot = __shfl_sync(0xffffffffu, slots, __ffs(m) - 1);
-                        } else {
-                            m = __ballot_sync(0xffffffffu, lane < GROUP && pn + lane < p1 && (entry >> 9) - 1 != slot);
-                            if (m) next_slot = (__shfl_sync(0xffffffffu, entry, __ffs(m) - 1) >> 9) - 1;
-                        }
-                        if (next_slot >= 0) next.load(P, next_slot, vrow);
-                    }
-                }
-                const uint32_t same = __ballot_sync(0xffffffffu, lane < cnt && slots == slot) >> j;
-                constexpr uint32_t FULL = STEP == 32 ? 0xffffffffu : (1u << STEP) - 1;
-                if ((same & FULL) == FULL) {
-                    float x[STEP];
-                    int col[STEP];
-#pragma unroll
-                    for (int i = 0; i < STEP; ++i) {
-                        col[i] = __shfl_sync(0xffffffffu, ent, j + i) & 511;
-                        tc::tmem_ld1(x[i], base + col[i]);
-                    }
-                    tc::tmem_wait_ld(x);
-                    if (slot >= 0) {
-#pragma unroll
-                        for (int i = 0; i < STEP; ++i) x[i] = add_adapter<R>(x[i], ubuf + (j + i) * rank, w, rank);
-                    }
-#pragma unroll
-                    for (int i = 0; i < STEP; ++i)
-                        if (in) Elem<ODT>::store(P.out, int64_t(b0 + col[i]) * P.out_stride + v, x[i]);
-                    j += STEP;
-                } else {
-                    float x[1];
-                    const int col = __shfl_sync(0xffffffffu, ent, j) & 511;
-                    tc::tmem_ld1(x[0], base + col);
-                    tc::tmem_wait_ld(x);
-                    if (slot >= 0) x[0] = add_adapter<R>(x[0], ubuf + j * rank, w, rank);
-                    if (in) Elem<ODT>::store(P.out, int64_t(b0 + col) * P.out_stride + v, x[0]);
-                    ++j;
+            for (int i = 0; i < BATCH; ++i) {
+                match[i] = 0;
+                const bool last = i == BATCH - 1;
+                if (last ? left != 0 : (left & (left - 1)) != 0) {
+                    const int slot = __shfl_sync(ALL, slots, __ffs(left) - 1);
+                    match[i] = __ballot_sync(ALL, slots == slot) & 0xffu;
+                    left &= ~match[i];
+                    if (last) up.load(P, cur = slot, v0, lane);
+                    else tile[i].load(P, slot, v0, lane);
                 }
             }
-            __syncwarp();
-            p = pn;
+#pragma unroll
+            for (int i = 0; i < BATCH - 1; ++i)
+                if (match[i]) apply(x, tile[i], u, unit0, unit1, match[i], t);
+            if (match[BATCH - 1]) apply(x, up, u, unit0, unit1, match[BATCH - 1], t);
         }
+    }
+};
+
+// Read window w of the accumulator, add the adapters' share and store it.
+template <int ODT>
+__device__ __forceinline__ void store_window(const Params& P, uint32_t base, int b0, int w, int v0, int ent,
+                                             const float (&add)[2][4], int lane) {
+    constexpr uint32_t ALL = 0xffffffffu;
+    const int g = lane >> 2, t = lane & 3;
+    float x[2][4];
+    tc::tmem_ld_window(x[0], base + 8 * w);
+    tc::tmem_ld_window(x[1], base + 8 * w + (16u << 16));
+    tc::tmem_wait_ld(x[0]);
+    tc::tmem_wait_ld(x[1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[0][i] += add[0][i];
+        x[1][i] += add[1][i];
+    }
+    if (ODT != FG_DTYPE_F32 && P.wide_out && v0 + 32 <= P.vocab) {
+        // 16-bit results: transpose 8 x 8 blocks so that a thread holds pairs of
+        // neighbouring rows of column g, then exchange among its four threads: eight
+        // neighbouring rows, one 16-byte store
+        uint32_t r[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t pack = uint32_t(to_bits<ODT>(x[h][2 * i])) |
+                                      (uint32_t(to_bits<ODT>(x[h][2 * i + 1])) << 16);
+                asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r[2 * h + i]) : "r"(pack));
+            }
+        const bool odd = t & 1, high = t & 2;
+        uint32_t s0 = __shfl_xor_sync(ALL, odd ? r[0] : r[1], 1), s1 = __shfl_xor_sync(ALL, odd ? r[2] : r[3], 1);
+        const uint32_t a0 = odd ? s0 : r[0], a1 = odd ? r[1] : s0;   // block `odd` of threads t & ~1, t | 1
+        const uint32_t a2 = odd ? s1 : r[2], a3 = odd ? r[3] : s1;   // block 2 + odd
+        s0 = __shfl_xor_sync(ALL, high ? a0 : a2, 2);
+        s1 = __shfl_xor_sync(ALL, high ? a1 : a3, 2);
+        const uint4 q = high ? make_uint4(s0, s1, a2, a3) : make_uint4(a0, a1, s0, s1);
+        const int eg = __shfl_sync(ALL, ent, g);
+        if (eg >= 0)
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(P.out) +
+                                      int64_t(b0 + (eg & 511)) * P.out_stride + v0 + 8 * t) = q;
+    } else {
+        const int e0 = __shfl_sync(ALL, ent, 2 * t), e1 = __shfl_sync(ALL, ent, 2 * t + 1);
+        const int64_t o0 = int64_t(b0 + (e0 & 511)) * P.out_stride, o1 = int64_t(b0 + (e1 & 511)) * P.out_stride;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int v = v0 + g + 16 * h + 8 * i;
+                if (v < P.vocab) {
+                    if (e0 >= 0) Elem<ODT>::store(P.out, o0 + v, x[h][2 * i]);
+                    if (e1 >= 0) Elem<ODT>::store(P.out, o1 + v, x[h][2 * i + 1]);
+                }
+            }
     }
 }
 
 // RC: rank / 16 held in registers (rounded up to 1, 2, 4 or 8), 0: no adapters.
 template <int CG, int DT, int ODT, int RC>
-__global__ void __launch_bounds__(PROJ_THREADS, 1)
+__global__ void __launch_bounds__(Epilogue<ODT, RC>::THREADS, 1)
 project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Params P) {
     extern __shared__ uint8_t dyn[];
     __shared__ Control C;
     constexpr bool PIECES = ODT == FG_DTYPE_F32;
+    constexpr int EPI_WARPS = Epilogue<ODT, RC>::WARPS;
     uint8_t* ring = dyn + ((1024 - (smem_u32(dyn) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? tc::cta_rank() : 0;
@@ -327,7 +426,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             mbar_init(&C.full[s], 1);
             mbar_init(&C.empty[s], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < P.accs; ++i) {
             mbar_init(&C.acc_full[i], 1);
             mbar_init(&C.acc_empty[i], CG * EPI_WARPS);
         }
@@ -348,60 +447,92 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
 
     if (warp == 0) {
         if (lane == 0) {
-            if (P.copy) tc::wait_prerequisites();   // the aligned rows come from down_kernel
-            int it = 0;
+            const uint32_t ring_a = smem_u32(ring);
+            const uint32_t full0 = CG == 2 ? tc::mapa(&C.full[0], 0) : smem_u32(&C.full[0]);
+            int stage = 0, used = 0;      // used: stages handed out so far, up to S
+            uint32_t parity = 1;          // of the ring's previous round
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step) {
                 const int v0 = ((t / P.ntile) * CG + rank) * TILE_V;
                 const int b0 = (t % P.ntile) * P.nt + rank * (P.nt / CG);
-                for (int kc = 0; kc < nk; kc += P.kb, ++it) {
-                    const int s = it % S;
-                    if (it >= S && !mbar_wait(&C.empty[s], ((it / S) - 1) & 1, &C.abort)) { ok = false; break; }
+                for (int kc = 0; kc < nk; kc += P.kb) {
+                    if (used == S && !mbar_wait(&C.empty[stage], parity, &C.abort)) { ok = false; break; }
                     const int boxes = min(P.kb, nk - kc);
-                    const uint32_t bar = CG == 2 ? tc::mapa(&C.full[s], 0) : smem_u32(&C.full[s]);
-                    if (rank == 0) mbar_arrive_expect_tx(&C.full[s], CG * boxes * box_bytes);
-                    uint32_t a = smem_u32(ring + s * stage_bytes);
-                    for (int q = 0; q < boxes; ++q, a += box_bytes) {
-                        tc::tma_load_2d<CG>(a, &wmap, (kc + q) * TILE_K, v0, bar);
-                        tc::tma_load_2d<CG>(a + A_BYTES, &xmap, (kc + q) * TILE_K, b0, bar);
+                    uint32_t a = ring_a + stage * stage_bytes;
+                    if (used < S) {
+                        if (++used == 1) {
+                            // the first round's weights do not wait for down_kernel
+                            int s1 = 0;
+                            for (int t1 = first; t1 < tiles && s1 < S; t1 += step)
+                                for (int k1 = 0; k1 < nk && s1 < S; k1 += P.kb, ++s1) {
+                                    const int n1 = min(P.kb, nk - k1);
+                                    if (rank == 0) mbar_arrive_expect_tx(&C.full[s1], CG * n1 * box_bytes);
+                                    for (int q = 0; q < n1; ++q)
+                                        tc::tma_load_2d<CG>(ring_a + s1 * stage_bytes + q * box_bytes, &wmap,
+                                                            (k1 + q) * TILE_K, ((t1 / P.ntile) * CG + rank) * TILE_V,
+                                                            full0 + 8 * s1);
+                                }
+                            if (P.copy) {
+                                tc::wait_prerequisites();   // the sorted rows come from down_kernel
+                                asm volatile("fence.proxy.async.global;" ::: "memory");
+                            }
+                        }
+                    } else {
+                        if (rank == 0) mbar_arrive_expect_tx(&C.full[stage], CG * boxes * box_bytes);
+                        for (int q = 0; q < boxes; ++q)
+                            tc::tma_load_2d<CG>(a + q * box_bytes, &wmap, (kc + q) * TILE_K, v0, full0 + 8 * stage);
+                    }
+                    for (int q = 0; q < boxes; ++q)
+                        tc::tma_load_2d<CG>(a + q * box_bytes + A_BYTES, &xmap, (kc + q) * TILE_K, b0,
+                                            full0 + 8 * stage);
+                    if (++stage == S) {
+                        stage = 0;
+                        parity ^= 1;
                     }
                 }
             }
             if (!ok) {
-                // gave up: let the copies in flight land before the block leaves
+                // gave up: let the copies in flight land before the block leaves (the pair's
+                // barriers are the first CTA's, so this is a wait by time)
                 *reinterpret_cast<volatile int*>(&C.abort) = 1;
-                if (rank == 0)
-                    for (int j = max(0, it - S); j < it; ++j)
-                        mbar_wait_for(&C.full[j % S], (j / S) & 1, WAIT_LIMIT_NS / 16);
-                for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 1000000;) {}
+                for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 10000000;) {}
             }
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             const uint32_t idesc = tc::instr_desc(DT, TILE_V * CG, P.nt);
-            int it = 0, n = 0;
+            const uint64_t desc0 = tc::operand_desc(smem_u32(ring));
+            int stage = 0, acc = 0;
+            uint32_t parity = 0, acc_parity = 1;   // a fresh barrier counts as passed with parity 1
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step) {
-                for (int k0 = 0; k0 < nk && ok; k0 += piece, ++n) {
-                    const int acc = n & 1, k1 = min(nk, k0 + piece);
-                    if (n >= 2 && !mbar_wait(&C.acc_empty[acc], ((n >> 1) - 1) & 1, &C.abort)) { ok = false; break; }
+                for (int k0 = 0; k0 < nk && ok; k0 += piece) {
+                    const int k1 = min(nk, k0 + piece);
+                    if (!mbar_wait(&C.acc_empty[acc], acc_parity, &C.abort)) { ok = false; break; }
                     tc::fence_after();
                     const uint32_t d = tmem + acc * P.nt;
-                    for (int kc = k0; kc < k1; kc += P.kb, ++it) {
-                        const int s = it % S;
-                        if (!mbar_wait(&C.full[s], (it / S) & 1, &C.abort)) { ok = false; break; }
+                    for (int kc = k0; kc < k1; kc += P.kb) {
+                        if (!mbar_wait(&C.full[stage], parity, &C.abort)) { ok = false; break; }
                         tc::fence_after();
                         const int boxes = min(P.kb, k1 - kc);
-                        for (int q = 0; q < boxes; ++q) {
-                            const uint32_t a = smem_u32(ring + s * stage_bytes + q * box_bytes);
-                            const uint64_t ad = tc::operand_desc(a), bd = tc::operand_desc(a + A_BYTES);
+                        uint64_t ad = desc0 + uint32_t(stage * stage_bytes) / 16;
+                        for (int q = 0; q < boxes; ++q, ad += box_bytes / 16) {
+                            const uint64_t bd = ad + A_BYTES / 16;
 #pragma unroll
                             for (int k = 0; k < TILE_K / 16; ++k)
                                 tc::mma<CG>(d, ad + 2 * k, bd + 2 * k, idesc, kc + q > k0 || k > 0);
                         }
-                        tc::commit<CG>(&C.empty[s]);
+                        tc::commit<CG>(&C.empty[stage]);
+                        if (++stage == S) {
+                            stage = 0;
+                            parity ^= 1;
+                        }
                     }
                     if (ok) tc::commit<CG>(&C.acc_full[acc]);
+                    if (++acc == P.accs) {
+                        acc = 0;
+                        acc_parity ^= 1;
+                    }
                 }
             }
             if (!ok) {
@@ -411,65 +542,83 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             }
         }
     } else {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
-        float* ubuf = reinterpret_cast<float*>(ring + S * stage_bytes) + (warp - 2) * U_FLOATS;
-        const uint32_t empty_bar[2] = {CG == 2 ? tc::mapa(&C.acc_empty[0], 0) : smem_u32(&C.acc_empty[0]),
-                                       CG == 2 ? tc::mapa(&C.acc_empty[1], 0) : smem_u32(&C.acc_empty[1])};
-        auto release = [&](int acc) {
+        const int quarter = warp & 3, part = (warp - 2) >> 2;   // of PARTS
+        constexpr int PARTS = EPI_WARPS / 4;
+        const uint32_t empty_bar = CG == 2 ? tc::mapa(&C.acc_empty[0], 0) : smem_u32(&C.acc_empty[0]);
+        int acc = 0;
+        uint32_t acc_parity = 0;
+        auto release = [&]() {   // the accumulator at hand is read; on to the next
             tc::fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (CG == 2) tc::arrive_cluster(empty_bar[acc]);
-                else mbar_arrive_a(empty_bar[acc]);
+                if (CG == 2) tc::arrive_cluster(empty_bar + 8 * acc);
+                else mbar_arrive_a(empty_bar + 8 * acc);
+            }
+            if (++acc == P.accs) {
+                acc = 0;
+                acc_parity ^= 1;
             }
         };
         tc::wait_prerequisites();   // U, the order and the status words come from down_kernel
-        int n = 0;
         bool ok = true;
         for (int t = first; t < tiles && ok; t += step) {
             const int v = ((t / P.ntile) * CG + rank) * TILE_V + quarter * 32 + lane, b0 = (t % P.ntile) * P.nt;
             const int rows = min(P.nt, P.batch - b0);
-            const int mid = (rows + 1) / 2;
+            const int windows = (rows + 7) / 8, w0 = windows * part / PARTS, w1 = windows * (part + 1) / PARTS;
+            const int vw = v - lane;   // the warp's first vocabulary row
             const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
-            if (PIECES && nk > piece) {
-                const int cols = P.nt / 2;   // this warp's share of the columns, a multiple of 8
-                float sum[MAX_NT / 2];
+            // the adapters' share of the first windows, while the products run
+            constexpr int EARLY = Epilogue<ODT, RC>::EARLY;
+            constexpr int R = RC > 0 ? RC : 1;
+            using W = Windows<DT, ODT, R>;
+            W win;
+            float add[EARLY > 0 ? EARLY : 1][2][4];
+            int ents[EARLY > 0 ? EARLY : 1];
+            if constexpr (EARLY > 0) {
+                if (vw < P.vocab) {
 #pragma unroll
-                for (int i = 0; i < MAX_NT / 2; ++i) sum[i] = 0.0f;
+                    for (int i = 0; i < EARLY; ++i) ents[i] = W::entry(P, b0, rows, w0 + i, lane);
+#pragma unroll
+                    for (int i = 0; i < EARLY; ++i)
+                        if (w0 + i < w1) win.adapters(add[i], P, b0, rows, w0 + i, vw, ents[i], lane);
+                }
+            }
+            if (PIECES && nk > piece) {
+                // this warp's columns: every PARTS-th block of eight
+                float sum[MAX_NT / PARTS];
+#pragma unroll
+                for (int i = 0; i < MAX_NT / PARTS; ++i) sum[i] = 0.0f;
                 uint32_t at = 0;
                 for (int k0 = 0; k0 < nk; k0 += piece) {
-                    ok = mbar_wait(&C.acc_full[n & 1], (n >> 1) & 1, &C.abort);
+                    ok = mbar_wait(&C.acc_full[acc], acc_parity, &C.abort);
                     if (!ok) break;
                     tc::fence_after();
-                    at = lanes + (n & 1) * P.nt + half * cols;
+                    at = lanes + acc * P.nt + part * 8;
 #pragma unroll
-                    for (int i = 0; i < MAX_NT / 2; i += 8) {
-                        if (i < cols) {
+                    for (int i = 0; i < MAX_NT / PARTS; i += 8) {
+                        if (part * 8 + i * PARTS < P.nt) {
                             float x[8];
-                            tc::tmem_ld8(x, at + i);
+                            tc::tmem_ld8(x, at + i * PARTS);
                             tc::tmem_wait_ld(x);
 #pragma unroll
                             for (int j = 0; j < 8; ++j) sum[i + j] += x[j];
                         }
                     }
-                    if (k0 + piece < nk) {
-                        release(n & 1);
-                        ++n;
-                    }
+                    if (k0 + piece < nk) release();
                 }
                 if (ok) {
                     // the whole sums go back to where the last piece was
 #pragma unroll
-                    for (int i = 0; i < MAX_NT / 2; i += 8)
-                        if (i < cols) tc::tmem_st8(sum + i, at + i);
+                    for (int i = 0; i < MAX_NT / PARTS; i += 8)
+                        if (part * 8 + i * PARTS < P.nt) tc::tmem_st8(sum + i, at + i * PARTS);
                     tc::tmem_wait_st();
                 }
                 tc::fence_before();
-                // the two warps of this quarter of the lanes, which go on or give up together
-                ok = !named_any(1 + quarter, 64, !ok);
+                // the warps of this quarter of the lanes, which go on or give up together
+                ok = !named_any(1 + quarter, 32 * PARTS, !ok);
                 tc::fence_after();
             } else {
-                ok = mbar_wait(&C.acc_full[n & 1], (n >> 1) & 1, &C.abort);
+                ok = mbar_wait(&C.acc_full[acc], acc_parity, &C.abort);
                 tc::fence_after();
             }
             if (!ok) {
@@ -478,10 +627,27 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                     for (int i = 0; i < rows; ++i) atomicOr(&P.out_status[b0 + i], FG_ROW_TIMEOUT);
                 break;
             }
-            finish_columns<DT, ODT, RC>(P, lanes + (n & 1) * P.nt, b0, half ? mid : 0, half ? rows : mid, v,
-                                        v < P.vocab, ubuf, lane);
-            release(n & 1);
-            ++n;
+            const uint32_t base = lanes + acc * P.nt;
+            if (vw < P.vocab) {
+                if constexpr (EARLY > 0) {
+#pragma unroll
+                    for (int i = 0; i < EARLY; ++i)
+                        if (w0 + i < w1) store_window<ODT>(P, base, b0, w0 + i, vw, ents[i], add[i], lane);
+                }
+                if constexpr (EARLY == 0) win = W{};
+                for (int w = w0 + EARLY; w < w1; ++w) {
+                    float more[2][4] = {};
+                    int ent = 8 * w + (lane & 7);
+                    if constexpr (RC > 0) {
+                        ent = W::entry(P, b0, rows, w, lane);
+                        win.adapters(more, P, b0, rows, w, vw, ent, lane);
+                    } else if (ent >= rows) {
+                        ent = -1;
+                    }
+                    store_window<ODT>(P, base, b0, w, vw, ent, more, lane);
+                }
+            }
+            release();
         }
     }
     tc::fence_before();

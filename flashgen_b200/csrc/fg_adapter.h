@@ -22,17 +22,21 @@ struct Params {
     const int32_t* adapters;
     void* out;
     int32_t* out_status;
-    float* u;                 // [B, rank] in the sorted order (workspace)
+    void* u;                  // [B, 3, 16 RC] in the sorted order: 16-bit parts of U times a power of two (workspace)
+    float* unit;              // [B] in the sorted order: that power's inverse (workspace)
     int32_t* order;           // [B] per batch tile: (slot + 1) << 9 | column, sorted (workspace)
-    void* copy;               // [B, copy_stride] aligned hidden rows, or null (workspace)
+    void* copy;               // [B, copy_stride] hidden rows, sorted and aligned, or null (workspace)
     int32_t batch, dim, vocab, rank, slots;
     int64_t down_stride, out_stride, copy_stride;
     int32_t ntile;            // batch tiles
+    int32_t sorted;           // rows of a tile in the order of their adapters (else as they come)
+    int32_t wide_out;         // rows of out 16-byte aligned
     int32_t nt;               // columns of a batch tile, a multiple of 16 up to 256
     // project_kernel
     int32_t nvt;              // vocabulary tiles of 128 (256 for a pair)
     int32_t stages;           // of the operand ring
     int32_t kb;               // 64-wide boxes of K in a stage
+    int32_t accs;             // accumulators of nt columns in tensor memory
     int32_t tmem_cols;
 };
 

@@ -17,7 +17,8 @@ int launch_project(const Params& P, const CUtensorMap& wmap, const CUtensorMap& 
     static std::atomic<bool> attr_set[host::kMaxDevices] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return FG_EDEVICE;
-    const int room = d->smem_optin - int(sizeof(Control)) - 256;
+    // what the SM has, less this kernel's static part and down_kernel's CTA beside it
+    const int room = std::min(d->smem_optin - int(sizeof(Control)) - 256, d->smem_per_sm - 5 * 1024);
     if (!attr_set[dev].load(std::memory_order_acquire)) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, room) != cudaSuccess)
             return FG_EDEVICE;
@@ -25,12 +26,11 @@ int launch_project(const Params& P, const CUtensorMap& wmap, const CUtensorMap& 
     }
     Params Q = P;
     const int stage = P.kb * (A_BYTES + P.nt / CG * TILE_K * 2);
-    const int ubytes = RC > 0 ? U_BYTES : 0;
-    Q.stages = std::min(MAX_STAGES, (room - 1024 - ubytes) / stage);
+    Q.stages = std::min(MAX_STAGES, (room - 1024) / stage);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(std::min(P.nvt * P.ntile, d->sms / CG) * CG);
-    cfg.blockDim = dim3(PROJ_THREADS);
-    cfg.dynamicSmemBytes = size_t(1024 + Q.stages * stage + ubytes);
+    cfg.blockDim = dim3(Epilogue<ODT, RC>::THREADS);
+    cfg.dynamicSmemBytes = size_t(1024 + Q.stages * stage);
     cfg.stream = st;
     cudaLaunchAttribute attr[2] = {};
     if (CG == 2) {
@@ -53,6 +53,16 @@ int launch_rank(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xma
                 host::DevInfo* d, cudaStream_t st) {
     const bool first = P.adapters || P.copy || P.out_status;
     if (first) {
+        // the same division of the SM's memory as project_kernel's, so that both fit beside each other
+        static std::atomic<bool> attr_set[host::kMaxDevices] = {};
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess) return FG_EDEVICE;
+        if (!attr_set[dev].load(std::memory_order_acquire)) {
+            if (cudaFuncSetAttribute(down_kernel<DT, RC ? RC : 1>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                     (int)cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+                return FG_EDEVICE;
+            attr_set[dev].store(true, std::memory_order_release);
+        }
         down_kernel<DT, RC ? RC : 1><<<P.batch, DOWN_THREADS, 0, st>>>(P);
         if (cudaGetLastError() != cudaSuccess) return FG_ELAUNCH;
     }
@@ -63,7 +73,7 @@ int launch_rank(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xma
 template <int DT, int ODT>
 int launch(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, bool pair, host::DevInfo* d,
            cudaStream_t st) {
-    const int rc = P.adapters && P.slots > 0 ? P.rank / 16 : 0;
+    const int rc = P.adapters && P.slots > 0 ? (P.rank + 15) / 16 : 0;
     if (rc == 0) return launch_rank<DT, ODT, 0>(P, wmap, xmap, pair, d, st);
     if (rc == 1) return launch_rank<DT, ODT, 1>(P, wmap, xmap, pair, d, st);
     if (rc == 2) return launch_rank<DT, ODT, 2>(P, wmap, xmap, pair, d, st);

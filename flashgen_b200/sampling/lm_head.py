@@ -53,7 +53,7 @@ class AdapterHead:
         self.vocab, self.dim = weight.shape
         self.device, self.dtype = weight.device, weight.dtype
         self.slots, self.rank = int(slots), int(rank)
-        self._rank = (self.rank + 15) // 16 * 16          # the bank's rank
+        self._rank = (self.rank + 7) // 8 * 8             # the bank's rank
         width = (self.dim + 7) // 8 * 8
         self._down = torch.zeros(self.slots, self._rank, width, dtype=self.dtype, device=self.device)
         self._up = torch.zeros(self.slots, self.vocab, self._rank, dtype=self.dtype, device=self.device)

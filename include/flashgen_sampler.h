@@ -333,7 +333,7 @@ int fg_token_logprobs_grad(const FgLogprobGradArgs* args, void* stream);
  * Layout: weight [vocab, dim] with weight_stride, down [slots, rank, dim] with
  * down_stride between the rows of one adapter and rank * down_stride between
  * adapters, up [slots, vocab, rank] dense. All three 16-byte aligned, the
- * strides multiples of 8 elements, rank a multiple of 16 up to
+ * strides multiples of 8 elements, rank a multiple of 8 up to
  * FG_ADAPTER_MAX_RANK (an adapter of lower rank has zero rows of down or zero
  * columns of up). hidden and out need only the alignment of their elements.
  *
@@ -362,7 +362,7 @@ typedef struct FgAdapterArgs {
     int32_t        batch;               /* B >= 0                                  */
     int32_t        dim;                 /* >= 1                                    */
     int32_t        vocab;               /* V >= 1                                  */
-    int32_t        rank;                /* 16 .. FG_ADAPTER_MAX_RANK, or any if slots == 0 */
+    int32_t        rank;                /* 8 .. FG_ADAPTER_MAX_RANK, or any if slots == 0 */
     int32_t        slots;               /* >= 0                                    */
     int32_t        reserved;            /* 0                                       */
     int64_t        hidden_stride;       /* elements between rows, >= dim           */

@@ -45,7 +45,7 @@ def _args(**kw):
 @pytest.mark.parametrize("bad", [
     dict(hidden=None), dict(weight=None), dict(out=None), dict(down=None), dict(up=None), dict(scales=None),
     dict(dtype=_lib.FG_DTYPE_F32), dict(out_dtype=_lib.FG_DTYPE_F16), dict(batch=-1), dict(dim=0), dict(vocab=0),
-    dict(rank=0), dict(rank=8), dict(rank=24), dict(rank=144), dict(slots=-1), dict(reserved=1),
+    dict(rank=0), dict(rank=4), dict(rank=20), dict(rank=136), dict(slots=-1), dict(reserved=1),
     dict(hidden_stride=59), dict(weight_stride=60), dict(weight_stride=56), dict(down_stride=56),
     dict(down_stride=60), dict(out_stride=99), dict(weight=264), dict(down=264), dict(up=264), dict(hidden=257),
     dict(out=258), dict(workspace=None), dict(workspace=128), dict(workspace_bytes=255)])
@@ -67,7 +67,7 @@ def test_workspace_size():
     f = _lib.load().fg_adapter_workspace_size
     assert f(64, 4096, 16, 8) >= 64 * 16 * 4
     assert f(64, 4096, 16, 0) > 0 and f(0, 4096, 16, 3) > 0
-    assert f(64, 4096, 24, 1) == 0 and f(-1, 4096, 16, 1) == 0 and f(1, 0, 16, 1) == 0
+    assert f(64, 4096, 20, 1) == 0 and f(-1, 4096, 16, 1) == 0 and f(1, 0, 16, 1) == 0
 
 
 def test_cpu_weight_is_refused():

@@ -1,12 +1,14 @@
 // fg_logprobs.cu — C ABI entry points of the token log probabilities and their
 // gradient: argument checks and launches.
 #include <algorithm>
+#include <atomic>
 
 #include "fg_internal.h"
 #include "fg_logprobs.cuh"
 
 namespace {
 
+using fg::host::DevInfo;
 using fg::host::elem_size;
 
 bool rows_ok(const void* p, int dtype, int64_t stride, int32_t vocab) {
@@ -15,10 +17,56 @@ bool rows_ok(const void* p, int dtype, int64_t stride, int32_t vocab) {
 
 constexpr int32_t kMaxRows = 1 << 30;
 
-template <int DT>
+// CTAs per row: more of them shorten a row but each pays the fixed part (reductions,
+// alternatives). Time in us of `waves` rounds of CTAs, two an SM, whose steps of
+// THREADS * UNROLL chunks take what HBM gives all of them, at least a load's latency.
+int ctas_per_row(int32_t batch, int vocab, int elem, const DevInfo* d) {
+    const int64_t chunks = int64_t(vocab) * elem / 16;
+    const int64_t slots = 2 * d->sms;
+    const double step_bytes = 16.0 * fg::lp::THREADS * fg::lp::UNROLL;
+    int best = 1;
+    double least = 1e30;
+    for (int G = 1; G <= fg::lp::MAX_G; G *= 2) {
+        if (G > 1 && chunks / G < fg::lp::THREADS) break;
+        const int64_t ctas = int64_t(batch) * G;
+        const int64_t part = (chunks + G - 1) / G;
+        const double steps = double(std::max<int64_t>(1, (part + fg::lp::THREADS - 1) / fg::lp::THREADS)) / fg::lp::UNROLL;
+        const double step_us = std::max(0.8, double(std::min(ctas, slots)) * step_bytes / 6.4e6);
+        const double us = double((ctas + slots - 1) / slots) * (steps * step_us + 2.0 + (G > 1 ? 0.7 : 0.0));
+        if (us < 0.97 * least) {
+            least = us;
+            best = G;
+        }
+    }
+    return best;
+}
+
+template <int DT, bool TOP>
 int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
-    fg::lp::logprob_kernel<DT><<<batch, fg::lp::THREADS, 0, st>>>(P);
-    return cudaGetLastError() == cudaSuccess ? FG_OK : FG_ELAUNCH;
+    DevInfo* d = nullptr;
+    const int rc = fg::host::device_info(&d);
+    if (rc != FG_OK) return rc;
+    auto kern = fg::lp::logprob_kernel<DT, TOP>;
+    static std::atomic<bool> attr_set[fg::host::kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return FG_EDEVICE;
+    if (!attr_set[dev].load(std::memory_order_acquire)) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+            return FG_EDEVICE;
+        attr_set[dev].store(true, std::memory_order_release);
+    }
+    const int G = ctas_per_row(batch, P.vocab, fg::Elem<DT>::SIZE, d);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(batch) * G);
+    cfg.blockDim = dim3(fg::lp::THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = G;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = G > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, P, G) == cudaSuccess ? FG_OK : FG_ELAUNCH;
 }
 
 template <int DT>
@@ -37,7 +85,7 @@ int launch_grad(const fg::lp::GradParams& P, int32_t batch, cudaStream_t st) {
         if (P.entropy) Q.entropy = P.entropy + lo;
         if (P.grad_logprobs) Q.grad_logprobs = P.grad_logprobs + lo;
         if (P.grad_entropy) Q.grad_entropy = P.grad_entropy + lo;
-        fg::lp::logprob_grad_kernel<DT><<<dim3(per_row, n), fg::lp::THREADS, 0, st>>>(Q);
+        fg::lp::logprob_grad_kernel<DT><<<dim3(per_row, n), fg::lp::GRAD_THREADS, 0, st>>>(Q);
     }
     return cudaGetLastError() == cudaSuccess ? FG_OK : FG_ELAUNCH;
 }
@@ -61,9 +109,12 @@ int fg_token_logprobs(const FgLogprobArgs* a, void* stream) {
     P.out_top_logprobs = a->out_top_logprobs; P.out_status = a->out_status;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (a->dtype) {
-        case FG_DTYPE_F32: return launch_forward<FG_DTYPE_F32>(P, a->batch, st);
-        case FG_DTYPE_F16: return launch_forward<FG_DTYPE_F16>(P, a->batch, st);
-        default: return launch_forward<FG_DTYPE_BF16>(P, a->batch, st);
+        case FG_DTYPE_F32: 
+            return P.top ? launch_forward<FG_DTYPE_F32, true>(P, a->batch, st) : launch_forward<FG_DTYPE_F32, false>(P, a->batch, st);
+        case FG_DTYPE_F16: 
+            return P.top ? launch_forward<FG_DTYPE_F16, true>(P, a->batch, st) : launch_forward<FG_DTYPE_F16, false>(P, a->batch, st);
+        default: 
+            return P.top ? launch_forward<FG_DTYPE_BF16, true>(P, a->batch, st) : launch_forward<FG_DTYPE_BF16, false>(P, a->batch, st);
     }
 }
 

@@ -71,11 +71,20 @@ int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
 
 template <int DT>
 int launch_grad(const fg::lp::GradParams& P, int32_t batch, cudaStream_t st) {
-    const int per_row = std::max(1, std::min(8, P.vocab / 2048));
-    for (int32_t lo = 0; lo < batch; lo += 65535) {
+    DevInfo* d = nullptr;
+    const int rc = fg::host::device_info(&d);
+    if (rc != FG_OK) return rc;
+    // steps of GRAD_THREADS * GRAD_UNROLL chunks: one a CTA while they do not fill the
+    // machine, up to four a CTA when there are many
+    const int64_t esz = fg::Elem<DT>::SIZE;
+    const int64_t step = int64_t(fg::lp::GRAD_THREADS) * fg::lp::GRAD_UNROLL * 16 / esz;
+    const int64_t steps = (P.vocab + step - 1) / step;
+    const int64_t each = std::max<int64_t>(1, std::min<int64_t>(4, steps * batch / (8 * d->sms)));
+    const int per_row = int((steps + each - 1) / each);
+    const int32_t rows = std::max(1, (1 << 30) / per_row);   // rows a launch
+    for (int32_t lo = 0; lo < batch; lo += rows) {
         fg::lp::GradParams Q = P;
-        const int32_t n = std::min<int32_t>(65535, batch - lo);
-        const int64_t esz = fg::Elem<DT>::SIZE;
+        const int32_t n = std::min(rows, batch - lo);
         Q.logits = reinterpret_cast<const char*>(P.logits) + lo * P.row_stride * esz;
         Q.out_grad = reinterpret_cast<char*>(P.out_grad) + lo * P.grad_stride * esz;
         if (P.tokens) Q.tokens = P.tokens + lo;
@@ -85,9 +94,10 @@ int launch_grad(const fg::lp::GradParams& P, int32_t batch, cudaStream_t st) {
         if (P.entropy) Q.entropy = P.entropy + lo;
         if (P.grad_logprobs) Q.grad_logprobs = P.grad_logprobs + lo;
         if (P.grad_entropy) Q.grad_entropy = P.grad_entropy + lo;
-        fg::lp::logprob_grad_kernel<DT><<<dim3(per_row, n), fg::lp::GRAD_THREADS, 0, st>>>(Q);
+        fg::lp::logprob_grad_kernel<DT><<<unsigned(n) * unsigned(per_row), fg::lp::GRAD_THREADS, 0, st>>>(Q, per_row);
+        if (cudaGetLastError() != cudaSuccess) return FG_ELAUNCH;
     }
-    return cudaGetLastError() == cudaSuccess ? FG_OK : FG_ELAUNCH;
+    return FG_OK;
 }
 
 }  // namespace

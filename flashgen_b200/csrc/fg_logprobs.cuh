@@ -589,9 +589,18 @@ __global__ void __launch_bounds__(THREADS, 2) logprob_kernel(const Params P, con
     }
 }
 
+// ---------------------------------------------------------------------------
+// Gradient: dx_j = p_j (a + b y_j) + 1[j == t] g / T with y_j = (x_j - m) c - L2,
+// p_j = 2^y_j, a = -(g + h H) / T and b = -h ln2 / T.
+//
+// Bound: HBM, the logits read and the gradient written once. Work is cut along the
+// gradient's 16-byte chunks; where the logits' rows are offset against the
+// gradient's, a thread takes the two chunks around its own and shifts them together.
+// ---------------------------------------------------------------------------
 constexpr int GRAD_THREADS = 256;
+constexpr int GRAD_UNROLL = 4;   // chunks in flight a thread
 
-// A coherent load: the gradient may overwrite the logits.
+// Coherent loads: the gradient may overwrite the logits.
 template <int DT>
 __device__ __forceinline__ float load_rw(const char* row, int64_t j) {
     if constexpr (DT == FG_DTYPE_F32) return reinterpret_cast<const float*>(row)[j];
@@ -599,32 +608,146 @@ __device__ __forceinline__ float load_rw(const char* row, int64_t j) {
     else return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[j]);
 }
 
-// dx_j = p_j (a + b y_j) + 1[j == t] g / T with y_j = (x_j - m) c - L2,
-// p_j = 2^y_j, a = -(g + h H) / T and b = -h ln2 / T.
+// The 16 bytes that start `shift` bytes into a:b.
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int shift) {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (shift & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (shift & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    if (shift & 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct GradRow {
+    float m, c, l2, a, b;
+    __device__ __forceinline__ float at(float x) const {
+        const float y = fmaxf(fmaf(x - m, c, -l2), Y_MIN);
+        return exp2_fast(y) * fmaf(b, y, a);
+    }
+    __device__ __forceinline__ float2 at(float2 x) const {
+        float2 y = fma2(add2(x, make_float2(-m, -m)), make_float2(c, c), make_float2(-l2, -l2));
+        y = make_float2(fmaxf(y.x, Y_MIN), fmaxf(y.y, Y_MIN));
+        const float2 d = fma2(make_float2(b, b), y, make_float2(a, a));
+        return make_float2(exp2_fast(y.x) * d.x, exp2_fast(y.y) * d.y);
+    }
+};
+
 template <int DT>
-__global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const GradParams P) {
-    const int64_t r = blockIdx.y;
+__device__ __forceinline__ uint4 pack_chunk(const float (&x)[Elem<DT>::VEC]) {
+    uint32_t w[4];
+    if constexpr (DT == FG_DTYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == FG_DTYPE_F16) {
+                const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// CTA blockIdx.x: part blockIdx.x % per_row of row blockIdx.x / per_row.
+template <int DT>
+__global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const GradParams P, const int per_row) {
+    constexpr int VEC = Elem<DT>::VEC, SIZE = Elem<DT>::SIZE;
+    const int64_t r = blockIdx.x / per_row;
+    const int part = blockIdx.x % per_row, tid = threadIdx.x;
     const int V = P.vocab;
-    const char* row = reinterpret_cast<const char*>(P.logits) + r * P.row_stride * Elem<DT>::SIZE;
-    char* out = reinterpret_cast<char*>(P.out_grad) + r * P.grad_stride * Elem<DT>::SIZE;
+    const char* in = reinterpret_cast<const char*>(P.logits) + r * P.row_stride * SIZE;
+    char* out = reinterpret_cast<char*>(P.out_grad) + r * P.grad_stride * SIZE;
     const int64_t tok = P.tokens ? P.tokens[r] : -1;
     const float T = P.temperature ? P.temperature[r] : 1.0f;
     const float g = (P.grad_logprobs && tok >= 0) ? P.grad_logprobs[r] : 0.0f;
     const float h = P.grad_entropy ? P.grad_entropy[r] : 0.0f;
-    const float m = P.max[r];
-    const float l2 = P.logsum[r] * LOG2E;
-    const float c = LOG2E / T;
-    float a = -(g + (h != 0.0f ? h * P.entropy[r] : 0.0f)) / T;
-    const float b = -h * LN2 / T;
-    const bool bad = !temperature_ok(T) || tok >= V || isnan(l2) || isnan(m);
-    const bool zero = (g == 0.0f && h == 0.0f) || (m == -INFINITY && !bad);
-    if (bad) a = __int_as_float(0x7fc00000);
-    for (int j = blockIdx.x * GRAD_THREADS + threadIdx.x; j < V; j += gridDim.x * GRAD_THREADS) {
+    GradRow G;
+    G.m = P.max[r];
+    G.l2 = P.logsum[r] * LOG2E;
+    G.c = LOG2E / T;
+    G.a = -(g + (h != 0.0f ? h * P.entropy[r] : 0.0f)) / T;
+    G.b = -h * LN2 / T;
+    const bool bad = !temperature_ok(T) || tok >= V || isnan(G.l2) || isnan(G.m);
+    const bool zero = (g == 0.0f && h == 0.0f) || (G.m == -INFINITY && !bad);
+    if (bad) G.a = __int_as_float(0x7fc00000);
+    const float hit = g / T;
+
+    const int head = min(V, int((16 - (reinterpret_cast<uintptr_t>(out) & 15)) & 15) / SIZE);
+    const int nvec = (V - head) / VEC;
+    uint4* dst = reinterpret_cast<uint4*>(out + int64_t(head) * SIZE);
+    const char* src = in + int64_t(head) * SIZE;
+    const int shift = int(reinterpret_cast<uintptr_t>(src) & 15);
+    const uint4* aligned = reinterpret_cast<const uint4*>(src - shift);
+    // chunks whose two aligned neighbours lie within the row
+    const int safe0 = shift > head * SIZE ? 1 : 0;
+    const int safe1 = shift == 0 ? nvec : (V - head) * SIZE + shift >= 32 ? ((V - head) * SIZE + shift) / 16 - 1 : 0;
+    const int c0 = int(int64_t(nvec) * part / per_row), c1 = int(int64_t(nvec) * (part + 1) / per_row);
+    for (int first = c0 + tid; first < c1; first += GRAD_UNROLL * GRAD_THREADS) {
+        uint4 v[GRAD_UNROLL];
+        if (!zero) {
+#pragma unroll
+            for (int u = 0; u < GRAD_UNROLL; ++u) {
+                const int i = first + u * GRAD_THREADS;
+                if (i >= c1) break;
+                if (shift == 0) {
+                    v[u] = aligned[i];
+                } else if (i >= safe0 && i < safe1) {
+                    v[u] = shifted(aligned[i], aligned[i + 1], shift);
+                } else {
+                    float x[VEC];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) x[e] = load_rw<DT>(src, int64_t(i) * VEC + e);
+                    v[u] = pack_chunk<DT>(x);   // back to the bits they came from
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < GRAD_UNROLL; ++u) {
+            const int i = first + u * GRAD_THREADS;
+            if (i >= c1) break;
+            float x[VEC];
+            if (zero) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[e] = 0.0f;
+            } else {
+                Elem<DT>::unpack(v[u], x);
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) {
+                    const float2 d = G.at(make_float2(x[e], x[e + 1]));
+                    x[e] = d.x;
+                    x[e + 1] = d.y;
+                }
+                const int64_t at = tok - (head + int64_t(i) * VEC);
+                if (at >= 0 && at < VEC) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (e == at) x[e] += hit;
+                }
+            }
+            dst[i] = pack_chunk<DT>(x);
+        }
+    }
+    // the ragged ends, an element a thread
+    const int tail = V - head - nvec * VEC;
+    if (part == 0 && tid < head + tail) {
+        const int j = tid < head ? tid : V - tail + (tid - head);
         float d = 0.0f;
         if (!zero) {
-            const float y = fmaxf((load_rw<DT>(row, j) - m) * c - l2, Y_MIN);
-            d = exp2f(y) * (a + b * y);
-            if (j == tok) d += g / T;
+            d = G.at(load_rw<DT>(in, j));
+            if (j == tok) d += hit;
         }
         Elem<DT>::store(out, j, d);
     }

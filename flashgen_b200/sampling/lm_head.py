@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .sampler import _DTYPES, _ptr, _status_error
+from .sampler import _DTYPES, _call, _ptr, _status_error
 
 
 def _dense_rows(t: torch.Tensor) -> torch.Tensor:
@@ -55,8 +55,9 @@ class AdapterHead:
         self.slots, self.rank = int(slots), int(rank)
         self._rank = (self.rank + 7) // 8 * 8             # the bank's rank
         width = (self.dim + 7) // 8 * 8
-        self._down = torch.zeros(self.slots, self._rank, width, dtype=self.dtype, device=self.device)
-        self._up = torch.zeros(self.slots, self.vocab, self._rank, dtype=self.dtype, device=self.device)
+        # a slot's contents count once its scale is not 0
+        self._down = torch.empty(self.slots, self._rank, width, dtype=self.dtype, device=self.device)
+        self._up = torch.empty(self.slots, self.vocab, self._rank, dtype=self.dtype, device=self.device)
         self._scales = torch.zeros(self.slots, dtype=torch.float32, device=self.device)
 
     def _slot(self, slot: int) -> int:
@@ -72,10 +73,10 @@ class AdapterHead:
                 up.shape != (self.vocab, r):
             raise ValueError(f"an adapter of this head is down [r, {self.dim}] and up [{self.vocab}, r] with "
                              f"r <= {self.rank}, got {tuple(down.shape)} and {tuple(up.shape)}")
-        self._down[slot].zero_()
-        self._down[slot, :r, :self.dim] = down
         if r < self._rank:
+            self._down[slot, r:] = 0
             self._up[slot, :, r:] = 0
+        self._down[slot, :r, :self.dim] = down
         self._up[slot, :, :r] = up
         self._scales[slot] = float(scale)
 
@@ -124,9 +125,7 @@ class AdapterHead:
             _DTYPES[self.dtype], _DTYPES[out.dtype], B, self.dim, self.vocab, self._rank, slots, 0,
             hidden.stride(0) if B > 1 else self.dim, self.weight.stride(0), self._down.stride(1),
             out.stride(0) if B > 1 else self.vocab)
-        with torch.cuda.device(self.device):
-            _lib.check(lib.fg_adapter_logits(a, torch.cuda.current_stream(self.device).cuda_stream),
-                       "fg_adapter_logits")
+        _call(self.device, lib.fg_adapter_logits, a, "fg_adapter_logits")
         if check_errors:
             msg = _status_error(status)
             if msg is not None:

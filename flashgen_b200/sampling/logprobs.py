@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from .. import _lib
-from .sampler import _DTYPES, _ptr, _row_logits, _status_error
+from .sampler import _DTYPES, _call, _ptr, _row_logits, _status_error
 
 
 class TokenLogprobs(NamedTuple):
@@ -83,8 +83,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     tokens = _vector(tokens, torch.int64, logits, "tokens")
     temperature = _vector(temperature, torch.float32, logits, "temperature")
     dev = logits.device
-    logprobs, entropy, peak, logsum = torch.empty((4, B), dtype=torch.float32, device=dev).unbind(0)
-    rank, status = torch.empty((2, B), dtype=torch.int32, device=dev).unbind(0)
+    logprobs, entropy, peak, logsum, rank, status = torch.empty((6, B), dtype=torch.float32, device=dev).unbind(0)
+    rank, status = rank.view(torch.int32), status.view(torch.int32)
     top_ids = top_lp = None
     if top > 0:
         top_ids = torch.empty((B, top), dtype=torch.int64, device=dev)
@@ -94,9 +94,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
             logits.data_ptr(), _DTYPES[logits.dtype], B, V, top, logits.stride(0) if B > 1 else V,
             _ptr(tokens), _ptr(temperature), logprobs.data_ptr(), entropy.data_ptr(), peak.data_ptr(),
             logsum.data_ptr(), rank.data_ptr(), _ptr(top_ids), _ptr(top_lp), status.data_ptr())
-        lib = _lib.load()
-        with torch.cuda.device(dev):
-            _lib.check(lib.fg_token_logprobs(a, torch.cuda.current_stream(dev).cuda_stream), "fg_token_logprobs")
+        _call(dev, _lib.load().fg_token_logprobs, a, "fg_token_logprobs")
         if check_errors:
             msg = _status_error(status)
             if msg is not None:
@@ -134,10 +132,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], ma
             rows.data_ptr(), _DTYPES[rows.dtype], B, V, 0, rows.stride(0) if B > 1 else V, _ptr(tokens),
             _ptr(temperature), max.data_ptr(), logsum.data_ptr(), _ptr(entropy), _ptr(grad_logprobs),
             _ptr(grad_entropy), out.data_ptr(), out.stride(0) if B > 1 else V)
-        lib = _lib.load()
-        with torch.cuda.device(rows.device):
-            _lib.check(lib.fg_token_logprobs_grad(a, torch.cuda.current_stream(rows.device).cuda_stream),
-                       "fg_token_logprobs_grad")
+        _call(rows.device, _lib.load().fg_token_logprobs_grad, a, "fg_token_logprobs_grad")
     return out
 
 

@@ -47,6 +47,19 @@ def _row_logits(logits: torch.Tensor) -> torch.Tensor:
     return logits
 
 
+def _call(dev: torch.device, fn, args, what: str) -> None:
+    """One C-ABI call on ``dev``'s current stream (the raw handle: a Stream
+    object and a device switch cost more than the small kernels)."""
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(args, stream)
+    if rc != _lib.FG_OK:
+        _lib.check(rc, what)
+
+
 def histories_to_csr(histories: Sequence[Sequence[int]], device) -> Tuple[torch.Tensor, torch.Tensor, int]:
     """Pack per-row token lists into CSR (ids int32, offsets int64) on ``device``."""
     lens = np.fromiter((len(h) for h in histories), dtype=np.int64, count=len(histories))

@@ -17,28 +17,24 @@ bool rows_ok(const void* p, int dtype, int64_t stride, int32_t vocab) {
 
 constexpr int32_t kMaxRows = 1 << 30;
 
-// CTAs per row: more of them shorten a row but each pays the fixed part (reductions,
-// alternatives). Time in us of `waves` rounds of CTAs, two an SM, whose steps of
-// THREADS * UNROLL chunks take what HBM gives all of them, at least a load's latency.
+// CTAs per row for a batch too small to fill the machine with one each: as many as find
+// room at once (four an SM), with at least two chunks for each of their threads.
 int ctas_per_row(int32_t batch, int vocab, int elem, const DevInfo* d) {
     const int64_t chunks = int64_t(vocab) * elem / 16;
-    const int64_t slots = 2 * d->sms;
-    const double step_bytes = 16.0 * fg::lp::THREADS * fg::lp::UNROLL;
-    int best = 1;
-    double least = 1e30;
-    for (int G = 1; G <= fg::lp::MAX_G; G *= 2) {
-        if (G > 1 && chunks / G < fg::lp::THREADS) break;
-        const int64_t ctas = int64_t(batch) * G;
-        const int64_t part = (chunks + G - 1) / G;
-        const double steps = double(std::max<int64_t>(1, (part + fg::lp::THREADS - 1) / fg::lp::THREADS)) / fg::lp::UNROLL;
-        const double step_us = std::max(0.8, double(std::min(ctas, slots)) * step_bytes / 6.4e6);
-        const double us = double((ctas + slots - 1) / slots) * (steps * step_us + 2.0 + (G > 1 ? 0.7 : 0.0));
-        if (us < 0.97 * least) {
-            least = us;
-            best = G;
-        }
-    }
-    return best;
+    int G = 1;
+    while (2 * G <= fg::lp::MAX_G && int64_t(batch) * 2 * G <= 4 * d->sms && chunks / (2 * G) >= 2 * fg::lp::THREADS)
+        G *= 2;
+    return G;
+}
+
+template <class K>
+bool set_once(K kern, std::atomic<bool>* done, cudaFuncAttribute attr, int value) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    if (done[dev].load(std::memory_order_acquire)) return true;
+    if (cudaFuncSetAttribute(kern, attr, value) != cudaSuccess) return false;
+    done[dev].store(true, std::memory_order_release);
+    return true;
 }
 
 template <int DT, bool TOP>
@@ -46,16 +42,21 @@ int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
     DevInfo* d = nullptr;
     const int rc = fg::host::device_info(&d);
     if (rc != FG_OK) return rc;
-    auto kern = fg::lp::logprob_kernel<DT, TOP>;
-    static std::atomic<bool> attr_set[fg::host::kMaxDevices] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return FG_EDEVICE;
-    if (!attr_set[dev].load(std::memory_order_acquire)) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-            return FG_EDEVICE;
-        attr_set[dev].store(true, std::memory_order_release);
-    }
     const int G = ctas_per_row(batch, P.vocab, fg::Elem<DT>::SIZE, d);
+    if (G == 1) {
+        auto kern = fg::lp::rows_kernel<DT, TOP>;
+        constexpr int smem = fg::lp::RING_BYTES;
+        static std::atomic<bool> sized[fg::host::kMaxDevices] = {}, carved[fg::host::kMaxDevices] = {};
+        if (!set_once(kern, sized, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ||
+            !set_once(kern, carved, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared))
+            return FG_EDEVICE;
+        const int grid = std::min<int64_t>(batch, fg::lp::CTAS_PER_SM * d->sms);
+        kern<<<grid, fg::lp::THREADS, smem, st>>>(P, batch);
+        return cudaGetLastError() == cudaSuccess ? FG_OK : FG_ELAUNCH;
+    }
+    auto kern = fg::lp::row_kernel<DT, TOP>;
+    static std::atomic<bool> done[fg::host::kMaxDevices] = {};
+    if (!set_once(kern, done, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return FG_EDEVICE;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(batch) * G);
     cfg.blockDim = dim3(fg::lp::THREADS);
@@ -65,7 +66,7 @@ int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
     attr.val.clusterDim.x = G;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = G > 1 ? 1 : 0;
+    cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, P, G) == cudaSuccess ? FG_OK : FG_ELAUNCH;
 }
 

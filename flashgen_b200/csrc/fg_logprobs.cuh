@@ -56,28 +56,42 @@ __device__ __forceinline__ bool temperature_ok(float T) { return T >= 1.17549435
 // ---------------------------------------------------------------------------
 // Forward: one pass over the logits.
 //
-// A cluster of G CTAs takes a row, each a slice of its 16-byte chunks. A thread
-// streams its chunks four at a time and keeps, in 32 bits: its largest logit; S and
-// Q (below) against a reference that follows its largest logit (lazily: a sum may
-// grow to 2^64 above it, so it is rescaled about once); the count of the logits ahead
-// of the token's. S and Q are sums of 2^y and 2^y y with y = x c - r: one FMA a
-// logit, the same r in every term, so r's rounding cancels in log2 S + r.
+// A thread takes 16-byte chunks four at a time and keeps, in 32 bits: its largest
+// logit; S and Q (above) against a reference that follows its largest logit (lazily: a
+// sum may grow to 2^64 above it, so it is rescaled about once); the count of the
+// logits ahead of the token's. S and Q are sums of 2^y and 2^y y with y = x c - r:
+// one FMA a logit, the same r in every term, so r's rounding cancels in log2 S + r.
 //
-// Alternatives without a second pass over the row: the top-th largest of 64 group
-// maxima bounds the top-th largest logit from below, so every alternative lies with a
-// thread whose own maximum reaches the bound; there are few such threads, and only
-// their chunks are read again (from L2). What reaches the bound is gathered, and a
-// candidate's place is the number of candidates ahead of it.
+// Alternatives without a second pass over the row: each thread leaves the maxima of up
+// to SLOTS stretches of its chunks. The top-th largest of 32 group maxima bounds the
+// top-th largest logit from below, so every alternative lies in a stretch whose maximum
+// reaches the bound; there are few, and only their chunks are read again (from L2).
+// What reaches the bound is gathered, and a candidate's place is the number of
+// candidates ahead of it.
 //
-// Bound: HBM, one read of the logits. The work per 16-bit logit is 5.5 instructions
-// and one ex2, about two thirds of what the SMs can issue in that time.
+// Two kernels share this. rows_kernel: persistent CTAs, CTAS_PER_SM an SM, a row each
+// at a time; a thread copies its own chunks to shared memory DEPTH steps ahead
+// (asynchronously, no other thread reads them), across the end of a row, so the next
+// row's logits arrive while a row is finished. row_kernel: a cluster of G CTAs a row,
+// for batches that leave SMs idle otherwise.
+//
+// Bound: HBM, one read of the logits, for fp32; instruction issue and the rows' ends for
+// 16-bit logits (8 instructions and one ex2 a logit).
 // ---------------------------------------------------------------------------
-constexpr int THREADS = 512;
+constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int UNROLL = 4;            // chunks in flight a thread
-constexpr int GROUPS = 64;           // of THREADS / 64 = 8 lanes
-constexpr int MAX_G = 16;
-constexpr int CAND = 1024;           // candidates held at once
+constexpr int CTAS_PER_SM = 3;       // of rows_kernel
+constexpr int UNROLL_LOG = 2;
+constexpr int UNROLL = 1 << UNROLL_LOG;   // chunks a thread takes at a time
+constexpr int STEP = UNROLL * THREADS;
+constexpr int DEPTH = 3;             // steps in flight in rows_kernel
+constexpr int RING_BYTES = DEPTH * STEP * 16;
+constexpr int SLOTS = 8;             // stretches of a thread's chunks
+constexpr int GROUPS = 32;           // of THREADS / 32 neighbouring lanes, for the bound
+constexpr int LANES = THREADS / GROUPS;
+constexpr int MAX_G = 8;
+constexpr int STRETCHES = 64;        // a warp reads again
+constexpr int CAND = 256;            // candidates held at once
 constexpr float R_STEP = 64.0f;      // how far above its reference a term may be (in log2)
 
 // Order of the alternatives: larger logit first, then smaller id. A larger code
@@ -124,16 +138,24 @@ template <> struct Chunk<FG_DTYPE_F32> {
         return make_float2(fmaxf(__uint_as_float(w[2 * pair]), -1e30f), fmaxf(__uint_as_float(w[2 * pair + 1]), -1e30f));
     }
     static constexpr int PAIRS = 2;   // per chunk
-    struct Count {
+    // the next value below x (finite)
+    __device__ __forceinline__ static float below(float x) {
+        const uint32_t u = __float_as_uint(x);
+        return __uint_as_float(x == 0.0f ? 0x80000001u : (u >> 31) ? u + 1 : u - 1);
+    }
+    using Threshold = float;
+    __device__ __forceinline__ static Threshold threshold(float x) { return x; }
+    struct Count {   // logits above a threshold
         int n = 0;
-        __device__ __forceinline__ void add(const uint32_t* w, float xt, bool or_equal) {
+        __device__ __forceinline__ void add(const uint32_t* w, Threshold t) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = __uint_as_float(w[i]);
-                n += (or_equal ? x >= xt : x > xt) ? 1 : 0;
-            }
+            for (int i = 0; i < 4; ++i) n += __uint_as_float(w[i]) > t ? 1 : 0;
         }
-        __device__ __forceinline__ int take() { return n; }
+        __device__ __forceinline__ int take() {
+            const int k = n;
+            n = 0;
+            return k;
+        }
     };
 };
 template <class T2, int DT> struct Chunk16 {
@@ -155,23 +177,30 @@ template <class T2, int DT> struct Chunk16 {
         T2 x = __hmax2(pack(w[pair]), pack(low));
         return unpack(*reinterpret_cast<uint32_t*>(&x));
     }
+    __device__ __forceinline__ static float below(float x) {
+        uint32_t u = DT == FG_DTYPE_F16 ? uint32_t(__half_as_ushort(__float2half_rn(x))) : __float_as_uint(x) >> 16;
+        u = x == 0.0f ? 0x8001u : (u >> 15) ? u + 1 : u - 1;
+        return DT == FG_DTYPE_F16 ? __half2float(__ushort_as_half(uint16_t(u))) : __uint_as_float(u << 16);
+    }
+    using Threshold = uint32_t;   // twice
+    __device__ __forceinline__ static Threshold threshold(float x) {
+        const uint32_t u = DT == FG_DTYPE_F16 ? uint32_t(__half_as_ushort(__float2half_rn(x))) : __float_as_uint(x) >> 16;
+        return u | (u << 16);
+    }
+    // A comparison leaves 0xffff in each half that is above. The plain sum of these
+    // words is 2^16 (L - H) - L for L low and H high halves above: no unpacking while
+    // L and H stay below 2^15.
     struct Count {
-        T2 n = pack(0u);   // up to 16 in each half
-        __device__ __forceinline__ void add(const uint32_t* w, float xt, bool or_equal) {
-            T2 t;
-            if constexpr (DT == FG_DTYPE_F16) t = __float2half2_rn(xt);
-            else t = __float2bfloat162_rn(xt);
-            if (or_equal) {
+        uint32_t n = 0;
+        __device__ __forceinline__ void add(const uint32_t* w, Threshold t) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) n = __hadd2(n, __hge2(pack(w[i]), t));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) n = __hadd2(n, __hgt2(pack(w[i]), t));
-            }
+            for (int i = 0; i < 4; ++i) n += __hgt2_mask(pack(w[i]), pack(t));
         }
         __device__ __forceinline__ int take() {
-            const float2 f = unpack(*reinterpret_cast<uint32_t*>(&n));
-            return int(f.x + f.y);
+            const uint32_t low = (0u - n) & 0xffffu;
+            const uint32_t high = (low - ((n + low) >> 16)) & 0xffffu;
+            n = 0;
+            return int(low + high);
         }
     };
 };
@@ -184,9 +213,9 @@ template <> struct Chunk<FG_DTYPE_BF16> : Chunk16<__nv_bfloat162, FG_DTYPE_BF16>
     }
 };
 
-// Running sums of one thread.
+// Running sums of one thread, even and odd logits apart.
 struct Sums {
-    float s = 0.0f, q = 0.0f;
+    float2 s = {0.0f, 0.0f}, q = {0.0f, 0.0f};
     float r = 0.0f;                  // the reference, in log2
     float limit = -9.9e29f;          // logits above it move the reference
     bool set = false;
@@ -194,23 +223,39 @@ struct Sums {
         if (m > limit) {
             const float to = m * c;
             const float f = set ? exp2_fast(r - to) : 0.0f;
-            q = set ? f * fmaf(r - to, s, q) : 0.0f;
-            s *= f;
+            const float d = set ? r - to : 0.0f;
+            q = make_float2(f * fmaf(d, s.x, q.x), f * fmaf(d, s.y, q.y));
+            s = make_float2(f * s.x, f * s.y);
             r = to;
             limit = m + R_STEP / c;
             set = true;
         }
     }
-    __device__ __forceinline__ void add(float x, float c) {   // x floored
-        const float y = fmaf(x, c, -r);
-        const float e = exp2_fast(y);
-        s += e;
-        q = fmaf(e, y, q);
+    // a step's sums on their own first: the long sums' rounding errors stay few
+    struct Part {
+        float2 s = {0.0f, 0.0f}, q = {0.0f, 0.0f};
+    };
+    __device__ __forceinline__ void term(Part& p, float2 x, float c) const {   // floored logits
+        const float2 y = fma2(x, make_float2(c, c), make_float2(-r, -r));
+        const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+        p.s = add2(p.s, e);
+        p.q = fma2(e, y, p.q);
+    }
+    __device__ __forceinline__ void add(const Part& p) {
+        s = add2(s, p.s);
+        q = add2(q, p.q);
     }
 };
 
+// The warp's maximum, NaN if any lane has one (redux on fp32, sm_100a).
+__device__ __forceinline__ float warp_max_nan(float x) {
+    float m;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
+    return m;
+}
+
 // What a warp, a CTA and a row add up to: S and Q against the largest logit.
-struct Stats {
+struct alignas(16) Stats {   // (other CTAs write one as 16 bytes)
     float m, s, q;
     int n;   // logits ahead of the token's
 };
@@ -226,33 +271,31 @@ __device__ __forceinline__ Stats merge(const Stats& a, float m, float c) {   // 
     return r;
 }
 
-// The top-th largest of 64 values, two a lane (a warp-wide bitonic sort of both
-// halves, then the larger ones of both).
-__device__ __forceinline__ float kth_of_64(float a, float b, int k, int lane) {
+// The k-th largest of the lanes' values (a warp-wide bitonic sort).
+__device__ __forceinline__ float kth_of_32(float a, int k, int lane) {
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
         for (int d = size >> 1; d > 0; d >>= 1) {
             const bool keep_max = ((lane & size) == 0) == ((lane & d) == 0);
-            const float oa = __shfl_xor_sync(0xffffffffu, a, d), ob = __shfl_xor_sync(0xffffffffu, b, d);
-            a = keep_max ? fmaxf(a, oa) : fminf(a, oa);
-            b = keep_max ? fmaxf(b, ob) : fminf(b, ob);
+            const float o = __shfl_xor_sync(0xffffffffu, a, d);
+            a = keep_max ? fmaxf(a, o) : fminf(a, o);
         }
-    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, b, 31));   // descending a against ascending b
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        const float o = __shfl_xor_sync(0xffffffffu, a, d);
-        a = (lane & d) == 0 ? fmaxf(a, o) : fminf(a, o);
-    }
     return __shfl_sync(0xffffffffu, a, k - 1);
 }
 
-struct Shared {
-    Stats warp[WARPS];
-    Stats cta[MAX_G];                       // every CTA of the cluster writes its entry
-    float groups[GROUPS];
-    int count;                              // candidates
+// A row's place in shared memory; what a row leaves before its first barrier alternates
+// between two places, since a thread may be a row ahead of another by then.
+struct alignas(128) Shared {
+    Stats warp[2][WARPS];
+    float groups[2][GROUPS];
+    int count[2];                                // candidates
+    uint16_t stretch[WARPS][STRETCHES];          // thread | slot << 8
+    float slots[SLOTS][THREADS];                 // a thread's stretches' maxima (its own column)
     uint64_t cand[CAND];
+};
+struct alignas(16) ClusterShared {
+    Stats cta[MAX_G];                            // every CTA of the cluster writes its entry
     uint64_t lists[MAX_G][FG_LOGPROB_MAX_TOP];   // the CTAs' best (in the first CTA)
 };
 
@@ -264,21 +307,39 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-// One row's geometry: scalars before the first and after the last whole chunk, and
-// this CTA's chunks.
+// One row's geometry and parameters: scalars before the first and after the last
+// whole chunk, and this CTA's chunks.
 template <int DT>
 struct Row {
     static constexpr int VEC = Elem<DT>::VEC, SIZE = Elem<DT>::SIZE;
     const char* p;
+    int64_t r, tok;
     int V, head, nvec, tail, c0, c1;
-    __device__ __forceinline__ Row(const Params& P, int64_t r, int part, int parts) {
+    int tchunk;        // chunks before the token's count equal logits as ahead of it, the others do not
+    float T, xt, c;
+    typename Chunk<DT>::Threshold above, from;   // thresholds after and before the token
+    bool given;
+    __device__ __forceinline__ Row(const Params& P, int64_t row, int part, int parts)
+        : Row(P, row, part, parts, P.tokens ? P.tokens[row] : -1, P.temperature ? P.temperature[row] : 1.0f,
+              token_logit(P, row, P.tokens ? P.tokens[row] : -1)) {}
+    __device__ __forceinline__ static float token_logit(const Params& P, int64_t row, int64_t token) {
+        return token >= 0 && token < P.vocab ? Elem<DT>::load(P.logits, row * P.row_stride + token) : INFINITY;
+    }
+    __device__ __forceinline__ Row(const Params& P, int64_t row, int part, int parts, int64_t token, float temperature,
+                                   float logit)
+        : r(row), tok(token), T(temperature), xt(logit) {
         p = reinterpret_cast<const char*>(P.logits) + r * P.row_stride * SIZE;
         V = P.vocab;
         head = min(V, int((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / SIZE);
         nvec = (V - head) / VEC;
         tail = V - head - nvec * VEC;
-        c0 = int(int64_t(nvec) * part / parts);
-        c1 = int(int64_t(nvec) * (part + 1) / parts);
+        c0 = nvec / parts * part + min(part, nvec % parts);
+        c1 = c0 + nvec / parts + (part < nvec % parts ? 1 : 0);
+        given = tok >= 0 && tok < V;
+        c = LOG2E / T;
+        tchunk = !given || tok < head ? -1 : int((tok - head) / VEC);
+        above = Chunk<DT>::threshold(xt);
+        from = Chunk<DT>::threshold(Chunk<DT>::below(xt));
     }
     __device__ __forceinline__ const uint4* chunks() const {
         return reinterpret_cast<const uint4*>(p + int64_t(head) * SIZE);
@@ -287,166 +348,205 @@ struct Row {
     __device__ __forceinline__ int scalar_id(int i) const { return i < head ? i : V - tail + (i - head); }
 };
 
-template <int DT, bool TOP>
-__global__ void __launch_bounds__(THREADS, 2) logprob_kernel(const Params P, const int G) {
-    __shared__ Shared sh;
-    constexpr int VEC = Elem<DT>::VEC;
+// What one thread gathers in the pass.
+template <int DT>
+struct Pass {
     using C = Chunk<DT>;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t r = blockIdx.x / G;
-    const int part = blockIdx.x % G;
-    if (G > 1) cluster_arrive();   // the others' shared memory stands once all have arrived
-    const Row<DT> row(P, r, part, G);
-    const int V = row.V;
-    const int64_t tok = P.tokens ? P.tokens[r] : -1;
-    const float T = P.temperature ? P.temperature[r] : 1.0f;
-    const bool given = tok >= 0 && tok < V;
-    const float c = LOG2E / T;
-    const float xt = given ? Elem<DT>::load(row.p, tok) : INFINITY;
-    // chunks before the token's count equal logits as ahead of it, the others do not
-    const int tchunk = !given || tok < row.head ? -1 : int((tok - row.head) / VEC);
-    if (tid == 0) sh.count = 0;
-
-    // ---- the pass ----
-    const uint4* chunks = row.chunks();
     Sums acc;
-    float vmax = -INFINITY;
+    typename C::Count above;
+    float vmax = -INFINITY;   // NaN if any logit is
+    float smax = -INFINITY;   // of the stretch at hand
     int n = 0;
-    for (int c0 = row.c0 + tid; c0 < row.c1; c0 += UNROLL * THREADS) {
-        uint32_t w[UNROLL * 4];
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int ci = c0 + u * THREADS;
-            const uint32_t none = DT == FG_DTYPE_F32 ? 0xff800000u : DT == FG_DTYPE_F16 ? 0xfc00fc00u : 0xff80ff80u;
-            uint4 v = make_uint4(none, none, none, none);   // -inf
-            if (ci < row.c1) v = __ldg(chunks + ci);
-            w[4 * u] = v.x; w[4 * u + 1] = v.y; w[4 * u + 2] = v.z; w[4 * u + 3] = v.w;
+    // a step is done: at the end of a stretch of 2^log steps its maximum is left behind
+    __device__ __forceinline__ void stretch(Shared& sh, int step, int log, bool last) {
+        if (((step + 1) & ((1 << log) - 1)) == 0 || last) {
+            sh.slots[step >> log][threadIdx.x] = smax;
+            smax = -INFINITY;
         }
+    }
+    // UNROLL chunks (those past the row's end hold -inf); t[u]: the threshold of chunk u
+    __device__ __forceinline__ void take(const uint32_t (&w)[4 * UNROLL], const Row<DT>& row,
+                                         const typename C::Threshold (&t)[UNROLL]) {
         const float m = C::max_of(w, UNROLL * 4);
         vmax = fmax_nan(vmax, m);
-        acc.follow(m, c);
-        float2 s2 = make_float2(0.0f, 0.0f), q2 = make_float2(0.0f, 0.0f);
-        const float2 cc = make_float2(c, c), rr = make_float2(-acc.r, -acc.r);
+        smax = fmaxf(smax, m);
+        acc.follow(m, row.c);
+        Sums::Part part;
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-            for (int i = 0; i < C::PAIRS; ++i) {
-                const float2 y = fma2(C::floored(w + 4 * u, i), cc, rr);
-                const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-                s2 = add2(s2, e);
-                q2 = fma2(e, y, q2);
-            }
-        acc.s += s2.x + s2.y;
-        acc.q += q2.x + q2.y;
-        typename C::Count cnt;
+            for (int i = 0; i < C::PAIRS; ++i) acc.term(part, C::floored(w + 4 * u, i), row.c);
+        acc.add(part);
+        if (m >= row.xt) {   // (chunks past the end hold -inf: never above a threshold)
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int ci = c0 + u * THREADS;
-            if (ci < row.c1) cnt.add(w + 4 * u, xt, ci < tchunk);
+            for (int u = 0; u < UNROLL; ++u) above.add(w + 4 * u, t[u]);
         }
-        n += cnt.take();
     }
-    // the ragged ends, a logit a thread, and the equal logits in the token's own chunk
-    const int scalars = part == 0 ? row.head + row.tail : 0;
-    if (tid < scalars) {
-        const int j = row.scalar_id(tid);
-        const float x = Elem<DT>::load(row.p, j);
-        vmax = fmax_nan(vmax, x);
-        acc.follow(x, c);
-        acc.add(fmaxf(x, DT == FG_DTYPE_F16 ? -65504.0f : -1e30f), c);
-        if (given) n += (x > xt || (x == xt && j < tok)) ? 1 : 0;
+    // ci: the first chunk's index
+    __device__ __forceinline__ void take(const uint32_t (&w)[4 * UNROLL], const Row<DT>& row, int ci) {
+        typename C::Threshold t[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) t[u] = ci + u * THREADS < row.tchunk ? row.from : row.above;
+        take(w, row, t);
     }
-    if (tchunk >= row.c0 && tchunk < row.c1 && tid < VEC) {
-        const int j = row.id(tchunk) + tid;
-        if (j < tok && Elem<DT>::load(row.p, j) == xt) n += 1;
+    // at least every 512 steps: 2^15 above in a half would be too many
+    __device__ __forceinline__ void settle() { n += above.take(); }
+    // The ragged ends, a logit a thread, and the equal logits in the token's own chunk.
+    // Their loads are begun before the pass, so that its end does not wait for them.
+    float end, own;
+    __device__ __forceinline__ void begin(const Row<DT>& row, int scalars, int tid) {
+        end = -INFINITY;
+        own = __int_as_float(0x7fc00000);
+        if (tid < scalars) end = Elem<DT>::load(row.p, row.scalar_id(tid));
+        if (row.tchunk >= row.c0 && row.tchunk < row.c1 && tid < Row<DT>::VEC && row.id(row.tchunk) + tid < row.tok)
+            own = Elem<DT>::load(row.p, row.id(row.tchunk) + tid);
     }
+    __device__ __forceinline__ void ends(const Row<DT>& row, int scalars, int tid) {
+        settle();
+        if (tid < scalars) {
+            const float low = DT == FG_DTYPE_F16 ? -65504.0f : -1e30f;
+            vmax = fmax_nan(vmax, end);
+            acc.follow(end, row.c);
+            Sums::Part part;
+            acc.term(part, make_float2(fmaxf(end, low), low), row.c);   // (low adds 0)
+            acc.add(part);
+            if (row.given) n += (end > row.xt || (end == row.xt && row.scalar_id(tid) < row.tok)) ? 1 : 0;
+        }
+        n += own == row.xt ? 1 : 0;
+        // nothing is below -inf: a masked token has every logit before it ahead of it
+        if (tid == 0 && row.xt == -INFINITY) n += max(0, min(row.c1, row.tchunk) - row.c0) * Row<DT>::VEC;
+    }
+};
+
+// Steps of a stretch (its log2), so that SLOTS stretches hold all steps.
+__device__ __forceinline__ int stretch_log(int steps) {
+    int log = 0;
+    while ((SLOTS << log) < steps) ++log;
+    return log;
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 no_logits() {   // a chunk of -inf
+    const uint32_t w = DT == FG_DTYPE_F32 ? 0xff800000u : DT == FG_DTYPE_F16 ? 0xfc00fc00u : 0xff80ff80u;
+    return make_uint4(w, w, w, w);
+}
+
+// From the threads' sums to the row's results; chunk i of the CTA's belongs to thread
+// (i - c0) % THREADS.
+template <int DT, bool TOP, bool CLUSTER>
+__device__ __forceinline__ void finish_row(const Params& P, Shared& sh, ClusterShared* cl, const Row<DT>& row,
+                                           const Pass<DT>& pass, int scalars, int part, int G, int flip) {
+    constexpr int VEC = Elem<DT>::VEC;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float c = row.c, T = row.T, vmax = pass.vmax;
+    const int64_t r = row.r;
+    const uint4* chunks = row.chunks();
 
     // ---- the warp, then the CTA ----
-    float wm = vmax;
+    if (TOP) {
+        float gm = vmax;
 #pragma unroll
-    for (int d = 1; d < 8; d <<= 1) wm = fmax_nan(wm, __shfl_xor_sync(0xffffffffu, wm, d));
-    if (TOP && (lane & 7) == 0) sh.groups[tid >> 3] = wm;
-#pragma unroll
-    for (int d = 8; d < 32; d <<= 1) wm = fmax_nan(wm, __shfl_xor_sync(0xffffffffu, wm, d));
+        for (int d = 1; d < LANES; d <<= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, d));
+        if ((lane & (LANES - 1)) == 0) sh.groups[flip][tid / LANES] = gm;
+    }
     {
-        Stats st{wm, 0.0f, 0.0f, n};
-        if (acc.set) {
-            const float d = fmaxf(fmaf(-wm, c, acc.r), Y_MIN);   // the reference against the warp's maximum
+        Stats st;
+        st.m = warp_max_nan(vmax);
+        st.n = __reduce_add_sync(0xffffffffu, pass.n);
+        st.s = st.q = 0.0f;
+        if (pass.acc.set) {
+            const float d = fmaxf(fmaf(-st.m, c, pass.acc.r), Y_MIN);   // the reference against the warp's maximum
             const float f = exp2_fast(d);
-            st.s = f * acc.s;
-            st.q = f * fmaf(d, acc.s, acc.q);
+            st.s = f * (pass.acc.s.x + pass.acc.s.y);
+            st.q = f * fmaf(d, pass.acc.s.x + pass.acc.s.y, pass.acc.q.x + pass.acc.q.y);
         }
+        float2 sq = make_float2(st.s, st.q);
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            st.s += __shfl_xor_sync(0xffffffffu, st.s, d);
-            st.q += __shfl_xor_sync(0xffffffffu, st.q, d);
-            st.n += __shfl_xor_sync(0xffffffffu, st.n, d);
-        }
-        if (lane == 0) sh.warp[warp] = st;
+        for (int d = 16; d > 0; d >>= 1)
+            sq = add2(sq, make_float2(__shfl_xor_sync(0xffffffffu, sq.x, d), __shfl_xor_sync(0xffffffffu, sq.y, d)));
+        st.s = sq.x;
+        st.q = sq.y;
+        if (lane == 0) sh.warp[flip][warp] = st;
     }
     __syncthreads();
-    auto fold = [&](const Stats* from, int count, bool recount) {   // every warp the same, a lane an entry
+    if (tid == 0) sh.count[flip ^ 1] = 0;   // everyone is done with the row before
+    // the sums of up to 16 entries, a lane an entry (same_max: all against one maximum)
+    auto fold = [&](const Stats* from, int count, bool same_max) {
         Stats st{-INFINITY, 0.0f, 0.0f, 0};
         if (lane < count) st = from[lane];
-        float m = st.m;
+        const float m = warp_max_nan(st.m);
+        if (!same_max) st = merge(st, m, c);
+        st.n = __reduce_add_sync(0xffffffffu, st.n);
+        float2 sq = make_float2(st.s, st.q);
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-        if (!recount) st = merge(st, m, c);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            st.s += __shfl_xor_sync(0xffffffffu, st.s, d);
-            st.q += __shfl_xor_sync(0xffffffffu, st.q, d);
-            st.n += __shfl_xor_sync(0xffffffffu, st.n, d);
-        }
-        st.m = m;
-        return st;
+        for (int d = 8; d > 0; d >>= 1)
+            sq = add2(sq, make_float2(__shfl_xor_sync(0xffffffffu, sq.x, d), __shfl_xor_sync(0xffffffffu, sq.y, d)));
+        return Stats{m, __shfl_sync(0xffffffffu, sq.x, 0), __shfl_sync(0xffffffffu, sq.y, 0), st.n};
     };
-    Stats all = fold(sh.warp, WARPS, false);
+    // Every warp needs the row's maximum; its sums only where results are written.
+    Stats all{0.0f, 0.0f, 0.0f, 0};
+    if (CLUSTER || TOP || warp == 0) all = fold(sh.warp[flip], WARPS, false);
+    else all.m = warp_max_nan(sh.warp[flip][lane & (WARPS - 1)].m);
 
     // ---- alternatives: the candidates of this CTA ----
     int ncand = 0;
     if (TOP) {
-        const float bound = kth_of_64(sh.groups[lane], sh.groups[lane + 32], P.top, lane);
-        const uint32_t winners = __ballot_sync(0xffffffffu, vmax >= bound);
-        auto load_chunk = [&](int ci, float (&x)[VEC]) { Elem<DT>::unpack(__ldg(chunks + ci), x); };
-        // gather: winner by winner, a chunk a lane
+        const float bound = kth_of_32(sh.groups[flip][lane], P.top, lane);
+        const bool wins = vmax >= bound;
+        const uint32_t winners = __ballot_sync(0xffffffffu, wins);
         auto put = [&](uint64_t code) {
-            const int at = atomicAdd(&sh.count, 1);
+            const int at = atomicAdd(&sh.count[flip], 1);
             if (at < CAND) sh.cand[at] = code;
         };
-        auto each_winner = [&](auto visit) {
-            for (uint32_t m = winners; m; m &= m - 1) {
-                const int first = row.c0 + (tid & ~31) + __ffs(m) - 1;
-                for (int c0 = first; c0 < row.c1; c0 += 32 * THREADS) visit(c0 + lane * THREADS);
-            }
-        };
         if (bound > -INFINITY) {
-            each_winner([&](int ci) {
-                if (ci < row.c1) {
-                    float x[VEC];
-                    load_chunk(ci, x);
+            // the warp's stretches that reach the bound, their chunks a lane each
+            const int steps = (row.c1 - row.c0 + STEP - 1) / STEP, log = stretch_log(steps);
+            const int used = (steps + (1 << log) - 1) >> log;
+            int total = 0;
+            if (winners) {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        if (x[e] >= bound) put(order_code(x[e], row.id(ci) + e));
+                for (int i = 0; i < SLOTS; ++i) {
+                    const bool in = wins && i < used && sh.slots[i][tid] >= bound;
+                    const uint32_t b = __ballot_sync(0xffffffffu, in);
+                    const int at = total + __popc(b & ((1u << lane) - 1));
+                    if (in && at < STRETCHES) sh.stretch[warp][at] = uint16_t(tid | (i << 8));
+                    total += __popc(b);
                 }
-            });
-            if (tid < scalars) {
-                const float x = Elem<DT>::load(row.p, row.scalar_id(tid));
-                if (x >= bound) put(order_code(x, row.scalar_id(tid)));
             }
+            __syncwarp();
+            if (total > STRETCHES) {
+                if (lane == 0) atomicAdd(&sh.count[flip], CAND + 1);   // too many
+                total = 0;
+            }
+#pragma unroll 2
+            for (int i = lane; i < total << (log + UNROLL_LOG); i += 32) {
+                const int e = sh.stretch[warp][i >> (log + UNROLL_LOG)], k = i & ((UNROLL << log) - 1);
+                const int ci = row.c0 + (((e >> 8) << log) + (k >> UNROLL_LOG)) * STEP + (k & (UNROLL - 1)) * THREADS + (e & 255);
+                if (ci < row.c1) {
+                    const uint4 v = __ldg(chunks + ci);
+                    if (Chunk<DT>::max_of(&v.x, 4) >= bound) {
+                        float x[VEC];
+                        Elem<DT>::unpack(v, x);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e)
+                            if (x[e] >= bound) put(order_code(x[e], row.id(ci) + e));
+                    }
+                }
+            }
+            if (tid < scalars && pass.end >= bound) put(order_code(pass.end, row.scalar_id(tid)));
         }
         __syncthreads();
-        ncand = sh.count;
+        ncand = sh.count[flip];
         if (ncand > CAND || !(bound > -INFINITY)) {
             // too many at or above the bound (ties, long runs in order), or a bound of -inf:
             // each warp keeps its best 32 in its lanes and inserts what beats the last
             __syncthreads();
-            if (tid == 0) sh.count = 0;
+            if (tid == 0) sh.count[flip] = 0;
             __syncthreads();
             uint64_t best = 0;
             auto insert = [&](uint64_t code) {
                 uint32_t better;
-                while ((better = __ballot_sync(0xffffffffu, code > __shfl_sync(0xffffffffu, best, 31)))) {
+                while ((better = __ballot_sync(0xffffffffu, code > shfl_u64(best, 31)))) {
                     const uint64_t v = shfl_u64(code, __ffs(better) - 1);
                     const uint64_t up = shfl_up_u64(best, 1);
                     const int place = __popc(__ballot_sync(0xffffffffu, best > v));
@@ -454,59 +554,66 @@ __global__ void __launch_bounds__(THREADS, 2) logprob_kernel(const Params P, con
                     if (lane == __ffs(better) - 1) code = 0;
                 }
             };
-            each_winner([&](int ci) {
-                float x[VEC];
-                const bool in = ci < row.c1;
-                if (in) load_chunk(ci, x);
+            for (uint32_t m = winners; m; m &= m - 1) {   // a winner at a time, a chunk a lane
+                const int first = row.c0 + (tid & ~31) + __ffs(m) - 1;
+                for (int c0 = first; c0 < row.c1; c0 += 32 * THREADS) {
+                    const int ci = c0 + lane * THREADS;
+                    float x[VEC];
+                    const bool in = ci < row.c1;
+                    if (in) Elem<DT>::unpack(__ldg(chunks + ci), x);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) insert(in ? order_code(x[e], row.id(ci) + e) : 0);
-            });
+                    for (int e = 0; e < VEC; ++e) insert(in ? order_code(x[e], row.id(ci) + e) : 0);
+                }
+            }
             if (scalars > 0 && warp == 0)
                 insert(lane < scalars ? order_code(Elem<DT>::load(row.p, row.scalar_id(lane)), row.scalar_id(lane)) : 0);
+            if (lane >= P.top) best = 0;
             if (best != 0) put(best);
             __syncthreads();
-            ncand = sh.count;
+            ncand = min(CAND, sh.count[flip]);
         }
     }
     // a candidate's place is the number of candidates ahead of it
-    auto place_of = [&](uint64_t code, const uint64_t* from, int count) {
+    auto place_of = [&](uint64_t code) {
         int ahead = 0;
-        for (int i = 0; i < count; ++i) ahead += from[i] > code;
+#pragma unroll 4
+        for (int i = 0; i < ncand; ++i) ahead += sh.cand[i] > code;
         return ahead;
     };
 
     // ---- the row ----
-    if (G > 1) {
+    if constexpr (CLUSTER) {
         cluster_wait();
         if (warp == 0 && lane < G) {
-            const uint32_t to = cluster_addr(&sh.cta[part], lane);
+            const uint32_t to = cluster_addr(&cl->cta[part], lane);
             asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};"
                          :: "r"(to), "f"(all.m), "f"(all.s), "f"(all.q), "f"(__int_as_float(all.n)) : "memory");
         }
         if (TOP) {
-            const uint32_t lists = cluster_addr(&sh.lists[part][0], 0);
-            for (int i = tid; i < ncand; i += THREADS) {
-                const int place = place_of(sh.cand[i], sh.cand, ncand);
+            const uint32_t lists = cluster_addr(&cl->lists[part][0], 0);
+            if (tid < ncand) {
+                const int place = place_of(sh.cand[tid]);
                 if (place < P.top)
-                    asm volatile("st.shared::cluster.u64 [%0], %1;" :: "r"(lists + 8 * place), "l"(sh.cand[i]) : "memory");
+                    asm volatile("st.shared::cluster.u64 [%0], %1;"
+                                 :: "r"(lists + 8 * place), "l"(sh.cand[tid]) : "memory");
             }
             if (tid < P.top && tid >= ncand)
                 asm volatile("st.shared::cluster.u64 [%0], %1;" :: "r"(lists + 8 * tid), "l"(uint64_t(0)) : "memory");
         }
         cluster_arrive();
         cluster_wait();
-        all = fold(sh.cta, G, false);
+        all = fold(cl->cta, G, false);
     }
     const float m = all.m;
     int status = 0;
     if (isnan(m)) status |= FG_ROW_NAN;
     if (m == INFINITY) status |= FG_ROW_POS_INF;
     if (m == -INFINITY) status |= FG_ROW_ALL_MASKED;
-    if (!temperature_ok(T) || tok >= V) status |= FG_ROW_BAD_PARAM;
+    if (!temperature_ok(T) || row.tok >= row.V) status |= FG_ROW_BAD_PARAM;
     const bool bad = (status & ~FG_ROW_ALL_MASKED) != 0;
     const bool empty = m == -INFINITY;
 
-    if (!bad && !empty && !C::one_pass_ok(m, c)) {
+    if (!bad && !empty && !Chunk<DT>::one_pass_ok(m, c)) {
         // the sums again, as differences from the row's maximum
         float s = 0.0f, q = 0.0f;
         auto add = [&](float x) {
@@ -528,20 +635,20 @@ __global__ void __launch_bounds__(THREADS, 2) logprob_kernel(const Params P, con
             q += __shfl_xor_sync(0xffffffffu, q, d);
         }
         __syncthreads();
-        if (lane == 0) sh.warp[warp] = Stats{m, s, q, 0};
+        if (lane == 0) sh.warp[flip][warp] = Stats{m, s, q, 0};
         __syncthreads();
-        Stats again = fold(sh.warp, WARPS, true);
-        if (G > 1) {
+        Stats again = fold(sh.warp[flip], WARPS, true);
+        if constexpr (CLUSTER) {
             cluster_arrive();   // everyone has read the first round's entries
             cluster_wait();
             if (warp == 0 && lane < G) {
-                const uint32_t to = cluster_addr(&sh.cta[part], lane);
+                const uint32_t to = cluster_addr(&cl->cta[part], lane);
                 asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};"
                              :: "r"(to), "f"(m), "f"(again.s), "f"(again.q), "f"(0.0f) : "memory");
             }
             cluster_arrive();
             cluster_wait();
-            again = fold(sh.cta, G, true);
+            again = fold(cl->cta, G, true);
         }
         all.s = again.s;
         all.q = again.q;
@@ -550,43 +657,193 @@ __global__ void __launch_bounds__(THREADS, 2) logprob_kernel(const Params P, con
     const float l2 = log2f(all.s);
     const float nan = __int_as_float(0x7fc00000);
     if (tid == 0) {
-        const float lpt = tok < 0 ? 0.0f : empty ? -INFINITY : (xt - m) / T - LN2 * l2;
+        const float lpt = row.tok < 0 ? 0.0f : empty ? -INFINITY : (row.xt - m) / T - LN2 * l2;
         if (P.out_logprobs) P.out_logprobs[r] = bad ? nan : lpt;
         if (P.out_entropy) P.out_entropy[r] = bad ? nan : empty ? 0.0f : LN2 * (l2 - all.q / all.s);
         if (P.out_max) P.out_max[r] = m;
         if (P.out_logsum) P.out_logsum[r] = bad ? nan : empty ? -INFINITY : LN2 * l2;
-        if (P.out_rank) P.out_rank[r] = (bad || tok < 0) ? -1 : all.n;
+        if (P.out_rank) P.out_rank[r] = (bad || row.tok < 0) ? -1 : all.n;
         if (P.out_status) P.out_status[r] = status;
     }
     if (TOP) {
+        const float per_t = 1.0f / T;
         auto write = [&](int i, bool none, uint64_t code) {
             const float x = funkey(uint32_t(code >> 32));
             if (P.out_top_ids) P.out_top_ids[r * P.top + i] = (none || bad) ? -1 : int64_t(uint32_t(~uint32_t(code)));
             if (P.out_top_logprobs)
                 P.out_top_logprobs[r * P.top + i] =
-                    bad ? nan : (none || x == -INFINITY) ? -INFINITY : (x - m) / T - LN2 * l2;
+                    bad ? nan : (none || x == -INFINITY) ? -INFINITY : (x - m) * per_t - LN2 * l2;
         };
-        const uint64_t* from = G > 1 ? &sh.lists[0][0] : sh.cand;
-        const int count = G > 1 ? G * FG_LOGPROB_MAX_TOP : ncand;
-        int valid = ncand;   // what there is to place
-        if (G > 1) valid = V;
-        for (int i = tid; i < count; i += THREADS) {
-            if (G > 1 && (i & (FG_LOGPROB_MAX_TOP - 1)) >= P.top) continue;
-            const uint64_t code = from[i];
-            if (code == 0) continue;
-            int place = 0;
-            if (G > 1) {
-                for (int g = 0; g < G; ++g)
-                    for (int j = 0; j < P.top; ++j) place += sh.lists[g][j] > code;
-            } else {
-                place = place_of(code, from, count);
+        if constexpr (CLUSTER) {
+            // G lists in order, an entry a thread
+            const int g = tid / FG_LOGPROB_MAX_TOP, j = tid % FG_LOGPROB_MAX_TOP;
+            if (g < G && j < P.top) {
+                const uint64_t code = cl->lists[g][j];
+                int place = 0;
+                for (int o = 0; o < G; ++o)
+#pragma unroll 4
+                    for (int i = 0; i < P.top; ++i) place += cl->lists[o][i] > code;
+                if (code != 0 && place < P.top) write(place, false, code);
             }
-            if (place < P.top) write(place, false, code);
+        } else if (tid < ncand) {
+            const int place = place_of(sh.cand[tid]);
+            if (place < P.top) write(place, false, sh.cand[tid]);
         }
         // past the vocabulary's end, and rows that have no alternatives to name
-        for (int i = tid; i < P.top; i += THREADS)
-            if (i >= min(valid, V) || bad) write(i, true, 0);
+        if (tid < P.top && (tid >= row.V || bad)) write(tid, true, 0);
     }
+}
+
+template <int DT, bool TOP>
+__global__ void __launch_bounds__(THREADS) row_kernel(const Params P, const int G) {
+    __shared__ Shared sh;
+    __shared__ ClusterShared cl;
+    static_assert(MAX_G * FG_LOGPROB_MAX_TOP <= THREADS && CAND <= THREADS && THREADS <= 256, "a thread an entry");
+    const int tid = threadIdx.x, part = blockIdx.x % G;
+    cluster_arrive();   // the others' shared memory stands once all have arrived
+    if (tid == 0) sh.count[0] = 0;
+    const Row<DT> row(P, blockIdx.x / G, part, G);
+    const uint4* chunks = row.chunks();
+    Pass<DT> pass;
+    const int scalars = part == 0 ? row.head + row.tail : 0;
+    pass.begin(row, scalars, tid);
+    const int steps = (row.c1 - row.c0 + STEP - 1) / STEP, log = stretch_log(steps);
+    uint4 ahead[UNROLL];
+    auto fetch = [&](int step) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int ci = row.c0 + step * STEP + u * THREADS + tid;
+            ahead[u] = no_logits<DT>();
+            if (ci < row.c1) ahead[u] = __ldg(chunks + ci);
+        }
+    };
+    fetch(0);
+    for (int step = 0; step < steps; ++step) {
+        uint32_t w[UNROLL * 4];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            w[4 * u] = ahead[u].x; w[4 * u + 1] = ahead[u].y; w[4 * u + 2] = ahead[u].z; w[4 * u + 3] = ahead[u].w;
+        }
+        fetch(step + 1);
+        pass.take(w, row, row.c0 + step * STEP + tid);
+        if (TOP) pass.stretch(sh, step, log, step + 1 == steps);
+        if ((step & 511) == 511) pass.settle();
+    }
+    pass.ends(row, scalars, tid);
+    finish_row<DT, TOP, true>(P, sh, &cl, row, pass, scalars, part, G, 0);
+}
+
+static_assert(sizeof(Shared) % 128 == 0 && offsetof(ClusterShared, cta) % 16 == 0 && sizeof(Stats) == 16, "alignment");
+
+template <int DT, bool TOP>
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) rows_kernel(const Params P, const int64_t batch) {
+    extern __shared__ __align__(128) uint4 ring[];   // [DEPTH][UNROLL][THREADS]
+    __shared__ Shared sh;
+    constexpr int SIZE = Elem<DT>::SIZE;
+    const int tid = threadIdx.x;
+    const uint32_t ring0 = smem_u32(ring) + 16 * tid, ring1 = ring0 + RING_BYTES;
+    if (tid == 0) sh.count[0] = 0;
+
+    // ---- the copies: `left` chunks of row `next` from `src` on ----
+    int64_t next = blockIdx.x;
+    const char* src = nullptr;
+    int left = 0;
+    auto open = [&]() {
+        const char* p = reinterpret_cast<const char*>(P.logits) + next * P.row_stride * SIZE;
+        const int head = min(P.vocab, int((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / SIZE);
+        left = (P.vocab - head) / Elem<DT>::VEC;
+        src = p + int64_t(head) * SIZE + 16 * tid;
+    };
+    // one step of this thread into a place of the ring (an empty step past the last row)
+    auto fetch = [&](uint32_t place) {
+        if (left >= STEP) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                             :: "r"(place + 16 * THREADS * u), "l"(src + 16 * THREADS * u) : "memory");
+        } else if (left > 0) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+                if (tid + u * THREADS < left)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                 :: "r"(place + 16 * THREADS * u), "l"(src + 16 * THREADS * u) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        src += 16 * STEP;
+        left -= STEP;
+        while (left <= 0 && next + gridDim.x < batch) {
+            next += gridDim.x;
+            open();
+        }
+    };
+    open();
+    while (left <= 0 && next + gridDim.x < batch) {
+        next += gridDim.x;
+        open();
+    }
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) fetch(ring0 + i * 16 * STEP);
+
+    uint32_t place = ring0;
+    int flip = 0;
+    int64_t tok = P.tokens ? P.tokens[blockIdx.x] : -1;
+    float T = P.temperature ? P.temperature[blockIdx.x] : 1.0f;
+    float xt = Row<DT>::token_logit(P, blockIdx.x, tok);
+    for (int64_t r = blockIdx.x; r < batch; r += gridDim.x, flip ^= 1) {
+        const Row<DT> row(P, r, 0, 1, tok, T, xt);
+        const bool more = r + gridDim.x < batch;
+        if (more) {   // the next row's, for when its turn comes
+            if (P.tokens) tok = P.tokens[r + gridDim.x];
+            if (P.temperature) T = P.temperature[r + gridDim.x];
+        }
+        Pass<DT> pass;
+        const int scalars = row.head + row.tail;
+        pass.begin(row, scalars, tid);
+        auto turn = [&]() {   // the values are used: the place is free
+            fetch(place);
+            place += 16 * STEP;
+            if (place == ring1) place = ring0;
+        };
+        const int steps = (row.nvec + STEP - 1) / STEP, log = stretch_log(steps);
+        int c0 = 0, step = 0;
+        for (; c0 + STEP <= row.nvec; c0 += STEP, ++step) {
+            asm volatile("cp.async.wait_group %0;" :: "n"(DEPTH - 1) : "memory");
+            uint32_t w[UNROLL * 4];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const uint4 v = lds_v4(place + 16 * THREADS * u);
+                w[4 * u] = v.x; w[4 * u + 1] = v.y; w[4 * u + 2] = v.z; w[4 * u + 3] = v.w;
+            }
+            if (unsigned(row.tchunk - c0) < unsigned(STEP)) {   // the token's own step
+                pass.take(w, row, c0 + tid);
+            } else {
+                typename Chunk<DT>::Threshold t[UNROLL];
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) t[u] = c0 < row.tchunk ? row.from : row.above;
+                pass.take(w, row, t);
+            }
+            turn();
+            if (TOP) pass.stretch(sh, step, log, step + 1 == steps);
+            if ((step & 511) == 511) pass.settle();
+        }
+        if (c0 < row.nvec) {
+            asm volatile("cp.async.wait_group %0;" :: "n"(DEPTH - 1) : "memory");
+            uint32_t w[UNROLL * 4];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                uint4 v = no_logits<DT>();
+                if (c0 + tid + u * THREADS < row.nvec) v = lds_v4(place + 16 * THREADS * u);
+                w[4 * u] = v.x; w[4 * u + 1] = v.y; w[4 * u + 2] = v.z; w[4 * u + 3] = v.w;
+            }
+            pass.take(w, row, c0 + tid);
+            turn();
+            if (TOP) pass.stretch(sh, step, log, true);
+        }
+        if (more) xt = Row<DT>::token_logit(P, r + gridDim.x, tok);
+        pass.ends(row, scalars, tid);
+        finish_row<DT, TOP, false>(P, sh, nullptr, row, pass, scalars, 0, 1, flip);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------

@@ -165,6 +165,125 @@ PYBIND11_MODULE(_C, m) {
           py::arg("logits"), py::arg("dtype"), py::arg("batch"), py::arg("vocab"), py::arg("row_stride") = 0,
           py::arg("hist_ids"), py::arg("hist_offsets"), py::arg("penalty"), py::arg("stream") = 0);
 
+    m.def("token_logprobs",
+          [](std::uintptr_t logits, int dtype, int32_t batch, int32_t vocab, int64_t row_stride,
+             std::uintptr_t tokens, std::uintptr_t temperature, int32_t top, std::uintptr_t out_logprobs,
+             std::uintptr_t out_entropy, std::uintptr_t out_max, std::uintptr_t out_logsum, std::uintptr_t out_rank,
+             std::uintptr_t out_top_ids, std::uintptr_t out_top_logprobs, std::uintptr_t out_status,
+             std::uintptr_t stream) {
+              FgLogprobArgs a{};
+              a.logits = ptr<const void>(logits);
+              a.dtype = dtype;
+              a.batch = batch;
+              a.vocab = vocab;
+              a.top = top;
+              a.row_stride = row_stride > 0 ? row_stride : vocab;
+              a.tokens = ptr<const int64_t>(tokens);
+              a.temperature = ptr<const float>(temperature);
+              a.out_logprobs = ptr<float>(out_logprobs);
+              a.out_entropy = ptr<float>(out_entropy);
+              a.out_max = ptr<float>(out_max);
+              a.out_logsum = ptr<float>(out_logsum);
+              a.out_rank = ptr<int32_t>(out_rank);
+              a.out_top_ids = ptr<int64_t>(out_top_ids);
+              a.out_top_logprobs = ptr<float>(out_top_logprobs);
+              a.out_status = ptr<int32_t>(out_status);
+              int rc;
+              {
+                  py::gil_scoped_release release;
+                  rc = fg_token_logprobs(&a, ptr<void>(stream));
+              }
+              check(rc, "fg_token_logprobs");
+          },
+          py::arg("logits"), py::arg("dtype"), py::arg("batch"), py::arg("vocab"), py::arg("row_stride") = 0,
+          py::arg("tokens") = 0, py::arg("temperature") = 0, py::arg("top") = 0, py::arg("out_logprobs") = 0,
+          py::arg("out_entropy") = 0, py::arg("out_max") = 0, py::arg("out_logsum") = 0, py::arg("out_rank") = 0,
+          py::arg("out_top_ids") = 0, py::arg("out_top_logprobs") = 0, py::arg("out_status") = 0,
+          py::arg("stream") = 0,
+          "fg_token_logprobs on device buffers (integers: device pointers; 0: absent).");
+
+    m.def("token_logprobs_grad",
+          [](std::uintptr_t logits, int dtype, int32_t batch, int32_t vocab, std::uintptr_t max,
+             std::uintptr_t logsum, std::uintptr_t out_grad, int64_t row_stride, int64_t grad_stride,
+             std::uintptr_t tokens, std::uintptr_t temperature, std::uintptr_t entropy,
+             std::uintptr_t grad_logprobs, std::uintptr_t grad_entropy, std::uintptr_t stream) {
+              FgLogprobGradArgs a{};
+              a.logits = ptr<const void>(logits);
+              a.dtype = dtype;
+              a.batch = batch;
+              a.vocab = vocab;
+              a.row_stride = row_stride > 0 ? row_stride : vocab;
+              a.tokens = ptr<const int64_t>(tokens);
+              a.temperature = ptr<const float>(temperature);
+              a.max = ptr<const float>(max);
+              a.logsum = ptr<const float>(logsum);
+              a.entropy = ptr<const float>(entropy);
+              a.grad_logprobs = ptr<const float>(grad_logprobs);
+              a.grad_entropy = ptr<const float>(grad_entropy);
+              a.out_grad = ptr<void>(out_grad);
+              a.grad_stride = grad_stride > 0 ? grad_stride : vocab;
+              int rc;
+              {
+                  py::gil_scoped_release release;
+                  rc = fg_token_logprobs_grad(&a, ptr<void>(stream));
+              }
+              check(rc, "fg_token_logprobs_grad");
+          },
+          py::arg("logits"), py::arg("dtype"), py::arg("batch"), py::arg("vocab"), py::arg("max"), py::arg("logsum"),
+          py::arg("out_grad"), py::arg("row_stride") = 0, py::arg("grad_stride") = 0, py::arg("tokens") = 0,
+          py::arg("temperature") = 0, py::arg("entropy") = 0, py::arg("grad_logprobs") = 0,
+          py::arg("grad_entropy") = 0, py::arg("stream") = 0,
+          "fg_token_logprobs_grad on device buffers (integers: device pointers; 0: absent).");
+
+    m.def("adapter_workspace_size",
+          [](int32_t batch, int32_t dim, int32_t rank, int32_t slots) {
+              return fg_adapter_workspace_size(batch, dim, rank, slots);
+          },
+          py::arg("batch"), py::arg("dim"), py::arg("rank") = 16, py::arg("slots") = 0);
+
+    m.def("adapter_logits",
+          [](std::uintptr_t hidden, std::uintptr_t weight, std::uintptr_t out, int dtype, int out_dtype,
+             int32_t batch, int32_t dim, int32_t vocab, std::uintptr_t workspace, size_t workspace_bytes,
+             std::uintptr_t down, std::uintptr_t up, std::uintptr_t scales, std::uintptr_t adapters, int32_t rank,
+             int32_t slots, std::uintptr_t out_status, int64_t hidden_stride, int64_t weight_stride,
+             int64_t down_stride, int64_t out_stride, std::uintptr_t stream) {
+              FgAdapterArgs a{};
+              a.hidden = ptr<const void>(hidden);
+              a.weight = ptr<const void>(weight);
+              a.down = ptr<const void>(down);
+              a.up = ptr<const void>(up);
+              a.scales = ptr<const float>(scales);
+              a.adapters = ptr<const int32_t>(adapters);
+              a.out = ptr<void>(out);
+              a.out_status = ptr<int32_t>(out_status);
+              a.workspace = ptr<void>(workspace);
+              a.workspace_bytes = workspace_bytes;
+              a.dtype = dtype;
+              a.out_dtype = out_dtype;
+              a.batch = batch;
+              a.dim = dim;
+              a.vocab = vocab;
+              a.rank = rank;
+              a.slots = slots;
+              a.hidden_stride = hidden_stride > 0 ? hidden_stride : dim;
+              a.weight_stride = weight_stride > 0 ? weight_stride : dim;
+              a.down_stride = down_stride > 0 ? down_stride : dim;
+              a.out_stride = out_stride > 0 ? out_stride : vocab;
+              int rc;
+              {
+                  py::gil_scoped_release release;
+                  rc = fg_adapter_logits(&a, ptr<void>(stream));
+              }
+              check(rc, "fg_adapter_logits");
+          },
+          py::arg("hidden"), py::arg("weight"), py::arg("out"), py::arg("dtype"), py::arg("out_dtype"),
+          py::arg("batch"), py::arg("dim"), py::arg("vocab"), py::arg("workspace"), py::arg("workspace_bytes"),
+          py::arg("down") = 0, py::arg("up") = 0, py::arg("scales") = 0, py::arg("adapters") = 0,
+          py::arg("rank") = 16, py::arg("slots") = 0, py::arg("out_status") = 0, py::arg("hidden_stride") = 0,
+          py::arg("weight_stride") = 0, py::arg("down_stride") = 0, py::arg("out_stride") = 0,
+          py::arg("stream") = 0,
+          "fg_adapter_logits on device buffers (integers: device pointers; 0: absent).");
+
     m.def("version", []() { return fg_version(); });
     m.def("strerror", [](int code) { return std::string(fg_strerror(code)); });
 }

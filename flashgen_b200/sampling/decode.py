@@ -15,6 +15,14 @@ step rebuilds the compact CSR view ``fg_sample`` reads (ids, int64 offsets)
 with device-only torch operations: a cumulative sum of the lengths and one
 scatter of the valid entries, so the step never synchronises with the host.
 A row whose history is full keeps its first ``capacity`` ids.
+
+A step can also return what a serving API reports beside the ids: each drawn
+id's log probability under the model's distribution (the logits before
+penalties and temperature) with its rank and the likeliest alternatives
+(``top_logprobs``), and keep each row's running sum, the field FlashGen declares
+and never fills (``CompletionOutput.cumulative_logprob``, flashgen/outputs.py:25).
+``step_hidden`` starts one product earlier, from the hidden states and an
+:class:`~flashgen_b200.sampling.lm_head.AdapterHead`.
 """
 from __future__ import annotations
 
@@ -24,6 +32,8 @@ import torch
 
 from .. import _lib
 from ..core.config import SamplingParams
+from .lm_head import AdapterHead
+from .logprobs import TokenLogprobs, token_logprobs
 from .sampler import PackedParams, _status_error, fused_sample, workspace_for
 
 
@@ -52,6 +62,8 @@ class DecodeBatch:
         self.status = torch.empty(self.B, dtype=torch.int32, device=self.device)
         self.out = torch.empty(self.B, dtype=torch.int64, device=self.device)
         self.check_errors = check_errors
+        self.last_logprobs: Optional[TokenLogprobs] = None    # of the last step, if it was asked for them
+        self.cumulative_logprob = torch.zeros(self.B, dtype=torch.float32, device=self.device)
 
     def set_history(self, row: int, ids: Sequence[int]) -> None:
         """Row `row`'s history so far (prompt and generated ids), from the host."""
@@ -75,11 +87,14 @@ class DecodeBatch:
         return self.csr_ids, self.csr_off, self.capacity
 
     def step(self, logits: torch.Tensor, uniforms: Optional[torch.Tensor] = None,
-             generator: Optional[torch.Generator] = None) -> torch.Tensor:
+             generator: Optional[torch.Generator] = None, top_logprobs: Optional[int] = None) -> torch.Tensor:
         """Sample one token per row from `logits` [B, V] (on this device) with the
         rows' penalties over their histories, append it to the histories and
         return the ids ([B] int64, on the device; the same buffer every step,
-        so read or copy it before the next step)."""
+        so read or copy it before the next step). With `top_logprobs` (0 to 32)
+        `last_logprobs` holds the drawn ids' log probabilities, ranks and that
+        many alternatives, and `cumulative_logprob` grows by them (rows without an
+        id, rank -1, add nothing)."""
         assert logits.shape == (self.B, self.V), (logits.shape, self.B, self.V)
         if uniforms is None:
             uniforms = torch.rand(self.B, device=self.device, generator=generator, dtype=torch.float32)
@@ -95,8 +110,19 @@ class DecodeBatch:
             msg = _status_error(self.status)
             if msg is not None:
                 raise RuntimeError(msg)
+        self.last_logprobs = None
+        if top_logprobs is not None:
+            self.last_logprobs = token_logprobs(logits, ids, top=top_logprobs)
+            self.cumulative_logprob += torch.where(ids >= 0, self.last_logprobs.logprobs,
+                                                   torch.zeros_like(self.cumulative_logprob))
         self._append(ids)
         return ids
+
+    def step_hidden(self, hidden: torch.Tensor, head: AdapterHead, adapters: Optional[torch.Tensor] = None,
+                    **kwargs) -> torch.Tensor:
+        """`step` from the hidden states [B, dim]: the logits are `head`'s, every
+        row with its own adapter (`adapters` [B] int32, negative: none)."""
+        return self.step(head.logits(hidden, adapters), **kwargs)
 
     def _append(self, ids: torch.Tensor) -> None:
         """Append each row's id (skipping error rows, id -1) on the device; a

@@ -187,14 +187,17 @@ constexpr int A_BYTES = TILE_V * TILE_K * 2;
 constexpr int MAX_STAGES = 12;
 // Epilogue warps, and how many windows of its tile each works out before the
 // products arrive (the others' adapters are added as they are read). With fp32
-// results the registers go to the sums: next to the ring there is no L1 left, and a
-// spilled register would wait for L2.
-template <int ODT, int RC>
+// results registers go to the sums, of fewer columns for a SMALL batch tile: next to
+// the ring there is no L1 left, and a spilled register would wait for L2.
+template <int ODT, int RC, bool SMALL>
 struct Epilogue {
     static constexpr bool PIECES = ODT == FG_DTYPE_F32;
-    static constexpr int WARPS = PIECES ? (RC <= 2 ? 16 : 8) : (RC <= 2 ? 12 : 8);
-    static constexpr int EARLY = RC == 0 || PIECES ? 0 : RC == 1 ? 3 : RC <= 4 ? 2 : 1;
+    static constexpr int WARPS = RC > 2 ? 8 : PIECES && !SMALL ? 16 : 12;
+    static constexpr int EARLY = RC == 0 || (PIECES && !SMALL) ? 0
+                                 : PIECES ? (RC == 1 ? 2 : RC == 4 ? 1 : 0) : (RC == 1 ? 3 : RC <= 4 ? 2 : 1);
     static constexpr int THREADS = 64 + 32 * WARPS;            // of the CTA
+    static constexpr int COLUMNS = SMALL ? SMALL_NT : MAX_NT;
+    static constexpr int SUMS = (COLUMNS / 8 + WARPS / 4 - 1) / (WARPS / 4) * 8;   // a warp's share, in eights
 };
 constexpr int PIECE_K = 8;                         // 64-wide steps of K per piece of an fp32 sum
 
@@ -346,6 +349,62 @@ struct Windows {
     }
 };
 
+// The adapters' share of the E windows from w0 on, as Windows::adapters, but slot by
+// slot over all of them: a slot's rows of up are loaded once, BATCH slots at a time.
+template <int DT, int ODT, int RC, int E>
+__device__ __forceinline__ void early_windows(float (&x)[E][2][4], const int (&ents)[E], const Params& P, int b0,
+                                              int rows, int w0, int w1, int v0, int lane) {
+    using W = Windows<DT, ODT, RC>;
+    constexpr uint32_t ALL = 0xffffffffu;
+    constexpr int BATCH = RC == 1 && ODT != FG_DTYPE_F32 ? 3 : RC <= 2 ? 2 : 1;
+    const int g = lane >> 2, t = lane & 3;
+    int slots[E];
+    uint32_t left = 0;   // columns still without their adapter, eight bits a window
+    uint2 u[E][RC][W::PARTS];
+    float unit[E][2];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][0][j] = x[i][1][j] = 0.0f;
+        slots[i] = w0 + i < w1 && ents[i] >= 0 ? (ents[i] >> 9) - 1 : -1;
+        left |= (__ballot_sync(ALL, slots[i] >= 0) & 0xffu) << (8 * i);
+        const int w = min(w0 + i, w1 - 1), p = 8 * w + 2 * t;
+        const uint2* src = reinterpret_cast<const uint2*>(P.u) + int64_t(b0 + min(8 * w + g, rows - 1)) * (12 * RC) + t;
+#pragma unroll
+        for (int c = 0; c < RC; ++c)
+#pragma unroll
+            for (int j = 0; j < W::PARTS; ++j) u[i][c][j] = src[j * 4 * RC + c * 4];
+        unit[i][0] = p < rows ? P.unit[b0 + p] : 0.0f;
+        unit[i][1] = p + 1 < rows ? P.unit[b0 + p + 1] : 0.0f;
+    }
+    while (left) {
+        UpTile<RC> tile[BATCH];
+        uint32_t match[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            match[k] = 0;
+            if (left) {
+                const int at = __ffs(left) - 1;
+                int mine = slots[0];
+#pragma unroll
+                for (int i = 1; i < E; ++i)
+                    if (at >= 8 * i) mine = slots[i];
+                const int slot = __shfl_sync(ALL, mine, at & 7);
+#pragma unroll
+                for (int i = 0; i < E; ++i) match[k] |= (__ballot_sync(ALL, slots[i] == slot) & 0xffu) << (8 * i);
+                left &= ~match[k];
+                tile[k].load(P, slot, v0, lane);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (match[k] >> (8 * i) & 0xffu)
+                    W::apply(x[i], tile[k], u[i], unit[i][0], unit[i][1], match[k] >> (8 * i), t);
+    }
+}
+
 // Read window w of the accumulator, add the adapters' share and store it.
 template <int ODT>
 __device__ __forceinline__ void store_window(const Params& P, uint32_t base, int b0, int w, int v0, int ent,
@@ -403,13 +462,14 @@ __device__ __forceinline__ void store_window(const Params& P, uint32_t base, int
 }
 
 // RC: rank / 16 held in registers (rounded up to 1, 2, 4 or 8), 0: no adapters.
-template <int CG, int DT, int ODT, int RC>
-__global__ void __launch_bounds__(Epilogue<ODT, RC>::THREADS, 1)
+// SMALL: fp32 results and a batch tile of at most SMALL_NT columns.
+template <int CG, int DT, int ODT, int RC, bool SMALL>
+__global__ void __launch_bounds__(Epilogue<ODT, RC, SMALL>::THREADS, 1)
 project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const Params P) {
     extern __shared__ uint8_t dyn[];
     __shared__ Control C;
     constexpr bool PIECES = ODT == FG_DTYPE_F32;
-    constexpr int EPI_WARPS = Epilogue<ODT, RC>::WARPS;
+    constexpr int EPI_WARPS = Epilogue<ODT, RC, SMALL>::WARPS;
     uint8_t* ring = dyn + ((1024 - (smem_u32(dyn) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? tc::cta_rank() : 0;
@@ -568,7 +628,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             const int vw = v - lane;   // the warp's first vocabulary row
             const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
             // the adapters' share of the first windows, while the products run
-            constexpr int EARLY = Epilogue<ODT, RC>::EARLY;
+            constexpr int EARLY = Epilogue<ODT, RC, SMALL>::EARLY;
             constexpr int R = RC > 0 ? RC : 1;
             using W = Windows<DT, ODT, R>;
             W win;
@@ -578,16 +638,15 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                 if (vw < P.vocab) {
 #pragma unroll
                     for (int i = 0; i < EARLY; ++i) ents[i] = W::entry(P, b0, rows, w0 + i, lane);
-#pragma unroll
-                    for (int i = 0; i < EARLY; ++i)
-                        if (w0 + i < w1) win.adapters(add[i], P, b0, rows, w0 + i, vw, ents[i], lane);
+                    if (w0 < w1) early_windows<DT, ODT, R, EARLY>(add, ents, P, b0, rows, w0, w1, vw, lane);
                 }
             }
             if (PIECES && nk > piece) {
                 // this warp's columns: every PARTS-th block of eight
-                float sum[MAX_NT / PARTS];
+                constexpr int SUMS = Epilogue<ODT, RC, SMALL>::SUMS;
+                float sum[SUMS];
 #pragma unroll
-                for (int i = 0; i < MAX_NT / PARTS; ++i) sum[i] = 0.0f;
+                for (int i = 0; i < SUMS; ++i) sum[i] = 0.0f;
                 uint32_t at = 0;
                 for (int k0 = 0; k0 < nk; k0 += piece) {
                     ok = mbar_wait(&C.acc_full[acc], acc_parity, &C.abort);
@@ -595,7 +654,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                     tc::fence_after();
                     at = lanes + acc * P.nt + part * 8;
 #pragma unroll
-                    for (int i = 0; i < MAX_NT / PARTS; i += 8) {
+                    for (int i = 0; i < SUMS; i += 8) {
                         if (part * 8 + i * PARTS < P.nt) {
                             float x[8];
                             tc::tmem_ld8(x, at + i * PARTS);
@@ -609,7 +668,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                 if (ok) {
                     // the whole sums go back to where the last piece was
 #pragma unroll
-                    for (int i = 0; i < MAX_NT / PARTS; i += 8)
+                    for (int i = 0; i < SUMS; i += 8)
                         if (part * 8 + i * PARTS < P.nt) tc::tmem_st8(sum + i, at + i * PARTS);
                     tc::tmem_wait_st();
                 }
@@ -634,7 +693,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                     for (int i = 0; i < EARLY; ++i)
                         if (w0 + i < w1) store_window<ODT>(P, base, b0, w0 + i, vw, ents[i], add[i], lane);
                 }
-                if constexpr (EARLY == 0) win = W{};
+                win = W{};
                 for (int w = w0 + EARLY; w < w1; ++w) {
                     float more[2][4] = {};
                     int ent = 8 * w + (lane & 7);

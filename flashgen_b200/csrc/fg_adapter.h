@@ -11,6 +11,7 @@ namespace adapt {
 
 constexpr int TILE_V = 128, TILE_K = 64;   // accumulator lanes; elements of a K step (128 bytes)
 constexpr int MAX_NT = 256;                // batch columns of a tile
+constexpr int SMALL_NT = 64;
 
 struct Params {
     const void* hidden;       // rows for the products: the caller's, or the aligned copy

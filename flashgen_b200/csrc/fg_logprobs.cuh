@@ -63,8 +63,8 @@ __device__ __forceinline__ bool temperature_ok(float T) { return T >= 1.17549435
 // one FMA a logit, the same r in every term, so r's rounding cancels in log2 S + r.
 //
 // Alternatives without a second pass over the row: each thread leaves the maxima of up
-// to SLOTS stretches of its chunks. The top-th largest of 32 group maxima bounds the
-// top-th largest logit from below, so every alternative lies in a stretch whose maximum
+// to SLOTS stretches of its chunks. The top-th largest of 32 or 64 group maxima bounds
+// the top-th largest logit from below, so every alternative lies in a stretch whose maximum
 // reaches the bound; there are few, and only their chunks are read again (from L2).
 // What reaches the bound is gathered, and a candidate's place is the number of
 // candidates ahead of it.
@@ -87,7 +87,7 @@ constexpr int STEP = UNROLL * THREADS;
 constexpr int DEPTH = 3;             // steps in flight in rows_kernel
 constexpr int RING_BYTES = DEPTH * STEP * 16;
 constexpr int SLOTS = 8;             // stretches of a thread's chunks
-constexpr int GROUPS = 32;           // of THREADS / 32 neighbouring lanes, for the bound
+constexpr int GROUPS = 64;           // of THREADS / 64 neighbouring lanes, for the bound
 constexpr int LANES = THREADS / GROUPS;
 constexpr int MAX_G = 8;
 constexpr int STRETCHES = 64;        // a warp reads again
@@ -271,17 +271,32 @@ __device__ __forceinline__ Stats merge(const Stats& a, float m, float c) {   // 
     return r;
 }
 
-// The k-th largest of the lanes' values (a warp-wide bitonic sort).
-__device__ __forceinline__ float kth_of_32(float a, int k, int lane) {
+// The k-th largest of 32 or 64 group maxima, one or two a lane: a warp-wide bitonic
+// sort (of both halves, then of the larger ones of both).
+template <bool TWO>
+__device__ __forceinline__ float kth_largest(float a, float b, int k, int lane) {
+    constexpr uint32_t ALL = 0xffffffffu;
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
         for (int d = size >> 1; d > 0; d >>= 1) {
             const bool keep_max = ((lane & size) == 0) == ((lane & d) == 0);
-            const float o = __shfl_xor_sync(0xffffffffu, a, d);
+            const float o = __shfl_xor_sync(ALL, a, d);
             a = keep_max ? fmaxf(a, o) : fminf(a, o);
+            if (TWO) {
+                const float p = __shfl_xor_sync(ALL, b, d);
+                b = keep_max ? fmaxf(b, p) : fminf(b, p);
+            }
         }
-    return __shfl_sync(0xffffffffu, a, k - 1);
+    if (TWO) {
+        a = fmaxf(a, __shfl_xor_sync(ALL, b, 31));   // descending a against ascending b
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            const float o = __shfl_xor_sync(ALL, a, d);
+            a = (lane & d) == 0 ? fmaxf(a, o) : fminf(a, o);
+        }
+    }
+    return __shfl_sync(ALL, a, k - 1);
 }
 
 // A row's place in shared memory; what a row leaves before its first barrier alternates
@@ -491,7 +506,12 @@ __device__ __forceinline__ void finish_row(const Params& P, Shared& sh, ClusterS
     // ---- alternatives: the candidates of this CTA ----
     int ncand = 0;
     if (TOP) {
-        const float bound = kth_of_32(sh.groups[flip][lane], P.top, lane);
+        // 32 groups are enough for a tight bound up to 16 alternatives (of n groups the
+        // k-th largest maximum lets about n (H_n - H_(n - k)) logits through: 31 for k = 20,
+        // but 130 for k = 32; of 64 groups 24 and 44)
+        const float g0 = sh.groups[flip][2 * lane], g1 = sh.groups[flip][2 * lane + 1];
+        const float bound = P.top <= 16 ? kth_largest<false>(fmaxf(g0, g1), 0.0f, P.top, lane)
+                                        : kth_largest<true>(g0, g1, P.top, lane);
         const bool wins = vmax >= bound;
         const uint32_t winners = __ballot_sync(0xffffffffu, wins);
         auto put = [&](uint64_t code) {
@@ -554,19 +574,30 @@ __device__ __forceinline__ void finish_row(const Params& P, Shared& sh, ClusterS
                     if (lane == __ffs(better) - 1) code = 0;
                 }
             };
-            for (uint32_t m = winners; m; m &= m - 1) {   // a winner at a time, a chunk a lane
-                const int first = row.c0 + (tid & ~31) + __ffs(m) - 1;
-                for (int c0 = first; c0 < row.c1; c0 += 32 * THREADS) {
-                    const int ci = c0 + lane * THREADS;
-                    float x[VEC];
-                    const bool in = ci < row.c1;
-                    if (in) Elem<DT>::unpack(__ldg(chunks + ci), x);
+            // the warp's chunks in the order of their ids, four loads in flight: once the list
+            // is full, a chunk counts only with a logit above its last (a later equal one loses)
+            for (int first = row.c0 + (tid & ~31); first < row.c1; first += 4 * THREADS) {
+                uint4 v[4];
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) insert(in ? order_code(x[e], row.id(ci) + e) : 0);
+                for (int u = 0; u < 4; ++u) {
+                    v[u] = no_logits<DT>();
+                    const int ci = first + u * THREADS + lane;
+                    if (ci < row.c1) v[u] = __ldg(chunks + ci);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int ci = first + u * THREADS + lane;
+                    const uint64_t last = shfl_u64(best, 31);
+                    const bool above = last == 0 || Chunk<DT>::max_of(&v[u].x, 4) > funkey(uint32_t(last >> 32));
+                    if (!__any_sync(0xffffffffu, ci < row.c1 && above)) continue;
+                    float x[VEC];
+                    Elem<DT>::unpack(v[u], x);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) insert(ci < row.c1 ? order_code(x[e], row.id(ci) + e) : 0);
                 }
             }
             if (scalars > 0 && warp == 0)
-                insert(lane < scalars ? order_code(Elem<DT>::load(row.p, row.scalar_id(lane)), row.scalar_id(lane)) : 0);
+                insert(lane < scalars ? order_code(pass.end, row.scalar_id(lane)) : 0);
             if (lane >= P.top) best = 0;
             if (best != 0) put(best);
             __syncthreads();

@@ -49,6 +49,8 @@ def _vector(t: Optional[torch.Tensor], dtype: torch.dtype, like: torch.Tensor, w
     """A per-row vector as the kernels read it: [B], dense, on the logits' device."""
     if t is None:
         return None
+    if t.dtype is dtype and t.dim() == 1 and t.shape[0] == like.shape[0] and t.device == like.device:
+        return t if t.is_contiguous() else t.contiguous()
     if t.shape != like.shape[:1]:
         raise ValueError(f"{what} must be [{like.shape[0]}], got {tuple(t.shape)}")
     if t.device != like.device:

@@ -17,12 +17,16 @@ bool rows_ok(const void* p, int dtype, int64_t stride, int32_t vocab) {
 
 constexpr int32_t kMaxRows = 1 << 30;
 
-// CTAs per row for a batch too small to fill the machine with one each: as many as find
-// room at once (four an SM), with at least two chunks for each of their threads.
+// CTAs per row for a batch too small to fill the machine with one each: as many as
+// find room at once (three an SM), with at least two chunks for each of their threads.
+// Clusters of eight find room less easily. With four an SM instead: 256 rows of 32000
+// f16 logits 14.4 us, not 12.4; eight CTAs a row for 50 rows of 128256 bf16 logits: 18.5 us,
+// four 14.4; one CTA for a row of 256000 f32 logits: 33.6 us, eight 12.4.
 int ctas_per_row(int32_t batch, int vocab, int elem, const DevInfo* d) {
     const int64_t chunks = int64_t(vocab) * elem / 16;
     int G = 1;
-    while (2 * G <= fg::lp::MAX_G && int64_t(batch) * 2 * G <= 4 * d->sms && chunks / (2 * G) >= 2 * fg::lp::THREADS)
+    while (2 * G <= fg::lp::MAX_G && int64_t(batch) * 2 * G <= (2 * G == 8 ? 2 : 3) * d->sms &&
+           chunks / (2 * G) >= 2 * fg::lp::THREADS)
         G *= 2;
     return G;
 }
@@ -54,9 +58,6 @@ int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
         kern<<<grid, fg::lp::THREADS, smem, st>>>(P, batch);
         return cudaGetLastError() == cudaSuccess ? FG_OK : FG_ELAUNCH;
     }
-    auto kern = fg::lp::row_kernel<DT, TOP>;
-    static std::atomic<bool> done[fg::host::kMaxDevices] = {};
-    if (!set_once(kern, done, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return FG_EDEVICE;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(batch) * G);
     cfg.blockDim = dim3(fg::lp::THREADS);
@@ -67,7 +68,12 @@ int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, P, G) == cudaSuccess ? FG_OK : FG_ELAUNCH;
+    return cudaLaunchKernelEx(&cfg, fg::lp::row_kernel<DT, TOP>, P, G) == cudaSuccess ? FG_OK : FG_ELAUNCH;
+}
+
+template <int DT>
+int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
+    return P.top ? launch_forward<DT, true>(P, batch, st) : launch_forward<DT, false>(P, batch, st);
 }
 
 template <int DT>
@@ -120,12 +126,9 @@ int fg_token_logprobs(const FgLogprobArgs* a, void* stream) {
     P.out_top_logprobs = a->out_top_logprobs; P.out_status = a->out_status;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (a->dtype) {
-        case FG_DTYPE_F32: 
-            return P.top ? launch_forward<FG_DTYPE_F32, true>(P, a->batch, st) : launch_forward<FG_DTYPE_F32, false>(P, a->batch, st);
-        case FG_DTYPE_F16: 
-            return P.top ? launch_forward<FG_DTYPE_F16, true>(P, a->batch, st) : launch_forward<FG_DTYPE_F16, false>(P, a->batch, st);
-        default: 
-            return P.top ? launch_forward<FG_DTYPE_BF16, true>(P, a->batch, st) : launch_forward<FG_DTYPE_BF16, false>(P, a->batch, st);
+        case FG_DTYPE_F32: return launch_forward<FG_DTYPE_F32>(P, a->batch, st);
+        case FG_DTYPE_F16: return launch_forward<FG_DTYPE_F16>(P, a->batch, st);
+        default: return launch_forward<FG_DTYPE_BF16>(P, a->batch, st);
     }
 }
 

@@ -108,7 +108,7 @@ class AdapterHead:
             out_dtype = self.dtype if out_dtype is None else out_dtype
             if out_dtype not in (self.dtype, torch.float32):
                 raise TypeError(f"out_dtype must be {self.dtype} or float32, got {out_dtype}")
-            out = torch.empty((B, self.vocab), dtype=out_dtype, device=self.device)
+            out = hidden.new_empty((B, self.vocab), dtype=out_dtype)
         elif out.shape != (B, self.vocab) or out.dtype not in (self.dtype, torch.float32) or \
                 out.device != self.device or out.stride(1) != 1 or (B > 1 and out.stride(0) < self.vocab):
             raise ValueError(f"out must be a row-major {self.dtype} or float32 [{B}, {self.vocab}] on {self.device}")
@@ -117,7 +117,7 @@ class AdapterHead:
         lib = _lib.load()
         slots = self.slots if adapters is not None else 0
         need = lib.fg_adapter_workspace_size(B, self.dim, self._rank, slots)
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        ws = hidden.new_empty(need, dtype=torch.uint8)
         status = torch.empty(B, dtype=torch.int32, device=self.device) if check_errors else None
         a = _lib.FgAdapterArgs(
             hidden.data_ptr(), self.weight.data_ptr(), self._down.data_ptr() or None, self._up.data_ptr() or None,

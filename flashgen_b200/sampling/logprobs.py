@@ -85,12 +85,12 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     tokens = _vector(tokens, torch.int64, logits, "tokens")
     temperature = _vector(temperature, torch.float32, logits, "temperature")
     dev = logits.device
-    logprobs, entropy, peak, logsum, rank, status = torch.empty((6, B), dtype=torch.float32, device=dev).unbind(0)
+    logprobs, entropy, peak, logsum, rank, status = logits.new_empty((6, B), dtype=torch.float32).unbind(0)
     rank, status = rank.view(torch.int32), status.view(torch.int32)
     top_ids = top_lp = None
     if top > 0:
-        top_ids = torch.empty((B, top), dtype=torch.int64, device=dev)
-        top_lp = torch.empty((B, top), dtype=torch.float32, device=dev)
+        top_ids = logits.new_empty((B, top), dtype=torch.int64)
+        top_lp = logits.new_empty((B, top), dtype=torch.float32)
     if B > 0:
         a = _lib.FgLogprobArgs(
             logits.data_ptr(), _DTYPES[logits.dtype], B, V, top, logits.stride(0) if B > 1 else V,
@@ -125,7 +125,7 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], ma
         raise ValueError("grad_entropy needs the forward call's entropy")
     entropy = _vector(entropy, torch.float32, rows, "entropy")
     if out is None:
-        out = torch.empty((B, V), dtype=rows.dtype, device=rows.device)
+        out = rows.new_empty((B, V))
     elif out.shape != rows.shape or out.dtype != rows.dtype or out.device != rows.device or \
             out.stride(1) != 1 or (B > 1 and out.stride(0) < V):
         raise ValueError(f"out must be a row-major {rows.dtype} [{B}, {V}] on {rows.device}")

@@ -76,7 +76,7 @@ __device__ __forceinline__ bool temperature_ok(float T) { return T >= 1.17549435
 //
 // Bound: HBM, one read of the logits, for fp32; instruction issue and the rows' ends for
 // 16-bit logits (8 instructions and one ex2 a logit). Measured: rows_kernel, 4096 x 152064
-// fp32 383 us (6.5 TB/s); 1024 x 128256 bf16 55 us (4.8 TB/s; issue 65 %, ex2 pipe 63 %),
+// fp32 367 us (6.8 TB/s); 1024 x 128256 bf16 55 us (4.8 TB/s; issue 65 %, ex2 pipe 63 %),
 // with 20 alternatives 68 us; 777 x 50257 bf16, one alternative, 31 us. row_kernel: 1 x 256000
 // fp32, 20 alternatives, 12.4 us (one launch and a chain of latencies), 100 x 128256 bf16
 // 16.7 us. CTAs an SM, those 1024 rows without and with alternatives: two 59 and 74 us,

@@ -45,16 +45,17 @@ def _rows(logits: torch.Tensor, what: str) -> torch.Tensor:
     return logits
 
 
-def _vector(t: Optional[torch.Tensor], dtype: torch.dtype, like: torch.Tensor, what: str) -> Optional[torch.Tensor]:
-    """A per-row vector as the kernels read it: [B], dense, on the logits' device."""
+def _vector(t: Optional[torch.Tensor], dtype: torch.dtype, shape: torch.Size, device: int,
+            what: str) -> Optional[torch.Tensor]:
+    """A per-row vector as the kernels read it: dense, of the rows' ``shape`` ([B]) on their device."""
     if t is None:
         return None
-    if t.dtype is dtype and t.dim() == 1 and t.shape[0] == like.shape[0] and t.device == like.device:
-        return t if t.is_contiguous() else t.contiguous()
-    if t.shape != like.shape[:1]:
-        raise ValueError(f"{what} must be [{like.shape[0]}], got {tuple(t.shape)}")
-    if t.device != like.device:
-        raise ValueError(f"{what} are on {t.device}, the logits on {like.device}")
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return t
+    if t.shape != shape:
+        raise ValueError(f"{what} must be [{shape[0]}], got {tuple(t.shape)}")
+    if t.get_device() != device:
+        raise ValueError(f"{what} are on {t.device}, the logits on cuda:{device}")
     if t.dtype != dtype:
         if t.dtype.is_floating_point != dtype.is_floating_point:
             raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
@@ -79,11 +80,12 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     """
     logits = _rows(logits, "logits")
     B, V = logits.shape
+    shape, index = logits.shape[:1], logits.get_device()
     top = int(top)
     if not 0 <= top <= _lib.FG_LOGPROB_MAX_TOP:
         raise ValueError(f"top must be in [0, {_lib.FG_LOGPROB_MAX_TOP}], got {top}")
-    tokens = _vector(tokens, torch.int64, logits, "tokens")
-    temperature = _vector(temperature, torch.float32, logits, "temperature")
+    tokens = _vector(tokens, torch.int64, shape, index, "tokens")
+    temperature = _vector(temperature, torch.float32, shape, index, "temperature")
     dev = logits.device
     logprobs, entropy, peak, logsum, rank, status = logits.new_empty((6, B), dtype=torch.float32).unbind(0)
     rank, status = rank.view(torch.int32), status.view(torch.int32)
@@ -115,15 +117,16 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], ma
     ``out`` may be ``logits`` itself: the gradient then replaces the logits."""
     rows = _rows(logits, "logits")
     B, V = rows.shape
-    tokens = _vector(tokens, torch.int64, rows, "tokens")
-    temperature = _vector(temperature, torch.float32, rows, "temperature")
-    max = _vector(max, torch.float32, rows, "max")
-    logsum = _vector(logsum, torch.float32, rows, "logsum")
-    grad_logprobs = _vector(grad_logprobs, torch.float32, rows, "grad_logprobs")
-    grad_entropy = _vector(grad_entropy, torch.float32, rows, "grad_entropy")
+    shape, index = rows.shape[:1], rows.get_device()
+    tokens = _vector(tokens, torch.int64, shape, index, "tokens")
+    temperature = _vector(temperature, torch.float32, shape, index, "temperature")
+    max = _vector(max, torch.float32, shape, index, "max")
+    logsum = _vector(logsum, torch.float32, shape, index, "logsum")
+    grad_logprobs = _vector(grad_logprobs, torch.float32, shape, index, "grad_logprobs")
+    grad_entropy = _vector(grad_entropy, torch.float32, shape, index, "grad_entropy")
     if grad_entropy is not None and entropy is None:
         raise ValueError("grad_entropy needs the forward call's entropy")
-    entropy = _vector(entropy, torch.float32, rows, "entropy")
+    entropy = _vector(entropy, torch.float32, shape, index, "entropy")
     if out is None:
         out = rows.new_empty((B, V))
     elif out.shape != rows.shape or out.dtype != rows.dtype or out.device != rows.device or \

@@ -107,6 +107,8 @@ __device__ __forceinline__ void down_dots(const Params& P, const uint16_t* src, 
 template <int DT, int RC>
 __global__ void __launch_bounds__(DOWN_THREADS) down_kernel(const Params P) {
     __shared__ float us[16 * RC];
+    // project_kernel may begin once this kernel has: by then what came before both is done
+    tc::wait_prerequisites();
     tc::launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int b = blockIdx.x;

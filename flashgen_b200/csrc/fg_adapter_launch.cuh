@@ -63,8 +63,16 @@ int launch_rank(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xma
                 return FG_EDEVICE;
             attr_set[dev].store(true, std::memory_order_release);
         }
-        down_kernel<DT, RC ? RC : 1><<<P.batch, DOWN_THREADS, 0, st>>>(P);
-        if (cudaGetLastError() != cudaSuccess) return FG_ELAUNCH;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(P.batch);
+        cfg.blockDim = dim3(DOWN_THREADS);
+        cfg.stream = st;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (cudaLaunchKernelEx(&cfg, down_kernel<DT, RC ? RC : 1>, P) != cudaSuccess) return FG_ELAUNCH;
     }
     if (pair) return launch_project<2, DT, ODT, RC, false>(P, wmap, xmap, first, d, st);
     // (ranks 17 to 32 do better with more warps: 50 rows, dim 2048, V 50257: 52 against 55 us)

@@ -41,6 +41,27 @@ bool set_once(K kern, std::atomic<bool>* done, cudaFuncAttribute attr, int value
     return true;
 }
 
+// A launch that may begin while the stream's previous kernel ends: the kernel itself
+// waits for that one before it touches memory.
+template <class... Params, class... Args>
+int launch_early(void (*kern)(Params...), unsigned grid, unsigned threads, size_t smem, unsigned cluster,
+                 cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? FG_OK : FG_ELAUNCH;
+}
+
 template <int DT, bool TOP>
 int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
     DevInfo* d = nullptr;
@@ -55,20 +76,9 @@ int launch_forward(const fg::lp::Params& P, int32_t batch, cudaStream_t st) {
             !set_once(kern, carved, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared))
             return FG_EDEVICE;
         const int grid = std::min<int64_t>(batch, fg::lp::CTAS_PER_SM * d->sms);
-        kern<<<grid, fg::lp::THREADS, smem, st>>>(P, batch);
-        return cudaGetLastError() == cudaSuccess ? FG_OK : FG_ELAUNCH;
+        return launch_early(kern, grid, fg::lp::THREADS, smem, 1, st, P, int64_t(batch));
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(batch) * G);
-    cfg.blockDim = dim3(fg::lp::THREADS);
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = G;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fg::lp::row_kernel<DT, TOP>, P, G) == cudaSuccess ? FG_OK : FG_ELAUNCH;
+    return launch_early(fg::lp::row_kernel<DT, TOP>, unsigned(batch) * G, fg::lp::THREADS, 0, G, st, P, G);
 }
 
 template <int DT>
@@ -101,8 +111,9 @@ int launch_grad(const fg::lp::GradParams& P, int32_t batch, cudaStream_t st) {
         if (P.entropy) Q.entropy = P.entropy + lo;
         if (P.grad_logprobs) Q.grad_logprobs = P.grad_logprobs + lo;
         if (P.grad_entropy) Q.grad_entropy = P.grad_entropy + lo;
-        fg::lp::logprob_grad_kernel<DT><<<unsigned(n) * unsigned(per_row), fg::lp::GRAD_THREADS, 0, st>>>(Q, per_row);
-        if (cudaGetLastError() != cudaSuccess) return FG_ELAUNCH;
+        const int rc = launch_early(fg::lp::logprob_grad_kernel<DT>, unsigned(n) * unsigned(per_row),
+                                    fg::lp::GRAD_THREADS, 0, 1, st, Q, per_row);
+        if (rc != FG_OK) return rc;
     }
     return FG_OK;
 }

@@ -49,6 +49,9 @@ struct GradParams {
     int64_t grad_stride;
 };
 
+// The stream's previous kernel is done and its results visible (launches may begin earlier).
+__device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Temperatures: positive, finite and not subnormal (1 / T stays finite).
 __device__ __forceinline__ bool temperature_ok(float T) { return T >= 1.17549435e-38f && T < INFINITY; }
 
@@ -738,6 +741,7 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const Params P, const int 
     const int tid = threadIdx.x, part = blockIdx.x % G;
     cluster_arrive();   // the others' shared memory stands once all have arrived
     if (tid == 0) sh.count[0] = 0;
+    wait_prerequisites();
     const Row<DT> row(P, blockIdx.x / G, part, G);
     const uint4* chunks = row.chunks();
     Pass<DT> pass;
@@ -779,6 +783,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) rows_kernel(const Params
     const int tid = threadIdx.x;
     const uint32_t ring0 = smem_u32(ring) + 16 * tid, ring1 = ring0 + RING_BYTES;
     if (tid == 0) sh.count[0] = 0;
+    wait_prerequisites();
 
     // ---- the copies: `left` chunks of row `next` from `src` on ----
     int64_t next = blockIdx.x;
@@ -968,6 +973,7 @@ __device__ __forceinline__ uint4 pack_chunk(const float (&x)[Elem<DT>::VEC]) {
 // CTA blockIdx.x: part blockIdx.x % per_row of row blockIdx.x / per_row.
 template <int DT>
 __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const GradParams P, const int per_row) {
+    wait_prerequisites();
     constexpr int VEC = Elem<DT>::VEC, SIZE = Elem<DT>::SIZE;
     const int64_t r = blockIdx.x / per_row;
     const int part = blockIdx.x % per_row, tid = threadIdx.x;

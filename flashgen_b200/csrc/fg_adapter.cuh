@@ -187,12 +187,13 @@ __global__ void __launch_bounds__(DOWN_THREADS) down_kernel(const Params P) {
 // accumulators in tensor memory: one tile's epilogue runs beside the next products.
 //
 // Bound: HBM up to about 128 rows (the weight, once), the tensor pipe above. Measured
-// (bf16, dim 4096, rank 16): 128256 words, one row 162 us (6.5 TB/s of weight), 64 rows of 32
-// adapters 199 us (5.3 TB/s); 32768 words, 1024 rows 264 us (1.04 PFLOP/s; SM clock held to
+// (bf16, dim 4096, rank 16): 128256 words, one row 161 us (6.5 TB/s of weight), 64 rows of 32
+// adapters 197 us (5.3 TB/s); 32768 words, 1024 rows 260 us (1.06 PFLOP/s; SM clock held to
 // 1.6 GHz by the power limit, tensor pipe active 57 %, 66 % without adapters, the epilogue's
 // loads and products being the difference). Few rows of a short weight: 64 rows, dim 2048,
-// 32000 words 31 us without adapters, 36 us with 16 of rank 8, 42 us with 32 of rank 16
-// (the fetches of the adapters' rows, a chain of latencies in each tile's epilogue).
+// 32000 words 28 us without adapters, 34.5 us with 16 of rank 8, 40 us with 32 of rank 16
+// (down_kernel's launch and the adapters' bytes; their rows fetched ahead of the epilogue,
+// to L2 or to shared memory by a warp of its own, gained nothing).
 //
 // fp32 results: the tensor core truncates when it adds a product to the
 // accumulator, and over hundreds of steps that bias shows in 32 bits. So the sum
@@ -524,6 +525,8 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     if (CG == 2) tc::cluster_sync();   // both CTAs' barriers stand
     tc::fence_after();
     const uint32_t tmem = C.tmem;
+    // down_kernel began after everything before it had ended; without it, wait for that here
+    if (!P.chained) tc::wait_prerequisites();
 
     if (warp == 0) {
         if (lane == 0) {

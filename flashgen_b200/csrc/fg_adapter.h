@@ -39,6 +39,7 @@ struct Params {
     int32_t kb;               // 64-wide boxes of K in a stage
     int32_t accs;             // accumulators of nt columns in tensor memory
     int32_t tmem_cols;
+    int32_t chained;          // down_kernel goes before
 };
 
 // Both launches of a call: operands of type DT, result of type ODT. `pair`: two

@@ -11,7 +11,7 @@ namespace fg {
 namespace adapt {
 
 template <int CG, int DT, int ODT, int RC, bool SMALL>
-int launch_project(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, bool dependent,
+int launch_project(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xmap, bool chained,
                    host::DevInfo* d, cudaStream_t st) {
     auto kern = project_kernel<CG, DT, ODT, RC, SMALL>;
     static std::atomic<bool> attr_set[host::kMaxDevices] = {};
@@ -25,6 +25,7 @@ int launch_project(const Params& P, const CUtensorMap& wmap, const CUtensorMap& 
         attr_set[dev].store(true, std::memory_order_release);
     }
     Params Q = P;
+    Q.chained = chained;
     const int stage = P.kb * (A_BYTES + P.nt / CG * TILE_K * 2);
     Q.stages = std::min(MAX_STAGES, (room - 1024) / stage);
     cudaLaunchConfig_t cfg{};
@@ -39,11 +40,9 @@ int launch_project(const Params& P, const CUtensorMap& wmap, const CUtensorMap& 
         attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
         ++cfg.numAttrs;
     }
-    if (dependent) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-        ++cfg.numAttrs;
-    }
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
     cfg.attrs = attr;
     return cudaLaunchKernelEx(&cfg, kern, wmap, xmap, Q) == cudaSuccess ? FG_OK : FG_ELAUNCH;
 }

@@ -79,11 +79,11 @@ __device__ __forceinline__ bool temperature_ok(float T) { return T >= 1.17549435
 //
 // Bound: HBM, one read of the logits, for fp32; instruction issue and the rows' ends for
 // 16-bit logits (8 instructions and one ex2 a logit). Measured: rows_kernel, 4096 x 152064
-// fp32 367 us (6.8 TB/s); 1024 x 128256 bf16 55 us (4.8 TB/s; issue 65 %, ex2 pipe 63 %),
-// with 20 alternatives 68 us; 777 x 50257 bf16, one alternative, 31 us. row_kernel: 1 x 256000
-// fp32, 20 alternatives, 12.4 us (one launch and a chain of latencies), 100 x 128256 bf16
-// 16.7 us. CTAs an SM, those 1024 rows without and with alternatives: two 59 and 74 us,
-// three 55 and 68, four 61 and 74 (fewer steps in flight each).
+// fp32 369 us (6.8 TB/s); 1024 x 128256 bf16 53 us (5.0 TB/s; issue 65 %, ex2 pipe 63 %),
+// with 20 alternatives 66 us; 777 x 50257 bf16, one alternative, 28 us. row_kernel: 1 x 256000
+// fp32, 20 alternatives, 10.6 us (one launch and a chain of latencies). CTAs an SM, those
+// 1024 rows without and with alternatives: two take 4 and 6 us more than three, four 6 and 6
+// (fewer steps in flight each).
 // ---------------------------------------------------------------------------
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
@@ -903,8 +903,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) rows_kernel(const Params
 // Bound: HBM, the logits read and the gradient written once. Work is cut along the
 // gradient's 16-byte chunks; where the logits' rows are offset against the
 // gradient's, a thread takes the two chunks around its own and shifts them together.
-// Measured: 1024 x 128256 bf16 88 us (6.0 TB/s; two chunks in flight a thread 93, one step
-// a CTA 105), 2048 x 50257 fp32 130 us (6.3 TB/s; 147, 146); 8 x 50257 fp32 4.2 us.
+// Measured: 1024 x 128256 bf16 86 us (6.1 TB/s; two chunks in flight a thread 4 us more,
+// one step a CTA 16 more), 2048 x 50257 fp32 129 us (6.4 TB/s; 17 more, 16 more); 8 x 50257
+// fp32 2.9 us.
 // ---------------------------------------------------------------------------
 constexpr int GRAD_THREADS = 256;
 constexpr int GRAD_UNROLL = 4;   // chunks in flight a thread

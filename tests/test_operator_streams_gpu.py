@@ -96,3 +96,30 @@ def test_back_to_back_calls_read_finished_inputs():
     want = chain(True)
     for _ in range(3):
         assert torch.equal(chain(False), want)
+
+
+@pytest.mark.parametrize("batch", [1, 40, 200])
+@pytest.mark.parametrize("with_adapters", [False, True])
+def test_the_head_reads_a_weight_written_just_before(batch, with_adapters):
+    vocab, dim = 40003, 512
+    versions = [torch.randn(vocab, dim, device="cuda").to(torch.bfloat16) * dim ** -0.5 for _ in range(4)]
+    hidden = torch.randn(batch, dim, device="cuda").to(torch.bfloat16)
+    weight = versions[0].clone()
+    head = AdapterHead(weight, slots=2, rank=8)
+    assert head.weight.data_ptr() == weight.data_ptr()
+    head.load(1, torch.randn(8, dim, device="cuda"), torch.randn(vocab, 8, device="cuda"), 0.1)
+    adapters = torch.arange(batch, device="cuda", dtype=torch.int32) % 3 - 1 if with_adapters else None
+
+    def run(sync):
+        out = []
+        for v in versions:
+            torch.mul(v, 1.0, out=weight)   # a kernel, not a copy
+            if sync:
+                torch.cuda.synchronize()
+            out.append(head.logits(hidden, adapters))
+            if sync:
+                torch.cuda.synchronize()
+        return out
+
+    for got, want in zip(run(False), run(True)):
+        assert torch.equal(got, want)

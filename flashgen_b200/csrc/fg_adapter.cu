@@ -113,11 +113,12 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
     P.order = reinterpret_cast<int32_t*>(ws + L.order);
     P.batch = a->batch; P.dim = a->dim; P.vocab = a->vocab; P.rank = a->rank; P.slots = a->slots;
     P.down_stride = a->down_stride; P.out_stride = a->out_stride; P.copy_stride = L.copy_stride;
-    // Sorting costs a copy of the hidden rows that the products wait for: up to 64
-    // rows it takes longer than it saves (64 rows of 32 adapters of rank 16, dim 2048,
-    // V 32000: 50 us sorted, 44 us not). TMA reads rows that start on 16-byte boundaries:
-    // others are copied first too.
-    P.sorted = a->slots > 0 && a->adapters != nullptr && a->batch > 64;
+    // Sorting costs a copy of the hidden rows that the products wait for; it saves fetches of
+    // adapters and products with them. Dim 2048, V 32000, 32 adapters of rank 16: 32 rows 36.8
+    // us sorted, 34.7 not; 48 rows 37.8, 37.0; 64 rows 38.4, 40.2 (with 4 adapters 35.0, 33.9;
+    // fp32 results, V 50257, 16 adapters 53, 61); 96 rows 41.8, 45.6. TMA reads rows that
+    // start on 16-byte boundaries: others are copied first too.
+    P.sorted = a->slots > 0 && a->adapters != nullptr && a->batch > 48;
     const bool copy = P.sorted || !aligned(a->hidden, 16) || (a->batch > 1 && a->hidden_stride % 8 != 0);
     P.wide_out = aligned(a->out, 16) && (a->batch == 1 || a->out_stride * elem_size(a->out_dtype) % 16 == 0);
     P.copy = copy ? ws + L.copy : nullptr;

@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(DOWN_THREADS) down_kernel(const Params P) {
 // adapters 197 us (5.3 TB/s); 32768 words, 1024 rows 260 us (1.06 PFLOP/s; SM clock held to
 // 1.6 GHz by the power limit, tensor pipe active 57 %, 66 % without adapters, the epilogue's
 // loads and products being the difference). Few rows of a short weight: 64 rows, dim 2048,
-// 32000 words 28 us without adapters, 34.5 us with 16 of rank 8, 40 us with 32 of rank 16
+// 32000 words 28 us without adapters, 35 us with 16 of rank 8, 38 us with 32 of rank 16
 // (down_kernel's launch and the adapters' bytes; their rows fetched ahead of the epilogue,
 // to L2 or to shared memory by a warp of its own, gained nothing).
 //
@@ -207,8 +207,8 @@ constexpr int MAX_STAGES = 12;
 // products arrive (the others' adapters are added as they are read). With fp32
 // results registers go to the sums, of fewer columns for a SMALL batch tile: next to
 // the ring there is no L1 left, and a spilled register would wait for L2.
-// Measured: 12 warps against 8, 64 rows, 16-bit results: 42.7 us, 45.5; 16 against 8, 256
-// rows, fp32: 99, 114; no early windows at those 64 rows: 49.6; SMALL, 8 rows, dim 2048,
+// Measured: 12 warps against 8, 64 rows not sorted, 16-bit results: 42.7 us, 45.5; 16 against
+// 8, 256 rows, fp32: 99, 114; no early windows at those 64 rows: 49.6; SMALL, 8 rows, dim 2048,
 // 50257 words, fp32: 43.6, without it 49.9.
 template <int ODT, int RC, bool SMALL>
 struct Epilogue {

@@ -63,6 +63,11 @@ __device__ __forceinline__ bool temperature_ok(float T) { return T >= 1.17549435
 // sum may grow to 2^64 above it, so it is rescaled about once); the count of the
 // logits ahead of the token's. S and Q are sums of 2^y and 2^y y with y = x c - r:
 // one FMA a logit, the same r in every term, so r's rounding cancels in log2 S + r.
+// That holds while the rounding is small: |r| stays below FAR, where it is at most half
+// a unit of y. A thread whose largest logit is below -3/4 FAR / c keeps no reference, and
+// a row whose maximum is not within FAR / (2 c) of 0 is summed a second time, from the
+// differences x - m: in the other rows all that was left out is FAR / 4 below the
+// maximum, where 2^y is 0.
 //
 // Alternatives without a second pass over the row: each thread leaves the maxima of up
 // to SLOTS stretches of its chunks. The top-th largest of 32 or 64 group maxima bounds
@@ -100,6 +105,7 @@ constexpr int MAX_G = 8;
 constexpr int STRETCHES = 64;        // a warp reads again
 constexpr int CAND = 256;            // candidates held at once
 constexpr float R_STEP = 64.0f;      // how far above its reference a term may be (in log2)
+constexpr float FAR = 0x1p24f;       // how far from 0 a reference may be (in log2)
 
 // Order of the alternatives: larger logit first, then smaller id. A larger code
 // comes first; 0 is below every element's code.
@@ -128,12 +134,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 
 // Chunk arithmetic per type. FLOOR replaces -inf (and anything below) in the sums so
 // that no term is 0 * inf; the one-pass sums are valid while the row's maximum stays
-// well above it and x c stays finite (one_pass_ok), other rows are summed again.
+// well above it and near enough to 0, and x c finite (one_pass_ok); other rows are
+// summed again.
 template <int DT> struct Chunk;
 template <> struct Chunk<FG_DTYPE_F32> {
     static constexpr int WORDS = 4;
     __device__ __forceinline__ static bool one_pass_ok(float m, float c) {
-        return m > -1e29f && m < 1e29f && c < 1e8f && c > 1e-20f;
+        return c > 1e-20f && c < 1e8f && fabsf(m * c) < 0.5f * FAR;   // (so |m| < 1e27)
     }
     // the largest logit of the words, NaN if any is
     __device__ __forceinline__ static float max_of(const uint32_t* w, int n) {
@@ -212,7 +219,9 @@ template <class T2, int DT> struct Chunk16 {
     };
 };
 template <> struct Chunk<FG_DTYPE_F16> : Chunk16<__half2, FG_DTYPE_F16> {
-    __device__ __forceinline__ static bool one_pass_ok(float m, float c) { return m > -60000.0f && c > 0.03f && c < 1e8f; }
+    __device__ __forceinline__ static bool one_pass_ok(float m, float c) {
+        return m > -60000.0f && c > 0.03f && c < 1e8f && fabsf(m * c) < 0.5f * FAR;
+    }
 };
 template <> struct Chunk<FG_DTYPE_BF16> : Chunk16<__nv_bfloat162, FG_DTYPE_BF16> {
     __device__ __forceinline__ static bool one_pass_ok(float m, float c) {
@@ -224,8 +233,9 @@ template <> struct Chunk<FG_DTYPE_BF16> : Chunk16<__nv_bfloat162, FG_DTYPE_BF16>
 struct Sums {
     float2 s = {0.0f, 0.0f}, q = {0.0f, 0.0f};
     float r = 0.0f;                  // the reference, in log2
-    float limit = -9.9e29f;          // logits above it move the reference
+    float limit;                     // logits above it move the reference
     bool set = false;
+    __device__ __forceinline__ explicit Sums(float T) : limit(fmaxf(-9.9e29f, -0.75f * FAR * LN2 * T)) {}
     __device__ __forceinline__ void follow(float m, float c) {   // m: the largest of the next logits
         if (m > limit) {
             const float to = m * c;
@@ -381,6 +391,7 @@ struct Pass {
     float vmax = -INFINITY;   // NaN if any logit is
     float smax = -INFINITY;   // of the stretch at hand
     int n = 0;
+    __device__ __forceinline__ explicit Pass(const Row<DT>& row) : acc(row.T) {}
     // a step is done: at the end of a stretch of 2^log steps its maximum is left behind
     __device__ __forceinline__ void stretch(Shared& sh, int step, int log, bool last) {
         if (((step + 1) & ((1 << log) - 1)) == 0 || last) {
@@ -751,7 +762,7 @@ __global__ void __launch_bounds__(THREADS) row_kernel(const Params P, const int 
     wait_prerequisites();
     const Row<DT> row(P, blockIdx.x / G, part, G);
     const uint4* chunks = row.chunks();
-    Pass<DT> pass;
+    Pass<DT> pass(row);
     const int scalars = part == 0 ? row.head + row.tail : 0;
     pass.begin(row, scalars, tid);
     const int steps = (row.c1 - row.c0 + STEP - 1) / STEP, log = stretch_log(steps);
@@ -844,7 +855,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) rows_kernel(const Params
             if (P.tokens) tok = P.tokens[r + gridDim.x];
             if (P.temperature) T = P.temperature[r + gridDim.x];
         }
-        Pass<DT> pass;
+        Pass<DT> pass(row);
         const int scalars = row.head + row.tail;
         pass.begin(row, scalars, tid);
         auto turn = [&]() {   // the values are used: the place is free

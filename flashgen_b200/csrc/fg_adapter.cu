@@ -121,6 +121,7 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
     P.sorted = a->slots > 0 && a->adapters != nullptr && a->batch > 48;
     const bool copy = P.sorted || !aligned(a->hidden, 16) || (a->batch > 1 && a->hidden_stride % 8 != 0);
     P.wide_out = aligned(a->out, 16) && (a->batch == 1 || a->out_stride * elem_size(a->out_dtype) % 16 == 0);
+    P.f32_out = a->out_dtype == FG_DTYPE_F32;
     P.copy = copy ? ws + L.copy : nullptr;
     P.hidden = copy ? P.copy : a->hidden;
     P.hidden_stride = copy || a->batch == 1 ? L.copy_stride : a->hidden_stride;

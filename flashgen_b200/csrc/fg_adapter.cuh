@@ -16,10 +16,15 @@
 // or leaves it; sorting keeps that to about one product per eight columns plus one
 // per adapter.
 //
-// U enters the tensor cores in its fp32 precision: a row of U is scaled by a power
-// of two to at most 1 and split into 16-bit parts (three of bf16 make 24 bits, two
-// of f16 make 22; two of bf16 where the result has 16 bits anyway), whose products
-// are summed in fp32; the power of two multiplies the sum.
+// U enters the tensor cores in its fp32 precision: a row of U is scaled by a power of
+// two and split into 16-bit parts, whose products are summed in fp32; the power of two
+// multiplies the sum. Three parts hold the 24 bits of a component. bf16 has the
+// exponents for them; rows of f16 are scaled to the top of its range, and lower parts
+// are scaled up once more (part_scale), their sums down: components down to 2^-41 of the
+// row's largest keep 23 bits. 16-bit results take two parts: 16 bits of bf16 for results
+// of 8 bits; f16, whose results have 11, 16 or more down to 2^-23 of the largest, and a
+// third part for rows with smaller components (16 bits down to 2^-36). Three for all: 1024
+// rows, dim 4096, V 32768, rank 64, bf16 423 us against 391.
 #pragma once
 
 #include <type_traits>
@@ -37,6 +42,13 @@ __device__ __forceinline__ int row_slot(const Params& P, int b) {
 }
 
 constexpr int DOWN_THREADS = 256;
+
+constexpr int U_PARTS = 3;   // 16-bit parts of a component of U
+// What part i (1, 2) is scaled up by against part i - 1.
+template <int DT>
+__device__ __forceinline__ constexpr float part_scale(bool f32_out, int i) {
+    return DT != FG_DTYPE_F16 ? 1.0f : f32_out ? 0x1p12f : i == 1 ? 1.0f : 0x1p24f;
+}
 
 template <int DT>
 __device__ __forceinline__ float from_bits(uint16_t b) {
@@ -158,20 +170,33 @@ __global__ void __launch_bounds__(DOWN_THREADS) down_kernel(const Params P) {
     }
     __syncthreads();
     if (warp == 0) {
-        float top = 0.0f;
-        for (int i = lane; i < 16 * RC; i += 32) top = fmaxf(top, fabsf(us[i]));
+        float top = 0.0f;   // the largest finite one
+        for (int i = lane; i < 16 * RC; i += 32) {
+            const float v = fabsf(us[i]);
+            top = fmaxf(top, v < INFINITY ? v : 0.0f);
+        }
         for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        // |U| 2^-e <= 1; outside [2^-100, 2^100] (and without a finite maximum) the row is left as it is
-        const bool plain = !(top >= 0x1p-100f && top <= 0x1p100f);
-        const int e = plain ? 0 : ilogbf(top) + 1;
+        // |U| 2^-e < 2^HIGH (2 for the largest of bf16); both powers finite
+        constexpr int HIGH = DT == FG_DTYPE_F16 ? 15 : 0;
+        const int e = top > 0.0f ? max(HIGH - 126, min(HIGH + 127, ilogbf(top) + 1)) - HIGH : 0;
         const float down = ldexpf(1.0f, -e);
-        if (lane == 0) P.unit[pos] = ldexpf(1.0f, e);
-        uint16_t* dst = reinterpret_cast<uint16_t*>(P.u) + int64_t(pos) * (3 * 16 * RC);
+        bool small = false;   // components that 16-bit results need the third part for: the unit's sign
+        for (int i = lane; i < 16 * RC; i += 32) {
+            const float v = fabsf(us[i]) * down;
+            small |= DT == FG_DTYPE_F16 && v > 0.0f && v < 0x1p-8f;
+        }
+        small = __any_sync(0xffffffffu, small);
+        if (lane == 0) P.unit[pos] = ldexpf(small ? -1.0f : 1.0f, e);
+        uint16_t* dst = reinterpret_cast<uint16_t*>(P.u) + int64_t(pos) * (U_PARTS * 16 * RC);
         for (int i = lane; i < 16 * RC; i += 32) {
             float v = us[i] * down;
 #pragma unroll
-            for (int part = 0; part < 3; ++part) {
-                const uint16_t h = to_bits<DT>(v);
+            for (int part = 0; part < U_PARTS; ++part) {
+                if (part > 0) v *= part_scale<DT>(P.f32_out, part);
+                // a subnormal operand costs the sum the bits between it and the type's least
+                // exponent: to fp32 results it is worth leaving to the next part
+                const bool later = DT == FG_DTYPE_F16 && P.f32_out && part == 0 && fabsf(v) < 0x1p-14f;
+                const uint16_t h = later ? uint16_t(0) : to_bits<DT>(v);
                 dst[part * 16 * RC + i] = h;
                 const float left = v - from_bits<DT>(h);
                 v = (left - left == 0.0f) ? left : 0.0f;   // inf and NaN live in the first part
@@ -290,7 +315,8 @@ struct UpTile {
 // time, their loads in flight together.
 template <int DT, int ODT, int RC>
 struct Windows {
-    static constexpr int PARTS = (DT == FG_DTYPE_BF16 && ODT == FG_DTYPE_F32) ? 3 : 2;
+    static constexpr int PARTS = ODT == FG_DTYPE_F32 ? U_PARTS : 2;   // held in registers
+    static constexpr bool LAST = PARTS < U_PARTS && DT == FG_DTYPE_F16;   // the third where a row needs it
     static constexpr int BATCH = RC == 1 && ODT != FG_DTYPE_F32 ? 3 : 1;
     static constexpr uint32_t ALL = 0xffffffffu;
     UpTile<RC> up;
@@ -303,23 +329,64 @@ struct Windows {
         return p < rows ? P.order[b0 + p] : -1;
     }
 
+    __device__ __forceinline__ static void product(float (&d)[2][4], const UpTile<RC>& tile, int c, const uint2& u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            warp_mma<DT>(d[h], tile.q[c][2 * h].x, tile.q[c][2 * h + 1].x, tile.q[c][2 * h].y, tile.q[c][2 * h + 1].y, u);
+    }
+    __device__ __forceinline__ static void scale_down(float (&d)[2][4], int part) {
+        constexpr bool F32 = ODT == FG_DTYPE_F32;
+        if (part_scale<DT>(F32, part) == 1.0f) return;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[h][j] *= 1.0f / part_scale<DT>(F32, part);
+    }
+
     // One adapter's product with the window; the columns in `match` take it, no other does.
     __device__ __forceinline__ static void apply(float (&x)[2][4], const UpTile<RC>& tile, const uint2 (&u)[RC][PARTS],
                                                  float unit0, float unit1, uint32_t match, int t) {
         float d[2][4] = {};
 #pragma unroll
-        for (int i = PARTS - 1; i >= 0; --i)
+        for (int i = PARTS - 1; i >= 0; --i) {
 #pragma unroll
-            for (int c = 0; c < RC; ++c)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    warp_mma<DT>(d[h], tile.q[c][2 * h].x, tile.q[c][2 * h + 1].x, tile.q[c][2 * h].y,
-                                 tile.q[c][2 * h + 1].y, u[c][i]);
+            for (int c = 0; c < RC; ++c) product(d, tile, c, u[c][i]);
+            if (i > 0) scale_down(d, i);
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (match >> (2 * t) & (i & 1 ? 2 : 1)) x[h][i] = d[h][i] * (i & 1 ? unit1 : unit0);
+                if (match >> (2 * t) & (i & 1 ? 2 : 1)) x[h][i] = d[h][i] * fabsf(i & 1 ? unit1 : unit0);
+    }
+
+    // Whether any of the columns in `match` needs the part of U that is not held in registers.
+    __device__ __forceinline__ static bool needs_last(float unit0, float unit1, uint32_t match, int t) {
+        if (!LAST) return false;
+        const uint32_t mine = match >> (2 * t);
+        return __any_sync(ALL, (unit0 < 0.0f && (mine & 1)) || (unit1 < 0.0f && (mine & 2)));
+    }
+    // That part's products with every adapter of the window (seldom run: apart from the
+    // others, whose instructions interleave).
+    __device__ __forceinline__ static void add_last(float (&x)[2][4], UpTile<RC>& tile, const Params& P, const uint2* src,
+                                                    int slots, int v0, float unit0, float unit1, int lane) {
+        const int t = lane & 3;
+        uint32_t left = __ballot_sync(ALL, slots >= 0) & 0xffu;
+        while (left) {
+            const int slot = __shfl_sync(ALL, slots, __ffs(left) - 1);
+            const uint32_t match = __ballot_sync(ALL, slots == slot) & 0xffu;
+            left &= ~match;
+            tile.load(P, slot, v0, lane);
+            float d[2][4] = {};
+#pragma unroll
+            for (int c = 0; c < RC; ++c) product(d, tile, c, src[PARTS * 4 * RC + c * 4]);
+            scale_down(d, PARTS);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (match >> (2 * t) & (i & 1 ? 2 : 1)) x[h][i] += d[h][i] * fabsf(i & 1 ? unit1 : unit0);
+        }
     }
 
     // The adapters' share of window w, eight columns by 32 vocabulary rows from v0 on:
@@ -332,9 +399,10 @@ struct Windows {
         for (int i = 0; i < 4; ++i) x[0][i] = x[1][i] = 0.0f;
         uint32_t left = __ballot_sync(ALL, slots >= 0) & 0xffu;   // columns still without their adapter
         if (left == 0) return;
+        const uint32_t all = left;
         // B fragments: parts of U for column g
         uint2 u[RC][PARTS];
-        const uint2* src = reinterpret_cast<const uint2*>(P.u) + int64_t(b0 + min(8 * w + g, rows - 1)) * (12 * RC) + t;
+        const uint2* src = reinterpret_cast<const uint2*>(P.u) + int64_t(b0 + min(8 * w + g, rows - 1)) * (U_PARTS * 4 * RC) + t;
 #pragma unroll
         for (int c = 0; c < RC; ++c)
 #pragma unroll
@@ -367,6 +435,10 @@ struct Windows {
                 if (match[i]) apply(x, tile[i], u, unit0, unit1, match[i], t);
             if (match[BATCH - 1]) apply(x, up, u, unit0, unit1, match[BATCH - 1], t);
         }
+        if (needs_last(unit0, unit1, all, t)) {
+            add_last(x, up, P, src, slots, v0, unit0, unit1, lane);
+            cur = -1;
+        }
     }
 };
 
@@ -383,18 +455,21 @@ __device__ __forceinline__ void early_windows(float (&x)[E][2][4], const int (&e
     uint32_t left = 0;   // columns still without their adapter, eight bits a window
     uint2 u[E][RC][W::PARTS];
     float unit[E][2];
+    auto src = [&](int i) {   // this thread's parts of U of window w0 + i
+        return reinterpret_cast<const uint2*>(P.u) +
+               int64_t(b0 + min(8 * min(w0 + i, w1 - 1) + g, rows - 1)) * (U_PARTS * 4 * RC) + t;
+    };
 #pragma unroll
     for (int i = 0; i < E; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[i][0][j] = x[i][1][j] = 0.0f;
         slots[i] = w0 + i < w1 && ents[i] >= 0 ? (ents[i] >> 9) - 1 : -1;
         left |= (__ballot_sync(ALL, slots[i] >= 0) & 0xffu) << (8 * i);
-        const int w = min(w0 + i, w1 - 1), p = 8 * w + 2 * t;
-        const uint2* src = reinterpret_cast<const uint2*>(P.u) + int64_t(b0 + min(8 * w + g, rows - 1)) * (12 * RC) + t;
+        const int p = 8 * min(w0 + i, w1 - 1) + 2 * t;
 #pragma unroll
         for (int c = 0; c < RC; ++c)
 #pragma unroll
-            for (int j = 0; j < W::PARTS; ++j) u[i][c][j] = src[j * 4 * RC + c * 4];
+            for (int j = 0; j < W::PARTS; ++j) u[i][c][j] = src(i)[j * 4 * RC + c * 4];
         unit[i][0] = p < rows ? P.unit[b0 + p] : 0.0f;
         unit[i][1] = p + 1 < rows ? P.unit[b0 + p + 1] : 0.0f;
     }
@@ -424,6 +499,12 @@ __device__ __forceinline__ void early_windows(float (&x)[E][2][4], const int (&e
                 if (match[k] >> (8 * i) & 0xffu)
                     W::apply(x[i], tile[k], u[i], unit[i][0], unit[i][1], match[k] >> (8 * i), t);
     }
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (W::needs_last(unit[i][0], unit[i][1], __ballot_sync(ALL, slots[i] >= 0) & 0xffu, t)) {
+            UpTile<RC> tile;
+            W::add_last(x[i], tile, P, src(i), slots[i], v0, unit[i][0], unit[i][1], lane);
+        }
 }
 
 // Read window w of the accumulator, add the adapters' share and store it.

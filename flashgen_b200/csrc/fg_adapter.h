@@ -23,8 +23,8 @@ struct Params {
     const int32_t* adapters;
     void* out;
     int32_t* out_status;
-    void* u;                  // [B, 3, 16 RC] in the sorted order: 16-bit parts of U times a power of two (workspace)
-    float* unit;              // [B] in the sorted order: that power's inverse (workspace)
+    void* u;                  // [B, 3, 16 RC] in the sorted order: 16-bit parts of U times powers of two (workspace)
+    float* unit;              // [B] in the sorted order: the first power's inverse, negative where 16-bit results need all parts (workspace)
     int32_t* order;           // [B] per batch tile: (slot + 1) << 9 | column, sorted (workspace)
     void* copy;               // [B, copy_stride] hidden rows, sorted and aligned, or null (workspace)
     int32_t batch, dim, vocab, rank, slots;
@@ -32,6 +32,7 @@ struct Params {
     int32_t ntile;            // batch tiles
     int32_t sorted;           // rows of a tile in the order of their adapters (else as they come)
     int32_t wide_out;         // rows of out 16-byte aligned
+    int32_t f32_out;
     int32_t nt;               // columns of a batch tile, a multiple of 16 up to 256
     // project_kernel
     int32_t nvt;              // vocabulary tiles of 128 (256 for a pair)

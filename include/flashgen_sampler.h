@@ -324,9 +324,11 @@ int fg_token_logprobs_grad(const FgLogprobGradArgs* args, void* stream);
  *             + scales[a] sum_i (sum_k hidden[b, k] down[a, i, k]) up[a, v, i]
  *
  * and without the second term where a < 0 or scales[a] == 0 (or adapters is NULL).
- * Products of the
- * 16-bit operands are summed in fp32, the inner sums of the second term stay in
- * fp32, and out is rounded once. A row reads its own adapter only: NaN or inf in
+ * Products of the 16-bit operands are summed in fp32 and out is rounded once. The
+ * inner sums of the second term are fp32; its outer product takes their 24 bits
+ * (float16: 23 for sums down to 2^-41 of the row's largest) for fp32 results and
+ * their first 16 bits (float16: 16 for sums down to 2^-36 of the row's largest) for
+ * 16-bit results. A row reads its own adapter only: NaN or inf in
  * another row's adapter cannot reach it. An id >= slots marks the row's
  * out_status FG_ROW_BAD_PARAM and leaves it without an adapter.
  *

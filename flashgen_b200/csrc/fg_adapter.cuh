@@ -500,17 +500,59 @@ __device__ __forceinline__ void early_windows(float (&x)[E][2][4], const int (&e
                     W::apply(x[i], tile[k], u[i], unit[i][0], unit[i][1], match[k] >> (8 * i), t);
     }
 #pragma unroll
-    for (int i = 0; i < E; ++i)
+    for (int i = 0; i < E; ++i) {
         if (W::needs_last(unit[i][0], unit[i][1], __ballot_sync(ALL, slots[i] >= 0) & 0xffu, t)) {
             UpTile<RC> tile;
             W::add_last(x[i], tile, P, src(i), slots[i], v0, unit[i][0], unit[i][1], lane);
         }
+    }
+}
+
+// An infinite element of up meets every part of a component, of which the lower ones may
+// be 0 or of the other sign: NaN where the product is infinite. So what came out NaN of an
+// adapter is summed again, in fp32 and from whole components (NaN stays NaN).
+template <int DT, int ODT, int RC>
+__device__ __forceinline__ void settle_nan(float (&x)[2][4], const Params& P, int b0, int w, int v0, int ent, int lane) {
+    constexpr uint32_t ALL = 0xffffffffu;
+    float all = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) all += x[0][i] + x[1][i];
+    if (!__any_sync(ALL, isnan(all))) return;
+    // (the lane anew, so that nothing worked out from it is kept for this path)
+    asm volatile("mov.u32 %0, %%laneid;" : "=r"(lane));
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int e = __shfl_sync(ALL, ent, 2 * t + j);
+        const int pos = b0 + 8 * w + 2 * t + j;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {   // one at a time: seldom run, and registers are short
+            float& y = x[i >> 1][2 * (i & 1) + j];
+            if (!isnan(y)) continue;    // (a column without an adapter has 0)
+            const uint16_t* u = reinterpret_cast<const uint16_t*>(P.u) + int64_t(pos) * (U_PARTS * 16 * RC);
+            const uint16_t* up = reinterpret_cast<const uint16_t*>(P.up) +
+                                 (int64_t((e >> 9) - 1) * P.vocab + min(v0 + g + 8 * i, P.vocab - 1)) * P.rank;
+            float sum = 0.0f;
+#pragma unroll 1
+            for (int r = 0; r < P.rank; ++r) {
+                float c = 0.0f;
+#pragma unroll
+                for (int part = U_PARTS - 1; part >= 0; --part) {
+                    c += from_bits<DT>(u[part * 16 * RC + r]);
+                    if (part > 0) c *= 1.0f / part_scale<DT>(ODT == FG_DTYPE_F32, part);
+                }
+                sum = fmaf(c, from_bits<DT>(up[r]), sum);
+            }
+            y = sum * fabsf(P.unit[pos]);
+        }
+    }
 }
 
 // Read window w of the accumulator, add the adapters' share and store it.
-template <int ODT>
+template <int DT, int ODT, int RC>
 __device__ __forceinline__ void store_window(const Params& P, uint32_t base, int b0, int w, int v0, int ent,
-                                             const float (&add)[2][4], int lane) {
+                                             float (&add)[2][4], int lane) {
+    if constexpr (RC > 0) settle_nan<DT, ODT, RC>(add, P, b0, w, v0, ent, lane);
     constexpr uint32_t ALL = 0xffffffffu;
     const int g = lane >> 2, t = lane & 3;
     float x[2][4];
@@ -795,7 +837,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                 if constexpr (EARLY > 0) {
 #pragma unroll
                     for (int i = 0; i < EARLY; ++i)
-                        if (w0 + i < w1) store_window<ODT>(P, base, b0, w0 + i, vw, ents[i], add[i], lane);
+                        if (w0 + i < w1) store_window<DT, ODT, RC>(P, base, b0, w0 + i, vw, ents[i], add[i], lane);
                 }
                 win = W{};
                 for (int w = w0 + EARLY; w < w1; ++w) {
@@ -807,7 +849,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                     } else if (ent >= rows) {
                         ent = -1;
                     }
-                    store_window<ODT>(P, base, b0, w, vw, ent, more, lane);
+                    store_window<DT, ODT, RC>(P, base, b0, w, vw, ent, more, lane);
                 }
             }
             release();

@@ -141,6 +141,19 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], ma
     return out
 
 
+class _Once(torch.autograd.Function):
+    """A gradient that is linked to what it was computed from: a backward pass
+    through it raises (``once_differentiable`` would not see the saved logits)."""
+
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("logprobs_and_entropy is differentiable once: its gradient has no gradient")
+
+
 class _LogprobsAndEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, temperature):
@@ -154,16 +167,20 @@ class _LogprobsAndEntropy(torch.autograd.Function):
         logits, tokens, temperature, peak, logsum, entropy = ctx.saved_tensors
         if grad_logprobs is None and grad_entropy is None:
             return None, None, None
-        grad = token_logprobs_grad(logits, tokens, peak, logsum, grad_logprobs, entropy=entropy,
-                                   grad_entropy=grad_entropy, temperature=temperature)
-        return grad.to(logits.dtype), None, None
+        with torch.no_grad():
+            grad = token_logprobs_grad(logits, tokens, peak, logsum, grad_logprobs, entropy=entropy,
+                                       grad_entropy=grad_entropy, temperature=temperature).to(logits.dtype)
+        if torch.is_grad_enabled():   # create_graph=True
+            grad = _Once.apply(grad, logits, grad_logprobs, grad_entropy)
+        return grad, None, None
 
 
 def logprobs_and_entropy(logits: torch.Tensor, tokens: torch.Tensor,
                          temperature: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Differentiable (with respect to ``logits``) log probabilities of
     ``tokens`` and entropies, both [B] float32: the two terms of a
-    policy-gradient loss with an entropy bonus.
+    policy-gradient loss with an entropy bonus. Differentiable once: a second
+    derivative raises.
 
     >>> lp, h = logprobs_and_entropy(logits, tokens)
     >>> (-(advantage * lp) - 0.01 * h).mean().backward()

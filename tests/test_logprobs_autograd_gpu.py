@@ -19,3 +19,38 @@ def test_second_derivatives_are_refused(cuda_device, which):
     with pytest.raises(RuntimeError, match="differentiable once"):
         (g,) = torch.autograd.grad(out, a, create_graph=True)
         torch.autograd.grad((g * g).sum(), a)
+
+
+@pytest.mark.parametrize("change", ["index", "mul", "fill"])
+def test_results_can_be_changed_in_place(cuda_device, change):
+    """Masking padded tokens in place, as a trainer does first."""
+    a, t = _case()
+    keep = torch.tensor([1.0, 0.0, 1.0], device="cuda")
+    lp, ent = logprobs_and_entropy(a, t)
+    for v in (lp, ent):
+        if change == "index":
+            v[1] = 0
+        elif change == "mul":
+            v.mul_(keep)
+        else:
+            v.masked_fill_(keep == 0, 0.0)
+    assert lp[1] == 0 and ent[1] == 0
+    (lp.sum() + 0.5 * ent.sum()).backward()
+    b = a.detach().clone().requires_grad_()
+    z = torch.log_softmax(b, 1)
+    (keep * (z.gather(1, t[:, None])[:, 0] - 0.5 * (z.exp() * z).sum(1))).sum().backward()
+    torch.testing.assert_close(a.grad, b.grad, atol=2e-6, rtol=0)     # both in fp32 on terms below 4
+    assert (a.grad[1] == 0).all()
+
+
+def test_one_result_changed_leaves_the_other(cuda_device):
+    """A detached result clamped for a report, and the statistics of a second call, change nothing saved."""
+    a, t = _case()
+    lp, ent = logprobs_and_entropy(a, t)
+    lp.detach().clamp_(max=-5)
+    ent.detach().zero_()
+    ent.sum().backward()
+    b = a.detach().clone().requires_grad_()
+    z = torch.log_softmax(b, 1)
+    (-(z.exp() * z).sum()).backward()
+    torch.testing.assert_close(a.grad, b.grad, atol=2e-6, rtol=0)

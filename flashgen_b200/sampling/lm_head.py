@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .sampler import _DTYPES, _call, _ptr, _status_error
+from .sampler import _DTYPES, _call, _ptr, _status_error, _written
 
 
 def _dense_rows(t: torch.Tensor) -> torch.Tensor:
@@ -104,7 +104,8 @@ class AdapterHead:
                 raise ValueError(f"adapters must be int32 [{B}] on {self.device}, got {adapters.dtype} "
                                  f"{tuple(adapters.shape)} on {adapters.device}")
             adapters = adapters.contiguous()
-        if out is None:
+        given = out is not None
+        if not given:
             out_dtype = self.dtype if out_dtype is None else out_dtype
             if out_dtype not in (self.dtype, torch.float32):
                 raise TypeError(f"out_dtype must be {self.dtype} or float32, got {out_dtype}")
@@ -126,6 +127,8 @@ class AdapterHead:
             hidden.stride(0) if B > 1 else self.dim, self.weight.stride(0), self._down.stride(1),
             out.stride(0) if B > 1 else self.vocab)
         _call(self.device, lib.fg_adapter_logits, a, "fg_adapter_logits")
+        if given:
+            _written(out)
         if check_errors:
             msg = _status_error(status)
             if msg is not None:

@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from .. import _lib
-from .sampler import _DTYPES, _call, _ptr, _row_logits, _status_error
+from .sampler import _DTYPES, _call, _ptr, _row_logits, _status_error, _written
 
 
 class TokenLogprobs(NamedTuple):
@@ -115,7 +115,8 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], ma
     """Gradient with respect to ``logits`` of ``sum(grad_logprobs * logprobs) +
     sum(grad_entropy * entropy)``, from the forward call's ``max``, ``logsum``
     and (with ``grad_entropy``) ``entropy``. The result has the logits' type.
-    ``out`` may be ``logits`` itself: the gradient then replaces the logits."""
+    ``out`` may be ``logits`` itself: the gradient then replaces the logits (a
+    graph that saved them raises when it goes back through them)."""
     rows = _rows(logits, "logits")
     B, V = rows.shape
     shape, index = rows.shape[:1], rows.get_device()
@@ -128,7 +129,8 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], ma
     if grad_entropy is not None and entropy is None:
         raise ValueError("grad_entropy needs the forward call's entropy")
     entropy = _vector(entropy, torch.float32, shape, index, "entropy")
-    if out is None:
+    given = out is not None
+    if not given:
         out = rows.new_empty((B, V))
     elif out.shape != rows.shape or out.dtype != rows.dtype or out.device != rows.device or \
             out.stride(1) != 1 or (B > 1 and out.stride(0) < V):
@@ -139,6 +141,8 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], ma
             _ptr(temperature), max.data_ptr(), logsum.data_ptr(), _ptr(entropy), _ptr(grad_logprobs),
             _ptr(grad_entropy), out.data_ptr(), out.stride(0) if B > 1 else V)
         _call(rows.device, _lib.load().fg_token_logprobs_grad, a, "fg_token_logprobs_grad")
+        if given:
+            _written(out)
     return out
 
 

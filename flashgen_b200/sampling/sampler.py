@@ -60,6 +60,13 @@ def _call(dev: torch.device, fn, args, what: str) -> None:
         _lib.check(rc, what)
 
 
+def _written(t: torch.Tensor) -> None:
+    """Tell autograd that a kernel wrote to ``t``: a graph that saved it raises
+    instead of going on with what it finds there."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def histories_to_csr(histories: Sequence[Sequence[int]], device) -> Tuple[torch.Tensor, torch.Tensor, int]:
     """Pack per-row token lists into CSR (ids int32, offsets int64) on ``device``."""
     lens = np.fromiter((len(h) for h in histories), dtype=np.int64, count=len(histories))

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from flashgen_b200.sampling.logprobs import logprobs_and_entropy
+from flashgen_b200.sampling.lm_head import AdapterHead
+from flashgen_b200.sampling.logprobs import logprobs_and_entropy, token_logprobs, token_logprobs_grad
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +55,29 @@ def test_one_result_changed_leaves_the_other(cuda_device):
     z = torch.log_softmax(b, 1)
     (-(z.exp() * z).sum()).backward()
     torch.testing.assert_close(a.grad, b.grad, atol=2e-6, rtol=0)
+
+
+def test_a_graph_notices_that_its_logits_were_written(cuda_device):
+    a, t = _case()
+    y = a * 1.0
+    lp, _ = logprobs_and_entropy(y, t)
+    r = token_logprobs(y.detach(), t)
+    token_logprobs_grad(y.detach(), t, r.max, r.logsum, r.logprobs, out=y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        lp.sum().backward()
+    head = AdapterHead(torch.randn(11, 64, device="cuda").half())
+    y = (a * 1.0).half()
+    lp, _ = logprobs_and_entropy(y, t)
+    head.logits(torch.randn(3, 64, device="cuda").half(), out=y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        lp.sum().backward()
+
+
+def test_out_under_inference_mode(cuda_device):
+    with torch.inference_mode():
+        x = torch.randn(3, 11, device="cuda")
+        r = token_logprobs(x)
+        token_logprobs_grad(x, None, r.max, r.logsum, None, entropy=r.entropy, grad_entropy=r.entropy, out=x)
+        head = AdapterHead(torch.randn(11, 64, device="cuda").half())
+        head.logits(torch.randn(3, 64, device="cuda").half(), out=x)
+    assert x.isfinite().all()

@@ -122,7 +122,7 @@ class DecodeBatch:
                     **kwargs) -> torch.Tensor:
         """`step` from the hidden states [B, dim]: the logits are `head`'s, every
         row with its own adapter (`adapters` [B] int32, negative: none)."""
-        return self.step(head.logits(hidden, adapters), **kwargs)
+        return self.step(head.logits(hidden.detach(), adapters), **kwargs)
 
     def _append(self, ids: torch.Tensor) -> None:
         """Append each row's id (skipping error rows, id -1) on the device; a

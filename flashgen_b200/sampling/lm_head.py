@@ -91,11 +91,14 @@ class AdapterHead:
         (``adapters`` [B] int32, negative: none). ``out_dtype`` is the head's
         type (default) or float32. ``check_errors`` reads the row status back
         and raises for slots outside the bank; without it such rows get the
-        shared logits alone."""
+        shared logits alone. There is no backward pass: a ``hidden`` that requires
+        a gradient is refused outside ``torch.no_grad()``."""
         if hidden.dim() != 2 or hidden.shape[1] != self.dim:
             raise ValueError(f"hidden must be [B, {self.dim}], got {tuple(hidden.shape)}")
         if hidden.dtype != self.dtype or hidden.device != self.device:
             raise TypeError(f"hidden must be {self.dtype} on {self.device}, got {hidden.dtype} on {hidden.device}")
+        if hidden.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("AdapterHead.logits has no backward pass: detach hidden or call it under torch.no_grad()")
         B = hidden.shape[0]
         if hidden.stride(1) != 1 or (B > 1 and hidden.stride(0) < self.dim):
             hidden = hidden.contiguous()

@@ -73,7 +73,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     statistics are float32 whatever the logits' type. ``check_errors`` reads
     the status back and raises for NaN, +inf or fully masked rows, bad
     temperatures and tokens outside the vocabulary; without it such rows are
-    marked in ``status``.
+    marked in ``status``. The results carry no gradient:
+    :func:`logprobs_and_entropy` is the differentiable form.
 
     >>> r = token_logprobs(logits, ids, top=5)
     >>> r.logprobs, r.top_ids, r.top_logprobs
@@ -185,9 +186,13 @@ def logprobs_and_entropy(logits: torch.Tensor, tokens: torch.Tensor,
     """Differentiable (with respect to ``logits``) log probabilities of
     ``tokens`` and entropies, both [B] float32: the two terms of a
     policy-gradient loss with an entropy bonus. Differentiable once: a second
-    derivative raises.
+    derivative raises. There is no gradient with respect to ``temperature``: one
+    that requires it is refused.
 
     >>> lp, h = logprobs_and_entropy(logits, tokens)
     >>> (-(advantage * lp) - 0.01 * h).mean().backward()
     """
+    if temperature is not None and temperature.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("logprobs_and_entropy has no gradient with respect to the temperature: detach it, "
+                           "or divide the logits by it")
     return _LogprobsAndEntropy.apply(logits, tokens, temperature)

@@ -66,3 +66,13 @@ def test_a_graph_that_is_not_used_again(stand_ins):
     z = torch.log_softmax(a, 1).gather(1, t[:, None]).sum() + (a ** 3).sum()
     (want,) = torch.autograd.grad(z, a)
     torch.testing.assert_close(g.detach(), want, atol=1e-5, rtol=0)
+
+
+def test_a_learned_temperature_is_refused(stand_ins):
+    a, t = _case()
+    T = torch.ones(3, requires_grad=True)
+    with pytest.raises(RuntimeError, match="temperature"):
+        L.logprobs_and_entropy(a, t, T)
+    lp, _ = L.logprobs_and_entropy(a, t, T.detach())
+    lp.sum().backward()
+    assert a.grad.isfinite().all()

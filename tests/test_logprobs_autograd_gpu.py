@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from flashgen_b200 import SamplingParams
+from flashgen_b200.sampling.decode import DecodeBatch
 from flashgen_b200.sampling.lm_head import AdapterHead
 from flashgen_b200.sampling.logprobs import logprobs_and_entropy, token_logprobs, token_logprobs_grad
 
@@ -81,3 +83,31 @@ def test_out_under_inference_mode(cuda_device):
         head = AdapterHead(torch.randn(11, 64, device="cuda").half())
         head.logits(torch.randn(3, 64, device="cuda").half(), out=x)
     assert x.isfinite().all()
+
+
+def test_gradients_that_do_not_exist_are_refused(cuda_device):
+    a, t = _case()
+    T = torch.ones(3, device="cuda").requires_grad_()
+    with pytest.raises(RuntimeError, match="temperature"):
+        logprobs_and_entropy(a, t, T)
+    with torch.no_grad():
+        logprobs_and_entropy(a, t, T)
+    lp, _ = logprobs_and_entropy(a / T[:, None], t, None)              # the way that the error names
+    lp.sum().backward()
+    assert T.grad.isfinite().all() and (T.grad != 0).any()
+    head = AdapterHead(torch.randn(11, 64, device="cuda").half())
+    hidden = torch.randn(3, 64, device="cuda").half().requires_grad_()
+    with pytest.raises(RuntimeError, match="backward"):
+        head.logits(hidden)
+    want = head.logits(hidden.detach())
+    with torch.no_grad():
+        assert torch.equal(head.logits(hidden), want)
+
+
+def test_a_served_step_takes_hidden_states_that_require_gradients(cuda_device):
+    head = AdapterHead(torch.randn(11, 64, device="cuda").half())
+    hidden = torch.randn(3, 64, device="cuda").half()
+    u = torch.full((3,), 0.5, device="cuda")
+    ids = [DecodeBatch([SamplingParams()] * 3, 11, capacity=4).step_hidden(h, head, uniforms=u, top_logprobs=2).clone()
+           for h in (hidden, hidden.clone().requires_grad_())]
+    assert torch.equal(*ids)

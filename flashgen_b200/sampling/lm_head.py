@@ -49,7 +49,7 @@ class AdapterHead:
         if slots < 0 or not 1 <= rank <= _lib.FG_ADAPTER_MAX_RANK:
             raise ValueError(f"slots must be >= 0 and rank in [1, {_lib.FG_ADAPTER_MAX_RANK}], "
                              f"got {slots} and {rank}")
-        self.weight = _dense_rows(weight)
+        self.weight = _dense_rows(weight.detach())
         self.vocab, self.dim = weight.shape
         self.device, self.dtype = weight.device, weight.dtype
         self.slots, self.rank = int(slots), int(rank)
@@ -65,8 +65,10 @@ class AdapterHead:
             raise IndexError(f"slot {slot} outside [0, {self.slots})")
         return slot
 
+    @torch.no_grad()
     def load(self, slot: int, down: torch.Tensor, up: torch.Tensor, scale: float = 1.0) -> None:
-        """Put an adapter into ``slot`` (on the current stream)."""
+        """Put an adapter into ``slot`` (on the current stream): its values, without
+        its graph."""
         self._slot(slot)
         r = down.shape[0] if down.dim() == 2 else -1
         if down.dim() != 2 or up.dim() != 2 or not 1 <= r <= self.rank or down.shape[1] != self.dim or \

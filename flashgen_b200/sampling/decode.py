@@ -66,10 +66,12 @@ class DecodeBatch:
         self.cumulative_logprob = torch.zeros(self.B, dtype=torch.float32, device=self.device)
 
     def set_history(self, row: int, ids: Sequence[int]) -> None:
-        """Row `row`'s history so far (prompt and generated ids), from the host."""
+        """Row `row`'s history so far (prompt and generated ids), from the host: a
+        request is admitted, and its running log probability starts at 0."""
         t = torch.as_tensor(list(ids)[: self.capacity], dtype=torch.int32)
         self.hist[row, : t.numel()] = t.to(self.device)
         self.lens[row] = t.numel()
+        self.cumulative_logprob[row] = 0.0
 
     def histories(self) -> List[List[int]]:
         """The rows' histories on the host (reads the device state)."""

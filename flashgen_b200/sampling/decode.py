@@ -97,6 +97,7 @@ class DecodeBatch:
         `last_logprobs` holds the drawn ids' log probabilities, ranks and that
         many alternatives, and `cumulative_logprob` grows by them (rows without an
         id, rank -1, add nothing)."""
+        self.last_logprobs = None          # also where this step fails
         assert logits.shape == (self.B, self.V), (logits.shape, self.B, self.V)
         if uniforms is None:
             uniforms = torch.rand(self.B, device=self.device, generator=generator, dtype=torch.float32)
@@ -112,7 +113,6 @@ class DecodeBatch:
             msg = _status_error(self.status)
             if msg is not None:
                 raise RuntimeError(msg)
-        self.last_logprobs = None
         if top_logprobs is not None:
             self.last_logprobs = token_logprobs(logits, ids, top=top_logprobs)
             self.cumulative_logprob += torch.where(ids >= 0, self.last_logprobs.logprobs,

@@ -123,8 +123,11 @@ class DecodeBatch:
     def step_hidden(self, hidden: torch.Tensor, head: AdapterHead, adapters: Optional[torch.Tensor] = None,
                     **kwargs) -> torch.Tensor:
         """`step` from the hidden states [B, dim]: the logits are `head`'s, every
-        row with its own adapter (`adapters` [B] int32, negative: none)."""
-        return self.step(head.logits(hidden.detach(), adapters), **kwargs)
+        row with its own adapter (`adapters` [B] int32, negative: none). With
+        `check_errors` a slot outside the head's bank raises, too."""
+        self.last_logprobs = None
+        logits = head.logits(hidden.detach(), adapters, check_errors=self.check_errors)
+        return self.step(logits, **kwargs)
 
     def _append(self, ids: torch.Tensor) -> None:
         """Append each row's id (skipping error rows, id -1) on the device; a

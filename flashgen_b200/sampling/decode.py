@@ -121,12 +121,13 @@ class DecodeBatch:
         return ids
 
     def step_hidden(self, hidden: torch.Tensor, head: AdapterHead, adapters: Optional[torch.Tensor] = None,
-                    **kwargs) -> torch.Tensor:
+                    out_dtype: Optional[torch.dtype] = None, **kwargs) -> torch.Tensor:
         """`step` from the hidden states [B, dim]: the logits are `head`'s, every
-        row with its own adapter (`adapters` [B] int32, negative: none). With
-        `check_errors` a slot outside the head's bank raises, too."""
+        row with its own adapter (`adapters` [B] int32, negative: none), of the
+        head's type or of `out_dtype` (float32: log probabilities and ties as the
+        sums give them). With `check_errors` a slot outside the head's bank raises, too."""
         self.last_logprobs = None
-        logits = head.logits(hidden.detach(), adapters, check_errors=self.check_errors)
+        logits = head.logits(hidden.detach(), adapters, out_dtype=out_dtype, check_errors=self.check_errors)
         return self.step(logits, **kwargs)
 
     def _append(self, ids: torch.Tensor) -> None:

@@ -43,3 +43,18 @@ def test_bad_adapters_raise_where_errors_are_checked(cuda_device):
     assert dec.last_logprobs is None and [len(h) for h in dec.histories()] == [1, 1, 1]
     ids = DecodeBatch([SamplingParams()] * 3, 500, capacity=8).step_hidden(hidden, head, bad)   # not checked: shared logits
     assert (ids >= 0).all()
+
+
+@pytest.mark.parametrize("out_dtype", [None, torch.float16, torch.float32])
+def test_logits_of_a_step_from_hidden_states(cuda_device, out_dtype):
+    head = _head()
+    hidden = torch.randn(3, 64, device="cuda").half()
+    ad = torch.tensor([0, 1, -1], dtype=torch.int32, device="cuda")
+    u = torch.full((3,), 0.3, device="cuda")
+    a, b = (DecodeBatch([SamplingParams()] * 3, 500, capacity=8) for _ in range(2))
+    ids = a.step_hidden(hidden, head, ad, out_dtype=out_dtype, uniforms=u, top_logprobs=3)
+    assert torch.equal(ids, b.step(head.logits(hidden, ad, out_dtype=out_dtype), uniforms=u, top_logprobs=3))
+    for x, y in zip(a.last_logprobs, b.last_logprobs):
+        assert torch.equal(x, y)
+    with pytest.raises(TypeError):
+        a.step_hidden(hidden, head, ad, out_dtype=torch.bfloat16)

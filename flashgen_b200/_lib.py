@@ -29,7 +29,7 @@ FG_ROW_GREEDY = 0x0200
 EXPORTED_SYMBOLS = ("fg_sample", "fg_sample_workspace_size", "fg_sample_candidates", "fg_sample_noalloc",
                     "fg_sample_set_split",
                     "fg_apply_repetition_penalty", "fg_argmax", "fg_token_logprobs", "fg_token_logprobs_grad",
-                    "fg_adapter_logits", "fg_adapter_workspace_size", "fg_strerror", "fg_version")
+                    "fg_adapter_logits", "fg_adapter_set_wait", "fg_adapter_workspace_size", "fg_strerror", "fg_version")
 
 
 class FgSampleArgs(ctypes.Structure):
@@ -187,6 +187,8 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.fg_token_logprobs_grad.restype = ctypes.c_int
         lib.fg_adapter_logits.argtypes = [ctypes.POINTER(FgAdapterArgs), ctypes.c_void_p]
         lib.fg_adapter_logits.restype = ctypes.c_int
+        lib.fg_adapter_set_wait.argtypes = [ctypes.c_int64, ctypes.c_int32]
+        lib.fg_adapter_set_wait.restype = ctypes.c_int
         lib.fg_adapter_workspace_size.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
         lib.fg_adapter_workspace_size.restype = ctypes.c_size_t
         lib.fg_strerror.argtypes = [ctypes.c_int]

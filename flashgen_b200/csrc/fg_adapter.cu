@@ -68,6 +68,10 @@ Layout layout(int64_t batch, int64_t dim, int64_t rank, int64_t slots) {
 
 constexpr int32_t kMaxRows = 1 << 20;
 
+// fg_adapter_set_wait
+std::atomic<int64_t> g_wait_ns{fg::adapt::DEFAULT_WAIT_NS};
+std::atomic<int32_t> g_withhold{-1};
+
 }  // namespace
 
 extern "C" {
@@ -76,6 +80,14 @@ size_t fg_adapter_workspace_size(int32_t batch, int32_t dim, int32_t rank, int32
     if (batch < 0 || batch > kMaxRows || dim < 1 || slots < 0) return 0;
     if (slots > 0 && (rank < 8 || rank > FG_ADAPTER_MAX_RANK || rank % 8 != 0)) return 0;
     return layout(batch, dim, rank, slots).total;
+}
+
+int fg_adapter_set_wait(int64_t limit_ns, int32_t withhold) {
+    if (limit_ns < 0 || limit_ns > fg::adapt::DEFAULT_WAIT_NS || withhold < -1 || withhold >= fg::adapt::MAX_ACC)
+        return FG_EINVAL;
+    g_wait_ns.store(limit_ns > 0 ? limit_ns : fg::adapt::DEFAULT_WAIT_NS, std::memory_order_relaxed);
+    g_withhold.store(withhold, std::memory_order_relaxed);
+    return FG_OK;
 }
 
 int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
@@ -143,7 +155,9 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
     // (1024 rows, 32768 words: one 264, two 277). A divisor of PIECE_K.
     P.kb = P.nt <= 64 ? 4 : P.nt <= 128 ? 2 : 1;
     P.tmem_cols = 32;
-    P.accs = std::min(8, 512 / P.nt);
+    P.accs = std::min(fg::adapt::MAX_ACC, 512 / P.nt);
+    P.wait_ns = uint64_t(g_wait_ns.load(std::memory_order_relaxed));
+    P.withhold = g_withhold.load(std::memory_order_relaxed);
     while (P.tmem_cols < P.accs * P.nt) P.tmem_cols *= 2;
     if (int64_t(P.nvt) * P.ntile > (1 << 30)) return FG_ENOTSUP;
     CUtensorMap wmap, xmap;

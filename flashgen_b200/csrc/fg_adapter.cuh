@@ -211,6 +211,12 @@ __global__ void __launch_bounds__(DOWN_THREADS) down_kernel(const Params P) {
 // epilogue (two or four per quarter of the accumulator's lanes). Two to eight
 // accumulators in tensor memory: one tile's epilogue runs beside the next products.
 //
+// Every wait is bounded (P.wait_ns). Where one runs out, the CTA (and its pair) stops
+// waiting: the loader and the issuing thread leave off, the epilogue warps write NaN for
+// all that they have not stored, so that nothing unwritten can be taken for logits, one
+// of them marks every row FG_ROW_TIMEOUT, and the CTA waits for its products and copies
+// in flight before it frees the tensor memory and leaves.
+//
 // Bound: HBM up to about 128 rows (the weight, once), the tensor pipe above. Measured
 // (bf16, dim 4096, rank 16): 128256 words, one row 161 us (6.5 TB/s of weight), 64 rows of 32
 // adapters 197 us (5.3 TB/s); 32768 words, 1024 rows 260 us (1.06 PFLOP/s; SM clock held to
@@ -247,8 +253,6 @@ struct Epilogue {
 };
 constexpr int PIECE_K = 8;                         // 64-wide steps of K per piece of an fp32 sum
 
-constexpr int MAX_ACC = 8;   // accumulators in tensor memory
-
 // Barrier over `threads` threads that also tells all of them whether any had `p`.
 __device__ __forceinline__ bool named_any(int id, int threads, bool p) {
     uint32_t r;
@@ -262,7 +266,8 @@ struct Control {
     uint64_t full[MAX_STAGES], empty[MAX_STAGES];
     uint64_t acc_full[MAX_ACC], acc_empty[MAX_ACC], drain;
     uint32_t tmem;
-    int abort;
+    int abort;      // someone's wait ran out: everyone stops waiting
+    int reported;   // the rows' status words say so
 };
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -370,6 +375,7 @@ struct Windows {
     // others, whose instructions interleave).
     __device__ __forceinline__ static void add_last(float (&x)[2][4], UpTile<RC>& tile, const Params& P, const uint2* src,
                                                     int slots, int v0, float unit0, float unit1, int lane) {
+        asm volatile("mov.u32 %0, %%laneid;" : "=r"(lane));   // (anew: nothing is kept for this path)
         const int t = lane & 3;
         uint32_t left = __ballot_sync(ALL, slots >= 0) & 0xffu;
         while (left) {
@@ -605,6 +611,17 @@ __device__ __forceinline__ void store_window(const Params& P, uint32_t base, int
     }
 }
 
+// NaN in the place of window w, whose products did not come.
+template <int ODT, int RC>
+__device__ __forceinline__ void store_nan(const Params& P, int b0, int rows, int w, int v0, int lane) {
+    if (v0 + lane >= P.vocab) return;
+#pragma unroll 1
+    for (int p = 8 * w; p < min(rows, 8 * w + 8); ++p) {
+        const int row = RC > 0 ? P.order[b0 + p] & 511 : p;
+        Elem<ODT>::store(P.out, int64_t(b0 + row) * P.out_stride + v0 + lane, __int_as_float(0x7fc00000));
+    }
+}
+
 // RC: rank / 16 held in registers (rounded up to 1, 2, 4 or 8), 0: no adapters.
 // SMALL: fp32 results and a batch tile of at most SMALL_NT columns.
 template <int CG, int DT, int ODT, int RC, bool SMALL>
@@ -631,11 +648,11 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             mbar_init(&C.empty[s], 1);
         }
         for (int i = 0; i < P.accs; ++i) {
-            mbar_init(&C.acc_full[i], 1);
+            mbar_init(&C.acc_full[i], i == P.withhold ? 2 : 1);
             mbar_init(&C.acc_empty[i], CG * EPI_WARPS);
         }
         mbar_init(&C.drain, 1);
-        C.abort = 0;
+        C.abort = C.reported = 0;
         fence_mbar_init();
         tc::prefetch_map(&wmap);
         tc::prefetch_map(&xmap);
@@ -651,6 +668,11 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     // down_kernel began after everything before it had ended; without it, wait for that here
     if (!P.chained) tc::wait_prerequisites();
 
+    auto give_up = [&]() {   // (the pair's other CTA cannot go on alone)
+        *reinterpret_cast<volatile int*>(&C.abort) = 1;
+        if (CG == 2) tc::store_cluster(tc::mapa(&C.abort, rank ^ 1), 1);
+    };
+    int filled = 0;   // stages that the loader has filled
     if (warp == 0) {
         if (lane == 0) {
             const uint32_t ring_a = smem_u32(ring);
@@ -662,7 +684,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                 const int v0 = ((t / P.ntile) * CG + rank) * TILE_V;
                 const int b0 = (t % P.ntile) * P.nt + rank * (P.nt / CG);
                 for (int kc = 0; kc < nk; kc += P.kb) {
-                    if (used == S && !mbar_wait(&C.empty[stage], parity, &C.abort)) { ok = false; break; }
+                    if (used == S && !mbar_wait(&C.empty[stage], parity, &C.abort, P.wait_ns)) { ok = false; break; }
                     const int boxes = min(P.kb, nk - kc);
                     uint32_t a = ring_a + stage * stage_bytes;
                     if (used < S) {
@@ -691,18 +713,14 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                     for (int q = 0; q < boxes; ++q)
                         tc::tma_load_2d<CG>(a + q * box_bytes + A_BYTES, &xmap, (kc + q) * TILE_K, b0,
                                             full0 + 8 * stage);
+                    ++filled;
                     if (++stage == S) {
                         stage = 0;
                         parity ^= 1;
                     }
                 }
             }
-            if (!ok) {
-                // gave up: let the copies in flight land before the block leaves (the pair's
-                // barriers are the first CTA's, so this is a wait by time)
-                *reinterpret_cast<volatile int*>(&C.abort) = 1;
-                for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 10000000;) {}
-            }
+            if (!ok) give_up();
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
@@ -714,11 +732,11 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             for (int t = first; t < tiles && ok; t += step) {
                 for (int k0 = 0; k0 < nk && ok; k0 += piece) {
                     const int k1 = min(nk, k0 + piece);
-                    if (!mbar_wait(&C.acc_empty[acc], acc_parity, &C.abort)) { ok = false; break; }
+                    if (!mbar_wait(&C.acc_empty[acc], acc_parity, &C.abort, P.wait_ns)) { ok = false; break; }
                     tc::fence_after();
                     const uint32_t d = tmem + acc * P.nt;
                     for (int kc = k0; kc < k1; kc += P.kb) {
-                        if (!mbar_wait(&C.full[stage], parity, &C.abort)) { ok = false; break; }
+                        if (!mbar_wait(&C.full[stage], parity, &C.abort, P.wait_ns)) { ok = false; break; }
                         tc::fence_after();
                         const int boxes = min(P.kb, k1 - kc);
                         uint64_t ad = desc0 + uint32_t(stage * stage_bytes) / 16;
@@ -741,11 +759,10 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                     }
                 }
             }
-            if (!ok) {
-                *reinterpret_cast<volatile int*>(&C.abort) = 1;
-                tc::commit<CG>(&C.drain);
-                mbar_wait_for(&C.drain, 0, WAIT_LIMIT_NS);
-            }
+            if (!ok) give_up();
+            // no product is in flight when this thread is done, whatever the others made of them
+            tc::commit_here<CG>(&C.drain);
+            mbar_wait_for(&C.drain, 0, WAIT_LIMIT_NS);
         }
     } else {
         const int quarter = warp & 3, part = (warp - 2) >> 2;   // of PARTS
@@ -766,8 +783,12 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             }
         };
         tc::wait_prerequisites();   // U, the order and the status words come from down_kernel
-        bool ok = true;
-        for (int t = first; t < tiles && ok; t += step) {
+        // a wait of the whole warp: all lanes go on or none
+        auto products_done = [&]() {
+            return __all_sync(0xffffffffu, mbar_wait(&C.acc_full[acc], acc_parity, &C.abort, P.wait_ns)) != 0;
+        };
+        bool gone = false;   // gave up
+        for (int t = first; t < tiles; t += step) {
             const int v = ((t / P.ntile) * CG + rank) * TILE_V + quarter * 32 + lane, b0 = (t % P.ntile) * P.nt;
             const int rows = min(P.nt, P.batch - b0);
             const int windows = (rows + 7) / 8, w0 = windows * part / PARTS, w1 = windows * (part + 1) / PARTS;
@@ -780,6 +801,12 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             W win;
             float add[EARLY > 0 ? EARLY : 1][2][4];
             int ents[EARLY > 0 ? EARLY : 1];
+            if (gone) {
+                if (vw < P.vocab)
+                    for (int w = w0; w < w1; ++w) store_nan<ODT, RC>(P, b0, rows, w, vw, lane);
+                continue;
+            }
+            bool ok = true;
             if constexpr (EARLY > 0) {
                 if (vw < P.vocab) {
 #pragma unroll
@@ -795,7 +822,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                 for (int i = 0; i < SUMS; ++i) sum[i] = 0.0f;
                 uint32_t at = 0;
                 for (int k0 = 0; k0 < nk; k0 += piece) {
-                    ok = mbar_wait(&C.acc_full[acc], acc_parity, &C.abort);
+                    ok = products_done();
                     if (!ok) break;
                     tc::fence_after();
                     at = lanes + acc * P.nt + part * 8;
@@ -823,14 +850,19 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                 ok = !named_any(1 + quarter, 32 * PARTS, !ok);
                 tc::fence_after();
             } else {
-                ok = mbar_wait(&C.acc_full[acc], acc_parity, &C.abort);
+                ok = products_done();
                 tc::fence_after();
             }
             if (!ok) {
-                *reinterpret_cast<volatile int*>(&C.abort) = 1;
-                if (P.out_status && threadIdx.x == 64)
-                    for (int i = 0; i < rows; ++i) atomicOr(&P.out_status[b0 + i], FG_ROW_TIMEOUT);
-                break;
+                gone = true;
+                if (lane == 0) {
+                    give_up();
+                    if (P.out_status && atomicExch(&C.reported, 1) == 0)
+                        for (int i = 0; i < P.batch; ++i) atomicOr(&P.out_status[i], FG_ROW_TIMEOUT);
+                }
+                __syncwarp();
+                t -= step;   // this tile again, as what was not stored
+                continue;
             }
             const uint32_t base = lanes + acc * P.nt;
             if (vw < P.vocab) {
@@ -857,6 +889,16 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     }
     tc::fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *reinterpret_cast<volatile int*>(&C.abort)) {
+        // the copies in flight land before the CTA leaves. A pair's loads are counted on the
+        // first CTA's barriers, to which both may not have brought all: a wait by time
+        if (CG == 1)
+            for (int s = 0; s < min(S, filled); ++s)
+                mbar_wait_for(&C.full[s], ((filled - 1 - s) / S) & 1, WAIT_LIMIT_NS);
+        else
+            for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 10000000;) {}
+    }
+    __syncwarp();
     if (CG == 2) tc::cluster_sync();   // no CTA leaves while its pair may still signal it
     if (warp == 1) {
         tc::fence_after();

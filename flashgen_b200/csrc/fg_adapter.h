@@ -12,6 +12,8 @@ namespace adapt {
 constexpr int TILE_V = 128, TILE_K = 64;   // accumulator lanes; elements of a K step (128 bytes)
 constexpr int MAX_NT = 256;                // batch columns of a tile
 constexpr int SMALL_NT = 64;
+constexpr int MAX_ACC = 8;                 // accumulators in tensor memory
+constexpr int64_t DEFAULT_WAIT_NS = 1000000000;   // limit of a wait: 1 s, far above any legitimate one
 
 struct Params {
     const void* hidden;       // rows for the products: the caller's, or the aligned copy
@@ -41,6 +43,8 @@ struct Params {
     int32_t accs;             // accumulators of nt columns in tensor memory
     int32_t tmem_cols;
     int32_t chained;          // down_kernel goes before
+    int32_t withhold;         // accumulator whose products are never reported (tests), or -1
+    uint64_t wait_ns;         // limit of each wait
 };
 
 // Both launches of a call: operands of type DT, result of type ODT. `pair`: two

@@ -148,16 +148,17 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
                  : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
     return ok != 0;
 }
-// Wait for phase `parity` of `bar` to complete. Gives up after WAIT_LIMIT_NS or
+// Wait for phase `parity` of `bar` to complete. Gives up after limit_ns or
 // as soon as *abort is set; returns false in that case.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                          uint64_t limit_ns = WAIT_LIMIT_NS) {
     if (mbar_test(bar, parity)) return true;
     uint64_t t0 = globaltimer_ns();
     for (uint32_t it = 0;; ++it) {
         if (mbar_test(bar, parity)) return true;
         if ((it & 63u) == 63u) {
             if (*abort) return false;
-            if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) return false;
+            if (globaltimer_ns() - t0 > limit_ns) return false;
         }
     }
 }

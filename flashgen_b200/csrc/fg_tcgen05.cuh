@@ -105,6 +105,15 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
             "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
             :: "r"(smem_u32(bar)), "h"(uint16_t(3)) : "memory");
 }
+// The same on this CTA's barrier alone.
+template <int CG>
+__device__ __forceinline__ void commit_here(uint64_t* bar) {
+    if constexpr (CG == 1)
+        commit<1>(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                     :: "r"(smem_u32(bar)) : "memory");
+}
 
 // ---- the pair --------------------------------------------------------------
 __device__ __forceinline__ uint32_t cta_rank() {
@@ -120,6 +129,9 @@ __device__ __forceinline__ uint32_t mapa(const void* p, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
     return a;
+}
+__device__ __forceinline__ void store_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" :: "r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(bar) : "memory");

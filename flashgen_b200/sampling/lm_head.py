@@ -93,7 +93,9 @@ class AdapterHead:
         (``adapters`` [B] int32, negative: none). ``out_dtype`` is the head's
         type (default) or float32. ``check_errors`` reads the row status back
         and raises for slots outside the bank; without it such rows get the
-        shared logits alone. There is no backward pass: a ``hidden`` that requires
+        shared logits alone. (A wait in the kernel that runs out raises, too;
+        unchecked, what was not computed is NaN, which the sampler marks.) There is
+        no backward pass: a ``hidden`` that requires
         a gradient is refused outside ``torch.no_grad()``."""
         if hidden.dim() != 2 or hidden.shape[1] != self.dim:
             raise ValueError(f"hidden must be [B, {self.dim}], got {tuple(hidden.shape)}")

@@ -339,6 +339,9 @@ int fg_token_logprobs_grad(const FgLogprobGradArgs* args, void* stream);
  * FG_ADAPTER_MAX_RANK (an adapter of lower rank has zero rows of down or zero
  * columns of up). hidden and out need only the alignment of their elements.
  *
+ * Every wait in the kernels is bounded. Where one runs out (1 s), what was not
+ * computed is NaN and every row's out_status has FG_ROW_TIMEOUT.
+ *
  * Workspace: fg_adapter_workspace_size bytes, 256-byte aligned, written and read
  * within the call (no initial value). Calls that may run concurrently need
  * separate workspaces.
@@ -374,6 +377,15 @@ typedef struct FgAdapterArgs {
 } FgAdapterArgs;
 
 int fg_adapter_logits(const FgAdapterArgs* args, void* stream);
+
+/*
+ * For tests of that report: the limit of each wait of the calls from now on
+ * (nanoseconds up to 10^9; 0: the default, 10^9), and an accumulator (0 .. 7) whose
+ * products are computed but never reported, so that the wait for them runs out
+ * (-1: none, the default). Process-wide (atomics, read once per call); FG_EINVAL
+ * for other values.
+ */
+int fg_adapter_set_wait(int64_t limit_ns, int32_t withhold);
 
 /* Bytes of workspace of fg_adapter_logits; 0 for an invalid shape. Host-only. */
 size_t fg_adapter_workspace_size(int32_t batch, int32_t dim, int32_t rank, int32_t slots);

@@ -708,8 +708,10 @@ __device__ __forceinline__ void finish_row(const Params& P, Shared& sh, ClusterS
     if (part != 0) return;
     const float l2 = log2f(all.s);
     const float nan = __int_as_float(0x7fc00000);
+    // one expression for the token and the alternatives: the same id has the same bits
+    auto logprob = [&](float x) { return __fmaf_rn(-LN2, l2, __fdiv_rn(x - m, T)); };
     if (tid == 0) {
-        const float lpt = row.tok < 0 ? 0.0f : empty ? -INFINITY : (row.xt - m) / T - LN2 * l2;
+        const float lpt = row.tok < 0 ? 0.0f : empty ? -INFINITY : logprob(row.xt);
         if (P.out_logprobs) P.out_logprobs[r] = bad ? nan : lpt;
         if (P.out_entropy) P.out_entropy[r] = bad ? nan : empty ? 0.0f : LN2 * (l2 - all.q / all.s);
         if (P.out_max) P.out_max[r] = m;
@@ -718,13 +720,12 @@ __device__ __forceinline__ void finish_row(const Params& P, Shared& sh, ClusterS
         if (P.out_status) P.out_status[r] = status;
     }
     if (TOP) {
-        const float per_t = 1.0f / T;
         auto write = [&](int i, bool none, uint64_t code) {
             const float x = funkey(uint32_t(code >> 32));
             if (P.out_top_ids) P.out_top_ids[r * P.top + i] = (none || bad) ? -1 : int64_t(uint32_t(~uint32_t(code)));
             if (P.out_top_logprobs)
                 P.out_top_logprobs[r * P.top + i] =
-                    bad ? nan : (none || x == -INFINITY) ? -INFINITY : (x - m) * per_t - LN2 * l2;
+                    bad ? nan : (none || x == -INFINITY) ? -INFINITY : logprob(x);
         };
         if constexpr (CLUSTER) {
             // G lists in order, an entry a thread

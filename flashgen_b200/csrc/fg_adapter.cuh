@@ -226,11 +226,13 @@ __global__ void __launch_bounds__(DOWN_THREADS) down_kernel(const Params P) {
 // (down_kernel's launch and the adapters' bytes; their rows fetched ahead of the epilogue,
 // to L2 or to shared memory by a warp of its own, gained nothing).
 //
-// fp32 results: the tensor core truncates when it adds a product to the
-// accumulator, and over hundreds of steps that bias shows in 32 bits. So the sum
-// over K is taken in pieces of PIECE_K, one accumulator each, and the epilogue warps
-// add the pieces in registers with rounding. A 16-bit
-// result does not see the difference and takes the whole sum in one piece.
+// The tensor core truncates when it adds products to the accumulator: over n elements
+// of one sign the sum loses about 0.05 n units of 2^-23. So the sum over K is taken in
+// pieces, one accumulator each, that the epilogue warps add with rounding. fp32 results
+// take pieces of PIECE_K steps and keep the sum in registers. For 16-bit results pieces of
+// LONG_K lose an eighth of half a unit of f16 at most (of one sign; a few 10^-6 of the
+// results' norm otherwise, by which one in 400 rounds to the other neighbour); the epilogue
+// adds a long dim's pieces in tensor memory, each to the next.
 // ---------------------------------------------------------------------------
 constexpr int A_BYTES = TILE_V * TILE_K * 2;
 constexpr int MAX_STAGES = 12;
@@ -251,7 +253,7 @@ struct Epilogue {
     static constexpr int COLUMNS = SMALL ? SMALL_NT : MAX_NT;
     static constexpr int SUMS = (COLUMNS / 8 + WARPS / 4 - 1) / (WARPS / 4) * 8;   // a warp's share, in eights
 };
-constexpr int PIECE_K = 8;                         // 64-wide steps of K per piece of an fp32 sum
+constexpr int PIECE_K = 8, LONG_K = 64;            // 64-wide steps of K per piece: of fp32 results, of 16-bit ones
 
 // Barrier over `threads` threads that also tells all of them whether any had `p`.
 __device__ __forceinline__ bool named_any(int id, int threads, bool p) {
@@ -613,7 +615,9 @@ __device__ __forceinline__ void store_window(const Params& P, uint32_t base, int
 
 // NaN in the place of window w, whose products did not come.
 template <int ODT, int RC>
-__device__ __forceinline__ void store_nan(const Params& P, int b0, int rows, int w, int v0, int lane) {
+__device__ __forceinline__ void store_nan(const Params& P, int b0, int rows, int w, int v0) {
+    int lane;
+    asm volatile("mov.u32 %0, %%laneid;" : "=r"(lane));   // (anew: nothing is kept for this path)
     if (v0 + lane >= P.vocab) return;
 #pragma unroll 1
     for (int p = 8 * w; p < min(rows, 8 * w + 8); ++p) {
@@ -638,7 +642,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
     const int box_bytes = A_BYTES + P.nt / CG * TILE_K * 2;   // one 64-wide step of K, this CTA's part
     const int stage_bytes = P.kb * box_bytes;
     const int nk = (P.dim + TILE_K - 1) / TILE_K;
-    const int piece = PIECES ? PIECE_K : nk;
+    const int piece = PIECES ? PIECE_K : LONG_K;
     const int tiles = P.nvt * P.ntile;
     const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
@@ -770,17 +774,23 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
         const uint32_t empty_bar = CG == 2 ? tc::mapa(&C.acc_empty[0], 0) : smem_u32(&C.acc_empty[0]);
         int acc = 0;
         uint32_t acc_parity = 0;
-        auto release = [&]() {   // the accumulator at hand is read; on to the next
+        auto free_acc = [&](int which) {   // an accumulator is read
             tc::fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (CG == 2) tc::arrive_cluster(empty_bar + 8 * acc);
-                else mbar_arrive_a(empty_bar + 8 * acc);
+                if (CG == 2) tc::arrive_cluster(empty_bar + 8 * which);
+                else mbar_arrive_a(empty_bar + 8 * which);
             }
+        };
+        auto next_acc = [&]() {
             if (++acc == P.accs) {
                 acc = 0;
                 acc_parity ^= 1;
             }
+        };
+        auto release = [&]() {   // the accumulator at hand is read; on to the next
+            free_acc(acc);
+            next_acc();
         };
         tc::wait_prerequisites();   // U, the order and the status words come from down_kernel
         // a wait of the whole warp: all lanes go on or none
@@ -803,7 +813,7 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
             int ents[EARLY > 0 ? EARLY : 1];
             if (gone) {
                 if (vw < P.vocab)
-                    for (int w = w0; w < w1; ++w) store_nan<ODT, RC>(P, b0, rows, w, vw, lane);
+                    for (int w = w0; w < w1; ++w) store_nan<ODT, RC>(P, b0, rows, w, vw);
                 continue;
             }
             bool ok = true;
@@ -847,6 +857,34 @@ project_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__
                 }
                 tc::fence_before();
                 // the warps of this quarter of the lanes, which go on or give up together
+                ok = !named_any(1 + quarter, 32 * PARTS, !ok);
+                tc::fence_after();
+            } else if (!PIECES && nk > piece) {
+                // this warp's columns of each piece take what the one before it holds
+                int before = -1;
+                for (int k0 = 0; k0 < nk; k0 += piece) {
+                    ok = products_done();
+                    if (!ok) break;
+                    tc::fence_after();
+                    if (before >= 0) {
+#pragma unroll 1
+                        for (int i = part * 8; i < P.nt; i += 8 * PARTS) {
+                            float x[8], y[8];
+                            tc::tmem_ld8(x, lanes + acc * P.nt + i);
+                            tc::tmem_ld8(y, lanes + before * P.nt + i);
+                            tc::tmem_wait_ld(x);
+                            tc::tmem_wait_ld(y);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) x[j] += y[j];
+                            tc::tmem_st8(x, lanes + acc * P.nt + i);
+                        }
+                        tc::tmem_wait_st();
+                        free_acc(before);
+                    }
+                    before = acc;
+                    if (k0 + piece < nk) next_acc();
+                }
+                tc::fence_before();
                 ok = !named_any(1 + quarter, 32 * PARTS, !ok);
                 tc::fence_after();
             } else {

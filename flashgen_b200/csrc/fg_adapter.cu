@@ -109,6 +109,11 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
     const size_t need = fg_adapter_workspace_size(a->batch, a->dim, a->rank, a->slots);
     if (a->workspace == nullptr || !aligned(a->workspace, 256) || a->workspace_bytes < need) return FG_EINVAL;
     if (a->batch == 0) return FG_OK;
+    const int64_t osz = elem_size(a->out_dtype);
+    const fg::host::Rows out{a->out, a->batch, a->out_stride * osz, a->vocab * osz};
+    if (fg::host::rows_meet(out, {a->hidden, a->batch, a->hidden_stride * 2, int64_t(a->dim) * 2}) ||
+        fg::host::rows_meet(out, {a->weight, a->vocab, a->weight_stride * 2, int64_t(a->dim) * 2}))
+        return FG_EINVAL;
     DevInfo* d = nullptr;
     const int rc = fg::host::device_info(&d);
     if (rc != FG_OK) return rc;

@@ -44,6 +44,27 @@ inline int elem_size(int dtype) {
         default: return 0;
     }
 }
+// `rows` rows of `bytes` bytes, `stride` bytes apart.
+struct Rows {
+    const void* p;
+    int64_t rows, stride, bytes;
+};
+// Whether a row of one shares memory with a row of the other (no more than arithmetic
+// on the ends unless the ranges they span meet).
+inline bool rows_meet(const Rows& a, const Rows& b) {
+    if (a.rows <= 0 || b.rows <= 0) return false;
+    const int64_t d = int64_t(reinterpret_cast<uintptr_t>(b.p) - reinterpret_cast<uintptr_t>(a.p));   // b against a
+    if (d >= (a.rows - 1) * a.stride + a.bytes || -d >= (b.rows - 1) * b.stride + b.bytes) return false;
+    for (int64_t i = 0; i < a.rows; ++i) {
+        const int64_t at = i * a.stride - d;         // row i of a from b's start on
+        if (at + a.bytes <= 0) continue;
+        // the last row of b that begins before the end of this one
+        int64_t j = b.stride > 0 ? (at + a.bytes - 1) / b.stride : 0;
+        if (j >= b.rows) j = b.rows - 1;
+        if (j * b.stride + b.bytes > at) return true;
+    }
+    return false;
+}
 inline int bits_for(int64_t v) {  // smallest b >= 1 with v <= 2^b
     int b = 1;
     while ((int64_t(1) << b) < v) ++b;

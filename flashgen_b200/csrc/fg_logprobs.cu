@@ -159,6 +159,12 @@ int fg_token_logprobs_grad(const FgLogprobGradArgs* a, void* stream) {
     P.tokens = a->tokens; P.temperature = a->temperature; P.max = a->max; P.logsum = a->logsum;
     P.entropy = a->entropy; P.grad_logprobs = a->grad_logprobs; P.grad_entropy = a->grad_entropy;
     P.out_grad = a->out_grad; P.grad_stride = a->grad_stride;
+    // the logits themselves may become the gradient (each thread reads what it writes), a
+    // part of them may not
+    const int64_t esz = elem_size(a->dtype), wide = a->vocab * esz;
+    if (a->out_grad != a->logits && fg::host::rows_meet({a->logits, a->batch, a->row_stride * esz, wide},
+                                                        {a->out_grad, a->batch, a->grad_stride * esz, wide}))
+        return FG_EINVAL;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (a->dtype) {
         case FG_DTYPE_F32: return launch_grad<FG_DTYPE_F32>(P, a->batch, st);

@@ -117,7 +117,8 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], ma
     sum(grad_entropy * entropy)``, from the forward call's ``max``, ``logsum``
     and (with ``grad_entropy``) ``entropy``. The result has the logits' type.
     ``out`` may be ``logits`` itself: the gradient then replaces the logits (a
-    graph that saved them raises when it goes back through them)."""
+    graph that saved them raises when it goes back through them). One that
+    shares memory with a part of them is refused."""
     rows = _rows(logits, "logits")
     B, V = rows.shape
     shape, index = rows.shape[:1], rows.get_device()

@@ -292,7 +292,8 @@ int fg_token_logprobs(const FgLogprobArgs* args, void* stream);
  *
  * computed in fp32 from the saved max, logsum and (with grad_entropy) entropy H
  * and rounded once to the logits' type. out_grad may be the logits buffer
- * itself (same pointer and stride): the gradient then replaces the logits. A
+ * itself (same pointer and stride): the gradient then replaces the logits; rows
+ * that share memory with the logits in any other way are FG_EINVAL. A
  * row with g = h = 0 and a row that is all -inf have gradient 0; a row whose
  * forward results are NaN has NaN.
  */
@@ -337,7 +338,8 @@ int fg_token_logprobs_grad(const FgLogprobGradArgs* args, void* stream);
  * adapters, up [slots, vocab, rank] dense. All three 16-byte aligned, the
  * strides multiples of 8 elements, rank a multiple of 8 up to
  * FG_ADAPTER_MAX_RANK (an adapter of lower rank has zero rows of down or zero
- * columns of up). hidden and out need only the alignment of their elements.
+ * columns of up). hidden and out need only the alignment of their elements; rows of
+ * out that share memory with rows of hidden or weight are FG_EINVAL.
  *
  * Every wait in the kernels is bounded. Where one runs out (1 s), what was not
  * computed is NaN and every row's out_status has FG_ROW_TIMEOUT.

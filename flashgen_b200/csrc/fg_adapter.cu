@@ -131,10 +131,14 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
     P.batch = a->batch; P.dim = a->dim; P.vocab = a->vocab; P.rank = a->rank; P.slots = a->slots;
     P.down_stride = a->down_stride; P.out_stride = a->out_stride; P.copy_stride = L.copy_stride;
     // Sorting costs a copy of the hidden rows that the products wait for; it saves fetches of
-    // adapters and products with them. Dim 2048, V 32000, 32 adapters of rank 16: 32 rows 36.8
-    // us sorted, 34.7 not; 48 rows 37.8, 37.0; 64 rows 38.4, 40.2 (with 4 adapters 35.0, 33.9;
-    // fp32 results, V 50257, 16 adapters 53, 61); 96 rows 41.8, 45.6. TMA reads rows that
-    // start on 16-byte boundaries: others are copied first too.
+    // adapters and products with them. Microseconds sorted and not, rank 16, 16-bit results,
+    // with 1, 4 and 32 adapters: dim 2048, V 32000, 32 rows 34.9 29.3, 35.4 29.2, 36.9 35.3; 48
+    // rows 35.1 33.7, 35.4 34.0, 37.8 37.3; 64 rows 35.1 33.9, 35.6 34.2, 38.7 40.9; 96 rows 38.0
+    // 37.8, 38.3 39.2, 43.0 46.8; V 50257, 128 rows 55.6 55.3, 55.9 58.6, 65.4 82.7; dim 4096, V
+    // 32768, 256 rows 86.9 84.2, 86.9 90.8, 91.5 119; V 128256, 64 rows 185 184, 187 185, 200 197.
+    // How many adapters a batch names is known on the device only: up to 64 rows of few
+    // adapters lose 1.5 us by the rule. TMA reads rows that start on 16-byte boundaries:
+    // others are copied first too.
     P.sorted = a->slots > 0 && a->adapters != nullptr && a->batch > 48;
     const bool copy = P.sorted || !aligned(a->hidden, 16) || (a->batch > 1 && a->hidden_stride % 8 != 0);
     P.wide_out = aligned(a->out, 16) && (a->batch == 1 || a->out_stride * elem_size(a->out_dtype) % 16 == 0);

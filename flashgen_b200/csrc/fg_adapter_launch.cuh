@@ -74,7 +74,9 @@ int launch_rank(const Params& P, const CUtensorMap& wmap, const CUtensorMap& xma
         if (cudaLaunchKernelEx(&cfg, down_kernel<DT, RC ? RC : 1>, P) != cudaSuccess) return FG_ELAUNCH;
     }
     if (pair) return launch_project<2, DT, ODT, RC, false>(P, wmap, xmap, first, d, st);
-    // (ranks 17 to 32 do better with more warps: 50 rows, dim 2048, V 50257: 52 against 55 us)
+    // (Ranks 17 to 32 do better with more warps around 32 rows: dim 2048, V 50257, rank 32, 32
+    // rows 52 us against 58, rank 20 51 against 55; 50 and 64 rows differ by less than their
+    // spread, 8 and 16 rows lose one to three: dim 4096, V 32000, 16 rows 60.2 against 58.6)
     if constexpr (ODT == FG_DTYPE_F32 && RC != 2)
         if (P.nt <= SMALL_NT) return launch_project<1, DT, ODT, RC, true>(P, wmap, xmap, first, d, st);
     return launch_project<1, DT, ODT, RC, false>(P, wmap, xmap, first, d, st);

@@ -20,8 +20,8 @@ constexpr int32_t kMaxRows = 1 << 30;
 // CTAs per row for a batch too small to fill the machine with one each: as many as
 // find room at once (three an SM), with at least two chunks for each of their threads.
 // Clusters of eight find room less easily. With four an SM instead: 256 rows of 32000
-// f16 logits 14.4 us, not 12.4; eight CTAs a row for 50 rows of 128256 bf16 logits: 18.5 us,
-// four 14.4; one CTA for a row of 256000 f32 logits: 33.6 us, eight 12.4.
+// f16 logits 12.0 us, not 10.9; eight CTAs a row for 50 rows of 128256 bf16 logits: 13.7 us,
+// four 11.7; one CTA for a row of 256000 f32 logits: 32 us, eight 9.6.
 int ctas_per_row(int32_t batch, int vocab, int elem, const DevInfo* d) {
     const int64_t chunks = int64_t(vocab) * elem / 16;
     int G = 1;
@@ -91,8 +91,10 @@ int launch_grad(const fg::lp::GradParams& P, int32_t batch, cudaStream_t st) {
     DevInfo* d = nullptr;
     const int rc = fg::host::device_info(&d);
     if (rc != FG_OK) return rc;
-    // steps of GRAD_THREADS * GRAD_UNROLL chunks: one a CTA while they do not fill the
-    // machine, up to four a CTA when there are many
+    // steps of GRAD_THREADS * GRAD_UNROLL chunks: one a CTA while there are fewer than eight
+    // for an SM, up to four a CTA when there are many (five CTAs are resident with 16-bit
+    // logits, six with fp32; cut for five instead, 100, 333 and 500 rows of 32001 and 64 and
+    // 1024 of 128256 logits take the same time)
     const int64_t esz = fg::Elem<DT>::SIZE;
     const int64_t step = int64_t(fg::lp::GRAD_THREADS) * fg::lp::GRAD_UNROLL * 16 / esz;
     const int64_t steps = (P.vocab + step - 1) / step;

@@ -35,8 +35,11 @@ class AdapterHead:
     >>> head.load(3, down, up, scale=alpha / r)          # down [r, dim], up [V, r], r <= rank
     >>> logits = head.logits(hidden, adapters)           # [B, dim], [B] int32 -> [B, V]
 
-    ``weight`` is used where it lies when its rows are 16-byte aligned and
-    copied once otherwise; adapters are copied into the bank.
+    ``weight`` is used where it lies when its rows are 16-byte aligned: later
+    in-place updates of it reach the head. Otherwise (an odd ``dim``, a sliced or
+    transposed weight) it is laid out anew once, which takes its memory a second
+    time, and the head keeps that snapshot: build a new head after an update.
+    Adapters are copied into the bank.
     """
 
     def __init__(self, weight: torch.Tensor, slots: int = 0, rank: int = 16):

@@ -88,8 +88,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     tokens = _vector(tokens, torch.int64, shape, index, "tokens")
     temperature = _vector(temperature, torch.float32, shape, index, "temperature")
     dev = logits.device
-    logprobs = logits.new_empty(B, dtype=torch.float32)   # (results that autograd hands out are no views)
-    entropy, peak, logsum, rank, status = logits.new_empty((5, B), dtype=torch.float32).unbind(0)
+    logprobs, entropy, peak, logsum, rank, status = logits.new_empty((6, B), dtype=torch.float32).unbind(0)
     rank, status = rank.view(torch.int32), status.view(torch.int32)
     top_ids = top_lp = None
     if top > 0:
@@ -167,7 +166,9 @@ class _LogprobsAndEntropy(torch.autograd.Function):
         r = token_logprobs(logits, tokens, temperature=temperature)
         ctx.save_for_backward(logits, tokens, temperature, r.max, r.logsum, r.entropy)
         ctx.set_materialize_grads(False)
-        return r.logprobs, r.entropy.clone()   # (the saved one stays as it is whatever the caller does)
+        # the caller may change both in place: neither is a view (set_ shares the memory, of which
+        # nothing else is read), and the entropy that is saved stays as it is
+        return r.logprobs.new_empty(0).set_(r.logprobs), r.entropy.clone()
 
     @staticmethod
     def backward(ctx, grad_logprobs, grad_entropy):

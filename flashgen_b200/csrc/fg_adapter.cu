@@ -148,9 +148,9 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
     P.hidden_stride = copy || a->batch == 1 ? L.copy_stride : a->hidden_stride;
     // batch tiles of equal width, at most 256 columns
     P.ntile = (a->batch + fg::adapt::MAX_NT - 1) / fg::adapt::MAX_NT;
-    // Two SMs share a product above 128 columns (dim 4096, 32768 words: 1024 rows 264 us
-    // against 268 with one SM each; dim 2048, 32000 words: 160 rows 55.2 against 57.5, but
-    // 96 rows 49.1 against 47.2).
+    // Two SMs share a product above 128 columns: dim 4096, 32768 words, 1024 rows 255 us against
+    // 258 with one SM each. Small batches go either way: dim 2048, 32000 words, 96 rows 41.4
+    // against 42.2, 160 rows 51 to 57 against 48; dim 4096, 128256 words, 128 rows 215 against 220.
     const int columns = (a->batch + P.ntile - 1) / P.ntile;
     const bool pair = columns > 128;
     // a pair's product takes its columns in steps of 32, a single CTA's in steps of 16
@@ -159,9 +159,9 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
     const int tile_v = fg::adapt::TILE_V * (pair ? 2 : 1);
     P.nvt = (a->vocab + tile_v - 1) / tile_v;
     // Steps of K a stage: loads of one row of the weight close to each other in time while
-    // the weight's bytes bound the call (dim 4096, 128256 words, one row: four steps 162 us,
-    // two 169, one 178; 128 rows: two 220, one 229), more stages when the products do
-    // (1024 rows, 32768 words: one 264, two 277). A divisor of PIECE_K.
+    // the weight's bytes bound the call (dim 4096, 128256 words, one row: four steps 165 us,
+    // two 168, one 178; 128 rows: two 219, one 226), more stages when the products do
+    // (1024 rows, 32768 words: one 255, two 264). A divisor of PIECE_K.
     P.kb = P.nt <= 64 ? 4 : P.nt <= 128 ? 2 : 1;
     P.tmem_cols = 32;
     P.accs = std::min(fg::adapt::MAX_ACC, 512 / P.nt);

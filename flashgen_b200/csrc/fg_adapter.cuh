@@ -111,9 +111,9 @@ __device__ __forceinline__ void down_dots(const Params& P, const uint16_t* src, 
 // the same adapter next to each other, ties in row order), its copy there, and U, a
 // warp per rank index (2 * RC of them each, their 16-byte loads in flight together).
 // Bound: latency, then L2 (each row reads its own adapter): one row of dim 4096 and
-// rank 16 takes 14 us, 1024 rows 28 us (cold caches, alone), beside project_kernel's first
+// rank 16 takes 17 us, 1024 rows 29 us (cold caches, alone), beside project_kernel's first
 // loads. Half the threads, so that this kernel fits beside project_kernel on an SM: the
-// call is 2 to 3 us slower at 64 rows, 15 us at rank 128, 6 us faster at 1024 rows.
+// call was 2 to 3 us slower at 64 rows, 15 us at rank 128, 6 us faster at 1024 rows.
 // It stages nothing in shared memory: project_kernel's CTAs take nearly all of it
 // and start beside this kernel's.
 template <int DT, int RC>
@@ -218,11 +218,11 @@ __global__ void __launch_bounds__(DOWN_THREADS) down_kernel(const Params P) {
 // in flight before it frees the tensor memory and leaves.
 //
 // Bound: HBM up to about 128 rows (the weight, once), the tensor pipe above. Measured
-// (bf16, dim 4096, rank 16): 128256 words, one row 161 us (6.5 TB/s of weight), 64 rows of 32
-// adapters 197 us (5.3 TB/s); 32768 words, 1024 rows 260 us (1.06 PFLOP/s; SM clock held to
-// 1.6 GHz by the power limit, tensor pipe active 57 %, 66 % without adapters, the epilogue's
-// loads and products being the difference). Few rows of a short weight: 64 rows, dim 2048,
-// 32000 words 28 us without adapters, 35 us with 16 of rank 8, 38 us with 32 of rank 16
+// (bf16, dim 4096, rank 16): 128256 words, one row 160 to 165 us (6.4 to 6.5 TB/s of weight),
+// 64 rows of 32 adapters 198 us (5.3 TB/s); 32768 words, 1024 rows 255 us (1.08 PFLOP/s; SM
+// clock held to 1.6 GHz by the power limit, tensor pipe active 58 %), 210 without adapters (the
+// epilogue's loads and products are the difference). Few rows of a short weight: 64 rows, dim
+// 2048, 32000 words 29 us without adapters, 37 us with 16 of rank 8, 39 us with 32 of rank 16
 // (down_kernel's launch and the adapters' bytes; their rows fetched ahead of the epilogue,
 // to L2 or to shared memory by a warp of its own, gained nothing).
 //
@@ -240,9 +240,9 @@ constexpr int MAX_STAGES = 12;
 // products arrive (the others' adapters are added as they are read). With fp32
 // results registers go to the sums, of fewer columns for a SMALL batch tile: next to
 // the ring there is no L1 left, and a spilled register would wait for L2.
-// Measured: 12 warps against 8, 64 rows not sorted, 16-bit results: 42.7 us, 45.5; 16 against
-// 8, 256 rows, fp32: 99, 114; no early windows at those 64 rows: 49.6; SMALL, 8 rows, dim 2048,
-// 50257 words, fp32: 43.6, without it 49.9.
+// Measured (dim 2048, 32000 words, rank 16): 12 warps against 8, 64 rows not sorted, 16-bit
+// results: 41 us, 45; 16 against 8, 256 rows, fp32: 66, 81; no early windows at those 64 rows:
+// 46; SMALL, 8 rows, 50257 words, fp32: 42, without it 45.
 template <int ODT, int RC, bool SMALL>
 struct Epilogue {
     static constexpr bool PIECES = ODT == FG_DTYPE_F32;

@@ -922,9 +922,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) rows_kernel(const Params
 // Bound: HBM, the logits read and the gradient written once. Work is cut along the
 // gradient's 16-byte chunks; where the logits' rows are offset against the
 // gradient's, a thread takes the two chunks around its own and shifts them together.
-// Measured: 1024 x 128256 bf16 86 us (6.1 TB/s; two chunks in flight a thread 4 us more,
-// one step a CTA 16 more), 2048 x 50257 fp32 129 us (6.4 TB/s; 17 more, 16 more); 8 x 50257
-// fp32 2.9 us.
+// Measured: 1024 x 128256 bf16 85 us (6.2 TB/s; two chunks in flight a thread 4 us more,
+// one step a CTA 16 more), 2048 x 50257 fp32 128 us (6.4 TB/s; 17 more, 16 more); 333 x
+// 32001 f16 13.6 us; 8 x 50257 fp32 2.9 us.
 // ---------------------------------------------------------------------------
 constexpr int GRAD_THREADS = 256;
 constexpr int GRAD_UNROLL = 4;   // chunks in flight a thread

@@ -27,8 +27,6 @@
 // rows, dim 4096, V 32768, rank 64, bf16 423 us against 391.
 #pragma once
 
-#include <type_traits>
-
 #include "fg_adapter.h"
 #include "fg_tcgen05.cuh"
 
@@ -271,14 +269,6 @@ struct Control {
     int abort;      // someone's wait ran out: everyone stops waiting
     int reported;   // the rows' status words say so
 };
-
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d)
-        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
-          "l"(*reinterpret_cast<uint64_t*>(&c)));
-    return *reinterpret_cast<float2*>(&d);
-}
 
 // D (16 x 8, fp32) += A (16 x 16) B (16 x 8) of 16-bit operands, on one warp.
 template <int DT>

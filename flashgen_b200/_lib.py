@@ -29,7 +29,8 @@ FG_ROW_GREEDY = 0x0200
 EXPORTED_SYMBOLS = ("fg_sample", "fg_sample_workspace_size", "fg_sample_candidates", "fg_sample_noalloc",
                     "fg_sample_set_split",
                     "fg_apply_repetition_penalty", "fg_argmax", "fg_token_logprobs", "fg_token_logprobs_grad",
-                    "fg_adapter_logits", "fg_adapter_set_wait", "fg_adapter_workspace_size", "fg_strerror", "fg_version")
+                    "fg_adapter_logits", "fg_adapter_set_wait", "fg_adapter_workspace_size",
+                    "fg_clip_grad_norm", "fg_clip_workspace_size", "fg_strerror", "fg_version")
 
 
 class FgSampleArgs(ctypes.Structure):
@@ -136,6 +137,33 @@ class FgAdapterArgs(ctypes.Structure):
     ]
 
 
+class FgGradTensor(ctypes.Structure):
+    """Mirror of ``FgGradTensor``."""
+
+    _fields_ = [
+        ("grad", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("count", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+    ]
+
+
+class FgClipArgs(ctypes.Structure):
+    """Mirror of ``FgClipArgs``."""
+
+    _fields_ = [
+        ("tensors", ctypes.c_void_p),
+        ("count", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("max_norm", ctypes.c_float),
+        ("scale", ctypes.c_float),
+        ("out_norm", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 FG_SAMPLE_WORKSPACE_MIN_BYTES = 256
 FG_ADAPTER_MAX_RANK = 128
 FG_LOGPROB_MAX_TOP = 32
@@ -191,6 +219,10 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.fg_adapter_set_wait.restype = ctypes.c_int
         lib.fg_adapter_workspace_size.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
         lib.fg_adapter_workspace_size.restype = ctypes.c_size_t
+        lib.fg_clip_grad_norm.argtypes = [ctypes.POINTER(FgClipArgs), ctypes.c_void_p]
+        lib.fg_clip_grad_norm.restype = ctypes.c_int
+        lib.fg_clip_workspace_size.argtypes = [ctypes.c_int32]
+        lib.fg_clip_workspace_size.restype = ctypes.c_size_t
         lib.fg_strerror.argtypes = [ctypes.c_int]
         lib.fg_strerror.restype = ctypes.c_char_p
         lib.fg_version.argtypes = []

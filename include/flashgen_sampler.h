@@ -392,6 +392,51 @@ int fg_adapter_set_wait(int64_t limit_ns, int32_t withhold);
 /* Bytes of workspace of fg_adapter_logits; 0 for an invalid shape. Host-only. */
 size_t fg_adapter_workspace_size(int32_t batch, int32_t dim, int32_t rank, int32_t slots);
 
+/*
+ * The global norm of a list of gradients, and the gradients scaled to at most a given
+ * norm:
+ *
+ *   norm = scale * sqrt(sum over all elements of all tensors g^2)
+ *   out  = g * scale * min(1, max_norm / (norm + 1e-6))
+ *
+ * `tensors` is a host array, read during the call; grad and out are device pointers
+ * to dense tensors of `count` elements (0 allowed), aligned to their element size.
+ * out may be grad itself (same type), NULL (that tensor counts for the norm only) or
+ * memory that meets no other tensor's gradients or results and no other part of its
+ * own (FG_EINVAL otherwise). The squares are summed in 64 bits whatever the type, in
+ * an order that does not depend on timing; products are rounded once to the result's
+ * type. A NaN norm makes every result NaN; an infinite one makes the finite ones 0.
+ * max_norm >= 0 (infinity: no clipping), scale positive and finite.
+ *
+ * Workspace: fg_clip_workspace_size bytes, 8-byte aligned, written and read within the
+ * call (no initial value). Calls that may run concurrently need separate workspaces.
+ *
+ * No reference counterpart (FlashGen does not train).
+ */
+typedef struct FgGradTensor {
+    const void* grad;
+    void*       out;
+    int64_t     count;
+    int32_t     dtype;                  /* FG_DTYPE_* of grad                      */
+    int32_t     out_dtype;              /* FG_DTYPE_* of out; any if out is NULL   */
+} FgGradTensor;
+
+typedef struct FgClipArgs {
+    const FgGradTensor* tensors;        /* [count] on the host                     */
+    int32_t        count;               /* >= 0                                    */
+    int32_t        reserved;            /* 0                                       */
+    float          max_norm;
+    float          scale;
+    float*         out_norm;            /* [1]                                     */
+    void*          workspace;
+    size_t         workspace_bytes;
+} FgClipArgs;
+
+int fg_clip_grad_norm(const FgClipArgs* args, void* stream);
+
+/* Bytes of workspace of fg_clip_grad_norm; 0 for an invalid count. Host-only. */
+size_t fg_clip_workspace_size(int32_t count);
+
 /* Human-readable name of a return code. */
 const char* fg_strerror(int code);
 

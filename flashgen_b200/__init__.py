@@ -8,6 +8,7 @@ their gradient, and an LM head with per-request low-rank adapters.
 """
 from .core.config import SamplingParams  # noqa: F401
 from .sampling.clip import clip_grad_norm, grad_norm  # noqa: F401
+from .sampling.linear import HeadBlock, fused_linear  # noqa: F401
 from .sampling.lm_head import AdapterHead  # noqa: F401
 from .sampling.logprobs import (TokenLogprobs, logprobs_and_entropy, token_logprobs,  # noqa: F401
                                 token_logprobs_grad)
@@ -15,4 +16,4 @@ from .sampling.sampler import Sampler  # noqa: F401
 
 __version__ = "0.1.0"
 __all__ = ["SamplingParams", "Sampler", "AdapterHead", "TokenLogprobs", "token_logprobs", "token_logprobs_grad",
-           "logprobs_and_entropy", "grad_norm", "clip_grad_norm"]
+           "logprobs_and_entropy", "grad_norm", "clip_grad_norm", "fused_linear", "HeadBlock"]

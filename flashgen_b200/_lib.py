@@ -30,7 +30,8 @@ EXPORTED_SYMBOLS = ("fg_sample", "fg_sample_workspace_size", "fg_sample_candidat
                     "fg_sample_set_split",
                     "fg_apply_repetition_penalty", "fg_argmax", "fg_token_logprobs", "fg_token_logprobs_grad",
                     "fg_adapter_logits", "fg_adapter_set_wait", "fg_adapter_workspace_size",
-                    "fg_clip_grad_norm", "fg_clip_workspace_size", "fg_strerror", "fg_version")
+                    "fg_clip_grad_norm", "fg_clip_workspace_size", "fg_linear", "fg_linear_workspace_size", "fg_linear_grad",
+                    "fg_linear_grad_workspace_size", "fg_strerror", "fg_version")
 
 
 class FgSampleArgs(ctypes.Structure):
@@ -164,9 +165,64 @@ class FgClipArgs(ctypes.Structure):
     ]
 
 
+class FgLinearArgs(ctypes.Structure):
+    """Mirror of ``FgLinearArgs``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("preact", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("dtype", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("inner", ctypes.c_int32),
+        ("outer", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("x_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+        ("preact_stride", ctypes.c_int64),
+    ]
+
+
+class FgLinearGradArgs(ctypes.Structure):
+    """Mirror of ``FgLinearGradArgs``."""
+
+    _fields_ = [
+        ("grad_out", ctypes.c_void_p),
+        ("x", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("preact", ctypes.c_void_p),
+        ("grad_x", ctypes.c_void_p),
+        ("grad_weight", ctypes.c_void_p),
+        ("grad_bias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("dtype", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("inner", ctypes.c_int32),
+        ("outer", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("grad_out_stride", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("weight_stride", ctypes.c_int64),
+        ("preact_stride", ctypes.c_int64),
+        ("grad_x_stride", ctypes.c_int64),
+        ("grad_weight_stride", ctypes.c_int64),
+    ]
+
+
 FG_SAMPLE_WORKSPACE_MIN_BYTES = 256
 FG_ADAPTER_MAX_RANK = 128
 FG_LOGPROB_MAX_TOP = 32
+FG_ACT_NONE, FG_ACT_RELU, FG_ACT_GELU, FG_ACT_GELU_TANH, FG_ACT_SILU = 0, 1, 2, 3, 4
 
 
 _lib = None
@@ -223,6 +279,11 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.fg_clip_grad_norm.restype = ctypes.c_int
         lib.fg_clip_workspace_size.argtypes = [ctypes.c_int32]
         lib.fg_clip_workspace_size.restype = ctypes.c_size_t
+        for name, args in (("fg_linear", FgLinearArgs), ("fg_linear_grad", FgLinearGradArgs)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
+            getattr(lib, name + "_workspace_size").argtypes = [ctypes.POINTER(args)]
+            getattr(lib, name + "_workspace_size").restype = ctypes.c_size_t
         lib.fg_strerror.argtypes = [ctypes.c_int]
         lib.fg_strerror.restype = ctypes.c_char_p
         lib.fg_version.argtypes = []

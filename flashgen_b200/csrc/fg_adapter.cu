@@ -5,6 +5,7 @@
 
 #include "fg_adapter.h"
 #include "fg_internal.h"
+#include "fg_tma.h"
 
 namespace {
 
@@ -12,41 +13,6 @@ using fg::host::DevInfo;
 using fg::host::elem_size;
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The driver's tensor-map encoder, through the runtime (the library links no libcuda).
-EncodeTiledFn encoder() {
-    static std::atomic<EncodeTiledFn> fn{nullptr};
-    EncodeTiledFn f = fn.load(std::memory_order_acquire);
-    if (f == nullptr) {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) !=
-                cudaSuccess || q != cudaDriverEntryPointSuccess)
-            return nullptr;
-        f = reinterpret_cast<EncodeTiledFn>(p);
-        fn.store(f, std::memory_order_release);
-    }
-    return f;
-}
-
-// A [rows, dim] matrix read in boxes of box_rows x 64 elements; columns past dim
-// and rows past `rows` read as zero.
-bool encode(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t dim, int64_t stride, int box_rows) {
-    EncodeTiledFn f = encoder();
-    if (f == nullptr) return false;
-    const cuuint64_t extent[2] = {cuuint64_t(dim), cuuint64_t(rows)};
-    const cuuint64_t pitch[1] = {cuuint64_t(stride) * 2};
-    const cuuint32_t box[2] = {cuuint32_t(fg::adapt::TILE_K), cuuint32_t(box_rows)};
-    const cuuint32_t step[2] = {1, 1};
-    return f(map, dtype == FG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-             const_cast<void*>(base), extent, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
 
 // Workspace: U in parts, its units, the order of the rows, their copy.
 struct Layout {
@@ -170,8 +136,8 @@ int fg_adapter_logits(const FgAdapterArgs* a, void* stream) {
     while (P.tmem_cols < P.accs * P.nt) P.tmem_cols *= 2;
     if (int64_t(P.nvt) * P.ntile > (1 << 30)) return FG_ENOTSUP;
     CUtensorMap wmap, xmap;
-    if (!encode(&wmap, a->dtype, a->weight, a->vocab, a->dim, a->weight_stride, fg::adapt::TILE_V) ||
-        !encode(&xmap, a->dtype, P.hidden, a->batch, a->dim, P.hidden_stride, pair ? P.nt / 2 : P.nt))
+    if (!fg::host::encode_rows(&wmap, a->dtype, a->weight, a->vocab, a->dim, a->weight_stride, fg::adapt::TILE_V) ||
+        !fg::host::encode_rows(&xmap, a->dtype, P.hidden, a->batch, a->dim, P.hidden_stride, pair ? P.nt / 2 : P.nt))
         return FG_EDEVICE;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const bool f32 = a->out_dtype == FG_DTYPE_F32;

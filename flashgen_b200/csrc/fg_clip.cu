@@ -13,7 +13,8 @@ using fg::host::elem_size;
 
 constexpr int32_t kMaxTensors = 1 << 20;
 
-int64_t launches_for(int64_t count) { return (count + fg::clip::MAX_TENSORS - 1) / fg::clip::MAX_TENSORS; }
+// Norm launches of `count` tensors at most: each of the three types may leave one list unfilled.
+int64_t launches_for(int64_t count) { return std::min(count, count / fg::clip::MAX_TENSORS + 3); }
 
 // A launch that may begin while the stream's previous kernel ends: the kernel itself
 // waits for that one before it touches memory.
@@ -66,6 +67,48 @@ bool results_meet(const FgGradTensor* t, int32_t n) {
     return false;
 }
 
+using ScaleKernel = void (*)(const fg::clip::List, const double*, int64_t, float, float, float*);
+ScaleKernel scale_kernel_of(int dt, int odt) {
+    using namespace fg::clip;
+    static const ScaleKernel table[3][3] = {{scale_kernel<0, 0>, scale_kernel<0, 1>, scale_kernel<0, 2>},
+                                            {scale_kernel<1, 0>, scale_kernel<1, 1>, scale_kernel<1, 2>},
+                                            {scale_kernel<2, 0>, scale_kernel<2, 1>, scale_kernel<2, 2>}};
+    return table[dt][odt];
+}
+
+// Calls launch(dtype, result type, list) for the tensors of each type (with `scaling` of
+// each pair of types that has results), MAX_TENSORS of them at a time.
+template <class F>
+int for_lists(const FgClipArgs& a, bool scaling, F launch) {
+    for (int dt = 0; dt < 3; ++dt)
+        for (int odt = 0; odt < (scaling ? 3 : 1); ++odt) {
+            fg::clip::List L;
+            L.count = 0;
+            int64_t chunks = 0;
+            for (int32_t i = 0; i <= a.count; ++i) {
+                if (L.count == fg::clip::MAX_TENSORS || (i == a.count && L.count > 0)) {
+                    L.chunks = uint32_t(chunks);
+                    const int rc = launch(dt, odt, L);
+                    if (rc != FG_OK) return rc;
+                    L.count = 0;
+                    chunks = 0;
+                }
+                if (i == a.count) break;
+                const FgGradTensor& t = a.tensors[i];
+                if (t.count == 0 || t.dtype != dt || (scaling && (t.out == nullptr || t.out_dtype != odt))) continue;
+                const int esz = elem_size(dt);
+                fg::clip::Item& it = L.items[L.count++];
+                it.in = t.grad; it.out = t.out; it.count = t.count;
+                it.first = uint32_t(chunks);
+                it.wide_in = reinterpret_cast<uintptr_t>(t.grad) % 16 == 0;
+                it.wide_out = reinterpret_cast<uintptr_t>(t.out) % std::min(16, 16 / esz * elem_size(odt)) == 0;
+                chunks += (t.count * esz + fg::clip::CHUNK_BYTES - 1) / fg::clip::CHUNK_BYTES;
+                if (chunks > (int64_t(1) << 31)) return FG_ENOTSUP;
+            }
+        }
+    return FG_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -97,59 +140,43 @@ int fg_clip_grad_norm(const FgClipArgs* a, void* stream) {
         return FG_ENOTSUP;
     }
     DevInfo* d = nullptr;
-    const int rc = fg::host::device_info(&d);
+    int rc = fg::host::device_info(&d);
     if (rc != FG_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     double* total = reinterpret_cast<double*>(a->workspace);
     double* partial = total + 1;
-    const int64_t cap = std::min<int64_t>(fg::clip::MAX_GRID, 8 * int64_t(d->sms));
+    const int64_t cap = std::min<int64_t>(fg::clip::MAX_GRID, 6 * int64_t(d->sms));   // what is resident at once
     int64_t partials = 0;
-    // pass 0: the sums; pass 1: the scaling (at least one launch, which writes the norm)
-    for (int pass = 0; pass < 2; ++pass) {
-        bool wrote = false;
-        for (int32_t lo = 0; lo < a->count || (pass == 1 && !wrote); lo += fg::clip::MAX_TENSORS) {
-            fg::clip::List L;
-            L.count = 0;
-            int64_t chunks = 0;
-            for (int32_t i = lo; i < std::min(a->count, lo + fg::clip::MAX_TENSORS); ++i) {
-                const FgGradTensor& t = a->tensors[i];
-                if (t.count == 0 || (pass == 1 && t.out == nullptr)) continue;
-                const int esz = elem_size(t.dtype);
-                fg::clip::Item& it = L.items[L.count++];
-                it.in = t.grad; it.out = t.out; it.count = t.count;
-                it.dtype = uint8_t(t.dtype); it.out_dtype = uint8_t(t.out_dtype);
-                it.first = uint32_t(chunks);
-                it.wide_in = reinterpret_cast<uintptr_t>(t.grad) % 16 == 0;
-                const int vec = t.out ? std::min(16, 16 / esz * elem_size(t.out_dtype)) : 16;
-                it.wide_out = t.out && reinterpret_cast<uintptr_t>(t.out) % vec == 0;
-                chunks += (t.count * esz + fg::clip::CHUNK_BYTES - 1) / fg::clip::CHUNK_BYTES;
-                if (chunks > (int64_t(1) << 31)) return FG_ENOTSUP;
-            }
-            L.chunks = uint32_t(chunks);
-            if (pass == 0) {
-                if (chunks == 0) continue;
-                const unsigned grid = unsigned(std::min(cap, chunks));
-                const int rc1 = launch_early(fg::clip::norm_kernel, grid, st, L, partial + partials);
-                if (rc1 != FG_OK) return rc1;
-                partials += grid;
-            } else {
-                if (chunks == 0 && wrote) continue;
-                if (chunks == 0 && lo + fg::clip::MAX_TENSORS < a->count) continue;   // a later launch writes the norm
-                const unsigned grid = unsigned(std::max<int64_t>(1, std::min(cap, chunks)));
-                const bool one = partials <= cap;
-                const int rc1 = launch_early(fg::clip::scale_kernel, grid, st, L, (const double*)(one ? partial : total),
-                                             one ? partials : int64_t(1), a->max_norm, a->scale,
-                                             wrote ? (float*)nullptr : a->out_norm);
-                if (rc1 != FG_OK) return rc1;
-                wrote = true;
-            }
-        }
-        if (pass == 0 && partials > cap) {
-            const int rc1 = launch_early(fg::clip::total_kernel, 1, st, (const double*)partial, partials, total);
-            if (rc1 != FG_OK) return rc1;
-        }
+    rc = for_lists(*a, false, [&](int dt, int, const fg::clip::List& L) {
+        const unsigned grid = unsigned(std::min<int64_t>(cap, L.chunks));
+        double* at = partial + partials;
+        partials += grid;
+        return launch_early(dt == FG_DTYPE_F32   ? fg::clip::norm_kernel<FG_DTYPE_F32>
+                            : dt == FG_DTYPE_F16 ? fg::clip::norm_kernel<FG_DTYPE_F16>
+                                                 : fg::clip::norm_kernel<FG_DTYPE_BF16>,
+                            grid, st, L, at);
+    });
+    if (rc != FG_OK) return rc;
+    // several launches' sums are added up once, not in every CTA
+    const bool one = partials <= cap;
+    if (!one && (rc = launch_early(fg::clip::total_kernel, 1, st, (const double*)partial, partials, total)) != FG_OK)
+        return rc;
+    const double* sums = one ? partial : total;
+    const int64_t count = one ? partials : 1;
+    float* norm = a->out_norm;   // until a launch writes it
+    rc = for_lists(*a, true, [&](int dt, int odt, const fg::clip::List& L) {
+        const unsigned grid = unsigned(std::min<int64_t>(cap, L.chunks));
+        const int r = launch_early(scale_kernel_of(dt, odt), grid, st, L, sums, count, a->max_norm, a->scale, norm);
+        norm = nullptr;
+        return r;
+    });
+    if (rc == FG_OK && norm != nullptr) {   // nothing to scale
+        fg::clip::List L;
+        L.count = 0;
+        L.chunks = 0;
+        rc = launch_early(scale_kernel_of(0, 0), 1, st, L, sums, count, a->max_norm, a->scale, norm);
     }
-    return FG_OK;
+    return rc;
 }
 
 }  // extern "C"

@@ -3,7 +3,8 @@
 //   norm = scale * sqrt(sum_i sum_j g_ij^2),   out_ij = g_ij * c,
 //   c    = scale * min(1, max_norm / (norm + 1e-6))
 //
-// Two launches over all tensors: norm_kernel leaves one partial sum a CTA, scale_kernel
+// Two launches over all tensors of one pair of types (more for lists of mixed types, or
+// of over MAX_TENSORS): norm_kernel leaves one partial sum a CTA, scale_kernel
 // adds them up in every CTA (a few hundred numbers, in the same order everywhere) and
 // scales. Tensors are cut into chunks of 16 KB, numbered through the list; a CTA takes
 // every gridDim-th chunk, so neither many small tensors nor one large one leave SMs
@@ -19,15 +20,14 @@ namespace clip {
 constexpr int THREADS = 256, UNROLL = 4;
 constexpr int CHUNK_BYTES = THREADS * UNROLL * 16;   // of a tensor's gradients
 constexpr int MAX_TENSORS = 96;                      // of a launch: their list is a kernel parameter (4 KB at most)
-constexpr int MAX_GRID = 1184;                       // partial sums of a launch
+constexpr int MAX_GRID = 1184;                       // CTAs, and partial sums, of a launch
 
 struct Item {
     const void* in;
     void* out;            // null: norm only
     int64_t count;
     uint32_t first;       // number of its first chunk
-    uint8_t dtype, out_dtype;
-    uint8_t wide_in, wide_out;   // 16-byte loads; stores of a whole vector
+    uint16_t wide_in, wide_out;   // 16-byte loads; stores of a whole vector
 };
 struct List {
     Item items[MAX_TENSORS];
@@ -73,7 +73,7 @@ __device__ __forceinline__ double squares(const uint4& q) {
 
 // The squares of elements [lo, hi) of a tensor (one chunk), this thread's share.
 template <int DT>
-__device__ __noinline__ double chunk_squares(const Item& it, int64_t lo, int64_t hi) {
+__device__ __forceinline__ double chunk_squares(const Item& it, int64_t lo, int64_t hi) {
     constexpr int VEC = Elem<DT>::VEC;
     double sum = 0.0;
     int64_t done = lo;
@@ -102,11 +102,8 @@ __device__ __forceinline__ int item_of(const List& L, uint32_t c, int t) {
     while (t + 1 < L.count && L.items[t + 1].first <= c) ++t;
     return t;
 }
-__device__ __forceinline__ int64_t chunk_elems(int dtype) {
-    return CHUNK_BYTES / (dtype == FG_DTYPE_F32 ? 4 : 2);
-}
-
 // Bound: HBM reads.
+template <int DT>
 __global__ void __launch_bounds__(THREADS, 6) norm_kernel(const __grid_constant__ List L, double* partial) {
     wait_prerequisites();
     launch_dependents();
@@ -115,13 +112,9 @@ __global__ void __launch_bounds__(THREADS, 6) norm_kernel(const __grid_constant_
     for (uint32_t c = blockIdx.x; c < L.chunks; c += gridDim.x) {
         t = item_of(L, c, t);
         const Item& it = L.items[t];
-        const int64_t step = chunk_elems(it.dtype), lo = int64_t(c - it.first) * step;
-        const int64_t hi = lo + step < it.count ? lo + step : it.count;
-        switch (it.dtype) {
-            case FG_DTYPE_F32: sum += chunk_squares<FG_DTYPE_F32>(it, lo, hi); break;
-            case FG_DTYPE_F16: sum += chunk_squares<FG_DTYPE_F16>(it, lo, hi); break;
-            default: sum += chunk_squares<FG_DTYPE_BF16>(it, lo, hi); break;
-        }
+        constexpr int64_t STEP = CHUNK_BYTES / Elem<DT>::SIZE;
+        const int64_t lo = int64_t(c - it.first) * STEP, hi = lo + STEP < it.count ? lo + STEP : it.count;
+        sum += chunk_squares<DT>(it, lo, hi);
     }
     sum = block_sum(sum);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -167,9 +160,8 @@ __device__ __forceinline__ void store_scaled(void* out, int64_t at, const uint4&
     }
 }
 
-// (not inlined: one of nine for a chunk, whose registers would add up)
 template <int DT, int ODT>
-__device__ __noinline__ void scale_chunk(const Item& it, int64_t lo, int64_t hi, float c) {
+__device__ __forceinline__ void scale_chunk(const Item& it, int64_t lo, int64_t hi, float c) {
     constexpr int VEC = Elem<DT>::VEC;
     int64_t done = lo;
     if (it.wide_in && it.wide_out) {
@@ -196,17 +188,9 @@ __device__ __noinline__ void scale_chunk(const Item& it, int64_t lo, int64_t hi,
     }
 }
 
-template <int DT>
-__device__ __forceinline__ void scale_chunk(const Item& it, int64_t lo, int64_t hi, float c) {
-    switch (it.out_dtype) {
-        case FG_DTYPE_F32: return scale_chunk<DT, FG_DTYPE_F32>(it, lo, hi, c);
-        case FG_DTYPE_F16: return scale_chunk<DT, FG_DTYPE_F16>(it, lo, hi, c);
-        default: return scale_chunk<DT, FG_DTYPE_BF16>(it, lo, hi, c);
-    }
-}
-
 // Bound: HBM, the second read as far as L2 does not hold it and the write.
-__global__ void __launch_bounds__(THREADS, 5) scale_kernel(const __grid_constant__ List L, const double* partial,
+template <int DT, int ODT>
+__global__ void __launch_bounds__(THREADS, 6) scale_kernel(const __grid_constant__ List L, const double* partial,
                                                         int64_t count, float max_norm, float scale, float* out_norm) {
     wait_prerequisites();
     launch_dependents();
@@ -226,13 +210,9 @@ __global__ void __launch_bounds__(THREADS, 5) scale_kernel(const __grid_constant
         const Item& it = L.items[t];
         // gradients that stay as they are
         if (c == 1.0f && it.out == it.in) continue;
-        const int64_t step = chunk_elems(it.dtype), lo = int64_t(ch - it.first) * step;
-        const int64_t hi = lo + step < it.count ? lo + step : it.count;
-        switch (it.dtype) {
-            case FG_DTYPE_F32: scale_chunk<FG_DTYPE_F32>(it, lo, hi, c); break;
-            case FG_DTYPE_F16: scale_chunk<FG_DTYPE_F16>(it, lo, hi, c); break;
-            default: scale_chunk<FG_DTYPE_BF16>(it, lo, hi, c); break;
-        }
+        constexpr int64_t STEP = CHUNK_BYTES / Elem<DT>::SIZE;
+        const int64_t lo = int64_t(ch - it.first) * STEP, hi = lo + STEP < it.count ? lo + STEP : it.count;
+        scale_chunk<DT, ODT>(it, lo, hi, c);
     }
 }
 

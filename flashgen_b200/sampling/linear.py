@@ -1,0 +1,193 @@
+"""The dense block in front of an LM head, fused: ``act(x W^T + bias) + residual``.
+
+Decoders put such blocks between the last hidden states and the head (the head
+transform of masked models, the residual block of a draft head). FlashGen runs
+them as a library product and a kernel each for bias, activation and addition
+(csrc/runtime/transformer.cu). :func:`fused_linear` is one kernel launch of the
+C ABI (``fg_linear``) whose epilogue does the rest, differentiable through
+``fg_linear_grad``; :class:`HeadBlock` keeps a block's parameters for
+``DecodeBatch.step_hidden``.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .. import _lib
+from .sampler import _DTYPES, _call, _ptr
+
+_ACTIVATIONS = {"none": _lib.FG_ACT_NONE, "relu": _lib.FG_ACT_RELU, "gelu": _lib.FG_ACT_GELU,
+                "gelu_tanh": _lib.FG_ACT_GELU_TANH, "silu": _lib.FG_ACT_SILU}
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A matrix as the kernels read it: rows of neighbouring elements that do not overlap."""
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _stride(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _room(size: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    return None if size == 0 else torch.empty(size, dtype=torch.uint8, device=like.device)
+
+
+def _forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
+             act: int, keep: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The block on matrices; with `keep` also the sums before the activation, in fp32 (the
+    gradient's slope at a rounded sum would lose the slope's last bits)."""
+    tokens, inner, outer = x.shape[0], x.shape[1], weight.shape[0]
+    out = x.new_empty((tokens, outer))
+    preact = x.new_empty((tokens, (outer + 3) // 4 * 4), dtype=torch.float32) if keep and act else None
+    if tokens == 0:
+        return out, preact
+    x, weight = _rows(x), _rows(weight)
+    lib = _lib.load()
+    a = _lib.FgLinearArgs(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), out.data_ptr(), _ptr(preact),
+                          None, 0, _DTYPES[x.dtype], tokens, inner, outer, act, 0, _stride(x), _stride(weight),
+                          _stride(residual), outer, _stride(preact))
+    room = _room(lib.fg_linear_workspace_size(a), x)
+    if room is not None:
+        a.workspace, a.workspace_bytes = room.data_ptr(), room.numel()
+    _call(x.device, lib.fg_linear, a, "fg_linear")
+    return out, preact
+
+
+class _Once(torch.autograd.Function):
+    """A gradient that is linked to what it was computed from: a backward pass
+    through it raises."""
+
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("fused_linear is differentiable once: its gradients have no gradients")
+
+
+class _FusedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        out, preact = _forward(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, preact)
+        ctx.act = act
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        x, weight, preact = ctx.saved_tensors
+        wanted = ctx.needs_input_grad
+        gx = gw = gb = None
+        if any(wanted[:3]):
+            with torch.no_grad():
+                gx, gw, gb = _gradients(grad, x, weight, preact, ctx.act, wanted)
+        grads = (gx, gw, gb, grad if wanted[3] else None)
+        if torch.is_grad_enabled():   # create_graph=True
+            grads = tuple(None if g is None or g is grad else _Once.apply(g, grad, x, weight) for g in grads)
+            grads = grads[:3] + (grad if wanted[3] else None,)
+        return (*grads, None)
+
+
+def _gradients(grad, x, weight, preact, act, wanted):
+    tokens, inner, outer = x.shape[0], x.shape[1], weight.shape[0]
+    g, x, weight = _rows(grad), _rows(x), _rows(weight)
+    gx = x.new_empty((tokens, inner)) if wanted[0] else None
+    gw = x.new_empty((outer, inner)) if wanted[1] else None
+    gb = x.new_empty((outer,)) if wanted[2] else None
+    lib = _lib.load()
+    # (an empty tensor has no address: the library wants one, and reads nothing there)
+    place = (gw if gw is not None else gb if gb is not None else weight).data_ptr() if tokens == 0 else 0
+    if tokens == 0 and gw is None and gb is None:
+        return gx, gw, gb
+    a = _lib.FgLinearGradArgs(
+        g.data_ptr() or place, x.data_ptr() or place, weight.data_ptr(), _ptr(preact) or place or None,
+        None if gx is None else gx.data_ptr() or place, _ptr(gw), _ptr(gb), None, 0, _DTYPES[x.dtype], tokens, inner,
+        outer, act, 0, _stride(g) if tokens else outer, _stride(x) if tokens else inner, _stride(weight),
+        (_stride(preact) or outer) if tokens else outer, inner, inner)
+    room = _room(lib.fg_linear_grad_workspace_size(a), x)
+    if room is not None:
+        a.workspace, a.workspace_bytes = room.data_ptr(), room.numel()
+    _call(x.device, lib.fg_linear_grad, a, "fg_linear_grad")
+    return gx, gw, gb
+
+
+def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                 residual: Optional[torch.Tensor] = None, *, activation: str = "none") -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual``: ``x`` [..., inner], ``weight`` [outer,
+    inner], ``bias`` [outer], ``residual`` of the result's shape [..., outer], all
+    float16 or all bfloat16; ``activation`` is "none", "relu", "gelu" (erf),
+    "gelu_tanh" or "silu". Products are summed in fp32, and bias, activation and
+    residual are applied to the fp32 sum, which is rounded once.
+
+    Differentiable with respect to all four (once: a second derivative raises).
+    For that the sums before the activation are kept in fp32, and their
+    gradients enter the two products of the backward pass rounded to the
+    operands' type.
+
+    ``x`` and ``weight`` are read where they lie when their rows are 16-byte
+    aligned (``inner`` a multiple of 8, as a rule); otherwise each call copies
+    them.
+
+    >>> y = fused_linear(hidden, weight, bias, hidden, activation="silu")
+    """
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"weight must be [outer, inner], got {tuple(weight.shape)}")
+    outer, inner = weight.shape
+    if x.dim() < 1 or x.shape[-1] != inner:
+        raise ValueError(f"x must be [..., {inner}], got {tuple(x.shape)}")
+    dtype, dev = weight.dtype, weight.device
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"weight must be float16 or bfloat16, got {dtype}")
+    shape = x.shape[:-1] + (outer,)
+    for t, what, want in ((x, "x", x.shape), (bias, "bias", (outer,)), (residual, "residual", shape)):
+        if t is None:
+            continue
+        if t.dtype != dtype or t.device != dev:
+            raise TypeError(f"{what} must be {dtype} on {dev} like the weight, got {t.dtype} on {t.device}")
+        if t.shape != want:
+            raise ValueError(f"{what} must be {list(want)}, got {list(t.shape)}")
+    if not weight.is_cuda:
+        raise RuntimeError(f"flashgen_b200 runs on the GPU only; the weight is on {dev}")
+    flat = x.dim() == 2
+    x2 = x if flat else x.reshape(-1, inner)
+    r2 = residual if residual is None or flat else residual.reshape(-1, outer)
+    if r2 is not None:
+        r2 = _rows(r2)
+    if bias is not None:
+        bias = bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
+        out = _FusedLinear.apply(x2, weight, bias, r2, act)
+    else:
+        out, _ = _forward(x2, weight, bias, r2, act, False)
+    return out if flat else out.view(shape)
+
+
+class HeadBlock:
+    """A dense block with its parameters: ``hidden + act(hidden W^T + bias)``, or
+    without the first term.
+
+    >>> block = HeadBlock(weight, bias, activation="silu")   # weight [dim, dim]
+    >>> ids = dec.step_hidden(hidden, head, block=block)
+    """
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, activation: str = "silu",
+                 residual: bool = True):
+        if weight.dim() != 2 or (residual and weight.shape[0] != weight.shape[1]):
+            raise ValueError(f"weight must be [outer, inner], square with a residual, got {tuple(weight.shape)}")
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+        self.weight, self.bias, self.activation, self.residual = weight, bias, activation, bool(residual)
+
+    def __call__(self, hidden: torch.Tensor) -> torch.Tensor:
+        return fused_linear(hidden, self.weight, self.bias, hidden if self.residual else None,
+                            activation=self.activation)

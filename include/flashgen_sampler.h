@@ -437,6 +437,102 @@ int fg_clip_grad_norm(const FgClipArgs* args, void* stream);
 /* Bytes of workspace of fg_clip_grad_norm; 0 for an invalid count. Host-only. */
 size_t fg_clip_workspace_size(int32_t count);
 
+/*
+ * A dense block with its bias, activation and residual in one product:
+ *
+ *   out[m, n] = act(sum_k x[m, k] weight[n, k] + bias[n]) + residual[m, n]
+ *
+ * All matrices are 16-bit, of one type; products are summed in fp32, and what follows is
+ * computed in fp32 and rounded once. bias and residual may be NULL. preact, if not NULL,
+ * receives the fp32 sums with the bias, which the gradient needs (activations other than
+ * FG_ACT_NONE). Any strides and any 2-byte alignment; x and weight are read where they
+ * lie when their rows are 16-byte aligned and copied to the workspace otherwise. out may
+ * be residual itself (same stride); results that meet inputs in any other way are
+ * FG_EINVAL.
+ *
+ * Every wait in the kernel is bounded (1 s); where one runs out, what was not computed is
+ * NaN.
+ *
+ * Workspace: fg_linear_workspace_size(args) bytes (0 for aligned x and weight), 256-byte
+ * aligned, written and read within the call. Calls that may run concurrently need separate
+ * workspaces.
+ *
+ * Replaces a library product and the element-wise kernels after it (FlashGen's
+ * csrc/runtime/transformer.cu).
+ */
+#define FG_ACT_NONE      0
+#define FG_ACT_RELU      1
+#define FG_ACT_GELU      2   /* z (1 + erf(z / sqrt 2)) / 2                          */
+#define FG_ACT_GELU_TANH 3   /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2    */
+#define FG_ACT_SILU      4   /* z / (1 + e^-z)                                       */
+
+typedef struct FgLinearArgs {
+    const void* x;                      /* [tokens, inner]                         */
+    const void* weight;                 /* [outer, inner]                          */
+    const void* bias;                   /* [outer] or NULL                         */
+    const void* residual;               /* [tokens, outer] or NULL                 */
+    void*       out;                    /* [tokens, outer]                         */
+    float*      preact;                 /* [tokens, outer] or NULL                 */
+    void*       workspace;
+    size_t      workspace_bytes;
+    int32_t     dtype;                  /* FG_DTYPE_F16 or FG_DTYPE_BF16           */
+    int32_t     tokens;                 /* >= 0                                    */
+    int32_t     inner;                  /* >= 1                                    */
+    int32_t     outer;                  /* >= 1                                    */
+    int32_t     activation;             /* FG_ACT_*                                */
+    int32_t     reserved;               /* 0                                       */
+    int64_t     x_stride;               /* elements between rows, >= inner         */
+    int64_t     weight_stride;
+    int64_t     residual_stride;        /* >= outer                                */
+    int64_t     out_stride;
+    int64_t     preact_stride;
+} FgLinearArgs;
+
+int fg_linear(const FgLinearArgs* args, void* stream);
+
+/* Bytes of workspace of fg_linear for these arguments; 0 also for an invalid shape. Host-only. */
+size_t fg_linear_workspace_size(const FgLinearArgs* args);
+
+/*
+ * Gradients of fg_linear. With dz = grad_out * act'(preact):
+ *
+ *   grad_x = dz weight      grad_weight = dz^T x      grad_bias = sum over tokens of dz
+ *
+ * (the residual's gradient is grad_out). Each of the three may be NULL. dz is rounded to
+ * the operands' type for the two products, and summed for the bias before that; sums are
+ * fp32, in an order that does not depend on timing. preact is read with activations other
+ * than FG_ACT_NONE, weight for grad_x, x for grad_weight. Strides, alignment, waits and
+ * workspace as in fg_linear. With no tokens the sums over them are 0.
+ */
+typedef struct FgLinearGradArgs {
+    const void*  grad_out;              /* [tokens, outer]                         */
+    const void*  x;                     /* [tokens, inner]                         */
+    const void*  weight;                /* [outer, inner]                          */
+    const float* preact;                /* [tokens, outer]                         */
+    void*        grad_x;                /* [tokens, inner] or NULL                 */
+    void*        grad_weight;           /* [outer, inner] or NULL                  */
+    void*        grad_bias;             /* [outer] or NULL                         */
+    void*        workspace;
+    size_t       workspace_bytes;
+    int32_t      dtype;
+    int32_t      tokens;
+    int32_t      inner;
+    int32_t      outer;
+    int32_t      activation;
+    int32_t      reserved;              /* 0                                       */
+    int64_t      grad_out_stride;
+    int64_t      x_stride;
+    int64_t      weight_stride;
+    int64_t      preact_stride;
+    int64_t      grad_x_stride;
+    int64_t      grad_weight_stride;
+} FgLinearGradArgs;
+
+int fg_linear_grad(const FgLinearGradArgs* args, void* stream);
+
+/* Bytes of workspace of fg_linear_grad for these arguments. Host-only. */
+size_t fg_linear_grad_workspace_size(const FgLinearGradArgs* args);
+
 /* Human-readable name of a return code. */
 const char* fg_strerror(int code);
 

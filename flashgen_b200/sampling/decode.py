@@ -32,6 +32,7 @@ import torch
 
 from .. import _lib
 from ..core.config import SamplingParams
+from .linear import HeadBlock
 from .lm_head import AdapterHead
 from .logprobs import TokenLogprobs, token_logprobs
 from .sampler import PackedParams, _status_error, fused_sample, workspace_for
@@ -121,13 +122,19 @@ class DecodeBatch:
         return ids
 
     def step_hidden(self, hidden: torch.Tensor, head: AdapterHead, adapters: Optional[torch.Tensor] = None,
-                    out_dtype: Optional[torch.dtype] = None, **kwargs) -> torch.Tensor:
+                    out_dtype: Optional[torch.dtype] = None, block: Optional[HeadBlock] = None,
+                    **kwargs) -> torch.Tensor:
         """`step` from the hidden states [B, dim]: the logits are `head`'s, every
         row with its own adapter (`adapters` [B] int32, negative: none), of the
         head's type or of `out_dtype` (float32: log probabilities and ties as the
-        sums give them). With `check_errors` a slot outside the head's bank raises, too."""
+        sums give them). With `block` the hidden states go through that dense block
+        first. With `check_errors` a slot outside the head's bank raises, too."""
         self.last_logprobs = None
-        logits = head.logits(hidden.detach(), adapters, out_dtype=out_dtype, check_errors=self.check_errors)
+        hidden = hidden.detach()
+        if block is not None:
+            with torch.no_grad():
+                hidden = block(hidden)
+        logits = head.logits(hidden, adapters, out_dtype=out_dtype, check_errors=self.check_errors)
         return self.step(logits, **kwargs)
 
     def _append(self, ids: torch.Tensor) -> None:

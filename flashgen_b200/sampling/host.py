@@ -27,7 +27,7 @@ class _Staging:
     """One set of pinned host buffers and their device twins."""
 
     def __init__(self, batch: int, device):
-        self.f32_h = torch.empty(7, batch, dtype=torch.float32).pin_memory()   # 5 params, uniforms, spare
+        self.f32_h = torch.empty(7, batch, dtype=torch.float32).pin_memory()   # 5 params, uniforms, min_p
         self.i32_h = torch.empty(batch, dtype=torch.int32).pin_memory()
         self.u8_h = torch.empty(batch, dtype=torch.uint8).pin_memory()
         self.ids_h = torch.empty(batch, dtype=torch.int64).pin_memory()
@@ -68,6 +68,8 @@ class HostBatchSampler:
         f = s.f32_h.numpy()
         f[0], f[1], f[2], f[3], f[4], f[5] = (params.temperature, params.top_p, params.repetition_penalty,
                                               params.presence_penalty, params.frequency_penalty, uniforms_h)
+        min_p = getattr(params, "min_p", None)
+        f[6] = 0.0 if min_p is None else min_p
         s.i32_h.numpy()[:] = params.top_k
         s.u8_h.numpy()[:] = params.greedy
         s.f32_d.copy_(s.f32_h, non_blocking=True)
@@ -88,6 +90,8 @@ class HostBatchSampler:
         packed.any_presence = bool(np.any(params.presence_penalty != 0.0))
         packed.any_frequency = bool(np.any(params.frequency_penalty != 0.0))
         packed.all_greedy = False
+        if min_p is not None and np.any(np.asarray(min_p) != 0.0):
+            packed.min_p = s.f32_d[6]
         fused_sample(self.logits_d, packed, s.f32_d[5], hist, out=self.ids_d, status=self.status_d)
         s.ids_h.copy_(self.ids_d, non_blocking=True)
         ev = torch.cuda.Event()

@@ -15,6 +15,7 @@ Differences a caller can observe, all deliberate:
 * Rows with ``temperature == 0`` are greedy (as in
   ``csrc/runtime/pipeline.cpp:284``); the reference's Python path would sample
   them at temperature 1.
+* ``SamplingParams.min_p`` (not in the reference) filters before top-k and top-p.
 * Penalties (repetition, presence, frequency) are applied inside ``sample``
   when ``token_histories`` is given; the reference only offers
   ``apply_repetition_penalty`` as a separate in-place helper (kept here too).
@@ -84,7 +85,9 @@ def histories_to_csr(histories: Sequence[Sequence[int]], device) -> Tuple[torch.
 class PackedParams:
     """Per-row parameters as device structure-of-arrays."""
 
-    def __init__(self, temperature, top_p, top_k, rep, presence, frequency, greedy, device):
+    min_p: Optional[torch.Tensor] = None      # [B] float32; None where no row has it
+
+    def __init__(self, temperature, top_p, top_k, rep, presence, frequency, greedy, device, min_p=None):
         B = len(temperature)
         host = np.empty((5, B), dtype=np.float32)
         host[0], host[1], host[2], host[3], host[4] = temperature, top_p, rep, presence, frequency
@@ -95,6 +98,8 @@ class PackedParams:
         self.any_presence = bool(np.any(np.asarray(presence) != 0.0))
         self.any_frequency = bool(np.any(np.asarray(frequency) != 0.0))
         self.all_greedy = bool(np.all(np.asarray(greedy) | (np.asarray(temperature) == 0.0)))
+        if min_p is not None and np.any(np.asarray(min_p) != 0.0):
+            self.min_p = torch.from_numpy(np.asarray(min_p, dtype=np.float32).copy()).to(device, non_blocking=True)
 
     @staticmethod
     def from_params(params: Sequence[SamplingParams], device) -> "PackedParams":
@@ -102,7 +107,8 @@ class PackedParams:
                             [p.top_k for p in params], [p.repetition_penalty for p in params],
                             [getattr(p, "presence_penalty", 0.0) for p in params],
                             [getattr(p, "frequency_penalty", 0.0) for p in params],
-                            [bool(p.greedy) for p in params], device)
+                            [bool(p.greedy) for p in params], device,
+                            [getattr(p, "min_p", 0.0) for p in params])
 
 
 _WORKSPACES = {}
@@ -127,7 +133,8 @@ def fused_sample(logits: torch.Tensor, packed: PackedParams, uniforms: torch.Ten
                  probs: Optional[torch.Tensor] = None, vocab_offset: int = 0, vocab_total: int = 0,
                  stream: Optional[torch.cuda.Stream] = None,
                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """One fg_sample call on device tensors (no checks beyond the C ABI's)."""
+    """One fg_sample call on device tensors (fg_sample_min_p where a row has min-p; no
+    checks beyond the C ABI's)."""
     lib = _lib.load()
     B, V = logits.shape
     if out is None:
@@ -151,6 +158,16 @@ def fused_sample(logits: torch.Tensor, packed: PackedParams, uniforms: torch.Ten
     a.out_status = _ptr(status)
     a.out_probs = _ptr(probs)
     st = stream if stream is not None else torch.cuda.current_stream(logits.device)
+    if packed.min_p is not None:
+        need = lib.fg_sample_min_p_workspace_size(B, V, a.hist_max_len if hist is not None else 0)
+        # of any content, unlike fg_sample's, whose counters stay zero between calls
+        with torch.cuda.stream(st):
+            own = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        _lib.set_workspace(a, own)
+        with torch.cuda.device(logits.device):
+            _lib.check(lib.fg_sample_min_p(_lib.FgMinPArgs(a, packed.min_p.data_ptr(), None, None), st.cuda_stream),
+                       "fg_sample_min_p")
+        return out
     if workspace is None:
         need = _lib.workspace_size(B, V, a.dtype, a.hist_max_len if hist is not None else 0)
         workspace = workspace_for(logits.device, st, need)

@@ -49,6 +49,8 @@ def local_candidates(shard: torch.Tensor, packed: PackedParams, uniforms: torch.
                      hist: Optional[Tuple[torch.Tensor, torch.Tensor, int]], vocab_offset: int,
                      vocab_total: int, cand_max: int, stream: Optional[torch.cuda.Stream] = None) -> Candidates:
     """Local stage on one GPU shard [B, V/G] (fg_sample_candidates)."""
+    if packed.min_p is not None:
+        raise ValueError("min_p needs the whole row's maximum, which a vocabulary shard does not have")
     lib = _lib.load()
     B, V = shard.shape
     dev = shard.device

@@ -533,6 +533,46 @@ int fg_linear_grad(const FgLinearGradArgs* args, void* stream);
 /* Bytes of workspace of fg_linear_grad for these arguments. Host-only. */
 size_t fg_linear_grad_workspace_size(const FgLinearGradArgs* args);
 
+/*
+ * Sampling with min-p. The chain of fg_sample with one more filter: per row, y being the
+ * penalised logits over the temperature and top their maximum,
+ *
+ *   min-p   keeps y_j >= top + log(min_p): a probability of at least min_p times the largest
+ *   top-k   of those (every value >= the k-th largest; k <= 0: off)
+ *   top-p   of those, renormalised: the descending prefix whose exclusive mass is <= top_p
+ *           of it, ties at the cut in ascending id order (>= 1: off)
+ *   draw    the first token, in that order, whose inclusive mass exceeds u times the
+ *           kept mass
+ *
+ * (min_p == 0 keeps everything but -inf: the result is then fg_sample's.) Probabilities
+ * are compared in 64 bits. Greedy rows take the first argmax of the penalised logits.
+ *
+ * `sample` is read as in fg_sample, with these differences: temperature, top_p, top_k
+ * (and min_p) may be NULL (1, 1, 0 and 0); there is no vocabulary sharding (vocab_offset 0,
+ * vocab_total 0 or vocab): a shard does not know the row's maximum; `workspace` is
+ * fg_sample_min_p_workspace_size bytes, 8-byte aligned, of any content, and calls that may
+ * run concurrently need separate ones. min_p outside [0, 1] is FG_ROW_BAD_PARAM.
+ *
+ * out_logprobs[r] is the log probability of the drawn id among the kept tokens (0 for greedy
+ * rows), out_kept[r] their number (1 for greedy rows); rows without an id have NaN and 0.
+ * Either may be NULL.
+ *
+ * Replaces a sort-based chain of filters; FlashGen's sampler has no min-p
+ * (flashgen/sampling/sampler.py:102-121).
+ */
+typedef struct FgMinPArgs {
+    FgSampleArgs   sample;
+    const float*   min_p;               /* [B] or NULL                             */
+    float*         out_logprobs;        /* [B] or NULL                             */
+    int32_t*       out_kept;            /* [B] or NULL                             */
+} FgMinPArgs;
+
+int fg_sample_min_p(const FgMinPArgs* args, void* stream);
+
+/* Bytes of workspace of fg_sample_min_p (hist_max_len 0 without penalties); 0 for an
+ * invalid shape. Host-only. */
+size_t fg_sample_min_p_workspace_size(int32_t batch, int32_t vocab, int32_t hist_max_len);
+
 /* Human-readable name of a return code. */
 const char* fg_strerror(int code);
 

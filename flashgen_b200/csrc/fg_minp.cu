@@ -12,7 +12,6 @@ using fg::host::elem_size;
 
 constexpr int32_t kMaxBatch = 1 << 24;
 constexpr int kMaxClusters = 64;    // of wide_kernel
-constexpr int kWideG = 8;           // its CTAs a row
 
 int slots_for(int64_t ids) {
     int s = 64;
@@ -70,20 +69,24 @@ int launch(fg::minp::Params P, DevInfo* d, cudaStream_t st) {
     static std::atomic<int> rows_smem[fg::host::kMaxDevices] = {}, wide_smem[fg::host::kMaxDevices] = {};
     const int esz = fg::Elem<DT>::SIZE;
     const int G = ctas_per_row(P.batch, P.vocab, esz, d);
-    const int smem = CAP * int(sizeof(Candidate) + 8) + (P.penalties ? P.slots * 8 : 0);
+    const int smem = RING_BYTES + CAP * int(sizeof(Candidate)) + (P.penalties ? P.slots * 8 : 0);
     if (!set_smem(rows_kernel<DT>, rows_smem, smem)) return FG_EDEVICE;
     int rc = launch_early(rows_kernel<DT>, unsigned(P.batch) * G, NT, smem, G, st, P);
     if (rc != FG_OK) return rc;
-    // the slice's keys in shared memory where they fit
-    const int fixed = bins_bytes(kWideG) + (P.penalties ? 4 * FILTER_WORDS : 0);
-    const int64_t chunks = int64_t(P.vocab) * esz / 16 + 1;
-    const int64_t keys = (chunks + kWideG - 1) / kWideG * (16 / esz) + 2 * (16 / esz);
-    const int room = d->smem_optin - int(sizeof(WideShared)) - 1024 - fixed;
-    P.cache = 4 * keys <= room ? int(keys) : 0;
-    const int wsmem = fixed + 4 * P.cache;
+    // wide_kernel: the slice's keys in shared memory where they fit; four CTAs a row where that
+    // leaves work for every SM
+    auto fixed = [&](int g) { return 16 * MEMBERS + bins_bytes(g) + (P.penalties ? 4 * FILTER_WORDS : 0); };
+    auto keys = [&](int g) {
+        const int64_t chunks = int64_t(P.vocab) * esz / 16 + 1;
+        return (chunks + g - 1) / g * (16 / esz) + 2 * (16 / esz);
+    };
+    const int room = d->smem_optin - int(sizeof(WideShared) + sizeof(ExpTable)) - 1024;
+    const int W = P.batch > d->sms / 8 && fixed(4) + 4 * keys(4) <= room ? 4 : 8;
+    P.cache = fixed(W) + 4 * keys(W) <= room ? int(keys(W)) : 0;
+    const int wsmem = fixed(W) + 4 * P.cache;
     if (!set_smem(wide_kernel<DT>, wide_smem, wsmem)) return FG_EDEVICE;
-    const int clusters = std::min({int(P.batch), kMaxClusters, d->sms / kWideG});
-    return launch_early(wide_kernel<DT>, unsigned(clusters * kWideG), WNT, wsmem, kWideG, st, P);
+    const int clusters = std::min({int(P.batch), kMaxClusters, d->sms / W});
+    return launch_early(wide_kernel<DT>, unsigned(clusters * W), WNT, wsmem, W, st, P);
 }
 
 }  // namespace

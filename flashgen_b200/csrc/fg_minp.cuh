@@ -20,12 +20,17 @@ namespace fg {
 namespace minp {
 
 constexpr int NT = 256;            // threads of rows_kernel
-constexpr int UNROLL = 8;          // 16-byte chunks a thread has in flight
-constexpr int CAP = 2048;          // candidates of a CTA's slice, and of a row
+constexpr int STAGES = 3;          // of a thread's ring of copies
+constexpr int UNROLL = 3;          // 16-byte chunks of a stage
+constexpr int CAP = 4096;          // candidates of a CTA's slice, and of a row
+constexpr int RBINS = 1024;        // bins of their masses
+constexpr int MEMBERS = 1024;      // tokens of one bin that are put in order
+constexpr int MAX_K = 512;         // top-k that rows_kernel takes without min-p
 constexpr int MAX_G = 8;           // CTAs that share a row
 constexpr int HIST_CAP = 4096;     // history ids of a row that rows_kernel takes
 constexpr int WNT = 512;           // threads of wide_kernel
 constexpr int BINS = 2048;         // of a radix step
+constexpr int RING_BYTES = STAGES * UNROLL * NT * 16;
 constexpr int FILTER_WORDS = 4096; // bits that say which columns may be in the history
 
 struct Params {
@@ -144,9 +149,55 @@ __device__ __forceinline__ void write_error(const Params& P, int r, uint32_t sta
     write_row(P, r, -1, __int_as_float(0x7fc00000), 0, status);
 }
 
-// round(2^S e^(y - top))
-__device__ __forceinline__ uint64_t mass_of(float y, float top, double scale) {
-    return __double2ull_rn(exp(double(y) - double(top)) * scale);
+// Masses: round(2^S e^(y - top)), right to 2^-42 of the mass. 64-bit
+// exponentials at the rate of this machine's 64-bit units were the longest part of a row's
+// decisions (3900 candidates: 11 us of 60), so e^d is taken in pairs of 32-bit numbers, by
+// table and polynomial (P. T. P. Tang, "Table-driven implementation of the exponential
+// function in IEEE floating-point arithmetic", ACM TOMS 15(2), 1989): with n the nearest
+// integer to d 64 / log 2, e^d = 2^(n / 64) e^r and |r| <= log 2 / 128; the table has
+// 2^(j / 64) as pairs.
+struct ExpTable {
+    float2 v[64];
+    __device__ __forceinline__ void fill() {   // by the first 64 threads
+        if (threadIdx.x < 64) {
+            const double t = exp2(double(threadIdx.x) / 64.0);
+            const float hi = float(t);
+            v[threadIdx.x] = make_float2(hi, float(t - double(hi)));
+        }
+    }
+};
+__device__ __forceinline__ uint64_t mass_of(float y, float top, const ExpTable& T, int shift) {
+    // d = y - top exactly, as a pair
+    const float d = __fsub_rn(y, top), back = __fadd_rn(d, top);
+    const float dl = __fadd_rn(__fsub_rn(y, back), __fsub_rn(__fsub_rn(back, d), top));
+    if (!(d > -44.0f)) return 0;   // 2^-63
+    // log 2 / 64 in three parts, of which the first two have 12 bits: n takes no more
+    constexpr float kPerLog2 = 92.332482616893656877f;              // 64 / log 2
+    constexpr float kC1 = 0x1.62ep-7f, kC2 = 0x1.0cp-21f, kC3 = -2.9760223436840126e-11f;
+    const float n = rintf(d * kPerLog2);
+    float rh = fmaf(-n, kC2, fmaf(-n, kC1, d));                     // both steps exact
+    float rl = fmaf(-n, kC3, dl);
+    const float sum = __fadd_rn(rh, rl);
+    rl = __fadd_rn(__fsub_rn(rh, sum), rl);
+    rh = sum;
+    // e^r - 1 as a pair
+    const float q = __fmul_rn(rh, rh), ql = fmaf(rh, rh, -q);       // r^2
+    const float cubic = __fmul_rn(__fmul_rn(q, rh), fmaf(rh, fmaf(rh, 1.0f / 120.0f, 1.0f / 24.0f), 1.0f / 6.0f));
+    const float half = __fmul_rn(0.5f, q);
+    const float sh = __fadd_rn(rh, half);
+    const float sl = __fadd_rn(__fadd_rn(__fsub_rn(half, __fsub_rn(sh, rh)), fmaf(rl, rh, rl)), fmaf(0.5f, ql, cubic));
+    // 2^(n / 64) e^r in units of 2^-S: the table's part, its product's high part and the rest
+    const int k = int(n), j = k & 63;
+    const float2 t = T.v[j];
+    const float wh = __fmul_rn(t.x, sh);
+    const float wl = __fadd_rn(fmaf(t.x, sh, -wh), fmaf(t.x, sl, fmaf(t.y, sh, t.y)));
+    const int e = shift + ((k - j) >> 6);                            // 62 at most
+    if (e < -1) return 0;
+    // a unit of the sum is 2^-(62 - e) of the result's: its bits below that are rounded once
+    const float up = 0x1p62f;
+    const int64_t m = __float2ll_rn(t.x * (up * 0.25f)) + __float2ll_rn(wh * (up * 0.25f)) + __float2ll_rn(wl * (up * 0.25f));
+    const int down = 60 - e;                                         // m is in units of 2^-60
+    return down <= 0 ? uint64_t(m) << -down : (uint64_t(m) + (uint64_t(1) << (down - 1))) >> down;
 }
 // The smallest key that min-p keeps below a maximum of `top`: y >= top + log(min_p) in 64 bits.
 __device__ __forceinline__ uint32_t least_key(const Row& row, float top) {
@@ -213,12 +264,13 @@ struct Shared {
     uint32_t top;        // key of the largest (penalised) logit seen
     uint32_t least;      // key of a lower bound of the K-th largest logit
     uint32_t count;      // candidates
+    uint32_t count_out;  // of this slice, as the others read it
     uint32_t flags;      // row status bits
-    uint32_t n;          // sorted candidates
-    uint32_t nk, np, at;
+    uint32_t n;          // members of a bin
+    uint32_t bin, bin_count, before_count, kth;
+    uint64_t before_mass;
     uint32_t warp[NT / 32];
     uint64_t sums[NT / 32];
-    uint64_t total;
 };
 struct Candidate {
     float x;
@@ -241,6 +293,46 @@ __device__ __forceinline__ float chunk_max(const uint4& q) {
     }
 }
 
+// Counts and masses of bins, the masses as two words: 64-bit atomics on shared memory
+// serialise far more.
+struct Bins32 {
+    uint32_t *count, *lo, *hi;
+    __device__ __forceinline__ void add(uint32_t b, uint64_t m) const {
+        reds_add(&count[b], 1u);
+        const uint32_t l = uint32_t(m);
+        uint32_t h = uint32_t(m >> 32);
+        if (l) h += atoms_add(&lo[b], l) + l < l;
+        if (h) reds_add(&hi[b], h);
+    }
+    __device__ __forceinline__ uint64_t mass(uint32_t b) const { return uint64_t(hi[b]) << 32 | lo[b]; }
+};
+// The bin of y below the row's maximum: of equal width down to `span` (32 at most, where a
+// mass is a unit or nothing), the last one for all that lies further below. Every step is
+// monotone, so bins are in the order of their keys.
+__device__ __forceinline__ float bin_scale(double log_min_p, int bins) {
+    return float(bins - 1) / fmaxf(1e-3f, fminf(32.0f, float(-log_min_p)));
+}
+__device__ __forceinline__ uint32_t bin_of(float top, float y, float scale, int bins) {
+    return min(uint32_t(bins - 1), uint32_t((top - y) * scale));
+}
+
+// `n` (a power of two, at least 32) numbers in descending order, by all threads.
+template <int THREADS>
+__device__ __forceinline__ void sort_descending(uint64_t* v, int n) {
+    for (int size = 2; size <= n; size <<= 1)
+        for (int d = size >> 1; d > 0; d >>= 1) {
+            for (int i = threadIdx.x; i < n / 2; i += THREADS) {
+                const int a = 2 * i - (i & (d - 1)), b = a + d;
+                const uint64_t x = v[a], y = v[b];
+                if (((a & size) == 0) == (x < y)) {
+                    v[a] = y;
+                    v[b] = x;
+                }
+            }
+            __syncthreads();
+        }
+}
+
 // A bound below which no logit can be kept when the largest is `top`. The slack covers the
 // roundings of x / T, of the maximum's quotient and of this product.
 __device__ __forceinline__ float bound_of(const Row& row, float top, float span) {
@@ -248,25 +340,64 @@ __device__ __forceinline__ float bound_of(const Row& row, float top, float span)
     return top - span - 0x1p-20f * (fabsf(top) + span);
 }
 
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_committed() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_done() {
+    asm volatile("cp.async.wait_group %0;" :: "n"(LEFT) : "memory");
+}
+
+// One 16-byte word of four, picked by an index.
+__device__ __forceinline__ uint32_t word_of(const uint4& q, int i) {
+    const uint32_t a = i & 1 ? q.y : q.x, b = i & 1 ? q.w : q.z;
+    return i & 2 ? b : a;
+}
+
+// Dynamic shared memory: the ring of copies (after the stream: bins and members of a bin),
+// the candidates, the history's table.
 template <int DT>
-__global__ void __launch_bounds__(NT) rows_kernel(const Params P, const int G) {
+__global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G) {
     using E = Elem<DT>;
     constexpr int VEC = E::VEC;
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ Shared S;
-    Candidate* cand = reinterpret_cast<Candidate*>(dyn);
-    uint64_t* sorted = reinterpret_cast<uint64_t*>(dyn + CAP * sizeof(Candidate));
-    uint2* table = reinterpret_cast<uint2*>(dyn + CAP * (sizeof(Candidate) + 8));
+    __shared__ ExpTable T;
+    Candidate* cand = reinterpret_cast<Candidate*>(dyn + RING_BYTES);
+    uint2* table = reinterpret_cast<uint2*>(cand + CAP);
+    uint64_t* members = reinterpret_cast<uint64_t*>(dyn);
+    Bins32 bins;
+    bins.count = reinterpret_cast<uint32_t*>(members + MEMBERS);
+    bins.lo = bins.count + RBINS;
+    bins.hi = bins.lo + RBINS;
+    static_assert(MEMBERS * 8 + RBINS * 12 <= RING_BYTES, "bins and members take the ring's place");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int r = blockIdx.x / G;
     const uint32_t rank = G > 1 ? cluster_rank() : 0;
     wait_prerequisites();
     launch_dependents();
 
-    if (rank == 0 && tid == 0) P.marks[r] = 0;
+    const Geom g = row_geom<E::SIZE>(P.logits, P.row_stride, P.vocab, r);
+    const int nch = int(g.ibytes / 16);
+    const int ch0 = int(int64_t(nch) * rank / G), ch1 = int(int64_t(nch) * (rank + 1) / G);
+    const uint4* chunks = reinterpret_cast<const uint4*>(g.interior);
+    const uint32_t ring = smem_u32(dyn) + 16 * tid;       // this thread's places, NT chunks apart
+    // stage k of the slice: its chunks ch0 + (k UNROLL + i) NT + tid
+    auto fetch = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            const int c = ch0 + (k * UNROLL + i) * NT + tid;
+            if (c < ch1) copy_async(ring + (k % STAGES * UNROLL + i) * NT * 16, chunks + c);
+        }
+        copies_committed();
+    };
+    const int stages = (ch1 - ch0 + UNROLL * NT - 1) / (UNROLL * NT);
+
     const Row row = load_row(P, r);
-    // a lower bound of the K-th largest comes from K chunks of the first tile
-    const bool by_k = row.K > 0 && row.K <= CAP / 4;
+    if (rank == 0 && tid == 0) P.marks[r] = 0;
+    // a lower bound of the K-th largest comes from K chunks of the first stages
+    const bool by_k = row.K > 0 && row.K <= MAX_K;
     auto hand_on = [&]() {
         if (rank == 0 && tid == 0) P.marks[r] = 1;
     };
@@ -278,28 +409,18 @@ __global__ void __launch_bounds__(NT) rows_kernel(const Params P, const int G) {
         hand_on();
         return;
     }
-    const Geom g = row_geom<E::SIZE>(P.logits, P.row_stride, P.vocab, r);
-    const int nch = int(g.ibytes / 16);
-    const int ch0 = int(int64_t(nch) * rank / G), ch1 = int(int64_t(nch) * (rank + 1) / G);
+#pragma unroll
+    for (int k = 0; k < STAGES; ++k) fetch(k);
     const bool first = rank == 0, last = int(rank) == G - 1;
     const int c_lo = first ? 0 : g.head + ch0 * VEC, c_hi = last ? P.vocab : g.head + ch1 * VEC;
-    const uint4* chunks = reinterpret_cast<const uint4*>(g.interior);
     const uint32_t mask = uint32_t(P.slots) - 1u;
     const bool pen = row.p.pen;
-
-    // the first tile's loads go out before anything waits
-    uint4 q[UNROLL];
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i) {
-        const int c = ch0 + i * NT + tid;
-        if (c < ch1) q[i] = __ldg(chunks + c);
-    }
+    T.fill();
     if (tid == 0) {
         S.top = KEY_NEG_INF;
         S.least = KEY_NEG_INF;
         S.count = 0;
         S.flags = 0;
-        S.n = 0;
     }
     if (pen)
         for (int i = tid; i <= int(mask); i += NT) table[i] = make_uint2(kEmptySlot, 0u);
@@ -322,16 +443,23 @@ __global__ void __launch_bounds__(NT) rows_kernel(const Params P, const int G) {
     auto in_history = [&](uint32_t col) { return pen && find_slot(table, mask, col) >= 0; };
     const float span = row.greedy ? 0.0f : float(-row.log_min_p) * row.p.T;
 
-    // the first tile's maximum, over what is not in the history
+    // the first stage's maximum, over what is not in the history
     {
+        copies_done<STAGES - 1>();
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
             const int c = ch0 + i * NT + tid;
             if (c >= ch1) break;
-            if (!(chunk_max<DT>(q[i]) > top)) continue;
+            const uint4 q = lds_v4(ring + i * NT * 16);
+            const float m = chunk_max<DT>(q);
+            if (!(m > top)) continue;
+            if (!pen) {
+                top = m;
+                continue;
+            }
             float x[VEC];
-            E::unpack(q[i], x);
+            E::unpack(q, x);
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
                 if (x[j] > top && !in_history(uint32_t(g.head + c * VEC + j))) top = x[j];
@@ -340,26 +468,35 @@ __global__ void __launch_bounds__(NT) rows_kernel(const Params P, const int G) {
         if (lane == 0) atomicMax(&S.top, key);
         __syncthreads();
         if (by_k) {
-            // the largest key, to 2^-11 of its range, that K chunks of the tile reach (the K-th
-            // largest logit is no smaller); a chunk with history columns counts for none
-            uint32_t key_of[UNROLL];
+            // the largest key, to 2^-20 of its range, that K chunks of the ring reach: the K-th
+            // largest logit is no smaller. A chunk whose largest is in the history counts for none
+            copies_done<0>();
+            constexpr int HELD = STAGES * UNROLL;
+            uint32_t key_of[HELD];
 #pragma unroll
-            for (int i = 0; i < UNROLL; ++i) {
+            for (int i = 0; i < HELD; ++i) {
                 const int c = ch0 + i * NT + tid;
                 key_of[i] = 0u;
                 if (c >= ch1) continue;
-                bool clean = true;
-                if (pen)
-                    for (int j = 0; j < VEC; ++j) clean = clean && !in_history(uint32_t(g.head + c * VEC + j));
-                const float m = chunk_max<DT>(q[i]);
-                if (clean && m == m) key_of[i] = fkey(m);
+                const uint4 q = lds_v4(ring + i * NT * 16);
+                const float m = chunk_max<DT>(q);
+                bool clean = m == m;
+                if (pen) {
+                    float x[VEC];
+                    E::unpack(q, x);
+                    int at = 0;
+#pragma unroll
+                    for (int j = 1; j < VEC; ++j) at = x[j] == m ? j : at;
+                    clean = clean && !in_history(uint32_t(g.head + c * VEC + at));
+                }
+                if (clean) key_of[i] = fkey(m);
             }
             uint32_t lo = KEY_NEG_INF, hi = S.top;
-            for (int step = 0; step < 20 && hi - lo > 1u; ++step) {
+            for (int step = 0; step < 20 && hi > lo; ++step) {
                 const uint32_t mid = lo + (hi - lo + 1) / 2;
                 uint32_t n = 0;
 #pragma unroll
-                for (int i = 0; i < UNROLL; ++i) n += key_of[i] >= mid;
+                for (int i = 0; i < HELD; ++i) n += key_of[i] >= mid;
                 n = __reduce_add_sync(0xffffffffu, n);
                 if (lane == 0) S.warp[warp] = n;
                 __syncthreads();
@@ -381,61 +518,84 @@ __global__ void __launch_bounds__(NT) rows_kernel(const Params P, const int G) {
         const float x = funkey(key);
         if (by_k && x > -INFINITY) bound = fmaxf(bound, x - 0x1p-20f * fabsf(x));
     };
-    auto refresh = [&](uint32_t key) {
-        seen = funkey(key);
-        bound = bound_of(row, seen, span);
-        with_k(S.least);
-    };
-    auto take = [&](float x, uint32_t col) {     // a logit that is not below the bound, or NaN
-        if (!(x > -INFINITY)) {
+    // the logits of a warp, one a lane, that are not below the bound (or NaN) become candidates
+    auto take = [&](float x, uint32_t col, bool in) {
+        if (in && !(x > -INFINITY)) {
             if (x != x && !in_history(col)) atomicOr(&S.flags, uint32_t(FG_ROW_NAN));
-            return;
+            in = false;
         }
-        if (in_history(col)) return;
-        if (x > seen) atomicMax(&S.top, fkey(x));
-        const uint32_t at = atomicAdd(&S.count, 1u);
-        if (at < uint32_t(CAP)) cand[at] = {x, col};
+        in = in && !in_history(col);
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (who == 0) return;
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&S.count, __popc(who));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+        if (in && at < uint32_t(CAP)) cand[at] = {x, col};
+        if (__any_sync(0xffffffffu, in && x > seen)) {
+            const uint32_t key = __reduce_max_sync(0xffffffffu, in ? fkey(x) : 0u);
+            if (lane == 0) atomicMax(&S.top, key);
+        }
     };
-    auto scan_chunk = [&](const uint4& v, int c) {
-        if (chunk_max<DT>(v) < bound) return;
-        float x[VEC];
-        E::unpack(v, x);
+    // a chunk a lane (lane's is chunk c0 + lane): those that reach the bound are gone through by
+    // the warp, 32 / VEC of them at a time, one element a lane
+    auto scan = [&](const uint4& q, int c0, bool valid) {
+        uint32_t hits = __ballot_sync(0xffffffffu, valid && !(chunk_max<DT>(q) < bound));
+        while (hits) {
+            int src = -1;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if (!(x[j] < bound)) take(x[j], uint32_t(g.head + c * VEC + j));
+            for (int k = 0; k < 32 / VEC; ++k) {
+                const int b = __ffs(hits) - 1;      // -1: no more
+                if (lane / VEC == k) src = b;
+                hits &= hits - 1u;
+            }
+            const int from = max(src, 0), e = lane % VEC;
+            uint4 w;
+            w.x = __shfl_sync(0xffffffffu, q.x, from);
+            w.y = __shfl_sync(0xffffffffu, q.y, from);
+            w.z = __shfl_sync(0xffffffffu, q.z, from);
+            w.w = __shfl_sync(0xffffffffu, q.w, from);
+            float x;
+            if constexpr (DT == FG_DTYPE_F32) {
+                x = __uint_as_float(word_of(w, e));
+            } else {
+                const uint32_t word = word_of(w, e >> 1), half = e & 1 ? word >> 16 : word & 0xffffu;
+                if constexpr (DT == FG_DTYPE_F16) x = __half2float(__ushort_as_half(uint16_t(half)));
+                else x = __uint_as_float(half << 16);
+            }
+            take(x, uint32_t(g.head + (c0 + from) * VEC + e), src >= 0 && !(x < bound));
+        }
+    };
+    // columns [lo, hi) one by one (fewer than a chunk), by the first warp
+    auto scan_columns = [&](int lo, int hi) {
+        if (warp != 0) return;
+        for (int c = lo; c < hi; c += 32) {
+            const bool in = c + lane < hi;
+            const float x = in ? E::load(g.row, c + lane) : 0.0f;
+            take(x, uint32_t(c + lane), in && !(x < bound));
+        }
     };
     auto scan_ragged = [&]() {
-        if (first)
-            for (int c = tid; c < g.head; c += NT) {
-                const float x = E::load(g.row, c);
-                if (!(x < bound)) take(x, uint32_t(c));
-            }
-        if (last)
-            for (int c = g.tail0 + tid; c < P.vocab; c += NT) {
-                const float x = E::load(g.row, c);
-                if (!(x < bound)) take(x, uint32_t(c));
-            }
+        if (first) scan_columns(0, g.head);
+        if (last) scan_columns(g.tail0, P.vocab);
     };
-    refresh(S.top);
+    for (int k = 0; k < stages; ++k) {
+        copies_done<STAGES - 1>();
+        seen = funkey(*reinterpret_cast<volatile uint32_t*>(&S.top));
+        bound = bound_of(row, seen, span);
+        with_k(S.least);
 #pragma unroll
-    for (int i = 0; i < UNROLL; ++i) {
-        const int c = ch0 + i * NT + tid;
-        if (c < ch1) scan_chunk(q[i], c);
+        for (int i = 0; i < UNROLL; ++i) {
+            const int c = ch0 + (k * UNROLL + i) * NT + tid;
+            scan(lds_v4(ring + (k % STAGES * UNROLL + i) * NT * 16), c - lane, c < ch1);
+        }
+        fetch(k + STAGES);   // (past the slice: an empty group, which keeps the count)
     }
-    for (int base = ch0 + UNROLL * NT; base < ch1; base += UNROLL * NT) {
-#pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
-            const int c = base + i * NT + tid;
-            if (c < ch1) q[i] = __ldg(chunks + c);
-        }
-        refresh(*reinterpret_cast<volatile uint32_t*>(&S.top));
-#pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
-            const int c = base + i * NT + tid;
-            if (c < ch1) scan_chunk(q[i], c);
-        }
+    if (stages == 0) {
+        seen = funkey(S.top);
+        bound = bound_of(row, seen, span);
     }
     scan_ragged();
+    copies_done<0>();
     __syncthreads();
 
     // the whole row's maximum and flags
@@ -460,7 +620,10 @@ __global__ void __launch_bounds__(NT) rows_kernel(const Params P, const int G) {
         // too many while the maximum was still rising: once more with the final bound (from L2)
         if (tid == 0) S.count = 0;
         __syncthreads();
-        for (int c = ch0 + tid; c < ch1; c += NT) scan_chunk(__ldg(chunks + c), c);
+        for (int c0 = ch0 + 32 * warp; c0 < ch1; c0 += NT) {
+            const bool in = c0 + lane < ch1;
+            scan(in ? __ldg(chunks + c0 + lane) : make_uint4(0u, 0u, 0u, 0u), c0, in);
+        }
         scan_ragged();
         __syncthreads();
     }
@@ -473,9 +636,11 @@ __global__ void __launch_bounds__(NT) rows_kernel(const Params P, const int G) {
         }
         __syncthreads();
     }
+    if (tid == 0) S.count_out = S.count;
+    __syncthreads();
     if (G > 1) cluster_sync();                    // every slice's candidates stand
-    over = false;
-    for (int i = 0; i < G; ++i) over = over || (G > 1 ? ld_cluster(mapa(&S.count, i)) : S.count) > uint32_t(CAP);
+    over = S.count_out > uint32_t(CAP);
+    for (int i = 0; i < G && G > 1; ++i) over = over || ld_cluster(mapa(&S.count_out, i)) > uint32_t(CAP);
 
     if (rank == 0) {
         // greedy rows with NaN or without a finite maximum: wide_kernel knows their first place
@@ -488,120 +653,218 @@ __global__ void __launch_bounds__(NT) rows_kernel(const Params P, const int G) {
         } else if ((flags & FG_ROW_BAD_PARAM) || (!row.greedy && (errors || !(ydiv(row.p, top_x) < INFINITY)))) {
             if (tid == 0) write_error(P, r, errors ? flags | errors : flags | FG_ROW_POS_INF);
         } else {
-            // ---- the candidates, exactly: (key of y, ~column), so that larger comes first
+            // ---- the other slices' candidates come to this CTA; the keys of all of them
             const float top = ydiv(row.p, top_x);
             const uint32_t least_k = row.greedy ? top_key : least_key(row, top);
-            for (int i = 0; i < G; ++i) {
-                const uint32_t n = G > 1 ? ld_cluster(mapa(&S.count, i)) : S.count;
-                const uint32_t src = G > 1 ? mapa(cand, i) : smem_u32(cand);
+            for (int i = 1; i < G; ++i) {
+                const uint32_t n = ld_cluster(mapa(&S.count_out, i)), src = mapa(cand, i);
                 for (uint32_t j = tid; j < n; j += NT) {
                     const uint64_t c = ld_cluster64(src + 8 * j);   // {x, col}
-                    const uint32_t key = fkey(ydiv(row.p, __uint_as_float(uint32_t(c))));
-                    if (key < least_k) continue;
-                    const uint32_t at = atomicAdd(&S.n, 1u);
-                    if (at < uint32_t(CAP)) sorted[at] = uint64_t(key) << 32 | uint32_t(~uint32_t(c >> 32));
+                    if (fkey(ydiv(row.p, __uint_as_float(uint32_t(c)))) < least_k) continue;
+                    const uint32_t at = atomicAdd(&S.count, 1u);
+                    if (at < uint32_t(CAP)) cand[at] = {__uint_as_float(uint32_t(c)), uint32_t(c >> 32)};
                 }
             }
+            for (int i = tid; i < RBINS; i += NT) bins.count[i] = bins.lo[i] = bins.hi[i] = 0u;
             __syncthreads();
-            const int n = int(S.n);
+            const int n = int(S.count);
+            uint64_t* keys = reinterpret_cast<uint64_t*>(cand);      // in place: key, ~column; 0: not kept
+            const float per_bin = bin_scale(row.log_min_p, RBINS);
+            const uint32_t status = flags | (row.greedy ? uint32_t(FG_ROW_GREEDY) : 0u);
             if (n > CAP) {
                 hand_on();
-            } else {
-                int room = 32;
-                while (room < n) room <<= 1;
-                for (int i = n + tid; i < room; i += NT) sorted[i] = 0;
+            } else if (row.greedy) {
+                uint32_t col = 0xffffffffu;
+                for (int i = tid; i < n; i += NT)
+                    if (fkey(cand[i].x) == top_key) col = min(col, cand[i].col);
+                col = __reduce_min_sync(0xffffffffu, col);
+                if (lane == 0) S.warp[warp] = col;
                 __syncthreads();
-                // bitonic, descending
-                for (int size = 2; size <= room; size <<= 1)
-                    for (int d = size >> 1; d > 0; d >>= 1) {
-                        for (int i = tid; i < room / 2; i += NT) {
-                            const int a = 2 * i - (i & (d - 1)), b = a + d;
-                            const uint64_t u = sorted[a], v = sorted[b];
-                            if (((a & size) == 0) == (u < v)) {
-                                sorted[a] = v;
-                                sorted[b] = u;
-                            }
-                        }
-                        __syncthreads();
-                    }
-                const uint32_t status = flags | (row.greedy ? uint32_t(FG_ROW_GREEDY) : 0u);
-                if (row.greedy) {
-                    if (tid == 0) write_row(P, r, int64_t(~uint32_t(sorted[0])) + P.vocab_offset, 0.0f, 1, status);
-                } else {
-                    // each thread the masses of CAP / NT neighbours
-                    constexpr int PER = CAP / NT;
-                    const double scale = double(uint64_t(1) << P.mass_shift);
-                    const uint32_t kth = row.K > 0 && row.K < n ? uint32_t(sorted[row.K - 1] >> 32) : 0u;
-                    uint64_t m[PER], sum = 0;
-                    uint32_t mine = 0;
+                if (tid == 0) {
+                    for (int w = 1; w < NT / 32; ++w) col = min(col, S.warp[w]);
+                    write_row(P, r, int64_t(col), 0.0f, 1, status);
+                }
+            } else {
+                for (int i = tid; i < n; i += NT) {
+                    const Candidate c = cand[i];
+                    const float y = ydiv(row.p, c.x);
+                    const uint32_t key = fkey(y);
+                    keys[i] = key < least_k ? 0 : uint64_t(key) << 32 | uint32_t(~c.col);
+                    if (key >= least_k)
+                        bins.add(bin_of(top, y, per_bin, RBINS), mass_of(y, top, T, P.mass_shift));
+                }
+                __syncthreads();
+                // each thread PB neighbouring bins and what lies above them
+                constexpr int PB = RBINS / NT;
+                uint64_t bm[PB], above_m = 0, all = 0;
+                uint32_t bn[PB], above_n = 0, count = 0;
 #pragma unroll
-                    for (int j = 0; j < PER; ++j) {
-                        const int i = tid * PER + j;
-                        const uint32_t key = i < n ? uint32_t(sorted[i] >> 32) : 0u;
-                        const bool in = i < n && key >= kth;
-                        m[j] = in ? mass_of(funkey(key), top, scale) : 0;
-                        mine += in;
-                        sum += m[j];
+                for (int j = 0; j < PB; ++j) {
+                    bm[j] = bins.mass(tid * PB + j);
+                    bn[j] = bins.count[tid * PB + j];
+                    above_m += bm[j];
+                    above_n += bn[j];
+                }
+                {
+                    const uint64_t im = warp_incl_scan_u64(above_m, lane);
+                    const uint32_t in = warp_incl_scan_u32(above_n, lane);
+                    if (lane == 31) {
+                        S.sums[warp] = im;
+                        S.warp[warp] = in;
                     }
-                    uint64_t upto = warp_incl_scan_u64(sum, lane);
-                    mine = __reduce_add_sync(0xffffffffu, mine);
-                    if (lane == 31) S.sums[warp] = upto;
-                    if (lane == 0) S.warp[warp] = mine;
-                    if (tid == 0) S.at = 0xffffffffu;
                     __syncthreads();
-                    uint64_t total = 0, before = upto - sum;
-                    int nk = 0;
+                    above_m = im - above_m;
+                    above_n = in - above_n;
 #pragma unroll
                     for (int w = 0; w < NT / 32; ++w) {
-                        if (w < warp) before += S.sums[w];
-                        total += S.sums[w];
-                        nk += int(S.warp[w]);
+                        if (w < warp) {
+                            above_m += S.sums[w];
+                            above_n += S.warp[w];
+                        }
+                        all += S.sums[w];
+                        count += S.warp[w];
                     }
                     __syncthreads();
-                    // top-p: the tokens whose mass before them is within its share
-                    int np = nk;
-                    uint64_t kept = total;
-                    if (row.p.use_p) {
-                        const uint64_t limit = part_of(row.p.top_p, total);
-                        uint64_t at = before, part = 0;
-                        uint32_t count = 0;
+                }
+                // The members of the bin in which the count or mass from the top passes `target`, with
+                // their places in descending order: a few by counting what lies above each of them,
+                // more by sorting. False where there are too many.
+                constexpr int PM = MEMBERS / NT;
+                uint64_t mk[PM], mm[PM], mb[PM];  // this thread's members, their masses, the mass before each
+                int mi[PM];                       // their places in the bin; -1: none
+                auto open_bin = [&](bool by_mass, uint64_t target, uint32_t floor_key) {
+                    uint64_t m = above_m;
+                    uint32_t c = above_n;
 #pragma unroll
-                        for (int j = 0; j < PER; ++j) {
-                            if (tid * PER + j < nk && at <= limit) {
-                                ++count;
-                                part += m[j];
-                            }
-                            at += m[j];
+                    for (int j = 0; j < PB; ++j) {
+                        const uint64_t from = by_mass ? m : c, to = from + (by_mass ? bm[j] : bn[j]);
+                        if (from <= target && target < to) {
+                            S.bin = tid * PB + j;
+                            S.bin_count = bn[j];
+                            S.before_mass = m;
+                            S.before_count = c;
                         }
-                        count = __reduce_add_sync(0xffffffffu, count);
-                        part = warp_incl_scan_u64(part, lane);
-                        if (lane == 31) {
-                            S.sums[warp] = part;
-                            S.warp[warp] = count;
+                        m += bm[j];
+                        c += bn[j];
+                    }
+                    if (tid == 0) S.n = 0;
+                    __syncthreads();
+                    if (S.bin_count > uint32_t(MEMBERS)) return false;
+                    const uint32_t b = S.bin;
+                    for (int i = tid; i < n; i += NT) {
+                        const uint64_t k = keys[i];
+                        if (uint32_t(k >> 32) < floor_key || k == 0) continue;
+                        if (bin_of(top, funkey(uint32_t(k >> 32)), per_bin, RBINS) == b)
+                            members[atomicAdd(&S.n, 1u)] = k;
+                    }
+                    __syncthreads();
+                    const int have = int(S.n);
+#pragma unroll
+                    for (int j = 0; j < PM; ++j) mi[j] = -1;
+                    if (have <= 64) {
+                        uint64_t* masses = members + 64;
+                        if (tid < have) {
+                            mk[0] = members[tid];
+                            masses[tid] = mm[0] = mass_of(funkey(uint32_t(mk[0] >> 32)), top, T, P.mass_shift);
                         }
                         __syncthreads();
-                        np = 0;
-                        kept = 0;
+                        if (tid < have) {
+                            mb[0] = S.before_mass;
+                            mi[0] = 0;
+                            for (int i = 0; i < have; ++i)
+                                if (members[i] > mk[0]) {
+                                    ++mi[0];
+                                    mb[0] += masses[i];
+                                }
+                        }
+                        return true;
+                    }
+                    int room = 128;
+                    while (room < have) room <<= 1;
+                    for (int i = have + tid; i < room; i += NT) members[i] = 0;
+                    __syncthreads();
+                    sort_descending<NT>(members, room);
+                    uint64_t sum = 0;
 #pragma unroll
-                        for (int w = 0; w < NT / 32; ++w) {
-                            np += int(S.warp[w]);
-                            kept += S.sums[w];
+                    for (int j = 0; j < PM; ++j) {
+                        const int i = tid * PM + j;
+                        if (i < have) {
+                            mi[j] = i;
+                            mk[j] = members[i];
+                            mm[j] = mass_of(funkey(uint32_t(mk[j] >> 32)), top, T, P.mass_shift);
+                            sum += mm[j];
                         }
                     }
-                    const uint64_t target = part_of(row.p.u, kept);
-                    uint64_t at = before;
+                    const uint64_t im = warp_incl_scan_u64(sum, lane);
+                    if (lane == 31) S.sums[warp] = im;
+                    __syncthreads();
+                    uint64_t before = S.before_mass + im - sum;
+                    for (int w = 0; w < warp; ++w) before += S.sums[w];
 #pragma unroll
-                    for (int j = 0; j < PER; ++j) {
-                        at += m[j];
-                        if (tid * PER + j < np && at > target && at - m[j] <= target) S.at = tid * PER + j;
+                    for (int j = 0; j < PM; ++j)
+                        if (mi[j] >= 0) {
+                            mb[j] = before;
+                            before += mm[j];
+                        }
+                    __syncthreads();
+                    return true;
+                };
+                // what lies above the bin and the members that `in` says: their number and mass
+                auto count_members = [&](auto in, uint32_t& number, uint64_t& mass) {
+                    uint32_t c = 0;
+                    uint64_t m = 0;
+#pragma unroll
+                    for (int j = 0; j < PM; ++j)
+                        if (mi[j] >= 0 && in(mk[j], mb[j])) {
+                            ++c;
+                            m += mm[j];
+                        }
+                    c = __reduce_add_sync(0xffffffffu, c);
+                    m = warp_incl_scan_u64(m, lane);
+                    if (lane == 31) {
+                        S.sums[warp] = m;
+                        S.warp[warp] = c;
                     }
                     __syncthreads();
-                    if (tid == 0) {
-                        const uint64_t c = sorted[S.at];
-                        const double y = double(funkey(uint32_t(c >> 32))) - double(top);
-                        write_row(P, r, int64_t(~uint32_t(c)) + P.vocab_offset,
-                                  float(y - log(double(kept) / scale)), np, status);
+                    number = S.before_count;
+                    mass = S.before_mass;
+                    for (int w = 0; w < NT / 32; ++w) {
+                        number += S.warp[w];
+                        mass += S.sums[w];
                     }
+                    __syncthreads();
+                };
+                bool fits = true;
+                uint32_t floor_key = least_k;
+                if (row.K > 0 && uint32_t(row.K) < count) {
+                    fits = open_bin(false, uint64_t(row.K - 1), floor_key);
+                    if (fits) {
+#pragma unroll
+                        for (int j = 0; j < PM; ++j)
+                            if (mi[j] >= 0 && int(S.before_count) + mi[j] == row.K - 1) S.kth = uint32_t(mk[j] >> 32);
+                        __syncthreads();
+                        floor_key = S.kth;
+                        count_members([&](uint64_t k, uint64_t) { return uint32_t(k >> 32) >= floor_key; }, count, all);
+                    }
+                }
+                uint64_t kept = all;
+                if (fits && row.p.use_p) {
+                    const uint64_t limit = part_of(row.p.top_p, all);
+                    fits = open_bin(true, limit, floor_key);
+                    if (fits) count_members([&](uint64_t, uint64_t before) { return before <= limit; }, count, kept);
+                }
+                const uint64_t target = fits ? part_of(row.p.u, kept) : 0;
+                fits = fits && open_bin(true, target, floor_key);
+                if (fits) {
+#pragma unroll
+                    for (int j = 0; j < PM; ++j)
+                        if (mi[j] >= 0 && mb[j] <= target && target < mb[j] + mm[j]) {
+                            const double y = double(funkey(uint32_t(mk[j] >> 32))) - double(top);
+                            const double sum = double(kept) / double(uint64_t(1) << P.mass_shift);
+                            write_row(P, r, int64_t(~uint32_t(mk[j])), float(y - log(sum)), int(count), status);
+                        }
+                } else {
+                    hand_on();
                 }
             }
         }
@@ -622,27 +885,29 @@ struct WideShared {
     uint32_t top, arg, nan_col, flags;   // this CTA's, read by the others
     uint16_t rows[WNT];
     uint32_t ties;
-    uint32_t bin;
+    uint32_t n;                          // members that this CTA has found, read by the first
+    uint32_t bin, before_count, at_count;
     uint64_t before_mass, at_mass;
-    uint32_t before_count, at_count;
+    uint32_t key, found_count, found_at; // a search's result, read from the first CTA
+    uint64_t found_mass;
+    uint32_t first;                      // place of the key's first member
 };
-// The bins of one radix step: this CTA's, its share of the cluster's, and all of the cluster's.
+// The bins of one step: this CTA's, its share of the cluster's, and all of the cluster's
+// (of the steps by keys, and of the first one, which every search of the row begins with).
 struct Bins {
-    uint64_t* mass;
-    uint32_t* count;
+    Bins32 mine;
     uint64_t* own_mass;
-    uint32_t* own_count;
     uint64_t* all_mass;
+    uint64_t* top_mass;
+    uint32_t* own_count;
     uint32_t* all_count;
-    uint64_t* top_mass;          // of the highest bits, kept for every search of the row
     uint32_t* top_count;
 };
 constexpr int bins_bytes(int G) { return 12 * (3 * BINS + BINS / G); }
 
-// Where a search has come to: keys with `prefix` above `shift` bits, what lies above them.
+// What a search has found: a key, the columns that share it and what lies above it.
 struct Found {
-    uint32_t key;                // low bits cleared below `shift`
-    int shift;
+    uint32_t key;
     uint64_t before_mass, at_mass;
     uint32_t before_count, at_count;
 };
@@ -654,20 +919,25 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
     constexpr int NW = WNT / 32;
     extern __shared__ __align__(16) uint8_t dyn[];
     __shared__ WideShared S;
+    __shared__ ExpTable T;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = cluster_rank();
     const int per = BINS / G;
+    uint64_t* members = reinterpret_cast<uint64_t*>(dyn);   // of a bin: this CTA's, and in the first CTA all
+    uint64_t* all_members = members + MEMBERS;
     Bins B;
-    B.mass = reinterpret_cast<uint64_t*>(dyn);
-    B.all_mass = B.mass + BINS;
+    B.all_mass = all_members + MEMBERS;
     B.top_mass = B.all_mass + BINS;
     B.own_mass = B.top_mass + BINS;
-    B.count = reinterpret_cast<uint32_t*>(B.own_mass + per);
-    B.all_count = B.count + BINS;
+    B.mine.count = reinterpret_cast<uint32_t*>(B.own_mass + per);
+    B.mine.lo = B.mine.count + BINS;
+    B.mine.hi = B.mine.lo + BINS;
+    B.all_count = B.mine.hi + BINS;
     B.top_count = B.all_count + BINS;
     B.own_count = B.top_count + BINS;
     uint32_t* filter = B.own_count + per;
     uint32_t* cache = filter + (P.penalties ? FILTER_WORDS : 0);
+    T.fill();
     wait_prerequisites();
     uint2* table = P.tables + int64_t(blockIdx.x / G) * P.wide_slots;
     const uint32_t mask = uint32_t(P.wide_slots) - 1u;
@@ -840,29 +1110,23 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
             if (rank == 0 && tid == 0) write_error(P, r, status);
         } else {
             uint32_t floor_key = least_key(row, top);
-            // bins of the keys that are >= floor_key and share `at`'s bits above `shift + bits`
-            auto fill = [&](uint32_t at, int shift, int bits, uint64_t* all_mass, uint32_t* all_count) {
-                for (int i = tid; i < BINS; i += WNT) {
-                    B.mass[i] = 0;
-                    B.count[i] = 0;
-                }
+            const float per_bin = bin_scale(row.log_min_p, BINS);
+            // the cluster's bins of the keys for which `bin` gives one (below 0: none)
+            auto fill = [&](auto bin, uint64_t* all_mass, uint32_t* all_count) {
+                for (int i = tid; i < BINS; i += WNT) B.mine.count[i] = B.mine.lo[i] = B.mine.hi[i] = 0u;
                 __syncthreads();
-                const uint32_t above = shift + bits >= 32 ? 0u : 0xffffffffu << (shift + bits);
-                const uint32_t low = (1u << bits) - 1u;
                 each_key([&](int, uint32_t k) {
-                    if (k < floor_key || ((k ^ at) & above)) return;
-                    const uint32_t b = k >> shift & low;
-                    atomicAdd(&B.count[b], 1u);
-                    const uint64_t m = mass_of(funkey(k), top, scale);
-                    if (m) atomicAdd(reinterpret_cast<unsigned long long*>(&B.mass[b]), (unsigned long long)m);
+                    const int b = bin(k);
+                    if (b >= 0) B.mine.add(uint32_t(b), mass_of(funkey(k), top, T, P.mass_shift));
                 });
                 cluster_sync();
                 for (int i = tid; i < per; i += WNT) {
                     uint64_t m = 0;
                     uint32_t n = 0;
                     for (int c = 0; c < G; ++c) {
-                        m += ld_cluster64(mapa(&B.mass[rank * per + i], c));
-                        n += ld_cluster(mapa(&B.count[rank * per + i], c));
+                        const int at = int(rank) * per + i;
+                        m += uint64_t(ld_cluster(mapa(&B.mine.hi[at], c))) << 32 | ld_cluster(mapa(&B.mine.lo[at], c));
+                        n += ld_cluster(mapa(&B.mine.count[at], c));
                     }
                     B.own_mass[i] = m;
                     B.own_count[i] = n;
@@ -874,17 +1138,16 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
                 }
                 __syncthreads();
             };
-            // the first bin, from the top, up to whose end there are more than `target` (count or mass)
-            auto descend = [&](Found& f, int bits, bool by_mass, uint64_t target, const uint64_t* all_mass,
-                               const uint32_t* all_count) {
+            // the first bin up to whose end the count or mass passes `target`, `f` being what lies
+            // before the bins; then before that bin
+            auto locate = [&](Found& f, bool by_mass, uint64_t target, const uint64_t* all_mass, const uint32_t* all_count) {
                 constexpr int PB = BINS / WNT;
                 uint64_t m[PB], sm = 0;
                 uint32_t n[PB], sn = 0;
 #pragma unroll
                 for (int j = 0; j < PB; ++j) {
-                    const int b = BINS - 1 - (tid * PB + j);
-                    m[j] = all_mass[b];
-                    n[j] = all_count[b];
+                    m[j] = all_mass[tid * PB + j];
+                    n[j] = all_count[tid * PB + j];
                     sm += m[j];
                     sn += n[j];
                 }
@@ -905,7 +1168,7 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
                 for (int j = 0; j < PB; ++j) {
                     const uint64_t from = by_mass ? bm : bn, to = from + (by_mass ? m[j] : n[j]);
                     if (from <= target && target < to) {
-                        S.bin = uint32_t(BINS - 1 - (tid * PB + j));
+                        S.bin = uint32_t(tid * PB + j);
                         S.before_mass = bm;
                         S.before_count = bn;
                         S.at_mass = m[j];
@@ -915,23 +1178,114 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
                     bn += n[j];
                 }
                 __syncthreads();
-                f.shift -= bits;
-                f.key |= S.bin << f.shift;
                 f.before_mass = S.before_mass;
                 f.before_count = S.before_count;
                 f.at_mass = S.at_mass;
                 f.at_count = S.at_count;
+                const uint32_t b = S.bin;
                 __syncthreads();
+                return b;
             };
-            // the key at which the count or mass from the top passes `target`
-            fill(0u, 21, 11, B.top_mass, B.top_count);
+            auto top_bin = [&](uint32_t k) { return bin_of(top, funkey(k), per_bin, BINS); };
+            fill([&](uint32_t k) { return k >= floor_key ? int(top_bin(k)) : -1; }, B.top_mass, B.top_count);
+            // the key at which the count or mass from the top passes `target`; whether the first CTA has
+            // its bin's members in order
+            bool in_order = false;
             auto search = [&](bool by_mass, uint64_t target) {
-                Found f{0u, 32, 0, 0, 0, 0};
-                descend(f, 11, by_mass, target, B.top_mass, B.top_count);
-                fill(f.key, 10, 11, B.all_mass, B.all_count);
-                descend(f, 11, by_mass, target, B.all_mass, B.all_count);
-                fill(f.key, 0, 10, B.all_mass, B.all_count);
-                descend(f, 10, by_mass, target, B.all_mass, B.all_count);
+                Found f{0u, 0, 0, 0, 0};
+                const uint32_t b = locate(f, by_mass, target, B.top_mass, B.top_count);
+                in_order = f.at_count <= uint32_t(MEMBERS);
+                if (in_order) {
+                    if (tid == 0) S.n = 0;
+                    __syncthreads();
+                    each_key([&](int c, uint32_t k) {
+                        if (k >= floor_key && top_bin(k) == b)
+                            members[atomicAdd(&S.n, 1u)] = uint64_t(k) << 32 | uint32_t(~uint32_t(c));
+                    });
+                    cluster_sync();
+                    if (rank == 0) {
+                        int have = 0;
+                        for (int c = 0; c < G; ++c) {
+                            const int n = int(ld_cluster(mapa(&S.n, c)));
+                            for (int i = tid; i < n; i += WNT) all_members[have + i] = ld_cluster64(mapa(&members[i], c));
+                            have += n;
+                        }
+                        int room = 32;
+                        while (room < have) room <<= 1;
+                        for (int i = have + tid; i < room; i += WNT) all_members[i] = 0;
+                        __syncthreads();
+                        sort_descending<WNT>(all_members, room);
+                        // the element that passes the target, then all that share its key
+                        constexpr int PM = MEMBERS / WNT;
+                        uint64_t m[PM], sum = 0;
+#pragma unroll
+                        for (int j = 0; j < PM; ++j) {
+                            const int i = tid * PM + j;
+                            m[j] = i < have ? mass_of(funkey(uint32_t(all_members[i] >> 32)), top, T, P.mass_shift) : 0;
+                            sum += m[j];
+                        }
+                        const uint64_t im = warp_incl_scan_u64(sum, lane);
+                        if (lane == 31) S.red64[warp] = im;
+                        __syncthreads();
+                        uint64_t at = f.before_mass + im - sum;
+                        for (int w = 0; w < warp; ++w) at += S.red64[w];
+                        if (!by_mass) {
+                            if (tid == 0) S.key = uint32_t(all_members[target - f.before_count] >> 32);
+                        } else {
+                            uint64_t before = at;
+#pragma unroll
+                            for (int j = 0; j < PM; ++j) {
+                                if (before <= target && target < before + m[j])
+                                    S.key = uint32_t(all_members[tid * PM + j] >> 32);
+                                before += m[j];
+                            }
+                        }
+                        __syncthreads();
+                        const uint32_t key = S.key;
+                        uint32_t same = 0;
+#pragma unroll
+                        for (int j = 0; j < PM; ++j) {
+                            const int i = tid * PM + j;
+                            if (i < have && uint32_t(all_members[i] >> 32) == key) {
+                                ++same;
+                                if (i == 0 || uint32_t(all_members[i - 1] >> 32) != key) {
+                                    S.first = uint32_t(i);
+                                    S.found_count = f.before_count + uint32_t(i);
+                                    S.found_mass = at;
+                                }
+                            }
+                            at += m[j];
+                        }
+                        same = __reduce_add_sync(0xffffffffu, same);
+                        if (lane == 0) S.red32[warp] = same;
+                        __syncthreads();
+                        if (tid == 0) {
+                            for (int w = 1; w < NW; ++w) same += S.red32[w];
+                            S.found_at = same;
+                        }
+                        __syncthreads();
+                    }
+                    cluster_sync();
+                    f.key = ld_cluster(mapa(&S.key, 0));
+                    f.before_count = ld_cluster(mapa(&S.found_count, 0));
+                    f.before_mass = ld_cluster64(mapa(&S.found_mass, 0));
+                    f.at_count = ld_cluster(mapa(&S.found_at, 0));
+                    f.at_mass = f.at_count * mass_of(funkey(f.key), top, T, P.mass_shift);
+                    return f;
+                }
+                // many share the bin: by the keys' bits, highest first (the bins' order is descending)
+                uint32_t key = 0;
+                int shift = 32;
+                for (int bits : {11, 11, 10}) {
+                    const uint32_t above = shift == 32 ? 0u : 0xffffffffu << shift, low = (1u << bits) - 1u;
+                    const int to = shift - bits;
+                    fill([&](uint32_t k) {
+                        return k >= floor_key && ((k ^ key) & above) == 0u && top_bin(k) == b ? int(low - (k >> to & low)) : -1;
+                    }, B.all_mass, B.all_count);
+                    shift = to;
+                    key |= (low - locate(f, by_mass, target, B.all_mass, B.all_count)) << shift;
+                }
+                f.key = key;
                 return f;
             };
             // everything that min-p keeps
@@ -1018,7 +1372,11 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
                 cluster_sync();
                 return col;
             };
-            drawn = int(column_of(f.key, nth));
+            // (without probabilities the first CTA alone writes, and may know the place)
+            if (in_order && !P.out_probs)
+                drawn = rank == 0 ? int(~uint32_t(all_members[S.first + nth])) : 0;
+            else
+                drawn = int(column_of(f.key, nth));
             if (P.out_probs) cut_col = cut_ties == 0xffffffffu ? 0xffffffffu : column_of(cut_key, cut_ties - 1);
             if (rank == 0 && tid == 0) {
                 const double y = double(funkey(f.key)) - double(top);

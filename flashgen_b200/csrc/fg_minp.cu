@@ -67,9 +67,10 @@ template <int DT>
 int launch(fg::minp::Params P, DevInfo* d, cudaStream_t st) {
     using namespace fg::minp;
     static std::atomic<int> rows_smem[fg::host::kMaxDevices] = {}, wide_smem[fg::host::kMaxDevices] = {};
+    static std::atomic<int> uncached_smem[fg::host::kMaxDevices] = {};
     const int esz = fg::Elem<DT>::SIZE;
     const int G = ctas_per_row(P.batch, P.vocab, esz, d);
-    const int smem = RING_BYTES + CAP * int(sizeof(Candidate)) + (P.penalties ? P.slots * 8 : 0);
+    const int smem = RING_BYTES + CAP * int(sizeof(Candidate)) + (P.penalties ? P.slots * 8 + ROW_FILTER * 4 : 0);
     if (!set_smem(rows_kernel<DT>, rows_smem, smem)) return FG_EDEVICE;
     int rc = launch_early(rows_kernel<DT>, unsigned(P.batch) * G, NT, smem, G, st, P);
     if (rc != FG_OK) return rc;
@@ -78,15 +79,17 @@ int launch(fg::minp::Params P, DevInfo* d, cudaStream_t st) {
     auto fixed = [&](int g) { return 16 * MEMBERS + bins_bytes(g) + (P.penalties ? 4 * FILTER_WORDS : 0); };
     auto keys = [&](int g) {
         const int64_t chunks = int64_t(P.vocab) * esz / 16 + 1;
-        return (chunks + g - 1) / g * (16 / esz) + 2 * (16 / esz);
+        return (chunks + g - 1) / g * (16 / esz) + 2 * (16 / esz) + KEY_PAD;
     };
     const int room = d->smem_optin - int(sizeof(WideShared) + sizeof(ExpTable)) - 1024;
     const int W = P.batch > d->sms / 8 && fixed(4) + 4 * keys(4) <= room ? 4 : 8;
-    P.cache = fixed(W) + 4 * keys(W) <= room ? int(keys(W)) : 0;
-    const int wsmem = fixed(W) + 4 * P.cache;
-    if (!set_smem(wide_kernel<DT>, wide_smem, wsmem)) return FG_EDEVICE;
+    const bool cached = fixed(W) + 4 * keys(W) <= room;
+    const int wsmem = fixed(W) + (cached ? 4 * int(keys(W)) : 0);
+    if (!set_smem(cached ? wide_kernel<DT, true> : wide_kernel<DT, false>, cached ? wide_smem : uncached_smem, wsmem))
+        return FG_EDEVICE;
     const int clusters = std::min({int(P.batch), kMaxClusters, d->sms / W});
-    return launch_early(wide_kernel<DT>, unsigned(clusters * W), WNT, wsmem, W, st, P);
+    return launch_early(cached ? wide_kernel<DT, true> : wide_kernel<DT, false>, unsigned(clusters * W), WNT, wsmem, W,
+                        st, P);
 }
 
 }  // namespace

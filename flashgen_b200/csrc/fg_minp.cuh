@@ -31,7 +31,7 @@ constexpr int HIST_CAP = 4096;     // history ids of a row that rows_kernel take
 constexpr int WNT = 512;           // threads of wide_kernel
 constexpr int BINS = 2048;         // of a radix step
 constexpr int RING_BYTES = STAGES * UNROLL * NT * 16;
-constexpr int FILTER_WORDS = 4096; // bits that say which columns may be in the history
+constexpr int ROW_FILTER = 2048, FILTER_WORDS = 4096;   // words of bits that say which columns may be in the history
 
 struct Params {
     const void* logits;
@@ -60,7 +60,6 @@ struct Params {
     int32_t hist_max_len;
     int32_t slots, wide_slots; // of a history table (powers of two)
     int32_t mass_shift;        // S
-    int32_t cache;             // keys that wide_kernel keeps in shared memory (0: none)
 };
 
 __device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -225,7 +224,7 @@ __device__ __forceinline__ int find_slot(const uint2* table, uint32_t mask, uint
     return -1;
 }
 // Inserts the row's ids; all threads. The table is empty. Returns status bits.
-template <int THREADS>
+template <int THREADS, int WORDS>
 __device__ __forceinline__ uint32_t count_history(const Params& P, const Row& row, uint2* table, uint32_t mask,
                                                   int64_t c_lo, int64_t c_hi, uint32_t* filter) {
     uint32_t bad = 0;
@@ -246,10 +245,8 @@ __device__ __forceinline__ uint32_t count_history(const Params& P, const Row& ro
             h = (h + 1u) & mask;
         }
         if (!done) bad |= FG_ROW_BAD_PARAM;   // more distinct ids than hist_max_len allows
-        if (filter) {
-            const uint32_t b = uint32_t(c - c_lo) & (FILTER_WORDS * 32 - 1);
-            atomicOr(&filter[b >> 5], 1u << (b & 31));
-        }
+        const uint32_t b = uint32_t(c - c_lo) & (WORDS * 32 - 1);
+        atomicOr(&filter[b >> 5], 1u << (b & 31));
     }
     return bad;
 }
@@ -366,6 +363,7 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
     __shared__ ExpTable T;
     Candidate* cand = reinterpret_cast<Candidate*>(dyn + RING_BYTES);
     uint2* table = reinterpret_cast<uint2*>(cand + CAP);
+    uint32_t* filter = reinterpret_cast<uint32_t*>(table + P.slots);
     uint64_t* members = reinterpret_cast<uint64_t*>(dyn);
     Bins32 bins;
     bins.count = reinterpret_cast<uint32_t*>(members + MEMBERS);
@@ -422,33 +420,51 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
         S.count = 0;
         S.flags = 0;
     }
-    if (pen)
+    if (pen) {
         for (int i = tid; i <= int(mask); i += NT) table[i] = make_uint2(kEmptySlot, 0u);
+        for (int i = tid; i < ROW_FILTER; i += NT) filter[i] = 0u;
+    }
     __syncthreads();
     if (pen) {
-        const uint32_t bad = count_history<NT>(P, row, table, mask, c_lo, c_hi, nullptr);
+        const uint32_t bad = count_history<NT, ROW_FILTER>(P, row, table, mask, c_lo, c_hi, filter);
         if (bad) atomicOr(&S.flags, bad);
         __syncthreads();
         uint32_t top = KEY_NEG_INF;
-        for (int i = tid; i <= int(mask); i += NT) {
-            if (table[i].x == kEmptySlot) continue;
-            const float x = penalize(row.p, E::load(g.row, table[i].x), table[i].y);
-            table[i].y = __float_as_uint(x);
-            if (x != x) atomicOr(&S.flags, uint32_t(FG_ROW_NAN));
-            else top = max(top, fkey(x));
+        constexpr int AHEAD = 8;   // loads of logits in flight
+        for (int base = tid; base <= int(mask); base += AHEAD * NT) {
+            uint2 e[AHEAD];
+            float x[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                e[j] = base + j * NT <= int(mask) ? table[base + j * NT] : make_uint2(kEmptySlot, 0u);
+                x[j] = e[j].x != kEmptySlot ? E::load(g.row, e[j].x) : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                if (e[j].x == kEmptySlot) continue;
+                const float v = penalize(row.p, x[j], e[j].y);
+                table[base + j * NT].y = __float_as_uint(v);
+                if (v != v) atomicOr(&S.flags, uint32_t(FG_ROW_NAN));
+                else top = max(top, fkey(v));
+            }
         }
         top = __reduce_max_sync(0xffffffffu, top);
         if (lane == 0) atomicMax(&S.top, top);
     }
-    auto in_history = [&](uint32_t col) { return pen && find_slot(table, mask, col) >= 0; };
+    auto in_history = [&](uint32_t col) {
+        if (!pen) return false;
+        const uint32_t b = (col - uint32_t(c_lo)) & (ROW_FILTER * 32 - 1);
+        return (filter[b >> 5] >> (b & 31) & 1u) != 0u && find_slot(table, mask, col) >= 0;
+    };
     const float span = row.greedy ? 0.0f : float(-row.log_min_p) * row.p.T;
 
-    // the first stage's maximum, over what is not in the history
+    // the maximum of the ring's first filling, over what is not in the history
+    constexpr int HELD = STAGES * UNROLL;
     {
-        copies_done<STAGES - 1>();
+        copies_done<0>();
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
+        for (int i = 0; i < HELD; ++i) {
             const int c = ch0 + i * NT + tid;
             if (c >= ch1) break;
             const uint4 q = lds_v4(ring + i * NT * 16);
@@ -470,8 +486,6 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
         if (by_k) {
             // the largest key, to 2^-20 of its range, that K chunks of the ring reach: the K-th
             // largest logit is no smaller. A chunk whose largest is in the history counts for none
-            copies_done<0>();
-            constexpr int HELD = STAGES * UNROLL;
             uint32_t key_of[HELD];
 #pragma unroll
             for (int i = 0; i < HELD; ++i) {
@@ -578,55 +592,62 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
         if (first) scan_columns(0, g.head);
         if (last) scan_columns(g.tail0, P.vocab);
     };
-    for (int k = 0; k < stages; ++k) {
-        copies_done<STAGES - 1>();
-        seen = funkey(*reinterpret_cast<volatile uint32_t*>(&S.top));
-        bound = bound_of(row, seen, span);
-        with_k(S.least);
+    uint32_t top_key = 0, flags = 0;
+    bool sick = false;
+    // A second pass where too many logits reached the bounds of their moments: with the final
+    // bound (from L2)
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+        if (pass == 0) {
+            seen = funkey(S.top);
+            bound = bound_of(row, seen, span);
+            with_k(S.least);
+        }
+#pragma unroll 1
+        for (int k = 0; k < stages; ++k) {
+            copies_done<STAGES - 1>();
+            if (pass == 0) {
+                seen = funkey(*reinterpret_cast<volatile uint32_t*>(&S.top));
+                bound = bound_of(row, seen, span);
+                with_k(S.least);
+            }
 #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
-            const int c = ch0 + (k * UNROLL + i) * NT + tid;
-            scan(lds_v4(ring + (k % STAGES * UNROLL + i) * NT * 16), c - lane, c < ch1);
-        }
-        fetch(k + STAGES);   // (past the slice: an empty group, which keeps the count)
-    }
-    if (stages == 0) {
-        seen = funkey(S.top);
-        bound = bound_of(row, seen, span);
-    }
-    scan_ragged();
-    copies_done<0>();
-    __syncthreads();
-
-    // the whole row's maximum and flags
-    uint32_t top_key = S.top, flags = S.flags, least = S.least;
-    if (G > 1) {
-        cluster_sync();
-        for (int i = 0; i < G; ++i) {
-            top_key = max(top_key, ld_cluster(mapa(&S.top, i)));
-            least = max(least, ld_cluster(mapa(&S.least, i)));
-            flags |= ld_cluster(mapa(&S.flags, i));
-        }
-        // (S.top and S.flags stay as they are until the last cluster_sync)
-    }
-    const float top_x = funkey(top_key);
-    seen = INFINITY;                              // from here on nothing raises the maximum
-    bound = bound_of(row, top_x, span);
-    with_k(least);
-    bool over = S.count > uint32_t(CAP);
-    const bool sick = (flags & FG_ROW_NAN) || top_key <= KEY_NEG_INF || !(top_x < INFINITY);
-    __syncthreads();
-    if (over && !sick) {
-        // too many while the maximum was still rising: once more with the final bound (from L2)
-        if (tid == 0) S.count = 0;
-        __syncthreads();
-        for (int c0 = ch0 + 32 * warp; c0 < ch1; c0 += NT) {
-            const bool in = c0 + lane < ch1;
-            scan(in ? __ldg(chunks + c0 + lane) : make_uint4(0u, 0u, 0u, 0u), c0, in);
+            for (int i = 0; i < UNROLL; ++i) {
+                const int c = ch0 + (k * UNROLL + i) * NT + tid;
+                scan(lds_v4(ring + (k % STAGES * UNROLL + i) * NT * 16), c - lane, c < ch1);
+            }
+            fetch(k + STAGES);   // (past the slice: an empty group, which keeps the count)
         }
         scan_ragged();
+        copies_done<0>();
+        __syncthreads();
+        if (pass == 1) break;
+        // the whole row's maximum and flags
+        top_key = S.top;
+        flags = S.flags;
+        uint32_t least = S.least;
+        if (G > 1) {
+            cluster_sync();
+            const uint32_t peer = uint32_t(min(lane, G - 1));
+            top_key = __reduce_max_sync(0xffffffffu, ld_cluster(mapa(&S.top, peer)));
+            least = __reduce_max_sync(0xffffffffu, ld_cluster(mapa(&S.least, peer)));
+            flags = __reduce_or_sync(0xffffffffu, ld_cluster(mapa(&S.flags, peer)));
+            // (S.top and S.flags stay as they are until the last cluster_sync)
+        }
+        sick = (flags & FG_ROW_NAN) || top_key <= KEY_NEG_INF || !(funkey(top_key) < INFINITY);
+        seen = INFINITY;                          // from here on nothing raises the maximum
+        bound = bound_of(row, funkey(top_key), span);
+        with_k(least);
+        const bool over = S.count > uint32_t(CAP);
+        if (!over || sick) break;
+        __syncthreads();
+        if (tid == 0) S.count = 0;
+#pragma unroll
+        for (int k = 0; k < STAGES; ++k) fetch(k);
         __syncthreads();
     }
+    const float top_x = funkey(top_key);
+    __syncthreads();
     if (pen && !sick) {
         for (int i = tid; i <= int(mask); i += NT) {
             const float x = __uint_as_float(table[i].y);
@@ -639,8 +660,8 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
     if (tid == 0) S.count_out = S.count;
     __syncthreads();
     if (G > 1) cluster_sync();                    // every slice's candidates stand
-    over = S.count_out > uint32_t(CAP);
-    for (int i = 0; i < G && G > 1; ++i) over = over || ld_cluster(mapa(&S.count_out, i)) > uint32_t(CAP);
+    const uint32_t slice_count = lane < G ? (G > 1 ? ld_cluster(mapa(&S.count_out, uint32_t(lane))) : S.count_out) : 0u;
+    const bool over = __any_sync(0xffffffffu, slice_count > uint32_t(CAP));
 
     if (rank == 0) {
         // greedy rows with NaN or without a finite maximum: wide_kernel knows their first place
@@ -656,15 +677,17 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
             // ---- the other slices' candidates come to this CTA; the keys of all of them
             const float top = ydiv(row.p, top_x);
             const uint32_t least_k = row.greedy ? top_key : least_key(row, top);
-            for (int i = 1; i < G; ++i) {
-                const uint32_t n = ld_cluster(mapa(&S.count_out, i)), src = mapa(cand, i);
-                for (uint32_t j = tid; j < n; j += NT) {
+            const uint32_t of_warp = __shfl_sync(0xffffffffu, slice_count, warp % MAX_G);
+            if (warp > 0 && warp < G) {           // a warp each
+                const uint32_t src = mapa(cand, uint32_t(warp));
+                for (uint32_t j = lane; j < of_warp; j += 32) {
                     const uint64_t c = ld_cluster64(src + 8 * j);   // {x, col}
                     if (fkey(ydiv(row.p, __uint_as_float(uint32_t(c)))) < least_k) continue;
                     const uint32_t at = atomicAdd(&S.count, 1u);
                     if (at < uint32_t(CAP)) cand[at] = {__uint_as_float(uint32_t(c)), uint32_t(c >> 32)};
                 }
             }
+            static_assert(NT / 32 >= MAX_G, "a warp for each slice");
             for (int i = tid; i < RBINS; i += NT) bins.count[i] = bins.lo[i] = bins.hi[i] = 0u;
             __syncthreads();
             const int n = int(S.count);
@@ -873,11 +896,12 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
 }
 
 // ---------------------------------------------------------------------------
-// wide_kernel: the rows of the list, one after the other on clusters of G CTAs, each a
-// slice of the row. The first pass leaves the order-preserving key of every y in shared
-// memory (where it fits); then each decision is a radix search over the keys by count or
-// by mass: 2048 bins of the highest bits, then of the next ones among the keys that
-// share those, summed over the cluster through distributed shared memory.
+// wide_kernel: the rows that rows_kernel has marked, one after the other on clusters of G
+// CTAs, each a slice of the row. The first pass leaves the order-preserving key of every y in
+// shared memory (CACHED; where a slice does not fit, every pass works them out anew). Counts
+// and masses of all that min-p keeps go into 2048 bins of y, summed over the cluster through
+// distributed shared memory; each decision then looks for its bin and puts that bin's
+// members in order, or, where many share it (ties), searches by their keys' bits.
 // ---------------------------------------------------------------------------
 struct WideShared {
     uint32_t red32[WNT / 32];
@@ -904,6 +928,7 @@ struct Bins {
     uint32_t* top_count;
 };
 constexpr int bins_bytes(int G) { return 12 * (3 * BINS + BINS / G); }
+constexpr int KEY_PAD = 16;              // keys that a cache has beside a slice's
 
 // What a search has found: a key, the columns that share it and what lies above it.
 struct Found {
@@ -912,7 +937,221 @@ struct Found {
     uint32_t before_count, at_count;
 };
 
-template <int DT>
+// This CTA's slice of a row, and its keys.
+template <int DT, bool CACHED>
+struct Slice {
+    using E = Elem<DT>;
+    static constexpr int VEC = E::VEC;
+    const Row& row;
+    Geom g;
+    int ch0, ch1, c_lo, c_hi;
+    bool first, last;
+    const uint2* table;      // the history, and which columns may be in it
+    uint32_t mask;
+    const uint32_t* filter;
+    uint32_t* cache;         // key of column c at c - c_lo + skew: the chunks' keys on 16-byte boundaries
+    int skew;
+
+    // (greedy rows: of the penalised logit itself)
+    __device__ __forceinline__ uint32_t key_of(int c, float x, bool& nan) const {
+        if (row.p.pen) {
+            const uint32_t b = uint32_t(c - c_lo) & (FILTER_WORDS * 32 - 1);
+            if (filter[b >> 5] >> (b & 31) & 1u) {
+                const int at = find_slot(table, mask, uint32_t(c));
+                if (at >= 0) x = penalize(row.p, x, *reinterpret_cast<const volatile uint32_t*>(&table[at].y));
+            }
+        }
+        nan = x != x;
+        return nan ? 0u : fkey(ydiv(row.p, x));
+    }
+    // The logits' keys, eight (four) at a time and the ragged ones one by one: f(column, n, keys, which are NaN).
+    template <class F>
+    __device__ __forceinline__ void read(F f) const {
+        const int ragged = (first ? g.head : 0) + (last ? c_hi - g.tail0 : 0), heads = first ? g.head : 0;
+        if (int(threadIdx.x) < ragged) {    // fewer than a warp's lanes
+            const int c = int(threadIdx.x) < heads ? int(threadIdx.x) : g.tail0 + int(threadIdx.x) - heads;
+            bool nan;
+            uint32_t k[VEC];
+            k[0] = key_of(c, E::load(g.row, c), nan);
+            f(c, 1, k, nan ? 1u : 0u);
+        }
+        const uint4* chunks = reinterpret_cast<const uint4*>(g.interior);
+        for (int b = ch0; b < ch1; b += 4 * WNT) {
+            uint4 q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int ch = b + i * WNT + int(threadIdx.x);
+                if (ch < ch1) q[i] = __ldg(chunks + ch);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int ch = b + i * WNT + int(threadIdx.x);
+                if (ch >= ch1) continue;
+                float x[VEC];
+                E::unpack(q[i], x);
+                uint32_t k[VEC], nans = 0;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    bool nan;
+                    k[j] = key_of(g.head + ch * VEC + j, x[j], nan);
+                    nans |= uint32_t(nan) << j;
+                }
+                f(g.head + ch * VEC, VEC, k, nans);
+            }
+        }
+    }
+    // f(column, key) for every column of the slice (CACHED: after `read` has filled the cache)
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        if constexpr (CACHED) {
+#pragma unroll 4
+            for (int c = c_lo + int(threadIdx.x); c < c_hi; c += WNT) f(c, cache[c - c_lo + skew]);
+        } else {
+            read([&](int c, int n, const uint32_t* k, uint32_t) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (j < n) f(c + j, k[j]);
+            });
+        }
+    }
+    __device__ __forceinline__ uint32_t key_at(int c) const {
+        if constexpr (CACHED) return cache[c - c_lo + skew];
+        bool nan;
+        return key_of(c, E::load(g.row, c), nan);
+    }
+};
+
+// The cluster's counts and masses by `bin` (below 0: not counted), in every CTA.
+template <class S_, class F>
+__device__ __forceinline__ void fill_bins(const S_& slice, const Bins& B, int G, int rank, F bin, float top,
+                                          const ExpTable& T, int shift, uint64_t* all_mass, uint32_t* all_count) {
+    const int tid = threadIdx.x, per = BINS / G;
+    for (int i = tid; i < BINS; i += WNT) B.mine.count[i] = B.mine.lo[i] = B.mine.hi[i] = 0u;
+    __syncthreads();
+    slice.each([&](int, uint32_t k) {
+        const int b = bin(k);
+        if (b >= 0) B.mine.add(uint32_t(b), mass_of(funkey(k), top, T, shift));
+    });
+    cluster_sync();
+    for (int i = tid; i < per; i += WNT) {
+        const int at = rank * per + i;
+        uint32_t lo[MAX_G], hi[MAX_G], n[MAX_G];
+#pragma unroll
+        for (int c = 0; c < MAX_G; ++c) {
+            lo[c] = c < G ? ld_cluster(mapa(&B.mine.lo[at], c)) : 0u;
+            hi[c] = c < G ? ld_cluster(mapa(&B.mine.hi[at], c)) : 0u;
+            n[c] = c < G ? ld_cluster(mapa(&B.mine.count[at], c)) : 0u;
+        }
+        uint64_t m = 0;
+        uint32_t count = 0;
+#pragma unroll
+        for (int c = 0; c < MAX_G; ++c) {
+            m += uint64_t(hi[c]) << 32 | lo[c];
+            count += n[c];
+        }
+        B.own_mass[i] = m;
+        B.own_count[i] = count;
+    }
+    cluster_sync();
+#pragma unroll
+    for (int j = 0; j < BINS / WNT; ++j) {
+        const int i = j * WNT + tid;
+        all_mass[i] = ld_cluster64(mapa(&B.own_mass[i % per], i / per));
+        all_count[i] = ld_cluster(mapa(&B.own_count[i % per], i / per));
+    }
+    __syncthreads();
+}
+// The first bin up to whose end the count or mass passes `target`, f being what lies before the
+// bins; f is then what lies before that bin, and the bin's own.
+__device__ __forceinline__ uint32_t locate(WideShared& S, Found& f, bool by_mass, uint64_t target,
+                                           const uint64_t* all_mass, const uint32_t* all_count) {
+    constexpr int PB = BINS / WNT;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint64_t m[PB], sm = 0;
+    uint32_t n[PB], sn = 0;
+#pragma unroll
+    for (int j = 0; j < PB; ++j) {
+        m[j] = all_mass[tid * PB + j];
+        n[j] = all_count[tid * PB + j];
+        sm += m[j];
+        sn += n[j];
+    }
+    const uint64_t im = warp_incl_scan_u64(sm, lane);
+    const uint32_t in = warp_incl_scan_u32(sn, lane);
+    if (lane == 31) {
+        S.red64[warp] = im;
+        S.red32[warp] = in;
+    }
+    __syncthreads();
+    uint64_t bm = f.before_mass + im - sm;
+    uint32_t bn = f.before_count + in - sn;
+#pragma unroll
+    for (int w = 0; w < WNT / 32; ++w)
+        if (w < warp) {
+            bm += S.red64[w];
+            bn += S.red32[w];
+        }
+#pragma unroll
+    for (int j = 0; j < PB; ++j) {
+        const uint64_t from = by_mass ? bm : bn, to = from + (by_mass ? m[j] : n[j]);
+        if (from <= target && target < to) {
+            S.bin = uint32_t(tid * PB + j);
+            S.before_mass = bm;
+            S.before_count = bn;
+            S.at_mass = m[j];
+            S.at_count = n[j];
+        }
+        bm += m[j];
+        bn += n[j];
+    }
+    __syncthreads();
+    f.before_mass = S.before_mass;
+    f.before_count = S.before_count;
+    f.at_mass = S.at_mass;
+    f.at_count = S.at_count;
+    const uint32_t b = S.bin;
+    __syncthreads();
+    return b;
+}
+// The n-th column, in ascending order, that has key k, in every CTA.
+template <class S_>
+__device__ __forceinline__ uint32_t column_of(const S_& slice, WideShared& S, int G, int rank, uint32_t k, uint32_t n) {
+    // each thread a run of the slice's neighbours
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int len = slice.c_hi - slice.c_lo, step = (len + WNT - 1) / WNT;
+    const int a = slice.c_lo + min(len, tid * step), z = min(slice.c_hi, a + step);
+    uint32_t ties = 0;
+    for (int c = a; c < z; ++c) ties += slice.key_at(c) == k;
+    const uint32_t upto = warp_incl_scan_u32(ties, lane);
+    if (lane == 31) S.red32[warp] = upto;
+    __syncthreads();
+    uint32_t before = upto - ties, mine = 0;
+    for (int w = 0; w < WNT / 32; ++w) {
+        if (w < warp) before += S.red32[w];
+        mine += S.red32[w];
+    }
+    if (tid == 0) {
+        S.ties = mine;
+        S.bin = 0xffffffffu;
+    }
+    cluster_sync();
+    for (int c = 0; c < rank; ++c) before += ld_cluster(mapa(&S.ties, c));
+    if (before <= n && n < before + ties) {
+        uint32_t left = n - before;
+        for (int c = a; c < z; ++c)
+            if (slice.key_at(c) == k && left-- == 0) {
+                S.bin = uint32_t(c);
+                break;
+            }
+    }
+    cluster_sync();
+    uint32_t col = lane < G ? ld_cluster(mapa(&S.bin, lane)) : 0xffffffffu;
+    col = __reduce_min_sync(0xffffffffu, col);
+    cluster_sync();
+    return col;
+}
+
+template <int DT, bool CACHED>
 __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int G) {
     using E = Elem<DT>;
     constexpr int VEC = E::VEC;
@@ -921,7 +1160,7 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
     __shared__ WideShared S;
     __shared__ ExpTable T;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t rank = cluster_rank();
+    const int rank = int(cluster_rank());
     const int per = BINS / G;
     uint64_t* members = reinterpret_cast<uint64_t*>(dyn);   // of a bin: this CTA's, and in the first CTA all
     uint64_t* all_members = members + MEMBERS;
@@ -942,462 +1181,311 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
     uint2* table = P.tables + int64_t(blockIdx.x / G) * P.wide_slots;
     const uint32_t mask = uint32_t(P.wide_slots) - 1u;
 
-    // the rows that carry rows_kernel's mark, in ascending order, by turns to the clusters
+    // the marked rows, in ascending order, by turns to the clusters
     const int clusters = gridDim.x / G, mine_of = blockIdx.x / G;
     int marked = 0;   // so far
     for (int base = 0; base < P.batch; base += WNT) {
-      const bool mark = base + tid < P.batch &&
-                        *reinterpret_cast<const volatile uint8_t*>(&P.marks[base + tid]) != 0;
-      const uint32_t vote = __ballot_sync(0xffffffffu, mark);
-      __syncthreads();
-      if (lane == 0) S.red32[warp] = __popc(vote);
-      __syncthreads();
-      int at = __popc(vote & ((1u << lane) - 1u)), found = 0;
-      for (int w = 0; w < NW; ++w) {
-          if (w < warp) at += int(S.red32[w]);
-          found += int(S.red32[w]);
-      }
-      if (mark) S.rows[at] = uint16_t(tid);
-      __syncthreads();
-      // the first of them whose turn is this cluster's
-      int item = (mine_of - marked % clusters + clusters) % clusters;
-      marked += found;
-      for (; item < found; item += clusters) {
-        const int r = base + S.rows[item];
-        const Row row = load_row(P, r);
-        const Geom g = row_geom<E::SIZE>(P.logits, P.row_stride, P.vocab, r);
-        const int nch = int(g.ibytes / 16);
-        const int ch0 = int(int64_t(nch) * rank / G), ch1 = int(int64_t(nch) * (rank + 1) / G);
-        const bool first = rank == 0, last = int(rank) == G - 1;
-        const int c_lo = first ? 0 : g.head + ch0 * VEC, c_hi = last ? P.vocab : g.head + ch1 * VEC;
-        const bool pen = row.p.pen;
-        const bool cached = P.cache > 0;
+        const bool mark = base + tid < P.batch && P.marks[base + tid] != 0;
+        const uint32_t vote = __ballot_sync(0xffffffffu, mark);
+        __syncthreads();
+        if (lane == 0) S.red32[warp] = __popc(vote);
+        __syncthreads();
+        int at = __popc(vote & ((1u << lane) - 1u)), found = 0;
+        for (int w = 0; w < NW; ++w) {
+            if (w < warp) at += int(S.red32[w]);
+            found += int(S.red32[w]);
+        }
+        if (mark) S.rows[at] = uint16_t(tid);
+        __syncthreads();
+        // the first of them whose turn is this cluster's
+        int item = (mine_of - marked % clusters + clusters) % clusters;
+        marked += found;
+        for (; item < found; item += clusters) {
+            const int r = base + S.rows[item];
+            const Row row = load_row(P, r);
+            const Geom g = row_geom<E::SIZE>(P.logits, P.row_stride, P.vocab, r);
+            const int nch = int(g.ibytes / 16);
+            Slice<DT, CACHED> slice{row, g};
+            slice.ch0 = int(int64_t(nch) * rank / G);
+            slice.ch1 = int(int64_t(nch) * (rank + 1) / G);
+            slice.first = rank == 0;
+            slice.last = rank == G - 1;
+            slice.c_lo = slice.first ? 0 : g.head + slice.ch0 * VEC;
+            slice.c_hi = slice.last ? P.vocab : g.head + slice.ch1 * VEC;
+            slice.table = table;
+            slice.mask = mask;
+            slice.filter = filter;
+            slice.cache = cache;
+            slice.skew = slice.first ? (VEC - g.head % VEC) % VEC : 0;
+            const bool pen = row.p.pen;
 
-        if (tid == 0) {
-            S.flags = 0;
-            S.top = KEY_NEG_INF;
-            S.arg = 0xffffffffu;
-            S.nan_col = 0xffffffffu;
-        }
-        if (pen) {
-            // the cluster shares one table; its CTAs insert and look up columns of their own
-            for (int i = int(rank) * WNT + tid; i <= int(mask); i += G * WNT) table[i] = make_uint2(kEmptySlot, 0u);
-            for (int i = tid; i < FILTER_WORDS; i += WNT) filter[i] = 0u;
-        }
-        cluster_sync();
-        if (pen) {
-            const uint32_t bad = count_history<WNT>(P, row, table, mask, c_lo, c_hi, filter);
-            if (bad) atomicOr(&S.flags, bad);
-            __syncthreads();
-        }
-        // the key of column c (greedy rows: of the penalised logit itself)
-        auto key_at = [&](int c, float x, bool* nan) {
+            if (tid == 0) {
+                S.flags = 0;
+                S.top = KEY_NEG_INF;
+                S.arg = 0xffffffffu;
+                S.nan_col = 0xffffffffu;
+            }
             if (pen) {
-                const uint32_t b = uint32_t(c - c_lo) & (FILTER_WORDS * 32 - 1);
-                if (filter[b >> 5] >> (b & 31) & 1u) {
-                    const int s = find_slot(table, mask, uint32_t(c));
-                    if (s >= 0) x = penalize(row.p, x, *reinterpret_cast<const volatile uint32_t*>(&table[s].y));
-                }
+                // the cluster shares one table; its CTAs insert and look up columns of their own
+                for (int i = rank * WNT + tid; i <= int(mask); i += G * WNT) table[i] = make_uint2(kEmptySlot, 0u);
+                for (int i = tid; i < FILTER_WORDS; i += WNT) filter[i] = 0u;
             }
-            *nan = x != x;
-            return *nan ? 0u : fkey(ydiv(row.p, x));
-        };
-        // every column of the slice: f(column, key, nan), in no order
-        auto each = [&](auto f) {
-            if (first)
-                for (int c = tid; c < g.head; c += WNT) {
-                    bool nan;
-                    const uint32_t k = key_at(c, E::load(g.row, c), &nan);
-                    f(c, k, nan);
-                }
-            const uint4* chunks = reinterpret_cast<const uint4*>(g.interior);
-            for (int b = ch0; b < ch1; b += 4 * WNT) {
-                uint4 q[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int ch = b + i * WNT + tid;
-                    if (ch < ch1) q[i] = __ldg(chunks + ch);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int ch = b + i * WNT + tid;
-                    if (ch >= ch1) break;
-                    float x[VEC];
-                    E::unpack(q[i], x);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        bool nan;
-                        const int c = g.head + ch * VEC + j;
-                        const uint32_t k = key_at(c, x[j], &nan);
-                        f(c, k, nan);
-                    }
-                }
+            cluster_sync();
+            if (pen) {
+                const uint32_t bad = count_history<WNT, FILTER_WORDS>(P, row, table, mask, slice.c_lo, slice.c_hi, filter);
+                if (bad) atomicOr(&S.flags, bad);
+                __syncthreads();
             }
-            if (last)
-                for (int c = g.tail0 + tid; c < P.vocab; c += WNT) {
-                    bool nan;
-                    const uint32_t k = key_at(c, E::load(g.row, c), &nan);
-                    f(c, k, nan);
-                }
-        };
-        auto each_key = [&](auto f) {   // the same without the NaN
-            if (cached) {
-                for (int i = tid; i < c_hi - c_lo; i += WNT) f(c_lo + i, cache[i]);
-            } else {
-                each([&](int c, uint32_t k, bool) { f(c, k); });
-            }
-        };
-        // ---- keys, the maximum and its first column, the first NaN
-        {
-            uint32_t top = KEY_NEG_INF, arg = 0xffffffffu, nan_col = 0xffffffffu;
-            each([&](int c, uint32_t k, bool nan) {
-                if (cached) cache[c - c_lo] = k;
-                if (nan) nan_col = min(nan_col, uint32_t(c));
-                else if (k > top || (k == top && uint32_t(c) < arg)) {
-                    top = k;
-                    arg = uint32_t(c);
-                }
-            });
-            const uint32_t wtop = __reduce_max_sync(0xffffffffu, top);
-            const uint32_t warg = __reduce_min_sync(0xffffffffu, top == wtop ? arg : 0xffffffffu);
-            nan_col = __reduce_min_sync(0xffffffffu, nan_col);
-            if (lane == 0) {
-                S.red32[warp] = wtop;
-                S.red64[warp] = warg;
-                if (nan_col != 0xffffffffu) atomicMin(&S.nan_col, nan_col);
-            }
-            __syncthreads();
-            if (tid == 0)
-                for (int w = 0; w < NW; ++w)
-                    if (S.red32[w] > S.top || (S.red32[w] == S.top && uint32_t(S.red64[w]) < S.arg)) {
-                        S.top = S.red32[w];
-                        S.arg = uint32_t(S.red64[w]);
-                    }
-        }
-        cluster_sync();
-        uint32_t top_key = KEY_NEG_INF, arg = 0xffffffffu, nan_col = 0xffffffffu, flags = 0;
-        for (int i = 0; i < G; ++i) {
-            const uint32_t k = ld_cluster(mapa(&S.top, i)), a = ld_cluster(mapa(&S.arg, i));
-            if (k > top_key || (k == top_key && a < arg)) {
-                top_key = k;
-                arg = a;
-            }
-            nan_col = min(nan_col, ld_cluster(mapa(&S.nan_col, i)));
-            flags |= ld_cluster(mapa(&S.flags, i));
-        }
-        const float top = funkey(top_key);
-        uint32_t errors = row.p.bad | (flags & FG_ROW_BAD_PARAM);
-        if (!row.greedy) {
-            if (nan_col != 0xffffffffu) errors |= FG_ROW_NAN;
-            else if (top_key <= KEY_NEG_INF) errors |= FG_ROW_ALL_MASKED;
-            else if (!(top < INFINITY)) errors |= FG_ROW_POS_INF;
-        }
-        const uint32_t status = flags | errors | FG_ROW_GENERAL_PATH | (row.greedy ? uint32_t(FG_ROW_GREEDY) : 0u);
-        // what is drawn: the column's key, and the kept set: keys above cut_key, and at cut_key the
-        // columns up to cut_col
-        int drawn = -1;
-        uint32_t cut_key = 0, cut_col = 0, kept_count = 0;
-        uint64_t kept = 0;
-        const double scale = double(uint64_t(1) << P.mass_shift);
-        if (!errors && row.greedy) {
-            // the first NaN counts as the maximum; a row of -inf has its first column
-            drawn = int(nan_col != 0xffffffffu ? nan_col : arg);
-            if (rank == 0 && tid == 0) write_row(P, r, drawn + P.vocab_offset, 0.0f, 1, status);
-            cut_key = nan_col != 0xffffffffu ? 0xffffffffu : top_key;
-            cut_col = uint32_t(drawn);
-            kept = uint64_t(1) << P.mass_shift;
-        } else if (errors) {
-            if (rank == 0 && tid == 0) write_error(P, r, status);
-        } else {
-            uint32_t floor_key = least_key(row, top);
-            const float per_bin = bin_scale(row.log_min_p, BINS);
-            // the cluster's bins of the keys for which `bin` gives one (below 0: none)
-            auto fill = [&](auto bin, uint64_t* all_mass, uint32_t* all_count) {
-                for (int i = tid; i < BINS; i += WNT) B.mine.count[i] = B.mine.lo[i] = B.mine.hi[i] = 0u;
-                __syncthreads();
-                each_key([&](int, uint32_t k) {
-                    const int b = bin(k);
-                    if (b >= 0) B.mine.add(uint32_t(b), mass_of(funkey(k), top, T, P.mass_shift));
-                });
-                cluster_sync();
-                for (int i = tid; i < per; i += WNT) {
-                    uint64_t m = 0;
-                    uint32_t n = 0;
-                    for (int c = 0; c < G; ++c) {
-                        const int at = int(rank) * per + i;
-                        m += uint64_t(ld_cluster(mapa(&B.mine.hi[at], c))) << 32 | ld_cluster(mapa(&B.mine.lo[at], c));
-                        n += ld_cluster(mapa(&B.mine.count[at], c));
-                    }
-                    B.own_mass[i] = m;
-                    B.own_count[i] = n;
-                }
-                cluster_sync();
-                for (int i = tid; i < BINS; i += WNT) {
-                    all_mass[i] = ld_cluster64(mapa(&B.own_mass[i % per], i / per));
-                    all_count[i] = ld_cluster(mapa(&B.own_count[i % per], i / per));
-                }
-                __syncthreads();
-            };
-            // the first bin up to whose end the count or mass passes `target`, `f` being what lies
-            // before the bins; then before that bin
-            auto locate = [&](Found& f, bool by_mass, uint64_t target, const uint64_t* all_mass, const uint32_t* all_count) {
-                constexpr int PB = BINS / WNT;
-                uint64_t m[PB], sm = 0;
-                uint32_t n[PB], sn = 0;
+            // ---- keys, the maximum and its first column, the first NaN
+            {
+                uint32_t top = KEY_NEG_INF, arg = 0xffffffffu, nan_col = 0xffffffffu;
+                slice.read([&](int c, int n, const uint32_t* k, uint32_t nans) {
+                    if constexpr (CACHED) {
+                        uint32_t* to = cache + (c - slice.c_lo + slice.skew);
+                        if (n == VEC) {
 #pragma unroll
-                for (int j = 0; j < PB; ++j) {
-                    m[j] = all_mass[tid * PB + j];
-                    n[j] = all_count[tid * PB + j];
-                    sm += m[j];
-                    sn += n[j];
-                }
-                const uint64_t im = warp_incl_scan_u64(sm, lane);
-                const uint32_t in = warp_incl_scan_u32(sn, lane);
-                if (lane == 31) {
-                    S.red64[warp] = im;
-                    S.red32[warp] = in;
-                }
-                __syncthreads();
-                uint64_t bm = f.before_mass + im - sm;
-                uint32_t bn = f.before_count + in - sn;
-                for (int w = 0; w < warp; ++w) {
-                    bm += S.red64[w];
-                    bn += S.red32[w];
-                }
-#pragma unroll
-                for (int j = 0; j < PB; ++j) {
-                    const uint64_t from = by_mass ? bm : bn, to = from + (by_mass ? m[j] : n[j]);
-                    if (from <= target && target < to) {
-                        S.bin = uint32_t(tid * PB + j);
-                        S.before_mass = bm;
-                        S.before_count = bn;
-                        S.at_mass = m[j];
-                        S.at_count = n[j];
-                    }
-                    bm += m[j];
-                    bn += n[j];
-                }
-                __syncthreads();
-                f.before_mass = S.before_mass;
-                f.before_count = S.before_count;
-                f.at_mass = S.at_mass;
-                f.at_count = S.at_count;
-                const uint32_t b = S.bin;
-                __syncthreads();
-                return b;
-            };
-            auto top_bin = [&](uint32_t k) { return bin_of(top, funkey(k), per_bin, BINS); };
-            fill([&](uint32_t k) { return k >= floor_key ? int(top_bin(k)) : -1; }, B.top_mass, B.top_count);
-            // the key at which the count or mass from the top passes `target`; whether the first CTA has
-            // its bin's members in order
-            bool in_order = false;
-            auto search = [&](bool by_mass, uint64_t target) {
-                Found f{0u, 0, 0, 0, 0};
-                const uint32_t b = locate(f, by_mass, target, B.top_mass, B.top_count);
-                in_order = f.at_count <= uint32_t(MEMBERS);
-                if (in_order) {
-                    if (tid == 0) S.n = 0;
-                    __syncthreads();
-                    each_key([&](int c, uint32_t k) {
-                        if (k >= floor_key && top_bin(k) == b)
-                            members[atomicAdd(&S.n, 1u)] = uint64_t(k) << 32 | uint32_t(~uint32_t(c));
-                    });
-                    cluster_sync();
-                    if (rank == 0) {
-                        int have = 0;
-                        for (int c = 0; c < G; ++c) {
-                            const int n = int(ld_cluster(mapa(&S.n, c)));
-                            for (int i = tid; i < n; i += WNT) all_members[have + i] = ld_cluster64(mapa(&members[i], c));
-                            have += n;
-                        }
-                        int room = 32;
-                        while (room < have) room <<= 1;
-                        for (int i = have + tid; i < room; i += WNT) all_members[i] = 0;
-                        __syncthreads();
-                        sort_descending<WNT>(all_members, room);
-                        // the element that passes the target, then all that share its key
-                        constexpr int PM = MEMBERS / WNT;
-                        uint64_t m[PM], sum = 0;
-#pragma unroll
-                        for (int j = 0; j < PM; ++j) {
-                            const int i = tid * PM + j;
-                            m[j] = i < have ? mass_of(funkey(uint32_t(all_members[i] >> 32)), top, T, P.mass_shift) : 0;
-                            sum += m[j];
-                        }
-                        const uint64_t im = warp_incl_scan_u64(sum, lane);
-                        if (lane == 31) S.red64[warp] = im;
-                        __syncthreads();
-                        uint64_t at = f.before_mass + im - sum;
-                        for (int w = 0; w < warp; ++w) at += S.red64[w];
-                        if (!by_mass) {
-                            if (tid == 0) S.key = uint32_t(all_members[target - f.before_count] >> 32);
+                            for (int j = 0; j < VEC; j += 4)
+                                *reinterpret_cast<uint4*>(to + j) = make_uint4(k[j], k[j + 1], k[j + 2], k[j + 3]);
                         } else {
-                            uint64_t before = at;
+                            to[0] = k[0];
+                        }
+                    }
+                    if (nans) nan_col = min(nan_col, uint32_t(c) + uint32_t(__ffs(nans) - 1));
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        if (j < n && !(nans >> j & 1u) && (k[j] > top || (k[j] == top && uint32_t(c + j) < arg))) {
+                            top = k[j];
+                            arg = uint32_t(c + j);
+                        }
+                });
+                const uint32_t wtop = __reduce_max_sync(0xffffffffu, top);
+                const uint32_t warg = __reduce_min_sync(0xffffffffu, top == wtop ? arg : 0xffffffffu);
+                nan_col = __reduce_min_sync(0xffffffffu, nan_col);
+                if (lane == 0) {
+                    S.red32[warp] = wtop;
+                    S.red64[warp] = warg;
+                    if (nan_col != 0xffffffffu) atomicMin(&S.nan_col, nan_col);
+                }
+                __syncthreads();
+                if (tid == 0)
+                    for (int w = 0; w < NW; ++w)
+                        if (S.red32[w] > S.top || (S.red32[w] == S.top && uint32_t(S.red64[w]) < S.arg)) {
+                            S.top = S.red32[w];
+                            S.arg = uint32_t(S.red64[w]);
+                        }
+            }
+            cluster_sync();
+            const uint32_t peer = uint32_t(min(lane, G - 1));
+            uint32_t top_key = ld_cluster(mapa(&S.top, peer)), arg = ld_cluster(mapa(&S.arg, peer));
+            uint32_t nan_col = ld_cluster(mapa(&S.nan_col, peer)), flags = ld_cluster(mapa(&S.flags, peer));
+            {
+                const uint32_t k = __reduce_max_sync(0xffffffffu, top_key);
+                arg = __reduce_min_sync(0xffffffffu, top_key == k ? arg : 0xffffffffu);
+                top_key = k;
+                nan_col = __reduce_min_sync(0xffffffffu, nan_col);
+                flags = __reduce_or_sync(0xffffffffu, flags);
+            }
+            const float top = funkey(top_key);
+            uint32_t errors = row.p.bad | (flags & FG_ROW_BAD_PARAM);
+            if (!row.greedy) {
+                if (nan_col != 0xffffffffu) errors |= FG_ROW_NAN;
+                else if (top_key <= KEY_NEG_INF) errors |= FG_ROW_ALL_MASKED;
+                else if (!(top < INFINITY)) errors |= FG_ROW_POS_INF;
+            }
+            const uint32_t status = flags | errors | FG_ROW_GENERAL_PATH | (row.greedy ? uint32_t(FG_ROW_GREEDY) : 0u);
+            // what is drawn, and the kept set: keys above cut_key, and at cut_key the columns up to cut_col
+            int drawn = -1;
+            uint32_t cut_key = 0, cut_col = 0;
+            uint64_t kept = 0;
+            const double unit = double(uint64_t(1) << P.mass_shift);
+            if (!errors && row.greedy) {
+                // the first NaN counts as the maximum; a row of -inf has its first column
+                drawn = int(nan_col != 0xffffffffu ? nan_col : arg);
+                if (rank == 0 && tid == 0) write_row(P, r, drawn, 0.0f, 1, status);
+            } else if (errors) {
+                if (rank == 0 && tid == 0) write_error(P, r, status);
+            } else {
+                uint32_t floor_key = least_key(row, top);
+                const float per_bin = bin_scale(row.log_min_p, BINS);
+                auto top_bin = [&](uint32_t k) { return bin_of(top, funkey(k), per_bin, BINS); };
+                fill_bins(slice, B, G, rank, [&](uint32_t k) { return k >= floor_key ? int(top_bin(k)) : -1; }, top, T,
+                          P.mass_shift, B.top_mass, B.top_count);
+                // everything that min-p keeps
+                uint64_t all = 0;
+                uint32_t count = 0;
+#pragma unroll
+                for (int j = 0; j < BINS / WNT; ++j) {
+                    all += B.top_mass[j * WNT + tid];
+                    count += B.top_count[j * WNT + tid];
+                }
+                all = warp_incl_scan_u64(all, lane);
+                count = __reduce_add_sync(0xffffffffu, count);
+                if (lane == 31) {
+                    S.red64[warp] = all;
+                    S.red32[warp] = count;
+                }
+                __syncthreads();
+                all = 0;
+                count = 0;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    all += S.red64[w];
+                    count += S.red32[w];
+                }
+                __syncthreads();
+                kept = all;
+                cut_key = floor_key;
+                uint32_t kept_count = count, cut_ties = 0xffffffffu;   // of the columns at cut_key
+                // top-k (0), the top-p cut (1), the draw (2)
+#pragma unroll 1
+                for (int step = 0; step < 3; ++step) {
+                    if (step == 0 && !(row.K > 0 && uint32_t(row.K) < count)) continue;
+                    if (step == 1 && !row.p.use_p) continue;
+                    const bool by_mass = step > 0;
+                    const uint64_t target = step == 0   ? uint64_t(row.K - 1)
+                                            : step == 1 ? part_of(row.p.top_p, all)
+                                                        : part_of(row.p.u, kept);
+                    // the key at which the count or mass from the top passes the target
+                    Found f{0u, 0, 0, 0, 0};
+                    const uint32_t b = locate(S, f, by_mass, target, B.top_mass, B.top_count);
+                    const bool in_order = f.at_count <= uint32_t(MEMBERS);
+                    if (in_order) {
+                        if (tid == 0) S.n = 0;
+                        __syncthreads();
+                        slice.each([&](int c, uint32_t k) {
+                            if (k >= floor_key && top_bin(k) == b)
+                                members[atomicAdd(&S.n, 1u)] = uint64_t(k) << 32 | uint32_t(~uint32_t(c));
+                        });
+                        cluster_sync();
+                        if (rank == 0) {
+                            // a warp or two for each CTA's members, behind those of the CTAs before it
+                            const uint32_t n = lane < G ? ld_cluster(mapa(&S.n, uint32_t(lane))) : 0u;
+                            const uint32_t upto = warp_incl_scan_u32(n, lane);
+                            const int have = int(__shfl_sync(0xffffffffu, upto, 31));
+                            const int c = warp % G;
+                            const int cn = int(__shfl_sync(0xffffffffu, n, c)), to = int(__shfl_sync(0xffffffffu, upto, c)) - cn;
+                            for (int i = warp / G * 32 + lane; i < cn; i += NW / G * 32)
+                                all_members[to + i] = ld_cluster64(mapa(&members[i], uint32_t(c)));
+                            int room = 32;
+                            while (room < have) room <<= 1;
+                            for (int i = have + tid; i < room; i += WNT) all_members[i] = 0;
+                            __syncthreads();
+                            sort_descending<WNT>(all_members, room);
+                            // the element that passes the target, then all that share its key
+                            constexpr int PM = MEMBERS / WNT;
+                            uint64_t m[PM], sum = 0;
 #pragma unroll
                             for (int j = 0; j < PM; ++j) {
-                                if (before <= target && target < before + m[j])
-                                    S.key = uint32_t(all_members[tid * PM + j] >> 32);
-                                before += m[j];
+                                const int i = tid * PM + j;
+                                m[j] = i < have ? mass_of(funkey(uint32_t(all_members[i] >> 32)), top, T, P.mass_shift) : 0;
+                                sum += m[j];
                             }
-                        }
-                        __syncthreads();
-                        const uint32_t key = S.key;
-                        uint32_t same = 0;
+                            const uint64_t im = warp_incl_scan_u64(sum, lane);
+                            if (lane == 31) S.red64[warp] = im;
+                            __syncthreads();
+                            uint64_t at_mass = f.before_mass + im - sum;
+                            for (int w = 0; w < warp; ++w) at_mass += S.red64[w];
+                            if (!by_mass) {
+                                if (tid == 0) S.key = uint32_t(all_members[target - f.before_count] >> 32);
+                            } else {
+                                uint64_t before = at_mass;
 #pragma unroll
-                        for (int j = 0; j < PM; ++j) {
-                            const int i = tid * PM + j;
-                            if (i < have && uint32_t(all_members[i] >> 32) == key) {
-                                ++same;
-                                if (i == 0 || uint32_t(all_members[i - 1] >> 32) != key) {
-                                    S.first = uint32_t(i);
-                                    S.found_count = f.before_count + uint32_t(i);
-                                    S.found_mass = at;
+                                for (int j = 0; j < PM; ++j) {
+                                    if (before <= target && target < before + m[j])
+                                        S.key = uint32_t(all_members[tid * PM + j] >> 32);
+                                    before += m[j];
                                 }
                             }
-                            at += m[j];
+                            __syncthreads();
+                            const uint32_t key = S.key;
+                            uint32_t same = 0;
+#pragma unroll
+                            for (int j = 0; j < PM; ++j) {
+                                const int i = tid * PM + j;
+                                if (i < have && uint32_t(all_members[i] >> 32) == key) {
+                                    ++same;
+                                    if (i == 0 || uint32_t(all_members[i - 1] >> 32) != key) {
+                                        S.first = uint32_t(i);
+                                        S.found_count = f.before_count + uint32_t(i);
+                                        S.found_mass = at_mass;
+                                    }
+                                }
+                                at_mass += m[j];
+                            }
+                            same = __reduce_add_sync(0xffffffffu, same);
+                            if (lane == 0) S.red32[warp] = same;
+                            __syncthreads();
+                            if (tid == 0) {
+                                for (int w = 1; w < NW; ++w) same += S.red32[w];
+                                S.found_at = same;
+                            }
+                            __syncthreads();
                         }
-                        same = __reduce_add_sync(0xffffffffu, same);
-                        if (lane == 0) S.red32[warp] = same;
-                        __syncthreads();
-                        if (tid == 0) {
-                            for (int w = 1; w < NW; ++w) same += S.red32[w];
-                            S.found_at = same;
+                        cluster_sync();
+                        f.key = ld_cluster(mapa(&S.key, 0));
+                        f.before_count = ld_cluster(mapa(&S.found_count, 0));
+                        f.before_mass = ld_cluster64(mapa(&S.found_mass, 0));
+                        f.at_count = ld_cluster(mapa(&S.found_at, 0));
+                        f.at_mass = f.at_count * mass_of(funkey(f.key), top, T, P.mass_shift);
+                    } else {
+                        // many share the bin: by the keys' bits, highest first (the bins' order is descending)
+                        uint32_t key = 0;
+                        int shift = 32;
+#pragma unroll 1
+                        for (int level = 0; level < 3; ++level) {
+                            const int bits = level < 2 ? 11 : 10;
+                            const uint32_t above = shift == 32 ? 0u : 0xffffffffu << shift, low = (1u << bits) - 1u;
+                            shift -= bits;
+                            fill_bins(slice, B, G, rank, [&](uint32_t k) {
+                                return k >= floor_key && ((k ^ key) & above) == 0u && top_bin(k) == b
+                                           ? int(low - (k >> shift & low)) : -1;
+                            }, top, T, P.mass_shift, B.all_mass, B.all_count);
+                            key |= (low - locate(S, f, by_mass, target, B.all_mass, B.all_count)) << shift;
                         }
-                        __syncthreads();
+                        f.key = key;
                     }
-                    cluster_sync();
-                    f.key = ld_cluster(mapa(&S.key, 0));
-                    f.before_count = ld_cluster(mapa(&S.found_count, 0));
-                    f.before_mass = ld_cluster64(mapa(&S.found_mass, 0));
-                    f.at_count = ld_cluster(mapa(&S.found_at, 0));
-                    f.at_mass = f.at_count * mass_of(funkey(f.key), top, T, P.mass_shift);
-                    return f;
-                }
-                // many share the bin: by the keys' bits, highest first (the bins' order is descending)
-                uint32_t key = 0;
-                int shift = 32;
-                for (int bits : {11, 11, 10}) {
-                    const uint32_t above = shift == 32 ? 0u : 0xffffffffu << shift, low = (1u << bits) - 1u;
-                    const int to = shift - bits;
-                    fill([&](uint32_t k) {
-                        return k >= floor_key && ((k ^ key) & above) == 0u && top_bin(k) == b ? int(low - (k >> to & low)) : -1;
-                    }, B.all_mass, B.all_count);
-                    shift = to;
-                    key |= (low - locate(f, by_mass, target, B.all_mass, B.all_count)) << shift;
-                }
-                f.key = key;
-                return f;
-            };
-            // everything that min-p keeps
-            uint64_t all = 0;
-            uint32_t count = 0;
-            for (int i = tid; i < BINS; i += WNT) {
-                all += B.top_mass[i];
-                count += B.top_count[i];
-            }
-            all = warp_incl_scan_u64(all, lane);
-            count = __reduce_add_sync(0xffffffffu, count);
-            if (lane == 31) {
-                S.red64[warp] = all;
-                S.red32[warp] = count;
-            }
-            __syncthreads();
-            all = 0;
-            count = 0;
-            for (int w = 0; w < NW; ++w) {
-                all += S.red64[w];
-                count += S.red32[w];
-            }
-            __syncthreads();
-            if (row.K > 0 && uint32_t(row.K) < count) {
-                const Found f = search(false, uint64_t(row.K - 1));
-                floor_key = f.key;
-                all = f.before_mass + f.at_mass;
-                count = f.before_count + f.at_count;
-            }
-            kept = all;
-            kept_count = count;
-            cut_key = floor_key;
-            uint32_t cut_ties = 0xffffffffu;      // of the columns at cut_key
-            if (row.p.use_p) {
-                const uint64_t limit = part_of(row.p.top_p, all);
-                const Found f = search(true, limit);
-                const uint64_t m = f.at_mass / f.at_count;
-                const uint64_t n = min(uint64_t(f.at_count), (limit - f.before_mass) / m + 1);
-                cut_key = f.key;
-                cut_ties = uint32_t(n);
-                kept = f.before_mass + n * m;
-                kept_count = f.before_count + uint32_t(n);
-            }
-            const uint64_t target = part_of(row.p.u, kept);
-            const Found f = search(true, target);
-            const uint32_t nth = uint32_t((target - f.before_mass) / (f.at_mass / f.at_count));
-            // the n-th column, in ascending order, that has key k (0xffffffff: there is none)
-            auto column_of = [&](uint32_t k, uint32_t n) {
-                // columns in order: each thread a run of the slice's neighbours
-                const int len = c_hi - c_lo, step = (len + WNT - 1) / WNT;
-                const int a = min(len, tid * step), z = min(len, a + step);
-                auto key_in_order = [&](int i) {
-                    if (cached) return cache[i];
-                    bool nan;
-                    return key_at(c_lo + i, E::load(g.row, c_lo + i), &nan);
-                };
-                uint32_t ties = 0;
-                for (int i = a; i < z; ++i) ties += key_in_order(i) == k;
-                const uint32_t upto = warp_incl_scan_u32(ties, lane);
-                if (lane == 31) S.red32[warp] = upto;
-                __syncthreads();
-                uint32_t before = upto - ties, mine = 0;
-                for (int w = 0; w < NW; ++w) {
-                    if (w < warp) before += S.red32[w];
-                    mine += S.red32[w];
-                }
-                if (tid == 0) {
-                    S.ties = mine;
-                    S.bin = 0xffffffffu;
-                }
-                cluster_sync();
-                for (uint32_t c = 0; c < rank; ++c) before += ld_cluster(mapa(&S.ties, c));
-                if (before <= n && n < before + ties) {
-                    uint32_t left = n - before;
-                    for (int i = a; i < z; ++i)
-                        if (key_in_order(i) == k && left-- == 0) {
-                            S.bin = uint32_t(c_lo + i);
-                            break;
+                    if (step == 0) {
+                        floor_key = cut_key = f.key;
+                        kept = all = f.before_mass + f.at_mass;
+                        kept_count = f.before_count + f.at_count;
+                    } else {
+                        const uint64_t m = f.at_mass / f.at_count;
+                        const uint32_t nth = uint32_t((target - f.before_mass) / m);   // of those that share the key
+                        if (step == 1) {
+                            cut_key = f.key;
+                            cut_ties = min(f.at_count, nth + 1);
+                            kept = f.before_mass + cut_ties * m;
+                            kept_count = f.before_count + cut_ties;
+                        } else {
+                            // (without probabilities the first CTA alone writes, and may know the place)
+                            if (in_order && !P.out_probs)
+                                drawn = rank == 0 ? int(~uint32_t(all_members[S.first + nth])) : 0;
+                            else
+                                drawn = int(column_of(slice, S, G, rank, f.key, nth));
+                            if (rank == 0 && tid == 0) {
+                                const double y = double(funkey(f.key)) - double(top);
+                                write_row(P, r, drawn, float(y - log(double(kept) / unit)), int(kept_count), status);
+                            }
                         }
+                    }
                 }
-                cluster_sync();
-                uint32_t col = 0xffffffffu;
-                for (int c = 0; c < G; ++c) col = min(col, ld_cluster(mapa(&S.bin, c)));
-                cluster_sync();
-                return col;
-            };
-            // (without probabilities the first CTA alone writes, and may know the place)
-            if (in_order && !P.out_probs)
-                drawn = rank == 0 ? int(~uint32_t(all_members[S.first + nth])) : 0;
-            else
-                drawn = int(column_of(f.key, nth));
-            if (P.out_probs) cut_col = cut_ties == 0xffffffffu ? 0xffffffffu : column_of(cut_key, cut_ties - 1);
-            if (rank == 0 && tid == 0) {
-                const double y = double(funkey(f.key)) - double(top);
-                write_row(P, r, drawn + P.vocab_offset, float(y - log(double(kept) / scale)), int(kept_count), status);
+                if (P.out_probs) cut_col = cut_ties == 0xffffffffu ? 0xffffffffu : column_of(slice, S, G, rank, cut_key, cut_ties - 1);
             }
+            if (P.out_probs) {
+                float* out = P.out_probs + int64_t(r) * P.vocab;
+                const double all = double(kept);
+                slice.each([&](int c, uint32_t k) {
+                    float p = 0.0f;
+                    if (drawn >= 0) {
+                        if (row.greedy) p = c == drawn ? 1.0f : 0.0f;
+                        else if (k > cut_key || (k == cut_key && uint32_t(c) <= cut_col))
+                            p = float(exp(double(funkey(k)) - double(top)) * unit / all);
+                    }
+                    out[c] = p;
+                });
+            }
+            cluster_sync();   // the next row's state replaces what the others may still read
         }
-        if (P.out_probs) {
-            float* out = P.out_probs + int64_t(r) * P.vocab;
-            const double all = double(kept);
-            each_key([&](int c, uint32_t k) {
-                float p = 0.0f;
-                if (drawn >= 0) {
-                    if (row.greedy) p = c == drawn ? 1.0f : 0.0f;
-                    else if (k > cut_key || (k == cut_key && uint32_t(c) <= cut_col))
-                        p = float(exp(double(funkey(k)) - double(top)) * scale / all);
-                }
-                out[c] = p;
-            });
-        }
-        cluster_sync();   // the next row's state replaces what the others may still read
-      }
     }
 }
 

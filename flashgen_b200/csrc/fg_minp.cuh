@@ -95,7 +95,6 @@ struct Row {
     bool greedy;
     int K;               // top-k; 0: off
     float min_p;
-    double log_min_p;    // -inf without min-p
     int64_t h0, h1;      // its history
 };
 __device__ __forceinline__ Row load_row(const Params& P, int r) {
@@ -134,8 +133,11 @@ __device__ __forceinline__ Row load_row(const Params& P, int r) {
     p.cls = row.greedy ? RC_GREEDY : RC_FULL;
     p.K = 0;
     row.K = !row.greedy && k > 0 && k < P.vocab ? k : 0;
-    row.log_min_p = row.greedy || row.min_p == 1.0f ? 0.0 : row.min_p > 0.0f ? log(double(row.min_p)) : -INFINITY;
     return row;
+}
+// log(min_p): -inf without min-p, 0 for greedy rows.
+__device__ __forceinline__ double log_min_p(const Row& row) {
+    return row.greedy || row.min_p == 1.0f ? 0.0 : row.min_p > 0.0f ? log(double(row.min_p)) : -INFINITY;
 }
 
 __device__ __forceinline__ void write_row(const Params& P, int r, int64_t id, float logprob, int kept, uint32_t status) {
@@ -155,14 +157,25 @@ __device__ __forceinline__ void write_error(const Params& P, int r, uint32_t sta
 // function in IEEE floating-point arithmetic", ACM TOMS 15(2), 1989): with n the nearest
 // integer to d 64 / log 2, e^d = 2^(n / 64) e^r and |r| <= log 2 / 128; the table has
 // 2^(j / 64) as pairs.
-struct ExpTable {
+struct ExpPairs {
+    float v[64][2];
+    constexpr ExpPairs() : v() {
+        for (int j = 0; j < 64; ++j) {
+            double t = 1.0, term = 1.0;   // e^x by its series, x = j log 2 / 64 < 0.69
+            for (int i = 1; i < 24; ++i) {
+                term *= j * (0.69314718055994530942 / 64.0) / i;
+                t += term;
+            }
+            v[j][0] = float(t);
+            v[j][1] = float(t - double(v[j][0]));
+        }
+    }
+};
+__device__ constexpr ExpPairs kExpPairs{};
+struct ExpTable {   // in shared memory
     float2 v[64];
     __device__ __forceinline__ void fill() {   // by the first 64 threads
-        if (threadIdx.x < 64) {
-            const double t = exp2(double(threadIdx.x) / 64.0);
-            const float hi = float(t);
-            v[threadIdx.x] = make_float2(hi, float(t - double(hi)));
-        }
+        if (threadIdx.x < 64) v[threadIdx.x] = make_float2(kExpPairs.v[threadIdx.x][0], kExpPairs.v[threadIdx.x][1]);
     }
 };
 __device__ __forceinline__ uint64_t mass_of(float y, float top, const ExpTable& T, int shift) {
@@ -199,9 +212,9 @@ __device__ __forceinline__ uint64_t mass_of(float y, float top, const ExpTable& 
     return down <= 0 ? uint64_t(m) << -down : (uint64_t(m) + (uint64_t(1) << (down - 1))) >> down;
 }
 // The smallest key that min-p keeps below a maximum of `top`: y >= top + log(min_p) in 64 bits.
-__device__ __forceinline__ uint32_t least_key(const Row& row, float top) {
-    if (!(row.log_min_p > -INFINITY)) return KEY_NEG_INF + 1u;
-    const uint32_t k = fkey(__double2float_ru(double(top) + row.log_min_p));
+__device__ __forceinline__ uint32_t least_key(double log_min_p, float top) {
+    if (!(log_min_p > -INFINITY)) return KEY_NEG_INF + 1u;
+    const uint32_t k = fkey(__double2float_ru(double(top) + log_min_p));
     return k > KEY_NEG_INF ? k : KEY_NEG_INF + 1u;
 }
 // What of a sum stays below a share of it: floor(share * sum).
@@ -266,6 +279,7 @@ struct Shared {
     uint32_t n;          // members of a bin
     uint32_t bin, bin_count, before_count, kth;
     uint64_t before_mass;
+    double log_min_p;
     uint32_t warp[NT / 32];
     uint64_t sums[NT / 32];
 };
@@ -346,12 +360,6 @@ __device__ __forceinline__ void copies_done() {
     asm volatile("cp.async.wait_group %0;" :: "n"(LEFT) : "memory");
 }
 
-// One 16-byte word of four, picked by an index.
-__device__ __forceinline__ uint32_t word_of(const uint4& q, int i) {
-    const uint32_t a = i & 1 ? q.y : q.x, b = i & 1 ? q.w : q.z;
-    return i & 2 ? b : a;
-}
-
 // Dynamic shared memory: the ring of copies (after the stream: bins and members of a bin),
 // the candidates, the history's table.
 template <int DT>
@@ -392,6 +400,9 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
     };
     const int stages = (ch1 - ch0 + UNROLL * NT - 1) / (UNROLL * NT);
 
+    // the first copies go out before anything else is known of the row
+#pragma unroll
+    for (int k = 0; k < STAGES; ++k) fetch(k);
     const Row row = load_row(P, r);
     if (rank == 0 && tid == 0) P.marks[r] = 0;
     // a lower bound of the K-th largest comes from K chunks of the first stages
@@ -401,14 +412,14 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
     };
     if (row.p.bad && !P.out_probs) {
         if (rank == 0 && tid == 0) write_error(P, r, row.p.bad);
+        copies_done<0>();
         return;
     }
     if (P.out_probs || (!row.greedy && row.min_p == 0.0f && !by_k) || row.h1 - row.h0 > HIST_CAP) {
         hand_on();
+        copies_done<0>();
         return;
     }
-#pragma unroll
-    for (int k = 0; k < STAGES; ++k) fetch(k);
     const bool first = rank == 0, last = int(rank) == G - 1;
     const int c_lo = first ? 0 : g.head + ch0 * VEC, c_hi = last ? P.vocab : g.head + ch1 * VEC;
     const uint32_t mask = uint32_t(P.slots) - 1u;
@@ -419,6 +430,7 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
         S.least = KEY_NEG_INF;
         S.count = 0;
         S.flags = 0;
+        S.log_min_p = log_min_p(row);   // (64 bits, by one thread: a microsecond of every thread's otherwise)
     }
     if (pen) {
         for (int i = tid; i <= int(mask); i += NT) table[i] = make_uint2(kEmptySlot, 0u);
@@ -456,7 +468,7 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
         const uint32_t b = (col - uint32_t(c_lo)) & (ROW_FILTER * 32 - 1);
         return (filter[b >> 5] >> (b & 31) & 1u) != 0u && find_slot(table, mask, col) >= 0;
     };
-    const float span = row.greedy ? 0.0f : float(-row.log_min_p) * row.p.T;
+    const float span = row.greedy ? 0.0f : -logf(row.min_p) * row.p.T;
 
     // the maximum of the ring's first filling, over what is not in the history
     constexpr int HELD = STAGES * UNROLL;
@@ -550,34 +562,38 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
             if (lane == 0) atomicMax(&S.top, key);
         }
     };
-    // a chunk a lane (lane's is chunk c0 + lane): those that reach the bound are gone through by
-    // the warp, 32 / VEC of them at a time, one element a lane
-    auto scan = [&](const uint4& q, int c0, bool valid) {
-        uint32_t hits = __ballot_sync(0xffffffffu, valid && !(chunk_max<DT>(q) < bound));
-        while (hits) {
-            int src = -1;
+    // a chunk a lane
+    auto scan = [&](const uint4& q, int c, bool valid) {
+        const float m = chunk_max<DT>(q);
+        if (!valid || m < bound) return;
+        float x[VEC];
+        E::unpack(q, x);
+        const uint32_t col = uint32_t(g.head + c * VEC);
+        uint32_t mine = 0;               // elements that reach the bound
 #pragma unroll
-            for (int k = 0; k < 32 / VEC; ++k) {
-                const int b = __ffs(hits) - 1;      // -1: no more
-                if (lane / VEC == k) src = b;
-                hits &= hits - 1u;
-            }
-            const int from = max(src, 0), e = lane % VEC;
-            uint4 w;
-            w.x = __shfl_sync(0xffffffffu, q.x, from);
-            w.y = __shfl_sync(0xffffffffu, q.y, from);
-            w.z = __shfl_sync(0xffffffffu, q.z, from);
-            w.w = __shfl_sync(0xffffffffu, q.w, from);
-            float x;
-            if constexpr (DT == FG_DTYPE_F32) {
-                x = __uint_as_float(word_of(w, e));
-            } else {
-                const uint32_t word = word_of(w, e >> 1), half = e & 1 ? word >> 16 : word & 0xffffu;
-                if constexpr (DT == FG_DTYPE_F16) x = __half2float(__ushort_as_half(uint16_t(half)));
-                else x = __uint_as_float(half << 16);
-            }
-            take(x, uint32_t(g.head + (c0 + from) * VEC + e), src >= 0 && !(x < bound));
+        for (int j = 0; j < VEC; ++j) mine |= uint32_t(!(x[j] < bound)) << j;
+        float most = m;
+        if (pen || !(bound > -INFINITY) || m != m) {
+            // history columns, -inf and NaN are none
+            most = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (mine >> j & 1u) {
+                    const bool other = in_history(col + j);
+                    if (x[j] != x[j] && !other) atomicOr(&S.flags, uint32_t(FG_ROW_NAN));
+                    if (other || !(x[j] > -INFINITY)) mine &= ~(1u << j);
+                    else most = fmaxf(most, x[j]);
+                }
         }
+        if (mine == 0u) return;
+        uint32_t at = atomicAdd(&S.count, uint32_t(__popc(mine)));
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (mine >> j & 1u) {
+                if (at < uint32_t(CAP)) cand[at] = {x[j], col + j};
+                ++at;
+            }
+        if (most > seen) atomicMax(&S.top, fkey(most));
     };
     // columns [lo, hi) one by one (fewer than a chunk), by the first warp
     auto scan_columns = [&](int lo, int hi) {
@@ -614,7 +630,7 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
 #pragma unroll
             for (int i = 0; i < UNROLL; ++i) {
                 const int c = ch0 + (k * UNROLL + i) * NT + tid;
-                scan(lds_v4(ring + (k % STAGES * UNROLL + i) * NT * 16), c - lane, c < ch1);
+                scan(lds_v4(ring + (k % STAGES * UNROLL + i) * NT * 16), c, c < ch1);
             }
             fetch(k + STAGES);   // (past the slice: an empty group, which keeps the count)
         }
@@ -663,36 +679,41 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
     const uint32_t slice_count = lane < G ? (G > 1 ? ld_cluster(mapa(&S.count_out, uint32_t(lane))) : S.count_out) : 0u;
     const bool over = __any_sync(0xffffffffu, slice_count > uint32_t(CAP));
 
+    // greedy rows with NaN or without a finite maximum: wide_kernel knows their first place
+    const bool wide = (sick && row.greedy) || (!sick && over);
+    const uint32_t errors = (flags & (FG_ROW_NAN | FG_ROW_BAD_PARAM)) |
+                            (flags & FG_ROW_NAN ? 0u : top_key <= KEY_NEG_INF ? uint32_t(FG_ROW_ALL_MASKED)
+                                                     : !(top_x < INFINITY)    ? uint32_t(FG_ROW_POS_INF) : 0u);
+    const bool decide = !wide && !(flags & FG_ROW_BAD_PARAM) && (row.greedy || !(errors || !(ydiv(row.p, top_x) < INFINITY)));
+    const float top = ydiv(row.p, top_x);
+    const uint32_t least_k = row.greedy ? top_key : least_key(S.log_min_p, top);
+    if (G > 1) {
+        // the other slices' candidates come to the first CTA, by a warp each
+        const uint32_t n = __shfl_sync(0xffffffffu, slice_count, warp % MAX_G);
+        if (rank == 0 && decide && warp > 0 && warp < G) {
+            const uint32_t src = mapa(cand, uint32_t(warp));
+            for (uint32_t j = lane; j < n; j += 32) {
+                const uint64_t c = ld_cluster64(src + 8 * j);   // {x, col}
+                if (fkey(ydiv(row.p, __uint_as_float(uint32_t(c)))) < least_k) continue;
+                const uint32_t at = atomicAdd(&S.count, 1u);
+                if (at < uint32_t(CAP)) cand[at] = {__uint_as_float(uint32_t(c)), uint32_t(c >> 32)};
+            }
+        }
+        static_assert(NT / 32 >= MAX_G, "a warp for each slice");
+        cluster_sync();                           // nobody leaves while its candidates may be read
+    }
     if (rank == 0) {
-        // greedy rows with NaN or without a finite maximum: wide_kernel knows their first place
-        const bool wide = (sick && row.greedy) || (!sick && over);
-        const uint32_t errors = (flags & (FG_ROW_NAN | FG_ROW_BAD_PARAM)) |
-                                (flags & FG_ROW_NAN ? 0u : top_key <= KEY_NEG_INF ? uint32_t(FG_ROW_ALL_MASKED)
-                                                         : !(top_x < INFINITY)    ? uint32_t(FG_ROW_POS_INF) : 0u);
         if (wide) {
             hand_on();
-        } else if ((flags & FG_ROW_BAD_PARAM) || (!row.greedy && (errors || !(ydiv(row.p, top_x) < INFINITY)))) {
+        } else if (!decide) {
             if (tid == 0) write_error(P, r, errors ? flags | errors : flags | FG_ROW_POS_INF);
         } else {
-            // ---- the other slices' candidates come to this CTA; the keys of all of them
-            const float top = ydiv(row.p, top_x);
-            const uint32_t least_k = row.greedy ? top_key : least_key(row, top);
-            const uint32_t of_warp = __shfl_sync(0xffffffffu, slice_count, warp % MAX_G);
-            if (warp > 0 && warp < G) {           // a warp each
-                const uint32_t src = mapa(cand, uint32_t(warp));
-                for (uint32_t j = lane; j < of_warp; j += 32) {
-                    const uint64_t c = ld_cluster64(src + 8 * j);   // {x, col}
-                    if (fkey(ydiv(row.p, __uint_as_float(uint32_t(c)))) < least_k) continue;
-                    const uint32_t at = atomicAdd(&S.count, 1u);
-                    if (at < uint32_t(CAP)) cand[at] = {__uint_as_float(uint32_t(c)), uint32_t(c >> 32)};
-                }
-            }
-            static_assert(NT / 32 >= MAX_G, "a warp for each slice");
+            // ---- the keys of all candidates
             for (int i = tid; i < RBINS; i += NT) bins.count[i] = bins.lo[i] = bins.hi[i] = 0u;
             __syncthreads();
             const int n = int(S.count);
             uint64_t* keys = reinterpret_cast<uint64_t*>(cand);      // in place: key, ~column; 0: not kept
-            const float per_bin = bin_scale(row.log_min_p, RBINS);
+            const float per_bin = bin_scale(S.log_min_p, RBINS);
             const uint32_t status = flags | (row.greedy ? uint32_t(FG_ROW_GREEDY) : 0u);
             if (n > CAP) {
                 hand_on();
@@ -892,7 +913,6 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
             }
         }
     }
-    if (G > 1) cluster_sync();                    // nobody leaves while its candidates may be read
 }
 
 // ---------------------------------------------------------------------------
@@ -1305,8 +1325,9 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
             } else if (errors) {
                 if (rank == 0 && tid == 0) write_error(P, r, status);
             } else {
-                uint32_t floor_key = least_key(row, top);
-                const float per_bin = bin_scale(row.log_min_p, BINS);
+                const double log_p = log_min_p(row);
+                uint32_t floor_key = least_key(log_p, top);
+                const float per_bin = bin_scale(log_p, BINS);
                 auto top_bin = [&](uint32_t k) { return bin_of(top, funkey(k), per_bin, BINS); };
                 fill_bins(slice, B, G, rank, [&](uint32_t k) { return k >= floor_key ? int(top_bin(k)) : -1; }, top, T,
                           P.mass_shift, B.top_mass, B.top_count);

@@ -76,7 +76,7 @@ int launch(fg::minp::Params P, DevInfo* d, cudaStream_t st) {
     if (rc != FG_OK) return rc;
     // wide_kernel: the slice's keys in shared memory where they fit; four CTAs a row where that
     // leaves work for every SM
-    auto fixed = [&](int g) { return 16 * MEMBERS + bins_bytes(g) + (P.penalties ? 4 * FILTER_WORDS : 0); };
+    auto fixed = [&](int g) { return 16 * MEMBERS + bins_bytes(g); };
     auto keys = [&](int g) {
         const int64_t chunks = int64_t(P.vocab) * esz / 16 + 1;
         return (chunks + g - 1) / g * (16 / esz) + 2 * (16 / esz) + KEY_PAD;
@@ -84,7 +84,7 @@ int launch(fg::minp::Params P, DevInfo* d, cudaStream_t st) {
     const int room = d->smem_optin - int(sizeof(WideShared) + sizeof(ExpTable)) - 1024;
     const int W = P.batch > d->sms / 8 && fixed(4) + 4 * keys(4) <= room ? 4 : 8;
     const bool cached = fixed(W) + 4 * keys(W) <= room;
-    const int wsmem = fixed(W) + (cached ? 4 * int(keys(W)) : 0);
+    const int wsmem = fixed(W) + 4 * (cached ? int(keys(W)) : P.penalties ? FILTER_WORDS : 0);
     if (!set_smem(cached ? wide_kernel<DT, true> : wide_kernel<DT, false>, cached ? wide_smem : uncached_smem, wsmem))
         return FG_EDEVICE;
     const int clusters = std::min({int(P.batch), kMaxClusters, d->sms / W});

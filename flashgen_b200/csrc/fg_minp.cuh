@@ -241,8 +241,15 @@ template <int THREADS, int WORDS>
 __device__ __forceinline__ uint32_t count_history(const Params& P, const Row& row, uint2* table, uint32_t mask,
                                                   int64_t c_lo, int64_t c_hi, uint32_t* filter) {
     uint32_t bad = 0;
-    for (int64_t i = row.h0 + threadIdx.x; i < row.h1; i += THREADS) {
-        const int64_t id = __ldg(P.hist_ids + i);
+    constexpr int AHEAD = 4;   // loads of ids in flight
+    for (int64_t at = row.h0 + threadIdx.x; at < row.h1; at += AHEAD * THREADS) {
+      int32_t ids[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) ids[j] = at + j * THREADS < row.h1 ? __ldg(P.hist_ids + at + j * THREADS) : 0;
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (at + j * THREADS >= row.h1) break;
+        const int64_t id = ids[j];
         if (id < 0 || id >= P.vocab_total) {
             bad |= FG_ROW_BAD_HISTORY;
             continue;
@@ -258,8 +265,11 @@ __device__ __forceinline__ uint32_t count_history(const Params& P, const Row& ro
             h = (h + 1u) & mask;
         }
         if (!done) bad |= FG_ROW_BAD_PARAM;   // more distinct ids than hist_max_len allows
-        const uint32_t b = uint32_t(c - c_lo) & (WORDS * 32 - 1);
-        atomicOr(&filter[b >> 5], 1u << (b & 31));
+        if constexpr (WORDS > 0) {
+            const uint32_t b = uint32_t(c - c_lo) & (WORDS * 32 - 1);
+            atomicOr(&filter[b >> 5], 1u << (b & 31));
+        }
+      }
     }
     return bad;
 }
@@ -280,7 +290,7 @@ struct Shared {
     uint32_t bin, bin_count, before_count, kth;
     uint64_t before_mass;
     double log_min_p;
-    uint32_t warp[NT / 32];
+    uint32_t warp[NT / 32], other[NT / 32];
     uint64_t sums[NT / 32];
 };
 struct Candidate {
@@ -302,6 +312,17 @@ __device__ __forceinline__ float chunk_max(const uint4& q) {
         const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
         return fmax_nan(__low2float(m), __high2float(m));
     }
+}
+
+// Where in a chunk its largest element is (`m`, not NaN).
+template <int DT>
+__device__ __forceinline__ int place_of(const uint4& q, float m) {
+    float x[Elem<DT>::VEC];
+    Elem<DT>::unpack(q, x);
+    int at = 0;
+#pragma unroll
+    for (int j = 1; j < Elem<DT>::VEC; ++j) at = x[j] == m ? j : at;
+    return at;
 }
 
 // Counts and masses of bins, the masses as two words: 64-bit atomics on shared memory
@@ -482,21 +503,14 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
             const uint4 q = lds_v4(ring + i * NT * 16);
             const float m = chunk_max<DT>(q);
             if (!(m > top)) continue;
-            if (!pen) {
-                top = m;
-                continue;
-            }
-            float x[VEC];
-            E::unpack(q, x);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (x[j] > top && !in_history(uint32_t(g.head + c * VEC + j))) top = x[j];
+            // (a chunk whose largest is in the history counts for none: the stream sees to the rest of it)
+            if (!pen || !in_history(uint32_t(g.head + c * VEC + place_of<DT>(q, m)))) top = m;
         }
         const uint32_t key = __reduce_max_sync(0xffffffffu, fkey(top));
         if (lane == 0) atomicMax(&S.top, key);
         __syncthreads();
         if (by_k) {
-            // the largest key, to 2^-20 of its range, that K chunks of the ring reach: the K-th
+            // the largest key, to 2^-17 of its range, that K chunks of the ring reach: the K-th
             // largest logit is no smaller. A chunk whose largest is in the history counts for none
             uint32_t key_of[HELD];
 #pragma unroll
@@ -506,30 +520,21 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
                 if (c >= ch1) continue;
                 const uint4 q = lds_v4(ring + i * NT * 16);
                 const float m = chunk_max<DT>(q);
-                bool clean = m == m;
-                if (pen) {
-                    float x[VEC];
-                    E::unpack(q, x);
-                    int at = 0;
-#pragma unroll
-                    for (int j = 1; j < VEC; ++j) at = x[j] == m ? j : at;
-                    clean = clean && !in_history(uint32_t(g.head + c * VEC + at));
-                }
-                if (clean) key_of[i] = fkey(m);
+                if (m == m && (!pen || !in_history(uint32_t(g.head + c * VEC + place_of<DT>(q, m))))) key_of[i] = fkey(m);
             }
             uint32_t lo = KEY_NEG_INF, hi = S.top;
-            for (int step = 0; step < 20 && hi > lo; ++step) {
+            for (int step = 0; step < 17 && hi > lo; ++step) {
                 const uint32_t mid = lo + (hi - lo + 1) / 2;
                 uint32_t n = 0;
 #pragma unroll
                 for (int i = 0; i < HELD; ++i) n += key_of[i] >= mid;
                 n = __reduce_add_sync(0xffffffffu, n);
-                if (lane == 0) S.warp[warp] = n;
+                uint32_t* sums = step & 1 ? S.warp : S.other;   // by turns: one barrier a step
+                if (lane == 0) sums[warp] = n;
                 __syncthreads();
                 n = 0;
 #pragma unroll
-                for (int w = 0; w < NT / 32; ++w) n += S.warp[w];
-                __syncthreads();
+                for (int w = 0; w < NT / 32; ++w) n += sums[w];
                 if (n >= uint32_t(row.K)) lo = mid;
                 else hi = mid - 1;
             }
@@ -974,7 +979,7 @@ struct Slice {
 
     // (greedy rows: of the penalised logit itself)
     __device__ __forceinline__ uint32_t key_of(int c, float x, bool& nan) const {
-        if (row.p.pen) {
+        if (!CACHED && row.p.pen) {
             const uint32_t b = uint32_t(c - c_lo) & (FILTER_WORDS * 32 - 1);
             if (filter[b >> 5] >> (b & 31) & 1u) {
                 const int at = find_slot(table, mask, uint32_t(c));
@@ -1195,7 +1200,7 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
     B.top_count = B.all_count + BINS;
     B.own_count = B.top_count + BINS;
     uint32_t* filter = B.own_count + per;
-    uint32_t* cache = filter + (P.penalties ? FILTER_WORDS : 0);
+    uint32_t* cache = filter;   // (one or the other)
     T.fill();
     wait_prerequisites();
     uint2* table = P.tables + int64_t(blockIdx.x / G) * P.wide_slots;
@@ -1248,19 +1253,29 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
             if (pen) {
                 // the cluster shares one table; its CTAs insert and look up columns of their own
                 for (int i = rank * WNT + tid; i <= int(mask); i += G * WNT) table[i] = make_uint2(kEmptySlot, 0u);
-                for (int i = tid; i < FILTER_WORDS; i += WNT) filter[i] = 0u;
+                if constexpr (!CACHED)
+                    for (int i = tid; i < FILTER_WORDS; i += WNT) filter[i] = 0u;
             }
             cluster_sync();
             if (pen) {
-                const uint32_t bad = count_history<WNT, FILTER_WORDS>(P, row, table, mask, slice.c_lo, slice.c_hi, filter);
+                const uint32_t bad = count_history<WNT, CACHED ? 0 : FILTER_WORDS>(P, row, table, mask, slice.c_lo,
+                                                                                  slice.c_hi, filter);
                 if (bad) atomicOr(&S.flags, bad);
                 __syncthreads();
             }
             // ---- keys, the maximum and its first column, the first NaN
             {
                 uint32_t top = KEY_NEG_INF, arg = 0xffffffffu, nan_col = 0xffffffffu;
-                slice.read([&](int c, int n, const uint32_t* k, uint32_t nans) {
-                    if constexpr (CACHED) {
+                auto meet = [&](int c, uint32_t k, bool nan) {
+                    if (nan) nan_col = min(nan_col, uint32_t(c));
+                    else if (k > top || (k == top && uint32_t(c) < arg)) {
+                        top = k;
+                        arg = uint32_t(c);
+                    }
+                };
+                if constexpr (CACHED) {
+                    // all columns' keys (0: NaN), then the history's over them
+                    slice.read([&](int c, int n, const uint32_t* k, uint32_t) {
                         uint32_t* to = cache + (c - slice.c_lo + slice.skew);
                         if (n == VEC) {
 #pragma unroll
@@ -1269,15 +1284,25 @@ __global__ void __launch_bounds__(WNT, 1) wide_kernel(const Params P, const int 
                         } else {
                             to[0] = k[0];
                         }
-                    }
-                    if (nans) nan_col = min(nan_col, uint32_t(c) + uint32_t(__ffs(nans) - 1));
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if (j < n && !(nans >> j & 1u) && (k[j] > top || (k[j] == top && uint32_t(c + j) < arg))) {
-                            top = k[j];
-                            arg = uint32_t(c + j);
+                    });
+                    __syncthreads();
+                    if (pen) {
+                        for (int i = tid; i <= int(mask); i += WNT) {
+                            const uint2 e = __ldcg(table + i);
+                            if (e.x == kEmptySlot || int(e.x) < slice.c_lo || int(e.x) >= slice.c_hi) continue;
+                            const float x = penalize(row.p, E::load(g.row, e.x), e.y);
+                            cache[int(e.x) - slice.c_lo + slice.skew] = x != x ? 0u : fkey(ydiv(row.p, x));
                         }
-                });
+                        __syncthreads();
+                    }
+                    slice.each([&](int c, uint32_t k) { meet(c, k, k == 0u); });
+                } else {
+                    slice.read([&](int c, int n, const uint32_t* k, uint32_t nans) {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j)
+                            if (j < n) meet(c + j, k[j], nans >> j & 1u);
+                    });
+                }
                 const uint32_t wtop = __reduce_max_sync(0xffffffffu, top);
                 const uint32_t warg = __reduce_min_sync(0xffffffffu, top == wtop ? arg : 0xffffffffu);
                 nan_col = __reduce_min_sync(0xffffffffu, nan_col);

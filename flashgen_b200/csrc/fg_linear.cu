@@ -195,11 +195,16 @@ GradLayout grad_layout(const FgLinearGradArgs& a) {
 }
 
 template <int DT>
-int launch_slope(const fg::lin::SlopeParams& S, void* grad_bias, cudaStream_t st) {
-    constexpr int cols = fg::lin::SLOPE_THREADS * 8;
-    const unsigned blocks = unsigned((S.tokens + fg::lin::SLOPE_ROWS - 1) / fg::lin::SLOPE_ROWS);
-    int rc = launch_early(fg::lin::slope_kernel<DT>, dim3(unsigned((S.outer + cols - 1) / cols), blocks),
-                          fg::lin::SLOPE_THREADS, 0, 1, st, S);
+int launch_slope(const fg::lin::SlopeParams& S, int act, void* grad_bias, cudaStream_t st) {
+    using namespace fg::lin;
+    const unsigned blocks = unsigned((S.tokens + SLOPE_ROWS - 1) / SLOPE_ROWS);
+    auto kern = act == FG_ACT_RELU        ? slope_kernel<DT, FG_ACT_RELU>
+                : act == FG_ACT_GELU      ? slope_kernel<DT, FG_ACT_GELU>
+                : act == FG_ACT_GELU_TANH ? slope_kernel<DT, FG_ACT_GELU_TANH>
+                : act == FG_ACT_SILU      ? slope_kernel<DT, FG_ACT_SILU>
+                                          : slope_kernel<DT, FG_ACT_NONE>;
+    int rc = launch_early(kern, dim3(unsigned((S.outer + SLOPE_COLS - 1) / SLOPE_COLS), blocks), SLOPE_THREADS, 0, 1,
+                          st, S);
     if (rc == FG_OK && grad_bias)
         rc = launch_early(fg::lin::bias_kernel<DT>, dim3(unsigned((S.outer + 31) / 32)), 256, 0, 1, st,
                           (const float*)S.sums, int(blocks), int(S.outer), (uint16_t*)grad_bias);
@@ -310,11 +315,11 @@ int fg_linear_grad(const FgLinearGradArgs* a, void* stream) {
         S.preact = a->activation != FG_ACT_NONE ? a->preact : nullptr; S.preact_stride = a->preact_stride;
         S.dz = written ? reinterpret_cast<uint16_t*>(room) : nullptr; S.dz_stride = round8(a->outer);
         S.sums = a->grad_bias ? reinterpret_cast<float*>(room + W.sums) : nullptr;
-        S.tokens = a->tokens; S.outer = a->outer; S.act = a->activation;
+        S.tokens = a->tokens; S.outer = a->outer;
         S.wide = tma_ready(a->grad_out, a->tokens, a->grad_out_stride) &&
                  (S.preact == nullptr || (aligned(S.preact, 16) && (a->tokens == 1 || a->preact_stride % 4 == 0)));
-        rc = a->dtype == FG_DTYPE_F16 ? launch_slope<FG_DTYPE_F16>(S, a->grad_bias, st)
-                                      : launch_slope<FG_DTYPE_BF16>(S, a->grad_bias, st);
+        rc = a->dtype == FG_DTYPE_F16 ? launch_slope<FG_DTYPE_F16>(S, a->activation, a->grad_bias, st)
+                                      : launch_slope<FG_DTYPE_BF16>(S, a->activation, a->grad_bias, st);
         if (rc != FG_OK) return rc;
         if (written) dz = {S.dz, a->tokens, a->outer, S.dz_stride};
     }

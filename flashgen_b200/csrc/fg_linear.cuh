@@ -33,44 +33,63 @@ __device__ __forceinline__ void logistic(float z, float& s, float& rest) {
     rest = z >= 0.0f ? t * q : q;
     if (z != z) s = rest = z;
 }
+// The first alone (of powers that do not leave the range).
+__device__ __forceinline__ float logistic(float z) {
+    const float t = exp_fast(-fabsf(z));
+    return __fdividef(z < 0.0f ? t : 1.0f, 1.0f + t);
+}
 constexpr float kGeluC = 0.7978845608028654f, kGeluD = 0.044715f;   // sqrt(2 / pi); the cubic term
 
-__device__ __forceinline__ float activate(int act, float z) {
-    switch (act) {
-        case FG_ACT_RELU: return z < 0.0f ? 0.0f : z;
-        case FG_ACT_SILU: {
-            float s, r;
-            logistic(z, s, r);
-            return z * s;
-        }
-        case FG_ACT_GELU: return 0.5f * z * erfcf(-0.7071067811865476f * z);
-        case FG_ACT_GELU_TANH: {
-            float s, r;
-            logistic(2.0f * kGeluC * fmaf(kGeluD * z * z, z, z), s, r);
-            return z * s;
-        }
-        default: return z;
-    }
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == FG_ACT_RELU) return z < 0.0f ? 0.0f : z;
+    if constexpr (ACT == FG_ACT_SILU) return z * logistic(z);
+    if constexpr (ACT == FG_ACT_GELU) return 0.5f * z * erfcf(-0.7071067811865476f * z);
+    if constexpr (ACT == FG_ACT_GELU_TANH)
+        return z * logistic(2.0f * kGeluC * fmaf(kGeluD * z * z, z, z));
+    return z;
 }
-__device__ __forceinline__ float slope(int act, float z) {
+template <int ACT>
+__device__ __forceinline__ float slope(float z) {
+    if constexpr (ACT == FG_ACT_RELU) return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
+    if constexpr (ACT == FG_ACT_SILU) {
+        float s, r;
+        logistic(z, s, r);
+        return fmaf(r == 0.0f ? 0.0f : z * s, r, s);
+    }
+    if constexpr (ACT == FG_ACT_GELU) {
+        const float density = 0.3989422804014327f * exp_fast(-0.5f * z * z);
+        return 0.5f * erfcf(-0.7071067811865476f * z) + (density == 0.0f ? 0.0f : z * density);
+    }
+    if constexpr (ACT == FG_ACT_GELU_TANH) {
+        float s, r;
+        logistic(2.0f * kGeluC * fmaf(kGeluD * z * z, z, z), s, r);
+        const float both = s * r;
+        return s + (both == 0.0f ? 0.0f : z * both * 2.0f * kGeluC * fmaf(3.0f * kGeluD * z, z, 1.0f));
+    }
+    return 1.0f;
+}
+// All of x, one choice for them together.
+template <int N>
+__device__ __forceinline__ void activate_all(int act, float (&x)[N]) {
     switch (act) {
-        case FG_ACT_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
-        case FG_ACT_SILU: {
-            float s, r;
-            logistic(z, s, r);
-            return fmaf(r == 0.0f ? 0.0f : z * s, r, s);
-        }
-        case FG_ACT_GELU: {
-            const float density = 0.3989422804014327f * exp_fast(-0.5f * z * z);
-            return 0.5f * erfcf(-0.7071067811865476f * z) + (density == 0.0f ? 0.0f : z * density);
-        }
-        case FG_ACT_GELU_TANH: {
-            float s, r;
-            logistic(2.0f * kGeluC * fmaf(kGeluD * z * z, z, z), s, r);
-            const float both = s * r;
-            return s + (both == 0.0f ? 0.0f : z * both * 2.0f * kGeluC * fmaf(3.0f * kGeluD * z, z, 1.0f));
-        }
-        default: return 1.0f;
+        case FG_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = activate<FG_ACT_RELU>(x[i]);
+            break;
+        case FG_ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = activate<FG_ACT_GELU>(x[i]);
+            break;
+        case FG_ACT_GELU_TANH:
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = activate<FG_ACT_GELU_TANH>(x[i]);
+            break;
+        case FG_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = activate<FG_ACT_SILU>(x[i]);
+            break;
+        default: break;
     }
 }
 
@@ -120,26 +139,60 @@ __device__ __forceinline__ float load_cluster(uint32_t addr) {
     return v;
 }
 
-// One column's results of this thread's lane.
+// This thread's lane of the results, N neighbouring columns at a time.
 template <int DT>
 struct Lane {
     const Params& P;
-    int l;
+    bool in;               // the lane is one of the result's
     float bias;
-    __device__ __forceinline__ Lane(const Params& p, int lane) : P(p), l(lane) {
-        bias = P.bias && l < P.L ? from_bits<DT>(reinterpret_cast<const uint16_t*>(P.bias)[l]) : 0.0f;
+    const uint16_t* residual;
+    uint16_t* out;
+    float* preact;
+    __device__ __forceinline__ Lane(const Params& p, int l) : P(p), in(l < p.L) {
+        bias = P.bias && in ? from_bits<DT>(reinterpret_cast<const uint16_t*>(P.bias)[l]) : 0.0f;
+        residual = P.residual ? reinterpret_cast<const uint16_t*>(P.residual) + l : nullptr;
+        out = reinterpret_cast<uint16_t*>(P.out) + l;
+        preact = P.preact ? P.preact + l : nullptr;
     }
-    __device__ __forceinline__ uint16_t residual(int c) const {
-        return P.residual && l < P.L && c < P.C
-                   ? reinterpret_cast<const uint16_t*>(P.residual)[int64_t(c) * P.residual_stride + l] : uint16_t(0);
+    template <int N>
+    __device__ __forceinline__ void load(int c, uint16_t (&r)[N]) const {
+        if (!residual || !in) return;
+        const uint16_t* p = residual + int64_t(c) * P.residual_stride;
+        if (c + N <= P.C) {
+#pragma unroll
+            for (int i = 0; i < N; ++i, p += P.residual_stride) r[i] = *p;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i, p += P.residual_stride)
+                if (c + i < P.C) r[i] = *p;
+        }
     }
-    __device__ __forceinline__ void store(int c, float sum, uint16_t r) const {
-        if (l >= P.L || c >= P.C) return;
-        float z = sum + bias;
-        if (P.preact) P.preact[int64_t(c) * P.preact_stride + l] = z;
-        z = activate(P.act, z);
-        if (P.residual) z += from_bits<DT>(r);
-        reinterpret_cast<uint16_t*>(P.out)[int64_t(c) * P.out_stride + l] = to_bits<DT>(z);
+    template <int N>
+    __device__ __forceinline__ void store(int c, float (&x)[N], const uint16_t (&r)[N]) const {
+        if (!in) return;
+        const int n = min(N, P.C - c);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] += bias;
+        if (preact) {
+            float* p = preact + int64_t(c) * P.preact_stride;
+#pragma unroll
+            for (int i = 0; i < N; ++i, p += P.preact_stride)
+                if (i < n) *p = x[i];
+        }
+        activate_all(P.act, x);
+        if (residual) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] += from_bits<DT>(r[i]);
+        }
+        uint16_t* p = out + int64_t(c) * P.out_stride;
+        if (n == N) {
+#pragma unroll
+            for (int i = 0; i < N; ++i, p += P.out_stride) *p = to_bits<DT>(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i, p += P.out_stride)
+                if (i < n) *p = to_bits<DT>(x[i]);
+        }
     }
 };
 
@@ -311,6 +364,9 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
         for (int t = first; t < tiles; t += step) {
             const int c0 = (t % P.nc) * P.nt;
             const Lane<DT> out(P, ((t / P.nc) * CG + half) * TILE_L + quarter * 32 + lane);
+            // the residual's columns come ahead: the first before the products are done
+            uint16_t next[16] = {};
+            if (P.splits == 1 && !gone) out.load(c0 + part * 16, next);
             int before = -1;
             for (int k0 = 0; k0 < nk && !gone; k0 += PIECE_K) {
                 // a wait of the whole warp: all lanes go on or none
@@ -341,8 +397,12 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
                 if (lane == 0) give_up();
                 __syncwarp();
                 if (P.splits == 1)
-                    for (int i = part * 16; i < P.nt; i += 16 * PARTS)
-                        for (int j = 0; j < 16; ++j) out.store(c0 + i + j, __int_as_float(0x7fc00000), 0);
+                    for (int i = part * 16; i < P.nt && c0 + i < P.C; i += 16 * PARTS) {
+                        float x[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[j] = __int_as_float(0x7fc00000);
+                        out.store(c0 + i, x, next);
+                    }
                 continue;
             }
             const uint32_t at = lanes + acc * P.nt;
@@ -354,10 +414,10 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
                     uint16_t r[16];
                     tmem_ld16(x, at + i);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) r[j] = out.residual(c0 + i + j);
+                    for (int j = 0; j < 16; ++j) r[j] = next[j];
+                    if (i + 16 * PARTS < P.nt) out.load(c0 + i + 16 * PARTS, next);
                     tc::tmem_wait_ld(x);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) out.store(c0 + i + j, x[j], r[j]);
+                    out.store(c0 + i, x, r);
                 }
             } else {
                 // this part of the sum, where the ring was: [column][lane]
@@ -394,7 +454,8 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
             const int hi = P.nt * (split + 1) / P.splits;
             for (int c = P.nt * split / P.splits + tid / TILE_L; c < hi; c += EPI_WARPS * 32 / TILE_L) {
                 if (c0 + c >= P.C) break;
-                const uint16_t r = out.residual(c0 + c);
+                uint16_t r[1] = {};
+                out.load(c0 + c, r);
                 float part[MAX_SPLITS];
 #pragma unroll
                 for (int q = 0; q < MAX_SPLITS; ++q)
@@ -403,7 +464,8 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
 #pragma unroll
                 for (int q = 1; q < MAX_SPLITS; ++q)
                     if (q < P.splits) sum += part[q];
-                out.store(c0 + c, sum, r);
+                float x[1] = {sum};
+                out.store(c0 + c, x, r);
             }
         }
     }
@@ -438,64 +500,74 @@ __global__ void __launch_bounds__(256) align_kernel(const uint16_t* src, int64_t
 }
 
 // dz = g * act'(z), rounded to the operands' type for the products, and its column sums
-// (of the products before rounding) over blocks of ROWS rows for the bias. A thread takes
-// eight columns. Bound: HBM (z in fp32: a rounded z would cost the slope its last bits).
-constexpr int SLOPE_ROWS = 64, SLOPE_THREADS = 128;
+// (of the products before rounding) over blocks of SLOPE_ROWS rows for the bias. A warp takes
+// 256 columns of a row, eight a thread; the block's warps the rows by turns. Bound: HBM (z in
+// fp32: a rounded z would cost the slope its last bits); gelu's error function takes as long.
+constexpr int SLOPE_ROWS = 32, SLOPE_THREADS = 256, SLOPE_COLS = 256;
 struct SlopeParams {
     const uint16_t* grad;
     const float* preact;      // null: act is none
     uint16_t* dz;             // null: the gradient serves as it is
     float* sums;              // [row blocks][outer], or null
     int64_t grad_stride, preact_stride, dz_stride;
-    int32_t tokens, outer, act;
+    int32_t tokens, outer;
     int32_t wide;             // rows of grad and preact on 16-byte boundaries
 };
-template <int DT>
+template <int DT, int ACT>
 __global__ void __launch_bounds__(SLOPE_THREADS) slope_kernel(const SlopeParams P) {
+    __shared__ float part[SLOPE_THREADS / 32][SLOPE_COLS];
     tc::wait_prerequisites();
     tc::launch_dependents();
-    const int n = (blockIdx.x * SLOPE_THREADS + threadIdx.x) * 8;
-    if (n >= P.outer) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n0 = blockIdx.x * SLOPE_COLS, n = n0 + lane * 8;
     const int m0 = blockIdx.y * SLOPE_ROWS, m1 = min(P.tokens, m0 + SLOPE_ROWS);
     const bool whole = P.wide && n + 8 <= P.outer;
     float sum[8] = {};
-#pragma unroll 4
-    for (int m = m0; m < m1; ++m) {
-        const uint16_t* g = P.grad + int64_t(m) * P.grad_stride + n;
-        const float* z = P.preact ? P.preact + int64_t(m) * P.preact_stride + n : nullptr;
-        float x[8], y[8];
-        if (whole) {
-            Elem<DT>::unpack(__ldg(reinterpret_cast<const uint4*>(g)), x);
-            if (z) {
-                const float4 a = __ldg(reinterpret_cast<const float4*>(z)), b = __ldg(reinterpret_cast<const float4*>(z) + 1);
-                y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w;
-                y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
+    if (n < P.outer) {
+#pragma unroll 2
+        for (int m = m0 + warp; m < m1; m += SLOPE_THREADS / 32) {
+            const uint16_t* g = P.grad + int64_t(m) * P.grad_stride + n;
+            float x[8], y[8];
+            if (whole) {
+                Elem<DT>::unpack(__ldg(reinterpret_cast<const uint4*>(g)), x);
+                if constexpr (ACT != FG_ACT_NONE) {
+                    const float4* z = reinterpret_cast<const float4*>(P.preact + int64_t(m) * P.preact_stride + n);
+                    const float4 a = __ldg(z), b = __ldg(z + 1);
+                    y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w;
+                    y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[j] = n + j < P.outer ? from_bits<DT>(g[j]) : 0.0f;
+                    y[j] = 0.0f;
+                    if constexpr (ACT != FG_ACT_NONE)
+                        if (n + j < P.outer) y[j] = P.preact[int64_t(m) * P.preact_stride + n + j];
+                }
             }
-        } else {
+            if constexpr (ACT != FG_ACT_NONE) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = n + j < P.outer ? from_bits<DT>(g[j]) : 0.0f;
-                y[j] = z && n + j < P.outer ? z[j] : 0.0f;
+                for (int j = 0; j < 8; ++j) x[j] *= slope<ACT>(y[j]);
             }
-        }
-        if (z) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= slope(P.act, y[j]);
-        }
+            for (int j = 0; j < 8; ++j) sum[j] += x[j];
+            if (P.dz) {
+                uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] += x[j];
-        if (P.dz) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = to_bits<DT>(x[2 * j]) | uint32_t(to_bits<DT>(x[2 * j + 1])) << 16;
-            *reinterpret_cast<uint4*>(P.dz + int64_t(m) * P.dz_stride + n) = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int j = 0; j < 4; ++j) w[j] = to_bits<DT>(x[2 * j]) | uint32_t(to_bits<DT>(x[2 * j + 1])) << 16;
+                *reinterpret_cast<uint4*>(P.dz + int64_t(m) * P.dz_stride + n) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
     }
     if (P.sums) {
-        float* s = P.sums + int64_t(blockIdx.y) * P.outer + n;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (n + j < P.outer) s[j] = sum[j];
+        for (int j = 0; j < 8; ++j) part[warp][lane * 8 + j] = sum[j];
+        __syncthreads();
+        const int c = threadIdx.x;
+        float s = part[0][c];
+#pragma unroll
+        for (int w = 1; w < SLOPE_THREADS / 32; ++w) s += part[w][c];
+        if (n0 + c < P.outer) P.sums[int64_t(blockIdx.y) * P.outer + n0 + c] = s;
     }
 }
 

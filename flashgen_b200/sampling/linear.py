@@ -37,14 +37,15 @@ def _room(size: int, like: torch.Tensor) -> Optional[torch.Tensor]:
 
 
 def _forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
-             act: int, keep: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """The block on matrices; with `keep` also the sums before the activation, in fp32 (the
-    gradient's slope at a rounded sum would lose the slope's last bits)."""
+             act: int, keep: bool) -> Tuple[torch.Tensor, ...]:
+    """The block on matrices; with `keep` also what the gradients read: x and the weight (their
+    aligned copies, where the call made some) and the sums before the activation, in fp32 (the
+    slope at a rounded sum would lose its last bits)."""
     tokens, inner, outer = x.shape[0], x.shape[1], weight.shape[0]
     out = x.new_empty((tokens, outer))
     preact = x.new_empty((tokens, (outer + 3) // 4 * 4), dtype=torch.float32) if keep and act else None
     if tokens == 0:
-        return out, preact
+        return out, x, weight, preact
     x, weight = _rows(x), _rows(weight)
     lib = _lib.load()
     a = _lib.FgLinearArgs(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), out.data_ptr(), _ptr(preact),
@@ -54,7 +55,21 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]
     if room is not None:
         a.workspace, a.workspace_bytes = room.data_ptr(), room.numel()
     _call(x.device, lib.fg_linear, a, "fg_linear")
-    return out, preact
+    if keep and room is not None:
+        # the workspace has x's copy, if one was made, then the weight's: rows of inner rounded up to 8
+        copies, width = room.view(x.dtype), (inner + 7) // 8 * 8
+        of_weight = 0
+        if not _aligned(x):
+            x = copies[:tokens * width].view(tokens, width)[:, :inner]
+            of_weight = (2 * tokens * width + 255) // 256 * 128
+        if not _aligned(weight):
+            weight = copies[of_weight:of_weight + outer * width].view(outer, width)[:, :inner]
+    return out, x, weight, preact
+
+
+def _aligned(t: torch.Tensor) -> bool:
+    """Whether the library reads the matrix where it lies: rows on 16-byte boundaries."""
+    return t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) % 8 == 0)
 
 
 class _Once(torch.autograd.Function):
@@ -73,19 +88,20 @@ class _Once(torch.autograd.Function):
 class _FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        out, preact = _forward(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, weight, preact)
+        out, x_read, weight_read, preact = _forward(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
+        # (the inputs themselves as well: a change of them before the backward pass is noticed)
+        ctx.save_for_backward(x, weight, x_read, weight_read, preact)
         ctx.act = act
         return out
 
     @staticmethod
     def backward(ctx, grad):
-        x, weight, preact = ctx.saved_tensors
+        x, weight, x_read, weight_read, preact = ctx.saved_tensors
         wanted = ctx.needs_input_grad
         gx = gw = gb = None
         if any(wanted[:3]):
             with torch.no_grad():
-                gx, gw, gb = _gradients(grad, x, weight, preact, ctx.act, wanted)
+                gx, gw, gb = _gradients(grad, x_read, weight_read, preact, ctx.act, wanted)
         grads = (gx, gw, gb, grad if wanted[3] else None)
         if torch.is_grad_enabled():   # create_graph=True
             grads = tuple(None if g is None or g is grad else _Once.apply(g, grad, x, weight) for g in grads)
@@ -168,7 +184,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
                                     (residual is not None and residual.requires_grad)):
         out = _FusedLinear.apply(x2, weight, bias, r2, act)
     else:
-        out, _ = _forward(x2, weight, bias, r2, act, False)
+        out = _forward(x2, weight, bias, r2, act, False)[0]
     return out if flat else out.view(shape)
 
 

@@ -101,7 +101,8 @@ int for_lists(const FgClipArgs& a, bool scaling, F launch) {
                 it.in = t.grad; it.out = t.out; it.count = t.count;
                 it.first = uint32_t(chunks);
                 it.wide_in = reinterpret_cast<uintptr_t>(t.grad) % 16 == 0;
-                it.wide_out = reinterpret_cast<uintptr_t>(t.out) % std::min(16, 16 / esz * elem_size(odt)) == 0;
+                // the results of one vector: 16 bytes of the wider type, as many of the other
+                it.wide_out = reinterpret_cast<uintptr_t>(t.out) % (16 / std::max(esz, elem_size(odt)) * elem_size(odt)) == 0;
                 chunks += (t.count * esz + fg::clip::CHUNK_BYTES - 1) / fg::clip::CHUNK_BYTES;
                 if (chunks > (int64_t(1) << 31)) return FG_ENOTSUP;
             }

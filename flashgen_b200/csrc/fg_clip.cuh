@@ -130,52 +130,73 @@ __global__ void __launch_bounds__(THREADS) total_kernel(const double* partial, i
     if (threadIdx.x == 0) *total = sum;
 }
 
-// One 16-byte vector of gradients, scaled, as VEC elements of the result's type.
+// What a thread loads and stores at once: 16 bytes of the wider type, so that both are
+// neighbouring bytes across a warp (16-byte loads of 16-bit gradients with two stores of 32-bit
+// results each wrote half sectors: 805 million bf16 gradients 990 us, 4.9 TB/s).
 template <int DT, int ODT>
-__device__ __forceinline__ void store_scaled(void* out, int64_t at, const uint4& q, float c) {
-    constexpr int VEC = Elem<DT>::VEC;
-    float x[VEC];
-    Elem<DT>::unpack(q, x);
+struct Vector {
+    static constexpr int N = 16 / (Elem<DT>::SIZE > Elem<ODT>::SIZE ? Elem<DT>::SIZE : Elem<ODT>::SIZE);
+};
+template <int BYTES> struct Words;
+template <> struct Words<16> { using T = uint4; };
+template <> struct Words<8> { using T = uint2; };
+
+template <int DT, int N, class W>
+__device__ __forceinline__ void unpack(const W& q, float (&x)[N]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&q);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) x[i] *= c;
-    if constexpr (ODT == FG_DTYPE_F32) {
-        float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
+    for (int i = 0; i < N; ++i) {
+        if constexpr (DT == FG_DTYPE_F32) x[i] = __uint_as_float(w[i]);
+        else if constexpr (DT == FG_DTYPE_BF16) x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        else x[i] = __half2float(__ushort_as_half(uint16_t(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
+    }
+}
+template <int ODT, int N, class W>
+__device__ __forceinline__ W pack(const float (&x)[N]) {
+    W q;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&q);
 #pragma unroll
-        for (int i = 0; i < VEC / 4; ++i) __stcs(p + i, make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
-    } else {
-        uint32_t w[VEC / 2];
-#pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) {
+    for (int i = 0; i < N; ++i) {
+        if constexpr (ODT == FG_DTYPE_F32) {
+            w[i] = __float_as_uint(x[i]);
+        } else if (i % 2 == 0) {
             if constexpr (ODT == FG_DTYPE_F16) {
-                const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                const __half2 h = __floats2half2_rn(x[i], x[i + 1]);
+                w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
             } else {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x[i], x[i + 1]);
+                w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
             }
         }
-        uint16_t* p = reinterpret_cast<uint16_t*>(out) + at;
-        if constexpr (VEC == 8) __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
-        else __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
     }
+    return q;
 }
 
 template <int DT, int ODT>
 __device__ __forceinline__ void scale_chunk(const Item& it, int64_t lo, int64_t hi, float c) {
-    constexpr int VEC = Elem<DT>::VEC;
+    constexpr int N = Vector<DT, ODT>::N;
+    using In = typename Words<N * Elem<DT>::SIZE>::T;
+    using Out = typename Words<N * Elem<ODT>::SIZE>::T;
+    constexpr int LOADS = CHUNK_BYTES / int(sizeof(In)) / THREADS;
     int64_t done = lo;
     if (it.wide_in && it.wide_out) {
-        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(it.in) + lo * Elem<DT>::SIZE);
-        const int vecs = int((hi - lo) / VEC);
-        uint4 q[UNROLL];
+        const In* p = reinterpret_cast<const In*>(reinterpret_cast<const char*>(it.in) + lo * Elem<DT>::SIZE);
+        Out* o = reinterpret_cast<Out*>(reinterpret_cast<char*>(it.out) + lo * Elem<ODT>::SIZE);
+        const int vecs = int((hi - lo) / N);
+        In q[LOADS];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
+        for (int u = 0; u < LOADS; ++u)
             if (u * THREADS + int(threadIdx.x) < vecs) q[u] = __ldcs(p + u * THREADS + threadIdx.x);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-            if (u * THREADS + int(threadIdx.x) < vecs)
-                store_scaled<DT, ODT>(it.out, lo + int64_t(u * THREADS + threadIdx.x) * VEC, q[u], c);
-        done = lo + int64_t(vecs) * VEC;
+        for (int u = 0; u < LOADS; ++u)
+            if (u * THREADS + int(threadIdx.x) < vecs) {
+                float x[N];
+                unpack<DT>(q[u], x);
+#pragma unroll
+                for (int i = 0; i < N; ++i) x[i] *= c;
+                __stcs(o + u * THREADS + threadIdx.x, pack<ODT, N, Out>(x));
+            }
+        done = lo + int64_t(vecs) * N;
     }
     // (not through the read-only cache: the result may replace what is read)
 #pragma unroll 4

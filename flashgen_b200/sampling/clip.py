@@ -11,16 +11,28 @@ from __future__ import annotations
 
 import array
 import math
+from operator import attrgetter
 from typing import List, Optional, Sequence, Union
 
 import torch
 
 from .. import _lib
-from .sampler import _DTYPES, _call, _written
+from .sampler import _DTYPES, _call
+
+# Lists are gone through by map: a training step has hundreds of tensors, and what Python does
+# for each of them takes longer than the kernels do.
+_dtype, _layout, _shape = attrgetter("dtype"), attrgetter("layout"), attrgetter("shape")
+_address, _count, _device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
+_dense, _inference = torch.Tensor.is_contiguous, torch.Tensor.is_inference
 
 
 def _list(tensors: Union[torch.Tensor, Sequence[torch.Tensor]], what: str) -> List[torch.Tensor]:
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    try:
+        if set(map(_layout, tensors)) <= {torch.strided} and set(map(_dtype, tensors)) <= _DTYPES.keys():
+            return tensors
+    except AttributeError:
+        pass
     for t in tensors:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what} must be tensors, got {type(t).__name__}")
@@ -34,28 +46,29 @@ def _norm(grads: List[torch.Tensor], out: Optional[List[torch.Tensor]], max_norm
     dev = grads[0].device
     if dev.type != "cuda":
         raise RuntimeError(f"flashgen_b200 runs on the GPU only; the gradients are on {dev}")
-    index = dev.index
-    for t in grads if out is None else grads + out:
-        if t.get_device() != index:
-            raise ValueError(f"gradients on {dev} and on {t.device}: one call works on one device")
-    flat = []
+    devices = set(map(_device, grads if out is None else grads + out))
+    if devices != {dev.index}:
+        raise ValueError(f"gradients on devices {sorted(devices)}: one call works on one device")
+    n = len(grads)
+    code = _DTYPES.__getitem__
+    codes = map(code, map(_dtype, grads))
+    table = array.array("q", bytes(32 * n))       # FgGradTensor, field by field
+    table[0::4] = array.array("q", map(_address, grads))
+    table[2::4] = array.array("q", map(_count, grads))
     if out is None:
-        for g in grads:
-            flat += (g.data_ptr(), 0, g.numel(), _DTYPES[g.dtype])
+        table[3::4] = array.array("q", codes)
     else:
-        for g, o in zip(grads, out):
-            flat += (g.data_ptr(), o.data_ptr(), g.numel(), _DTYPES[g.dtype] | _DTYPES[o.dtype] << 32)
-    table = array.array("q", flat)       # FgGradTensor, field by field
+        table[1::4] = array.array("q", map(_address, out))
+        table[3::4] = array.array("q", [g | o << 32 for g, o in zip(codes, map(code, map(_dtype, out)))])
     lib = _lib.load()
-    need = lib.fg_clip_workspace_size(len(grads))
+    need = lib.fg_clip_workspace_size(n)
     if need == 0:
-        raise ValueError(f"too many tensors: {len(grads)}")
-    room = torch.empty(need + 8, dtype=torch.uint8, device=dev)   # the norm, then the workspace
-    norm = room[:4].view(torch.float32).squeeze(0)
+        raise ValueError(f"too many tensors: {n}")
+    room = torch.empty(need // 4 + 2, dtype=torch.float32, device=dev)   # the norm, then the workspace
     at = room.data_ptr()
-    a = _lib.FgClipArgs(table.buffer_info()[0], len(grads), 0, max_norm, scale, at, at + 8, need)
+    a = _lib.FgClipArgs(table.buffer_info()[0], n, 0, max_norm, scale, at, at + 8, need)
     _call(dev, lib.fg_clip_grad_norm, a, "fg_clip_grad_norm")
-    return norm
+    return room[0]
 
 
 def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], *, scale: float = 1.0) -> torch.Tensor:
@@ -99,24 +112,28 @@ def clip_grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm:
     given = grads if out is None else _list(out, "out")
     if len(given) != len(grads):
         raise ValueError(f"{len(grads)} gradients, {len(given)} results")
-    if out is not None:
-        for g, o in zip(grads, given):
-            if g.shape != o.shape:
-                raise ValueError(f"out must have the gradients' shapes, got {tuple(o.shape)} for {tuple(g.shape)}")
+    if out is not None and list(map(_shape, grads)) != list(map(_shape, given)):
+        g, o = next((g, o) for g, o in zip(grads, given) if g.shape != o.shape)
+        raise ValueError(f"out must have the gradients' shapes, got {tuple(o.shape)} for {tuple(g.shape)}")
     with torch.no_grad():
         src, dst = grads, given
-        if not all([t.is_contiguous() for t in (grads if out is None else grads + given)]):
+        if not all(map(_dense, grads if out is None else grads + given)):
             # others go through a dense copy, and the results back through one
             src = [g.contiguous() for g in grads]
             dst = [s if o is g else o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format)
                    for g, s, o in zip(grads, src, given)]
             _apart(given)
         norm = _norm(src, dst, max_norm, scale)
-        for o, d in zip(given, dst):
-            if o is not d:
-                o.copy_(d)
-            else:
-                _written(o)
+        written = given
+        if dst is not given:
+            written = [o for o, d in zip(given, dst) if o is d]
+            for o, d in zip(given, dst):
+                if o is not d:
+                    o.copy_(d)
+        # a graph that saved one of them raises instead of going on with what it finds there
+        if any(map(_inference, written)):
+            written = [t for t in written if not t.is_inference()]
+        torch.autograd.graph.increment_version(written)
     if check_errors and not math.isfinite(float(norm)):
         raise RuntimeError(f"the gradients' norm is {float(norm)}")
     return norm

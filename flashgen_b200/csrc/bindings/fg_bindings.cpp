@@ -11,6 +11,7 @@
 // fg_strerror's text, the reference's error behaviour on the Python side.
 #include <cstdint>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include <pybind11/pybind11.h>
@@ -23,7 +24,7 @@ namespace py = pybind11;
 namespace {
 
 // The reference's C++ SamplingParams (csrc/include/request.hpp:14-22), with
-// the presence and frequency penalties of the sampler added.
+// the presence and frequency penalties and the min-p of the sampler added.
 struct SamplingParams {
     float temperature = 1.0f;
     float top_p = 0.9f;
@@ -31,6 +32,7 @@ struct SamplingParams {
     float repetition_penalty = 1.0f;
     float presence_penalty = 0.0f;
     float frequency_penalty = 0.0f;
+    float min_p = 0.0f;
     bool greedy = false;
     int max_tokens = 128;
     std::vector<int> stop_token_ids = {50256};  // EOS for GPT-2
@@ -59,6 +61,7 @@ PYBIND11_MODULE(_C, m) {
         .def_readwrite("repetition_penalty", &SamplingParams::repetition_penalty)
         .def_readwrite("presence_penalty", &SamplingParams::presence_penalty)
         .def_readwrite("frequency_penalty", &SamplingParams::frequency_penalty)
+        .def_readwrite("min_p", &SamplingParams::min_p)
         .def_readwrite("greedy", &SamplingParams::greedy)
         .def_readwrite("max_tokens", &SamplingParams::max_tokens)
         .def_readwrite("stop_token_ids", &SamplingParams::stop_token_ids);
@@ -283,6 +286,174 @@ PYBIND11_MODULE(_C, m) {
           py::arg("weight_stride") = 0, py::arg("down_stride") = 0, py::arg("out_stride") = 0,
           py::arg("stream") = 0,
           "fg_adapter_logits on device buffers (integers: device pointers; 0: absent).");
+
+    m.attr("ACT_NONE") = (int)FG_ACT_NONE;
+    m.attr("ACT_RELU") = (int)FG_ACT_RELU;
+    m.attr("ACT_GELU") = (int)FG_ACT_GELU;
+    m.attr("ACT_GELU_TANH") = (int)FG_ACT_GELU_TANH;
+    m.attr("ACT_SILU") = (int)FG_ACT_SILU;
+
+    m.def("sample_min_p_workspace_size",
+          [](int32_t batch, int32_t vocab, int32_t hist_max_len) {
+              return fg_sample_min_p_workspace_size(batch, vocab, hist_max_len);
+          },
+          py::arg("batch"), py::arg("vocab"), py::arg("hist_max_len") = 0);
+
+    m.def("sample_min_p",
+          [](std::uintptr_t logits, int dtype, int32_t batch, int32_t vocab, int64_t row_stride,
+             std::uintptr_t min_p, std::uintptr_t uniforms, std::uintptr_t out_ids, std::uintptr_t workspace,
+             size_t workspace_bytes, std::uintptr_t temperature, std::uintptr_t top_p, std::uintptr_t top_k,
+             std::uintptr_t status, std::uintptr_t out_logprobs, std::uintptr_t out_kept,
+             std::uintptr_t repetition_penalty, std::uintptr_t presence_penalty, std::uintptr_t frequency_penalty,
+             std::uintptr_t greedy, std::uintptr_t hist_ids, std::uintptr_t hist_offsets, int32_t hist_max_len,
+             std::uintptr_t stream) {
+              FgMinPArgs a{};
+              a.sample.logits = ptr<const void>(logits);
+              a.sample.dtype = dtype;
+              a.sample.batch = batch;
+              a.sample.vocab = vocab;
+              a.sample.row_stride = row_stride > 0 ? row_stride : vocab;
+              a.sample.hist_ids = ptr<const int32_t>(hist_ids);
+              a.sample.hist_offsets = ptr<const int64_t>(hist_offsets);
+              a.sample.hist_max_len = hist_max_len;
+              a.sample.temperature = ptr<const float>(temperature);
+              a.sample.top_p = ptr<const float>(top_p);
+              a.sample.top_k = ptr<const int32_t>(top_k);
+              a.sample.repetition_penalty = ptr<const float>(repetition_penalty);
+              a.sample.presence_penalty = ptr<const float>(presence_penalty);
+              a.sample.frequency_penalty = ptr<const float>(frequency_penalty);
+              a.sample.greedy = ptr<const uint8_t>(greedy);
+              a.sample.uniforms = ptr<const float>(uniforms);
+              a.sample.out_ids = ptr<int64_t>(out_ids);
+              a.sample.out_status = ptr<int32_t>(status);
+              a.sample.workspace = ptr<void>(workspace);
+              a.sample.workspace_bytes = workspace_bytes;
+              a.min_p = ptr<const float>(min_p);
+              a.out_logprobs = ptr<float>(out_logprobs);
+              a.out_kept = ptr<int32_t>(out_kept);
+              int rc;
+              {
+                  py::gil_scoped_release release;
+                  rc = fg_sample_min_p(&a, ptr<void>(stream));
+              }
+              check(rc, "fg_sample_min_p");
+          },
+          py::arg("logits"), py::arg("dtype"), py::arg("batch"), py::arg("vocab"), py::arg("row_stride") = 0,
+          py::arg("min_p") = 0, py::arg("uniforms"), py::arg("out_ids"), py::arg("workspace"),
+          py::arg("workspace_bytes"), py::arg("temperature") = 0, py::arg("top_p") = 0, py::arg("top_k") = 0,
+          py::arg("status") = 0, py::arg("out_logprobs") = 0, py::arg("out_kept") = 0,
+          py::arg("repetition_penalty") = 0, py::arg("presence_penalty") = 0, py::arg("frequency_penalty") = 0,
+          py::arg("greedy") = 0, py::arg("hist_ids") = 0, py::arg("hist_offsets") = 0, py::arg("hist_max_len") = 0,
+          py::arg("stream") = 0, "fg_sample_min_p on device buffers (integers: device pointers; 0: absent).");
+
+    m.def("linear",
+          [](std::uintptr_t x, std::uintptr_t weight, std::uintptr_t out, int dtype, int32_t tokens, int32_t inner,
+             int32_t outer, int activation, std::uintptr_t bias, std::uintptr_t residual, std::uintptr_t preact,
+             std::uintptr_t workspace, size_t workspace_bytes, int64_t x_stride, int64_t weight_stride,
+             int64_t residual_stride, int64_t out_stride, int64_t preact_stride, std::uintptr_t stream) {
+              FgLinearArgs a{};
+              a.x = ptr<const void>(x);
+              a.weight = ptr<const void>(weight);
+              a.bias = ptr<const void>(bias);
+              a.residual = ptr<const void>(residual);
+              a.out = ptr<void>(out);
+              a.preact = ptr<float>(preact);
+              a.workspace = ptr<void>(workspace);
+              a.workspace_bytes = workspace_bytes;
+              a.dtype = dtype;
+              a.tokens = tokens;
+              a.inner = inner;
+              a.outer = outer;
+              a.activation = activation;
+              a.x_stride = x_stride > 0 ? x_stride : inner;
+              a.weight_stride = weight_stride > 0 ? weight_stride : inner;
+              a.residual_stride = residual_stride > 0 ? residual_stride : outer;
+              a.out_stride = out_stride > 0 ? out_stride : outer;
+              a.preact_stride = preact_stride > 0 ? preact_stride : outer;
+              int rc;
+              {
+                  py::gil_scoped_release release;
+                  rc = fg_linear(&a, ptr<void>(stream));
+              }
+              check(rc, "fg_linear");
+          },
+          py::arg("x"), py::arg("weight"), py::arg("out"), py::arg("dtype"), py::arg("tokens"), py::arg("inner"),
+          py::arg("outer"), py::arg("activation") = 0, py::arg("bias") = 0, py::arg("residual") = 0,
+          py::arg("preact") = 0, py::arg("workspace") = 0, py::arg("workspace_bytes") = 0, py::arg("x_stride") = 0,
+          py::arg("weight_stride") = 0, py::arg("residual_stride") = 0, py::arg("out_stride") = 0,
+          py::arg("preact_stride") = 0, py::arg("stream") = 0,
+          "fg_linear on device buffers (integers: device pointers; 0: absent).");
+
+    m.def("linear_grad",
+          [](std::uintptr_t grad_out, std::uintptr_t x, std::uintptr_t weight, int dtype, int32_t tokens, int32_t inner,
+             int32_t outer, int activation, std::uintptr_t preact, std::uintptr_t grad_x, std::uintptr_t grad_weight,
+             std::uintptr_t grad_bias, std::uintptr_t workspace, size_t workspace_bytes, int64_t grad_out_stride,
+             int64_t x_stride, int64_t weight_stride, int64_t preact_stride, int64_t grad_x_stride,
+             int64_t grad_weight_stride, std::uintptr_t stream) {
+              FgLinearGradArgs a{};
+              a.grad_out = ptr<const void>(grad_out);
+              a.x = ptr<const void>(x);
+              a.weight = ptr<const void>(weight);
+              a.preact = ptr<const float>(preact);
+              a.grad_x = ptr<void>(grad_x);
+              a.grad_weight = ptr<void>(grad_weight);
+              a.grad_bias = ptr<void>(grad_bias);
+              a.workspace = ptr<void>(workspace);
+              a.workspace_bytes = workspace_bytes;
+              a.dtype = dtype;
+              a.tokens = tokens;
+              a.inner = inner;
+              a.outer = outer;
+              a.activation = activation;
+              a.grad_out_stride = grad_out_stride > 0 ? grad_out_stride : outer;
+              a.x_stride = x_stride > 0 ? x_stride : inner;
+              a.weight_stride = weight_stride > 0 ? weight_stride : inner;
+              a.preact_stride = preact_stride > 0 ? preact_stride : outer;
+              a.grad_x_stride = grad_x_stride > 0 ? grad_x_stride : inner;
+              a.grad_weight_stride = grad_weight_stride > 0 ? grad_weight_stride : inner;
+              int rc;
+              {
+                  py::gil_scoped_release release;
+                  rc = fg_linear_grad(&a, ptr<void>(stream));
+              }
+              check(rc, "fg_linear_grad");
+          },
+          py::arg("grad_out"), py::arg("x"), py::arg("weight"), py::arg("dtype"), py::arg("tokens"), py::arg("inner"),
+          py::arg("outer"), py::arg("activation") = 0, py::arg("preact") = 0, py::arg("grad_x") = 0,
+          py::arg("grad_weight") = 0, py::arg("grad_bias") = 0, py::arg("workspace") = 0,
+          py::arg("workspace_bytes") = 0, py::arg("grad_out_stride") = 0, py::arg("x_stride") = 0,
+          py::arg("weight_stride") = 0, py::arg("preact_stride") = 0, py::arg("grad_x_stride") = 0,
+          py::arg("grad_weight_stride") = 0, py::arg("stream") = 0,
+          "fg_linear_grad on device buffers (integers: device pointers; 0: absent).");
+
+    m.def("clip_workspace_size", [](int32_t count) { return fg_clip_workspace_size(count); }, py::arg("count"));
+
+    m.def("clip_grad_norm",
+          [](const std::vector<std::tuple<std::uintptr_t, std::uintptr_t, int64_t, int, int>>& tensors, float max_norm,
+             float scale, std::uintptr_t out_norm, std::uintptr_t workspace, size_t workspace_bytes,
+             std::uintptr_t stream) {
+              std::vector<FgGradTensor> list;
+              for (const auto& t : tensors)
+                  list.push_back({ptr<const void>(std::get<0>(t)), ptr<void>(std::get<1>(t)), std::get<2>(t),
+                                  std::get<3>(t), std::get<4>(t)});
+              FgClipArgs a{};
+              a.tensors = list.data();
+              a.count = (int32_t)list.size();
+              a.max_norm = max_norm;
+              a.scale = scale;
+              a.out_norm = ptr<float>(out_norm);
+              a.workspace = ptr<void>(workspace);
+              a.workspace_bytes = workspace_bytes;
+              int rc;
+              {
+                  py::gil_scoped_release release;
+                  rc = fg_clip_grad_norm(&a, ptr<void>(stream));
+              }
+              check(rc, "fg_clip_grad_norm");
+          },
+          py::arg("tensors"), py::arg("max_norm"), py::arg("scale") = 1.0f, py::arg("out_norm"), py::arg("workspace"),
+          py::arg("workspace_bytes"), py::arg("stream") = 0,
+          "fg_clip_grad_norm on a list of (gradient, result or 0, elements, type, result's type).");
 
     m.def("version", []() { return fg_version(); });
     m.def("strerror", [](int code) { return std::string(fg_strerror(code)); });

@@ -45,6 +45,28 @@ bool set_smem(K kern, std::atomic<int>* done, int bytes) {
     return true;
 }
 
+// Whether a cluster of sixteen CTAs with `smem` bytes each finds room (asked once a size and device).
+template <class K>
+bool sixteen_fit(K kern, std::atomic<int>* largest, int smem) {
+    int dev = 0, active = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    if (largest[dev].load(std::memory_order_acquire) >= smem) return true;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(fg::minp::NT);
+    cfg.dynamicSmemBytes = size_t(smem);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 16;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&active, kern, &cfg) != cudaSuccess || active < 1) return false;
+    largest[dev].store(smem, std::memory_order_release);
+    return true;
+}
+
 int launch_early(void (*kern)(fg::minp::Params, int), unsigned grid, unsigned threads, size_t smem, int cluster,
                  cudaStream_t st, const fg::minp::Params& P) {
     cudaLaunchConfig_t cfg{};
@@ -69,20 +91,23 @@ int launch(fg::minp::Params P, DevInfo* d, cudaStream_t st) {
     static std::atomic<int> rows_smem[fg::host::kMaxDevices] = {}, wide_smem[fg::host::kMaxDevices] = {};
     static std::atomic<int> uncached_smem[fg::host::kMaxDevices] = {};
     const int esz = fg::Elem<DT>::SIZE;
-    const int G = ctas_per_row(P.batch, P.vocab, esz, d);
+    int G = ctas_per_row(P.batch, P.vocab, esz, d);
     const int smem = RING_BYTES + CAP * int(sizeof(Candidate)) + (P.penalties ? P.slots * 8 + ROW_FILTER * 4 : 0);
+    static std::atomic<int> sixteen[fg::host::kMaxDevices] = {};
     if (!set_smem(rows_kernel<DT>, rows_smem, smem)) return FG_EDEVICE;
+    if (G > 8 && !sixteen_fit(rows_kernel<DT>, sixteen, smem)) G = 8;
     int rc = launch_early(rows_kernel<DT>, unsigned(P.batch) * G, NT, smem, G, st, P);
     if (rc != FG_OK) return rc;
-    // wide_kernel: the slice's keys in shared memory where they fit; four CTAs a row where that
-    // leaves work for every SM
+    // wide_kernel: the slice's keys in shared memory where they fit
     auto fixed = [&](int g) { return 16 * MEMBERS + bins_bytes(g); };
     auto keys = [&](int g) {
         const int64_t chunks = int64_t(P.vocab) * esz / 16 + 1;
         return (chunks + g - 1) / g * (16 / esz) + 2 * (16 / esz) + KEY_PAD;
     };
     const int room = d->smem_optin - int(sizeof(WideShared) + sizeof(ExpTable)) - 1024;
-    const int W = P.batch > d->sms / 8 && fixed(4) + 4 * keys(4) <= room ? 4 : 8;
+    // Four CTAs a row where that leaves work for every SM: 43 wide rows of 128256 with histories
+    // 142 us, with eight CTAs each 200; four wide rows 41 us, 36.
+    const int W = P.batch > d->sms / 8 && fixed(4) + 4 * keys(4) <= room ? 4 : WIDE_G;
     const bool cached = fixed(W) + 4 * keys(W) <= room;
     const int wsmem = fixed(W) + 4 * (cached ? int(keys(W)) : P.penalties ? FILTER_WORDS : 0);
     if (!set_smem(cached ? wide_kernel<DT, true> : wide_kernel<DT, false>, cached ? wide_smem : uncached_smem, wsmem))

@@ -26,7 +26,8 @@ constexpr int CAP = 4096;          // candidates of a CTA's slice, and of a row
 constexpr int RBINS = 1024;        // bins of their masses
 constexpr int MEMBERS = 1024;      // tokens of one bin that are put in order
 constexpr int MAX_K = 512;         // top-k that rows_kernel takes without min-p
-constexpr int MAX_G = 8;           // CTAs that share a row
+constexpr int MAX_G = 16;          // CTAs that share a row
+constexpr int WIDE_G = 8;          // in wide_kernel
 constexpr int HIST_CAP = 4096;     // history ids of a row that rows_kernel takes
 constexpr int WNT = 512;           // threads of wide_kernel
 constexpr int BINS = 2048;         // of a radix step
@@ -567,39 +568,54 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
             if (lane == 0) atomicMax(&S.top, key);
         }
     };
-    // a chunk a lane
-    auto scan = [&](const uint4& q, int c, bool valid) {
-        const float m = chunk_max<DT>(q);
-        if (!valid || m < bound) return;
-        float x[VEC];
-        E::unpack(q, x);
-        const uint32_t col = uint32_t(g.head + c * VEC);
-        uint32_t mine = 0;               // elements that reach the bound
+    // A thread's chunks of a stage, in the ring from `place` on (the first is chunk c0, the others
+    // NT chunks apart): their elements that reach the bound take places together, and come out of
+    // the ring one by one, so that a warp's steps are those of its busiest lane.
+    auto scan = [&](uint32_t place, int c0) {
+        uint32_t mine = 0;               // VEC bits a chunk
+        float most = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) mine |= uint32_t(!(x[j] < bound)) << j;
-        float most = m;
-        if (pen || !(bound > -INFINITY) || m != m) {
-            // history columns, -inf and NaN are none
-            most = -INFINITY;
+        for (int i = 0; i < UNROLL; ++i) {
+            const uint4 q = lds_v4(place + i * NT * 16);
+            const float m = chunk_max<DT>(q);
+            if (c0 + i * NT >= ch1 || m < bound) continue;
+            float x[VEC];
+            E::unpack(q, x);
+            uint32_t bits = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (mine >> j & 1u) {
-                    const bool other = in_history(col + j);
-                    if (x[j] != x[j] && !other) atomicOr(&S.flags, uint32_t(FG_ROW_NAN));
-                    if (other || !(x[j] > -INFINITY)) mine &= ~(1u << j);
-                    else most = fmaxf(most, x[j]);
-                }
+            for (int j = 0; j < VEC; ++j) bits |= uint32_t(!(x[j] < bound)) << j;
+            if (pen || !(bound > -INFINITY) || m != m) {
+                // history columns, -inf and NaN are none
+                const uint32_t col = uint32_t(g.head + (c0 + i * NT) * VEC);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (bits >> j & 1u) {
+                        const bool other = in_history(col + j);
+                        if (x[j] != x[j] && !other) atomicOr(&S.flags, uint32_t(FG_ROW_NAN));
+                        if (other || !(x[j] > -INFINITY)) bits &= ~(1u << j);
+                        else most = fmaxf(most, x[j]);
+                    }
+            } else {
+                most = fmaxf(most, m);
+            }
+            mine |= bits << (i * VEC);
         }
         if (mine == 0u) return;
         uint32_t at = atomicAdd(&S.count, uint32_t(__popc(mine)));
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if (mine >> j & 1u) {
-                if (at < uint32_t(CAP)) cand[at] = {x[j], col + j};
-                ++at;
-            }
+        do {
+            const int b = __ffs(mine) - 1, i = b / VEC, j = b % VEC;
+            mine &= mine - 1u;
+            const uint32_t from = place + i * NT * 16 + j * E::SIZE;
+            float x;
+            if constexpr (DT == FG_DTYPE_F32) x = __uint_as_float(lds_u32(from));
+            else if constexpr (DT == FG_DTYPE_F16) x = __half2float(__ushort_as_half(uint16_t(lds_u16(from))));
+            else x = __uint_as_float(lds_u16(from) << 16);
+            if (at < uint32_t(CAP)) cand[at] = {x, uint32_t(g.head + (c0 + i * NT) * VEC + j)};
+            ++at;
+        } while (mine);
         if (most > seen) atomicMax(&S.top, fkey(most));
     };
+    static_assert(UNROLL * VEC <= 32, "a bit for each element of a stage");
     // columns [lo, hi) one by one (fewer than a chunk), by the first warp
     auto scan_columns = [&](int lo, int hi) {
         if (warp != 0) return;
@@ -632,11 +648,7 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
                 bound = bound_of(row, seen, span);
                 with_k(S.least);
             }
-#pragma unroll
-            for (int i = 0; i < UNROLL; ++i) {
-                const int c = ch0 + (k * UNROLL + i) * NT + tid;
-                scan(lds_v4(ring + (k % STAGES * UNROLL + i) * NT * 16), c, c < ch1);
-            }
+            scan(ring + k % STAGES * (UNROLL * NT * 16), ch0 + k * UNROLL * NT + tid);
             fetch(k + STAGES);   // (past the slice: an empty group, which keeps the count)
         }
         scan_ragged();
@@ -694,9 +706,10 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
     const uint32_t least_k = row.greedy ? top_key : least_key(S.log_min_p, top);
     if (G > 1) {
         // the other slices' candidates come to the first CTA, by a warp each
-        const uint32_t n = __shfl_sync(0xffffffffu, slice_count, warp % MAX_G);
-        if (rank == 0 && decide && warp > 0 && warp < G) {
-            const uint32_t src = mapa(cand, uint32_t(warp));
+        for (int peer = warp; peer < G; peer += NT / 32) {
+            const uint32_t n = __shfl_sync(0xffffffffu, slice_count, peer);
+            if (rank != 0 || !decide || peer == 0) continue;
+            const uint32_t src = mapa(cand, uint32_t(peer));
             for (uint32_t j = lane; j < n; j += 32) {
                 const uint64_t c = ld_cluster64(src + 8 * j);   // {x, col}
                 if (fkey(ydiv(row.p, __uint_as_float(uint32_t(c)))) < least_k) continue;
@@ -704,7 +717,6 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
                 if (at < uint32_t(CAP)) cand[at] = {__uint_as_float(uint32_t(c)), uint32_t(c >> 32)};
             }
         }
-        static_assert(NT / 32 >= MAX_G, "a warp for each slice");
         cluster_sync();                           // nobody leaves while its candidates may be read
     }
     if (rank == 0) {
@@ -1060,9 +1072,9 @@ __device__ __forceinline__ void fill_bins(const S_& slice, const Bins& B, int G,
     cluster_sync();
     for (int i = tid; i < per; i += WNT) {
         const int at = rank * per + i;
-        uint32_t lo[MAX_G], hi[MAX_G], n[MAX_G];
+        uint32_t lo[WIDE_G], hi[WIDE_G], n[WIDE_G];
 #pragma unroll
-        for (int c = 0; c < MAX_G; ++c) {
+        for (int c = 0; c < WIDE_G; ++c) {
             lo[c] = c < G ? ld_cluster(mapa(&B.mine.lo[at], c)) : 0u;
             hi[c] = c < G ? ld_cluster(mapa(&B.mine.hi[at], c)) : 0u;
             n[c] = c < G ? ld_cluster(mapa(&B.mine.count[at], c)) : 0u;
@@ -1070,7 +1082,7 @@ __device__ __forceinline__ void fill_bins(const S_& slice, const Bins& B, int G,
         uint64_t m = 0;
         uint32_t count = 0;
 #pragma unroll
-        for (int c = 0; c < MAX_G; ++c) {
+        for (int c = 0; c < WIDE_G; ++c) {
             m += uint64_t(hi[c]) << 32 | lo[c];
             count += n[c];
         }

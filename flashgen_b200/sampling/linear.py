@@ -10,7 +10,7 @@ C ABI (``fg_linear``) whose epilogue does the rest, differentiable through
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional
 
 import torch
 
@@ -32,44 +32,37 @@ def _stride(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _room(size: int, like: torch.Tensor) -> Optional[torch.Tensor]:
-    return None if size == 0 else torch.empty(size, dtype=torch.uint8, device=like.device)
-
-
 def _forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
-             act: int, keep: bool) -> Tuple[torch.Tensor, ...]:
-    """The block on matrices; with `keep` also what the gradients read: x and the weight (their
-    aligned copies, where the call made some) and the sums before the activation, in fp32 (the
-    slope at a rounded sum would lose its last bits)."""
+             act: int, keep: bool):
+    """The block on matrices. With `keep` also what the gradients read: x and the weight as
+    (tensor, byte offset, stride) each, the aligned copies where the call made some, and the sums
+    before the activation, in fp32 (the slope at a rounded sum would lose its last bits)."""
     tokens, inner, outer = x.shape[0], x.shape[1], weight.shape[0]
     out = x.new_empty((tokens, outer))
     preact = x.new_empty((tokens, (outer + 3) // 4 * 4), dtype=torch.float32) if keep and act else None
     if tokens == 0:
-        return out, x, weight, preact
+        return out, (x, 0, inner), (weight, 0, inner), preact
     x, weight = _rows(x), _rows(weight)
+    xs, ws = _stride(x), _stride(weight)
+    xp, wp = x.data_ptr(), weight.data_ptr()
     lib = _lib.load()
-    a = _lib.FgLinearArgs(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), out.data_ptr(), _ptr(preact),
-                          None, 0, _DTYPES[x.dtype], tokens, inner, outer, act, 0, _stride(x), _stride(weight),
+    a = _lib.FgLinearArgs(xp, wp, _ptr(bias), _ptr(residual), out.data_ptr(), _ptr(preact),
+                          None, 0, _DTYPES[x.dtype], tokens, inner, outer, act, 0, xs, ws,
                           _stride(residual), outer, _stride(preact))
-    room = _room(lib.fg_linear_workspace_size(a), x)
-    if room is not None:
+    # rows on 16-byte boundaries are read where they lie
+    copy_x, copy_w = xp % 16 != 0 or (tokens > 1 and xs % 8 != 0), wp % 16 != 0 or (outer > 1 and ws % 8 != 0)
+    room = None
+    if copy_x or copy_w:
+        room = torch.empty(lib.fg_linear_workspace_size(a), dtype=torch.uint8, device=x.device)
         a.workspace, a.workspace_bytes = room.data_ptr(), room.numel()
     _call(x.device, lib.fg_linear, a, "fg_linear")
-    if keep and room is not None:
-        # the workspace has x's copy, if one was made, then the weight's: rows of inner rounded up to 8
-        copies, width = room.view(x.dtype), (inner + 7) // 8 * 8
-        of_weight = 0
-        if not _aligned(x):
-            x = copies[:tokens * width].view(tokens, width)[:, :inner]
-            of_weight = (2 * tokens * width + 255) // 256 * 128
-        if not _aligned(weight):
-            weight = copies[of_weight:of_weight + outer * width].view(outer, width)[:, :inner]
-    return out, x, weight, preact
-
-
-def _aligned(t: torch.Tensor) -> bool:
-    """Whether the library reads the matrix where it lies: rows on 16-byte boundaries."""
-    return t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or t.stride(0) % 8 == 0)
+    if not keep:
+        return out, None, None, None
+    # the workspace has x's copy, if one was made, then the weight's: rows of inner rounded up to 8
+    width = (inner + 7) // 8 * 8
+    x_read = (room, 0, width) if copy_x else (x, 0, xs)
+    w_read = (room, (2 * tokens * width + 255) // 256 * 256 if copy_x else 0, width) if copy_w else (weight, 0, ws)
+    return out, x_read, w_read, preact
 
 
 class _Once(torch.autograd.Function):
@@ -88,46 +81,46 @@ class _Once(torch.autograd.Function):
 class _FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        out, x_read, weight_read, preact = _forward(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
-        # (the inputs themselves as well: a change of them before the backward pass is noticed)
-        ctx.save_for_backward(x, weight, x_read, weight_read, preact)
+        out, x_read, w_read, preact = _forward(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
+        if x_read is not None:
+            # (the inputs themselves as well: a change of them before the backward pass is noticed)
+            ctx.save_for_backward(x, weight, x_read[0], w_read[0], preact)
+            ctx.places = x_read[1:] + w_read[1:]
         ctx.act = act
         return out
 
     @staticmethod
     def backward(ctx, grad):
-        x, weight, x_read, weight_read, preact = ctx.saved_tensors
         wanted = ctx.needs_input_grad
         gx = gw = gb = None
         if any(wanted[:3]):
-            with torch.no_grad():
-                gx, gw, gb = _gradients(grad, x_read, weight_read, preact, ctx.act, wanted)
-        grads = (gx, gw, gb, grad if wanted[3] else None)
-        if torch.is_grad_enabled():   # create_graph=True
-            grads = tuple(None if g is None or g is grad else _Once.apply(g, grad, x, weight) for g in grads)
-            grads = grads[:3] + (grad if wanted[3] else None,)
-        return (*grads, None)
+            x, weight, x_read, w_read, preact = ctx.saved_tensors
+            gx, gw, gb = _gradients(grad.detach(), x, weight, x_read, w_read, ctx.places, preact, ctx.act, wanted)
+            if torch.is_grad_enabled():   # create_graph=True
+                gx, gw, gb = (None if g is None else _Once.apply(g, grad, x, weight) for g in (gx, gw, gb))
+        return gx, gw, gb, grad if wanted[3] else None, None
 
 
-def _gradients(grad, x, weight, preact, act, wanted):
+def _gradients(grad, x, weight, x_read, w_read, places, preact, act, wanted):
     tokens, inner, outer = x.shape[0], x.shape[1], weight.shape[0]
-    g, x, weight = _rows(grad), _rows(x), _rows(weight)
-    gx = x.new_empty((tokens, inner)) if wanted[0] else None
-    gw = x.new_empty((outer, inner)) if wanted[1] else None
-    gb = x.new_empty((outer,)) if wanted[2] else None
-    lib = _lib.load()
-    # (an empty tensor has no address: the library wants one, and reads nothing there)
-    place = (gw if gw is not None else gb if gb is not None else weight).data_ptr() if tokens == 0 else 0
-    if tokens == 0 and gw is None and gb is None:
+    gx = torch.empty((tokens, inner), dtype=x.dtype, device=x.device) if wanted[0] else None
+    gw = torch.empty((outer, inner), dtype=x.dtype, device=x.device) if wanted[1] else None
+    gb = torch.empty((outer,), dtype=x.dtype, device=x.device) if wanted[2] else None
+    if tokens == 0:      # sums over nothing
+        for g in (gw, gb):
+            if g is not None:
+                g.zero_()
         return gx, gw, gb
+    g = _rows(grad)
+    lib = _lib.load()
     a = _lib.FgLinearGradArgs(
-        g.data_ptr() or place, x.data_ptr() or place, weight.data_ptr(), _ptr(preact) or place or None,
-        None if gx is None else gx.data_ptr() or place, _ptr(gw), _ptr(gb), None, 0, _DTYPES[x.dtype], tokens, inner,
-        outer, act, 0, _stride(g) if tokens else outer, _stride(x) if tokens else inner, _stride(weight),
-        (_stride(preact) or outer) if tokens else outer, inner, inner)
-    room = _room(lib.fg_linear_grad_workspace_size(a), x)
-    if room is not None:
-        a.workspace, a.workspace_bytes = room.data_ptr(), room.numel()
+        g.data_ptr(), x_read.data_ptr() + places[0], w_read.data_ptr() + places[2], _ptr(preact), _ptr(gx), _ptr(gw),
+        _ptr(gb), None, 0, _DTYPES[x.dtype], tokens, inner, outer, act, 0, _stride(g), places[1], places[3],
+        _stride(preact), inner, inner)
+    size = lib.fg_linear_grad_workspace_size(a)
+    if size:
+        room = torch.empty(size, dtype=torch.uint8, device=x.device)
+        a.workspace, a.workspace_bytes = room.data_ptr(), size
     _call(x.device, lib.fg_linear_grad, a, "fg_linear_grad")
     return gx, gw, gb
 

@@ -52,7 +52,7 @@ def _call(dev: torch.device, fn, args, what: str) -> None:
     """One C-ABI call on ``dev``'s current stream (the raw handle: a Stream
     object and a device switch cost more than the small kernels)."""
     stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if torch.cuda.current_device() == dev.index:
+    if torch._C._cuda_getDevice() == dev.index:
         rc = fn(args, stream)
     else:
         with torch.cuda.device(dev):

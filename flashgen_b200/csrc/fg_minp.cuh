@@ -14,6 +14,8 @@
 // wide_kernel, which selects by radix over the whole row.
 #pragma once
 
+#include <cfloat>
+
 #include "fg_row.cuh"
 
 namespace fg {
@@ -367,10 +369,9 @@ __device__ __forceinline__ void sort_descending(uint64_t* v, int n) {
 }
 
 // A bound below which no logit can be kept when the largest is `top`. The slack covers the
-// roundings of x / T, of the maximum's quotient and of this product.
+// roundings of x / T, of the maximum's quotient and of this product. Finite, so that -inf is below it.
 __device__ __forceinline__ float bound_of(const Row& row, float top, float span) {
-    if (row.greedy) return top;
-    return top - span - 0x1p-20f * (fabsf(top) + span);
+    return fmaxf(row.greedy ? top : top - span - 0x1p-20f * (fabsf(top) + span), -FLT_MAX);
 }
 
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
@@ -570,47 +571,37 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
     };
     // A thread's chunks of a stage, in the ring from `place` on (the first is chunk c0, the others
     // NT chunks apart): their elements that reach the bound take places together, and come out of
-    // the ring one by one, so that a warp's steps are those of its busiest lane.
+    // the ring one by one, so that a warp's steps are those of its busiest lane. Columns of the
+    // history and NaN leave -inf in their places.
     auto scan = [&](uint32_t place, int c0) {
         uint32_t mine = 0;               // VEC bits a chunk
-        float most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
             const uint4 q = lds_v4(place + i * NT * 16);
-            const float m = chunk_max<DT>(q);
-            if (c0 + i * NT >= ch1 || m < bound) continue;
+            if (c0 + i * NT >= ch1 || chunk_max<DT>(q) < bound) continue;
             float x[VEC];
             E::unpack(q, x);
-            uint32_t bits = 0;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) bits |= uint32_t(!(x[j] < bound)) << j;
-            if (pen || !(bound > -INFINITY) || m != m) {
-                // history columns, -inf and NaN are none
-                const uint32_t col = uint32_t(g.head + (c0 + i * NT) * VEC);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (bits >> j & 1u) {
-                        const bool other = in_history(col + j);
-                        if (x[j] != x[j] && !other) atomicOr(&S.flags, uint32_t(FG_ROW_NAN));
-                        if (other || !(x[j] > -INFINITY)) bits &= ~(1u << j);
-                        else most = fmaxf(most, x[j]);
-                    }
-            } else {
-                most = fmaxf(most, m);
-            }
-            mine |= bits << (i * VEC);
+            for (int j = 0; j < VEC; ++j) mine |= uint32_t(!(x[j] < bound)) << (i * VEC + j);
         }
         if (mine == 0u) return;
         uint32_t at = atomicAdd(&S.count, uint32_t(__popc(mine)));
+        float most = -INFINITY;
         do {
             const int b = __ffs(mine) - 1, i = b / VEC, j = b % VEC;
             mine &= mine - 1u;
-            const uint32_t from = place + i * NT * 16 + j * E::SIZE;
+            const uint32_t from = place + i * NT * 16 + j * E::SIZE, col = uint32_t(g.head + (c0 + i * NT) * VEC + j);
             float x;
             if constexpr (DT == FG_DTYPE_F32) x = __uint_as_float(lds_u32(from));
             else if constexpr (DT == FG_DTYPE_F16) x = __half2float(__ushort_as_half(uint16_t(lds_u16(from))));
             else x = __uint_as_float(lds_u16(from) << 16);
-            if (at < uint32_t(CAP)) cand[at] = {x, uint32_t(g.head + (c0 + i * NT) * VEC + j)};
+            if (in_history(col)) x = -INFINITY;
+            if (x != x) {
+                atomicOr(&S.flags, uint32_t(FG_ROW_NAN));
+                x = -INFINITY;
+            }
+            most = fmaxf(most, x);
+            if (at < uint32_t(CAP)) cand[at] = {x, col};
             ++at;
         } while (mine);
         if (most > seen) atomicMax(&S.top, fkey(most));
@@ -630,7 +621,7 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
         if (last) scan_columns(g.tail0, P.vocab);
     };
     uint32_t top_key = 0, flags = 0;
-    bool sick = false;
+    bool sick = false, flat = false;
     // A second pass where too many logits reached the bounds of their moments: with the final
     // bound (from L2)
 #pragma unroll 1
@@ -647,6 +638,9 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
                 seen = funkey(*reinterpret_cast<volatile uint32_t*>(&S.top));
                 bound = bound_of(row, seen, span);
                 with_k(S.least);
+                // a flat row: too many before half of it, when the bound has hardly risen any more
+                flat = 2 * k < stages && *reinterpret_cast<volatile uint32_t*>(&S.count) > 3u * CAP / 2u;
+                if (flat) break;
             }
             scan(ring + k % STAGES * (UNROLL * NT * 16), ch0 + k * UNROLL * NT + tid);
             fetch(k + STAGES);   // (past the slice: an empty group, which keeps the count)
@@ -671,8 +665,10 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
         seen = INFINITY;                          // from here on nothing raises the maximum
         bound = bound_of(row, funkey(top_key), span);
         with_k(least);
+        // (what a slice without the end of its stream knows of the row does not matter: it is handed on)
+        flat = __syncthreads_or(flat);
         const bool over = S.count > uint32_t(CAP);
-        if (!over || sick) break;
+        if (!over || sick || flat) break;
         __syncthreads();
         if (tid == 0) S.count = 0;
 #pragma unroll
@@ -690,11 +686,13 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
         }
         __syncthreads();
     }
-    if (tid == 0) S.count_out = S.count;
+    constexpr uint32_t FLAT = 0xffffffffu;        // this slice's stream was not gone through
+    if (tid == 0) S.count_out = flat ? FLAT : S.count;
     __syncthreads();
     if (G > 1) cluster_sync();                    // every slice's candidates stand
     const uint32_t slice_count = lane < G ? (G > 1 ? ld_cluster(mapa(&S.count_out, uint32_t(lane))) : S.count_out) : 0u;
     const bool over = __any_sync(0xffffffffu, slice_count > uint32_t(CAP));
+    if (__any_sync(0xffffffffu, slice_count == FLAT)) sick = false;   // what is known of the row is not all of it
 
     // greedy rows with NaN or without a finite maximum: wide_kernel knows their first place
     const bool wide = (sick && row.greedy) || (!sick && over);

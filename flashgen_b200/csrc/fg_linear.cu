@@ -76,8 +76,14 @@ struct Cut {
 };
 
 // The cut with the least estimated time, in SM clocks. A step of K takes a CTA 2 nt clocks
-// of tensor pipe, or its operands' bytes at what L2 gives one SM while all of them read;
-// a wave ends with its last tile's epilogue.
+// of tensor pipe, or its operands' bytes at what L2 gave an SM while all of them read (64 bytes
+// a clock, 46 each of a pair); a wave ends with its last tile's epilogue, a split sum with the
+// parts' way through the cluster. Microseconds measured, bf16, bias, SiLU and residual, for
+// columns a tile x splits (pairs: p): 1 token of 4096 x 4096 16 x 4 11.1, 16 x 2 14.3, 16 x 1 20.1;
+// 64 tokens 64 x 4 13.7, 64 x 2 17.4, 16 x 1 20.8; 256 tokens 256 x 4 22.1, 128 x 2 22.3, 64 x 1
+// 23.2, p64 25.3; 512 tokens 128 x 1 25.6, p128 28.3, p256 30.2; 1024 tokens p256 32.5, 256 x 1 33.2,
+// 128 x 1 44.7; 2048 tokens p256 55.8, 256 x 1 57.6; 1024 tokens of 1024 x 1024 64 x 1 9.4, p64 10.5,
+// 128 x 1 10.8; 1 token of 2048 x 2048 16 x 4 6.9, 16 x 8 11.2.
 Cut choose(int64_t L, int64_t C, int64_t K, bool b_mn, int sms) {
     const int64_t steps = (K + TILE_K - 1) / TILE_K;
     Cut best{1, 64, 1};
@@ -93,11 +99,12 @@ Cut choose(int64_t L, int64_t C, int64_t K, bool b_mn, int sms) {
             last = nt;
             const int64_t tiles = (L + TILE_L * cg - 1) / (TILE_L * cg) * ((C + nt - 1) / nt);
             for (int s = 1; s <= (cg == 1 ? fg::lin::MAX_SPLITS : 1) && s <= steps; s *= 2) {
-                if (s > 1 && tiles * s > sms) break;
+                // (clusters of eight find less room than their CTAs: 16 of them take two turns)
+                if (s > 1 && tiles * s > (s == 8 ? sms * 3 / 4 : s == 4 ? sms * 15 / 16 : sms)) break;
                 const double waves = double((tiles * cg * s + sms - 1) / sms);
                 const double bytes = 16384.0 + nt / cg * 128.0;
-                const double step = std::max(2.0 * nt, bytes / 64.0);
-                const double time = waves * (double((steps + s - 1) / s) * step) + 12.0 * nt + (s > 1 ? 2500.0 : 0.0);
+                const double step = std::max(2.0 * nt, bytes / (cg == 1 ? 64.0 : 46.0));
+                const double time = waves * (double((steps + s - 1) / s) * step) + 12.0 * nt + (s > 1 ? 2500.0 + 16.0 * nt : 0.0);
                 if (time < least) {
                     least = time;
                     best = {cg, nt, s};

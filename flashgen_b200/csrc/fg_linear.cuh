@@ -196,6 +196,43 @@ struct Lane {
     }
 };
 
+// N pairs of columns, GROUPS apart from pair p on: the splits' parts of them, which lie in the
+// CTAs' shared memory `at` bytes behind `ring`, added in the order of the splits. All parts of
+// a few pairs, or one split's parts of several, are on their way together.
+constexpr int GROUPS = EPI_WARPS * 32 / TILE_L;
+template <int DT, int N>
+__device__ __forceinline__ void add_parts(const Params& P, const Lane<DT>& out, const uint8_t* ring, uint32_t at, int c0,
+                                          int p, int pairs) {
+    constexpr int TOGETHER = N == 1 ? MAX_SPLITS : 2;
+    float x[N][2] = {};
+    uint16_t r[N][2] = {};
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (p + j * GROUPS < pairs) out.load(c0 + 2 * (p + j * GROUPS), r[j]);
+#pragma unroll 1
+    for (int q = 0; q < P.splits; q += TOGETHER) {
+        float part[TOGETHER][N][2];
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int c = 2 * min(p + j * GROUPS, pairs - 1) + i;
+                    part[k][j][i] = q + k < P.splits ? load_cluster(tc::mapa(ring, q + k) + at + c * TILE_L * 4) : 0.0f;
+                }
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) x[j][i] += part[k][j][i];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (p + j * GROUPS < pairs && c0 + 2 * (p + j * GROUPS) < P.C) out.store(c0 + 2 * (p + j * GROUPS), x[j], r[j]);
+}
+
 // Persistent over its tiles, one CTA an SM (CG = 1) or a pair of CTAs for two (CG = 2:
 // 256 lanes). Warp 0 loads (TMA), warp 1 issues the products, eight warps are the
 // epilogue, two for each quarter of the accumulator's lanes. Accumulators take turns, so
@@ -451,21 +488,15 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
             const int c0 = (first % P.nc) * P.nt;
             const int tid = threadIdx.x - 64, l = tid % TILE_L;
             const Lane<DT> out(P, (first / P.nc) * TILE_L + l);
-            const int hi = P.nt * (split + 1) / P.splits;
-            for (int c = P.nt * split / P.splits + tid / TILE_L; c < hi; c += EPI_WARPS * 32 / TILE_L) {
-                if (c0 + c >= P.C) break;
-                uint16_t r[1] = {};
-                out.load(c0 + c, r);
-                float part[MAX_SPLITS];
-#pragma unroll
-                for (int q = 0; q < MAX_SPLITS; ++q)
-                    part[q] = q < P.splits ? load_cluster(tc::mapa(reinterpret_cast<float*>(ring) + c * TILE_L + l, q)) : 0.0f;
-                float sum = part[0];
-#pragma unroll
-                for (int q = 1; q < MAX_SPLITS; ++q)
-                    if (q < P.splits) sum += part[q];
-                float x[1] = {sum};
-                out.store(c0 + c, x, r);
+            // this CTA's columns (an even number), two at a time by each part of the threads
+            const int lo = P.nt * split / P.splits, pairs = (P.nt * (split + 1) / P.splits - lo) / 2;
+            const int group = tid / TILE_L;
+            const uint32_t at = smem_u32(reinterpret_cast<float*>(ring) + l) - smem_u32(ring) + lo * TILE_L * 4;
+            if (pairs <= GROUPS) {
+                if (group < pairs) add_parts<DT, 1>(P, out, ring, at, c0 + lo, group, pairs);
+            } else {
+#pragma unroll 1
+                for (int p = group; p < pairs; p += 4 * GROUPS) add_parts<DT, 4>(P, out, ring, at, c0 + lo, p, pairs);
             }
         }
     }

@@ -110,7 +110,7 @@ constexpr int BLOCK_BYTES = 64 * TILE_K * 2;       // an MN-major box: 64 elemen
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int MAX_ACC = 4;
-constexpr int PIECE_K = 64;                        // K steps of one accumulation
+template <int DT> struct Pieces { static constexpr int STEPS = DT == FG_DTYPE_BF16 ? 256 : 64; };   // of K, one accumulation
 
 struct Control {
     uint64_t full[MAX_STAGES], empty[MAX_STAGES];
@@ -196,6 +196,15 @@ struct Lane {
     }
 };
 
+// Tile t's place: along the lanes within a band of BAND tiles first, then along the columns, so
+// that what runs at the same time is a square of the result and shares its operands in L2.
+constexpr int BAND = 8;
+__device__ __forceinline__ void place_of(const Params& P, int t, int& lt, int& ct) {
+    const int band = t / (BAND * P.nc), l0 = band * BAND, high = min(BAND, P.nl - l0), in = t - l0 * P.nc;
+    lt = l0 + in % high;
+    ct = in / high;
+}
+
 // N pairs of columns, GROUPS apart from pair p on: the splits' parts of them, which lie in the
 // CTAs' shared memory `at` bytes behind `ring`, added in the order of the splits. All parts of
 // a few pairs, or one split's parts of several, are on their way together.
@@ -243,8 +252,9 @@ __device__ __forceinline__ void add_parts(const Params& P, const Lane<DT>& out, 
 // adds up its share of the columns, in the order of the parts.
 //
 // The tensor core truncates when it accumulates (about 0.05 n units of 2^-23 over n
-// elements of one sign), so the sum is taken in pieces of 4096 (an eighth of half a unit
-// of float16 at most), which the epilogue adds with rounding.
+// elements of one sign), so the sum is taken in pieces, which the epilogue adds with
+// rounding: of 4096 for float16 (an eighth of half a unit of the result at most), of 16384
+// for bfloat16 (a twentieth).
 //
 // Every wait is bounded (P.wait_ns). Where one runs out, the CTA (and its pair) stops
 // waiting, the epilogue writes NaN for what it has not stored, and the CTA lets its
@@ -264,6 +274,7 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
     const int stage_bytes = A_BYTES + cols * TILE_K * 2;
     const int nk_all = (P.K + TILE_K - 1) / TILE_K;
     const int k_lo = nk_all * split / P.splits, nk = nk_all * (split + 1) / P.splits - k_lo;   // this CTA's steps
+    constexpr int PIECE = Pieces<DT>::STEPS;
     const int tiles = P.nl * P.nc;
     const int share = CG * P.splits;                          // CTAs of a tile
     const int first = blockIdx.x / share, step = gridDim.x / share;
@@ -308,8 +319,9 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
             uint32_t parity = 1;   // of the ring's previous round: a fresh barrier counts as passed with parity 1
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step) {
-                const int l0 = ((t / P.nc) * CG + half) * TILE_L;
-                const int c0 = (t % P.nc) * P.nt + half * cols;
+                int lt, ct;
+                place_of(P, t, lt, ct);
+                const int l0 = (lt * CG + half) * TILE_L, c0 = ct * P.nt + half * cols;
                 for (int k = k_lo; k < k_lo + nk; ++k) {
                     if (!mbar_wait(&C.empty[stage], parity, &C.abort, P.wait_ns)) { ok = false; break; }
                     if (half == 0) mbar_arrive_expect_tx(&C.full[stage], CG * stage_bytes);
@@ -345,8 +357,8 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
             uint32_t parity = 0, acc_parity = 1;
             bool ok = true;
             for (int t = first; t < tiles && ok; t += step) {
-                for (int k0 = 0; k0 < nk && ok; k0 += PIECE_K) {
-                    const int k1 = min(nk, k0 + PIECE_K);
+                for (int k0 = 0; k0 < nk && ok; k0 += PIECE) {
+                    const int k1 = min(nk, k0 + PIECE);
                     if (!mbar_wait(&C.acc_empty[acc], acc_parity, &C.abort, P.wait_ns)) { ok = false; break; }
                     tc::fence_after();
                     const uint32_t d = tmem + acc * P.nt;
@@ -399,13 +411,15 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
         };
         bool gone = false;   // gave up
         for (int t = first; t < tiles; t += step) {
-            const int c0 = (t % P.nc) * P.nt;
-            const Lane<DT> out(P, ((t / P.nc) * CG + half) * TILE_L + quarter * 32 + lane);
+            int lt, ct;
+            place_of(P, t, lt, ct);
+            const int c0 = ct * P.nt;
+            const Lane<DT> out(P, (lt * CG + half) * TILE_L + quarter * 32 + lane);
             // the residual's columns come ahead: the first before the products are done
             uint16_t next[16] = {};
             if (P.splits == 1 && !gone) out.load(c0 + part * 16, next);
             int before = -1;
-            for (int k0 = 0; k0 < nk && !gone; k0 += PIECE_K) {
+            for (int k0 = 0; k0 < nk && !gone; k0 += PIECE) {
                 // a wait of the whole warp: all lanes go on or none
                 gone = !__all_sync(0xffffffffu, mbar_wait(&C.acc_full[acc], acc_parity, &C.abort, P.wait_ns));
                 if (gone) break;
@@ -428,7 +442,7 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
                     free_acc(before);
                 }
                 before = acc;
-                if (k0 + PIECE_K < nk) next_acc();
+                if (k0 + PIECE < nk) next_acc();
             }
             if (gone) {
                 if (lane == 0) give_up();
@@ -485,9 +499,11 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
     if (CG == 1 && P.splits > 1) {
         tc::cluster_sync();   // every part stands
         if (warp >= 2) {
-            const int c0 = (first % P.nc) * P.nt;
+            int lt, ct;
+            place_of(P, first, lt, ct);
+            const int c0 = ct * P.nt;
             const int tid = threadIdx.x - 64, l = tid % TILE_L;
-            const Lane<DT> out(P, (first / P.nc) * TILE_L + l);
+            const Lane<DT> out(P, lt * TILE_L + l);
             // this CTA's columns (an even number), two at a time by each part of the threads
             const int lo = P.nt * split / P.splits, pairs = (P.nt * (split + 1) / P.splits - lo) / 2;
             const int group = tid / TILE_L;
@@ -612,7 +628,7 @@ __global__ void __launch_bounds__(256) bias_kernel(const float* sums, int blocks
     const int col = blockIdx.x * 32 + (threadIdx.x & 31), p = threadIdx.x >> 5;
     float s = 0.0f;
     if (col < outer) {
-#pragma unroll 4
+#pragma unroll 8
         for (int b = blocks * p / 8; b < blocks * (p + 1) / 8; ++b) s += sums[int64_t(b) * outer + col];
     }
     part[p][threadIdx.x & 31] = s;

@@ -2,8 +2,8 @@
 
 Tolerances, element by element, h being half a step of the type (eps / 2):
 * a sum of products: the tensor core loses up to 0.05 n units of 2^-23 over n elements of a
-  piece (4096 at most), and a few more in the additions after it, of the sum of magnitudes
-  S: e(S) = (0.05 min(n, 4096) + 4 + n / 4096) 2^-23 S;
+  piece (at most p = 4096 of float16, 16384 of bfloat16), and a few more in the additions after
+  it, of the sum of magnitudes S: e(S) = (0.05 min(n, p) + 4 + n / p) 2^-23 S;
 * the activations' slopes are at most 1.13, and their own error a few units in 2^-22 of
   the larger of |act(z)| and |z| 2^-3 (e^x by a product and ex2, one division): 2^-20 of it;
 * the result: h of itself, or half the least subnormal step;
@@ -34,9 +34,13 @@ def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
 
+def sum_units(n, dtype):
+    piece = 4096 if dtype is F16 else 16384
+    return (0.05 * min(n, piece) + 4 + n / piece) * 2.0 ** -23
+
+
 def sum_error(a, b):
-    n = a.shape[1]
-    return (0.05 * min(n, 4096) + 4 + n / 4096) * 2.0 ** -23 * (a.double().abs() @ b.double().abs().T)
+    return sum_units(a.shape[1], a.dtype) * (a.double().abs() @ b.double().abs().T)
 
 
 def close(got, want, slack):
@@ -79,7 +83,7 @@ def test_forward(cuda_device, size, dtype, act):
     check_forward(fused_linear(x, w, b, r, activation=act), x, w, b, r, act)
 
 
-@pytest.mark.parametrize("size", [(5, 16384, 300), (300, 12345, 260), (1000, 9000, 130)])
+@pytest.mark.parametrize("size", [(5, 16384, 300), (300, 12345, 260), (1000, 9000, 130), (40, 40000, 128)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_long_sums_of_one_sign(cuda_device, size, dtype):
     x, w, b, r, _ = tensors(*size, dtype)
@@ -133,7 +137,7 @@ def check_gradients(grads, gy, x, w, b, act):
         ea = e if a is dz else e.T
         ma = m if a is dz else m.T
         n = a.shape[1]
-        acc = (0.05 * min(n, 4096) + 4 + n / 4096) * 2.0 ** -23
+        acc = sum_units(n, x.dtype)
         want = a @ c.T
         close(got, want, (ea + acc * ma) @ c.abs().T)
         if act != "relu" and want.norm() > 0 and got.numel() > 50:

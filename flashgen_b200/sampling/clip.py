@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import array
 import math
+from itertools import chain, repeat
 from operator import attrgetter
 from typing import List, Optional, Sequence, Union
 
@@ -52,14 +53,12 @@ def _norm(grads: List[torch.Tensor], out: Optional[List[torch.Tensor]], max_norm
     n = len(grads)
     code = _DTYPES.__getitem__
     codes = map(code, map(_dtype, grads))
-    table = array.array("q", bytes(32 * n))       # FgGradTensor, field by field
-    table[0::4] = array.array("q", map(_address, grads))
-    table[2::4] = array.array("q", map(_count, grads))
     if out is None:
-        table[3::4] = array.array("q", codes)
+        fields = zip(map(_address, grads), repeat(0), map(_count, grads), codes)
     else:
-        table[1::4] = array.array("q", map(_address, out))
-        table[3::4] = array.array("q", [g | o << 32 for g, o in zip(codes, map(code, map(_dtype, out)))])
+        both = [g | o << 32 for g, o in zip(codes, map(code, map(_dtype, out)))]
+        fields = zip(map(_address, grads), map(_address, out), map(_count, grads), both)
+    table = array.array("q", list(chain.from_iterable(fields)))       # FgGradTensor, field by field
     lib = _lib.load()
     need = lib.fg_clip_workspace_size(n)
     if need == 0:

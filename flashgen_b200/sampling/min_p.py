@@ -69,6 +69,8 @@ def sample_min_p(logits: torch.Tensor, uniforms: torch.Tensor, min_p: torch.Tens
     if B > 1 and logits.stride(0) < V:     # rows that share memory (expand)
         logits = logits.contiguous()
     dev, f32 = logits.device, torch.float32
+    if uniforms is None or min_p is None:
+        raise TypeError("uniforms and min_p must be tensors of one value a row")
     uniforms = _vector(uniforms, f32, B, dev, "uniforms")
     min_p = _vector(min_p, f32, B, dev, "min_p")
     temperature = _vector(temperature, f32, B, dev, "temperature")
@@ -95,24 +97,21 @@ def sample_min_p(logits: torch.Tensor, uniforms: torch.Tensor, min_p: torch.Tens
             longest = 0
     lib = _lib.load()
     need = lib.fg_sample_min_p_workspace_size(B, V, longest)
-    # one allocation: ids (8 bytes a row), then log probabilities, kept and status (4 each), then the workspace
-    room = torch.empty(20 * B + 4 * (B & 1) + need, dtype=torch.uint8, device=dev)
-    out = room[:8 * B].view(torch.int64)
-    words = room[8 * B:20 * B].view(torch.int32).view(3, B)
-    logprobs, kept, status = words[0].view(f32), words[1], words[2]
-    r = MinPSample(out, logprobs, kept, status)
+    out = torch.empty(B, dtype=torch.int64, device=dev)
+    logprobs, kept, status = torch.empty((3, B), dtype=f32, device=dev).unbind(0)
+    r = MinPSample(out, logprobs, kept.view(torch.int32), status.view(torch.int32))
     if B == 0:
         return r
-    at = room.data_ptr()
+    room = torch.empty(need, dtype=torch.uint8, device=dev)
     a = _lib.FgMinPArgs(
         _lib.FgSampleArgs(logits.data_ptr(), _DTYPES[logits.dtype], B, V, longest, logits.stride(0) if B > 1 else V,
                           0, 0, _ptr(ids), _ptr(offsets), _ptr(temperature), _ptr(top_p), _ptr(top_k),
                           _ptr(repetition_penalty), _ptr(presence_penalty), _ptr(frequency_penalty), _ptr(greedy),
-                          uniforms.data_ptr(), at, at + 16 * B, None, at + 20 * B + 4 * (B & 1), need),
-        _ptr(min_p), at + 8 * B, at + 12 * B)
+                          uniforms.data_ptr(), out.data_ptr(), status.data_ptr(), None, room.data_ptr(), need),
+        _ptr(min_p), logprobs.data_ptr(), kept.data_ptr())
     _call(dev, lib.fg_sample_min_p, a, "fg_sample_min_p")
     if check_errors:
-        msg = _status_error(status)
+        msg = _status_error(r.status)
         if msg is not None:
             raise RuntimeError(msg)
     return r

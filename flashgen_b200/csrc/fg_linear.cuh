@@ -258,9 +258,9 @@ __device__ __forceinline__ void add_parts(const Params& P, const Lane<DT>& out, 
 //
 // Bound: the weight's bytes for a few tokens (1 token, 4096 x 4096, bf16: 10 us with its 33.6 MB,
 // floor 5.1; the launch, the ring's fill and the parts' exchange are the rest), the tensor pipe
-// and the power limit for many (8192 tokens, 4096 x 4096: forward with SiLU, residual and fp32 sums
-// 200 us, dx 180 us = 1.53 PFLOP/s, tensor pipe active 83 %; dW 205 us, 256 tiles over 74 pairs).
-// 1024 tokens: 33 us, one wave of 64 pairs whose start and epilogue no other tile covers.
+// for many (8192 tokens, 4096 x 4096, launches alone: forward with SiLU, residual and fp32 sums
+// 200 us, dx 179 us = 1.53 PFLOP/s, tensor pipe active 83 %; dW 206 us, 256 tiles over 74 pairs),
+// in a long loop at the clock that the power limit leaves. 1024 tokens: 34 us, one wave of 64 pairs whose start and epilogue no other tile covers.
 //
 // Every wait is bounded (P.wait_ns). Where one runs out, the CTA (and its pair) stops
 // waiting, the epilogue writes NaN for what it has not stored, and the CTA lets its

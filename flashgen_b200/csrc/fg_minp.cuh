@@ -15,11 +15,10 @@
 // min-p and no small top-k, or flat rows) go to wide_kernel, which does the same over whole
 // rows, a cluster each.
 //
-// Measured (one B200, kernels alone, inputs past L2): 1 x 256000 fp32 18.5 us; 256 x 32000 bf16
-// masked, mixed parameters 61; 1024 x 128256 bf16 153 (rows_kernel 100, four flat rows in
-// wide_kernel 45); 512 x 128256 bf16 mixed with histories 180 to 240 (as many as 43 rows
-// are wide). A sort of every row's candidates and 64-bit exponentials took 1036 us for the
-// 1024 rows.
+// Measured (one B200, kernels alone, inputs rotated): 1 x 256000 fp32 18.7 us; 256 x 32000 bf16
+// masked, mixed parameters 61; 1024 x 128256 bf16 153; 512 x 128256 bf16, mixed, with histories
+// 237. A sort of every row's candidates, 64-bit exponentials and loads to registers together
+// took 1036 us for the 1024 rows, the step that replaced the three 460.
 #pragma once
 
 #include <cfloat>
@@ -288,12 +287,12 @@ __device__ __forceinline__ uint32_t count_history(const Params& P, const Row& ro
 // ---------------------------------------------------------------------------
 // rows_kernel: one cluster of G CTAs a row, each a slice of it.
 //
-// Bound: HBM reads while rows stream (6.7 TB/s between the 6 us at their start and the 5 at
-// their end; 1024 x 128256 bf16 in all 100 us, 2.6 TB/s), the last flat rows after that. A
+// Bound: HBM reads and, as 1024 x 128256 bf16 run at 2.6 TB/s in all (101 us, issue slots 38 %),
+// the starts and ends of rows that no copy covers and the last flat rows. A
 // 16-byte chunk costs a packed maximum and one comparison; the chunks that reach the bound, a
 // few hundred of a row, are looked at element by element. The copies go through a ring in shared
-// memory: loads to registers were held back by the little L1 that the candidates leave
-// (1024 rows 800 us). Three CTAs an SM (two with histories).
+// memory: the candidates leave loads to registers little L1. Three CTAs an SM (two with
+// histories).
 // ---------------------------------------------------------------------------
 struct Shared {
     uint32_t top;        // key of the largest (penalised) logit seen

@@ -1,6 +1,7 @@
 // fg_minp.cu — C ABI entry points of sampling with min-p: argument checks and launches.
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 
 #include "fg_internal.h"
 #include "fg_minp.cuh"
@@ -25,7 +26,9 @@ size_t marks_bytes(int64_t batch) { return size_t(std::max<int64_t>(batch, 1) + 
 // Distinct columns of a row's history at most.
 int64_t distinct(int32_t hist_max_len, int32_t vocab) { return std::max(1, std::min(hist_max_len, vocab)); }
 
-// CTAs a row: as many as find room at once (four an SM) with two tiles' loads for each.
+// CTAs a row: a power of two of which the batch fills no more than three an SM, with half a round
+// of copies for each. Kernels alone: one row of 256000 fp32 with 1, 2, 4, 8 CTAs 41.6, 30, 25, 22
+// us; 1024 rows of 128256 bf16 182, 207, 254, 340 us.
 int ctas_per_row(int32_t batch, int vocab, int elem, const DevInfo* d) {
     const int64_t chunks = int64_t(vocab) * elem / 16;
     int G = 1;
@@ -35,10 +38,16 @@ int ctas_per_row(int32_t batch, int vocab, int elem, const DevInfo* d) {
     return G;
 }
 
+// Raises a kernel's limit of dynamic shared memory to `bytes`. Under a lock: of two threads the
+// one that needs less must not take back what the other has just set.
+std::mutex limits;
+
 template <class K>
 bool set_smem(K kern, std::atomic<int>* done, int bytes) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    if (done[dev].load(std::memory_order_acquire) >= bytes) return true;
+    std::lock_guard<std::mutex> lock(limits);
     if (done[dev].load(std::memory_order_acquire) >= bytes) return true;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
     done[dev].store(bytes, std::memory_order_release);
@@ -105,8 +114,10 @@ int launch(fg::minp::Params P, DevInfo* d, cudaStream_t st) {
         return (chunks + g - 1) / g * (16 / esz) + 2 * (16 / esz) + KEY_PAD;
     };
     const int room = d->smem_optin - int(sizeof(WideShared) + sizeof(ExpTable)) - 1024;
-    // Four CTAs a row where that leaves work for every SM: 43 wide rows of 128256 with histories
-    // 142 us, with eight CTAs each 200; four wide rows 41 us, 36.
+    // Four CTAs a row where the batch can have work for every SM; how many rows are wide is not known
+    // here. wide_kernel with four and with eight CTAs a row: 512 x 128256 bf16, mixed, with
+    // histories 142 and 200 us; but where few rows are wide, eight are faster: 1024 x 128256 bf16
+    // 55 and 41, 256 x 32000 bf16 38 and 36, 37 x 50257 f16 with histories 51 and 44.
     const int W = P.batch > d->sms / 8 && fixed(4) + 4 * keys(4) <= room ? 4 : WIDE_G;
     const bool cached = fixed(W) + 4 * keys(W) <= room;
     const int wsmem = fixed(W) + 4 * (cached ? int(keys(W)) : P.penalties ? FILTER_WORDS : 0);

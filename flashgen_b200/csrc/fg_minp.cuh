@@ -253,33 +253,33 @@ __device__ __forceinline__ uint32_t count_history(const Params& P, const Row& ro
     uint32_t bad = 0;
     constexpr int AHEAD = 4;   // loads of ids in flight
     for (int64_t at = row.h0 + threadIdx.x; at < row.h1; at += AHEAD * THREADS) {
-      int32_t ids[AHEAD];
+        int32_t ids[AHEAD];
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) ids[j] = at + j * THREADS < row.h1 ? __ldg(P.hist_ids + at + j * THREADS) : 0;
+        for (int j = 0; j < AHEAD; ++j) ids[j] = at + j * THREADS < row.h1 ? __ldg(P.hist_ids + at + j * THREADS) : 0;
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        if (at + j * THREADS >= row.h1) break;
-        const int64_t id = ids[j];
-        if (id < 0 || id >= P.vocab_total) {
-            bad |= FG_ROW_BAD_HISTORY;
-            continue;
+        for (int j = 0; j < AHEAD; ++j) {
+            if (at + j * THREADS >= row.h1) break;
+            const int64_t id = ids[j];
+            if (id < 0 || id >= P.vocab_total) {
+                bad |= FG_ROW_BAD_HISTORY;
+                continue;
+            }
+            const int64_t c = id - P.vocab_offset;
+            if (c < c_lo || c >= c_hi) continue;
+            uint32_t h = col_hash(uint32_t(c), mask);
+            bool done = false;
+            for (uint32_t n = 0; n <= mask && !done; ++n) {
+                const uint32_t k = atomicCAS(&table[h].x, kEmptySlot, uint32_t(c));
+                done = k == kEmptySlot || k == uint32_t(c);
+                if (done) atomicAdd(&table[h].y, 1u);
+                h = (h + 1u) & mask;
+            }
+            if (!done) bad |= FG_ROW_BAD_PARAM;   // more distinct ids than hist_max_len allows
+            if constexpr (WORDS > 0) {
+                const uint32_t b = uint32_t(c - c_lo) & (WORDS * 32 - 1);
+                atomicOr(&filter[b >> 5], 1u << (b & 31));
+            }
         }
-        const int64_t c = id - P.vocab_offset;
-        if (c < c_lo || c >= c_hi) continue;
-        uint32_t h = col_hash(uint32_t(c), mask);
-        bool done = false;
-        for (uint32_t n = 0; n <= mask && !done; ++n) {
-            const uint32_t k = atomicCAS(&table[h].x, kEmptySlot, uint32_t(c));
-            done = k == kEmptySlot || k == uint32_t(c);
-            if (done) atomicAdd(&table[h].y, 1u);
-            h = (h + 1u) & mask;
-        }
-        if (!done) bad |= FG_ROW_BAD_PARAM;   // more distinct ids than hist_max_len allows
-        if constexpr (WORDS > 0) {
-            const uint32_t b = uint32_t(c - c_lo) & (WORDS * 32 - 1);
-            atomicOr(&filter[b >> 5], 1u << (b & 31));
-        }
-      }
     }
     return bad;
 }

@@ -319,6 +319,37 @@ def test_streams_and_graphs(cuda_device):
         check(r, logits, u2, q)
 
 
+def test_two_threads(cuda_device):
+    # sizes that need different amounts of shared memory, with histories and without, side by side
+    import threading
+
+    rng = np.random.default_rng(15)
+    jobs = []
+    for v, h in ((700, 0), (5000, 40), (20000, 1500), (40000, 0), (70000, 4000), (9000, 9)):
+        logits, u, p = rows(6, v, F32, rng), rng.random(6, dtype=np.float32), draw_params(6, rng)
+        history = [rng.integers(0, v, h) for _ in range(6)] if h else None
+        pen = {"rep": np.full(6, 1.3, np.float32)} if h else None
+        jobs.append((logits, u, p, pen, history))
+    torch.cuda.synchronize()
+    got, start = [None] * len(jobs), threading.Barrier(len(jobs))
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait(timeout=60)
+            got[i] = [call(*jobs[i]) for _ in range(5)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for job, results in zip(jobs, got):
+        assert results is not None
+        for r in results:
+            check(r, *job)
+
+
 def test_no_rows(cuda_device):
     r = sample_min_p(torch.zeros(0, 50, device="cuda"), torch.zeros(0, device="cuda"), torch.zeros(0, device="cuda"))
     assert r.ids.shape == (0,) and r.logprobs.shape == (0,)

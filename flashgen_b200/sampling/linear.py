@@ -138,6 +138,11 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     gradients enter the two products of the backward pass rounded to the
     operands' type.
 
+    A step can be captured into a CUDA graph, forward and backward together, from
+    leaves that no graph of an uncaptured step is alive for: autograd would tie the
+    captured backward pass to that step's stream, which ends the capture and may
+    end the process. Drop such results first, or capture from fresh leaves.
+
     ``x`` and ``weight`` are read where they lie when their rows are 16-byte
     aligned (``inner`` a multiple of 8, as a rule); otherwise each call copies
     them.

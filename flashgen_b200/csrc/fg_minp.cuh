@@ -707,11 +707,12 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
 
     // greedy rows with NaN or without a finite maximum: wide_kernel knows their first place
     const bool wide = (sick && row.greedy) || (!sick && over);
-    const uint32_t errors = (flags & (FG_ROW_NAN | FG_ROW_BAD_PARAM)) |
-                            (flags & FG_ROW_NAN ? 0u : top_key <= KEY_NEG_INF ? uint32_t(FG_ROW_ALL_MASKED)
-                                                     : !(top_x < INFINITY)    ? uint32_t(FG_ROW_POS_INF) : 0u);
-    const bool decide = !wide && !(flags & FG_ROW_BAD_PARAM) && (row.greedy || !(errors || !(ydiv(row.p, top_x) < INFINITY)));
+    // (finite logits may divide to an infinity: the divided maximum says what the row has)
     const float top = ydiv(row.p, top_x);
+    const uint32_t errors = (flags & (FG_ROW_NAN | FG_ROW_BAD_PARAM)) |
+                            (flags & FG_ROW_NAN ? 0u : top == -INFINITY    ? uint32_t(FG_ROW_ALL_MASKED)
+                                                     : !(top < INFINITY) ? uint32_t(FG_ROW_POS_INF) : 0u);
+    const bool decide = !wide && !(flags & FG_ROW_BAD_PARAM) && (row.greedy || !errors);
     const uint32_t least_k = row.greedy ? top_key : least_key(S.log_min_p, top);
     if (G > 1) {
         // the other slices' candidates come to the first CTA, by a warp each
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
         if (wide) {
             hand_on();
         } else if (!decide) {
-            if (tid == 0) write_error(P, r, errors ? flags | errors : flags | FG_ROW_POS_INF);
+            if (tid == 0) write_error(P, r, flags | errors);
         } else {
             // ---- the keys of all candidates
             for (int i = tid; i < RBINS; i += NT) bins.count[i] = bins.lo[i] = bins.hi[i] = 0u;

@@ -34,14 +34,15 @@ def _stride(t: Optional[torch.Tensor]) -> int:
 
 def _forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
              act: int, keep: bool):
-    """The block on matrices. With `keep` also what the gradients read: x and the weight as
-    (tensor, byte offset, stride) each, the aligned copies where the call made some, and the sums
-    before the activation, in fp32 (the slope at a rounded sum would lose its last bits)."""
+    """The block on matrices. With `keep` also what the gradients read: x and the weight, each as a
+    matrix (place None) or as the aligned copy that the call made (the workspace, and the copy's
+    place in it: byte offset and stride), and the sums before the activation, in fp32 (the slope
+    at a rounded sum would lose its last bits)."""
     tokens, inner, outer = x.shape[0], x.shape[1], weight.shape[0]
     out = x.new_empty((tokens, outer))
     preact = x.new_empty((tokens, (outer + 3) // 4 * 4), dtype=torch.float32) if keep and act else None
     if tokens == 0:
-        return out, (x, 0, inner), (weight, 0, inner), preact
+        return out, (x, None), (weight, None), preact
     x, weight = _rows(x), _rows(weight)
     xs, ws = _stride(x), _stride(weight)
     xp, wp = x.data_ptr(), weight.data_ptr()
@@ -60,8 +61,8 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]
         return out, None, None, None
     # the workspace has x's copy, if one was made, then the weight's: rows of inner rounded up to 8
     width = (inner + 7) // 8 * 8
-    x_read = (room, 0, width) if copy_x else (x, 0, xs)
-    w_read = (room, (2 * tokens * width + 255) // 256 * 256 if copy_x else 0, width) if copy_w else (weight, 0, ws)
+    x_read = (room, (0, width)) if copy_x else (x, None)
+    w_read = (room, ((2 * tokens * width + 255) // 256 * 256 if copy_x else 0, width)) if copy_w else (weight, None)
     return out, x_read, w_read, preact
 
 
@@ -84,8 +85,9 @@ class _FusedLinear(torch.autograd.Function):
         out, x_read, w_read, preact = _forward(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
         if x_read is not None:
             # (the inputs themselves as well: a change of them before the backward pass is noticed)
-            ctx.save_for_backward(x, weight, x_read[0], w_read[0], preact)
-            ctx.places = x_read[1:] + w_read[1:]
+            ctx.save_for_backward(x, weight, None if x_read[0] is x else x_read[0],
+                                  None if w_read[0] is weight else w_read[0], preact)
+            ctx.places, ctx.sizes = (x_read[1], w_read[1]), (x.shape[0], x.shape[1], weight.shape[0])
         ctx.act = act
         return out
 
@@ -95,33 +97,56 @@ class _FusedLinear(torch.autograd.Function):
         gx = gw = gb = None
         if any(wanted[:3]):
             x, weight, x_read, w_read, preact = ctx.saved_tensors
-            gx, gw, gb = _gradients(grad.detach(), x, weight, x_read, w_read, ctx.places, preact, ctx.act, wanted)
+            gx, gw, gb = _gradients(grad.detach(), x if x_read is None else x_read,
+                                    weight if w_read is None else w_read, ctx.places, preact, ctx.sizes, ctx.act, wanted)
             if torch.is_grad_enabled():   # create_graph=True
                 gx, gw, gb = (None if g is None else _Once.apply(g, grad, x, weight) for g in (gx, gw, gb))
         return gx, gw, gb, grad if wanted[3] else None, None
 
 
-def _gradients(grad, x, weight, x_read, w_read, places, preact, act, wanted):
-    tokens, inner, outer = x.shape[0], x.shape[1], weight.shape[0]
-    gx = torch.empty((tokens, inner), dtype=x.dtype, device=x.device) if wanted[0] else None
-    gw = torch.empty((outer, inner), dtype=x.dtype, device=x.device) if wanted[1] else None
-    gb = torch.empty((outer,), dtype=x.dtype, device=x.device) if wanted[2] else None
+def _saved(t: torch.Tensor, place, rows: int, cols: int, like: torch.Tensor, dtype: torch.dtype):
+    """What forward saved, as it came back, with its address and row stride. Hooks on saved tensors
+    (offloading) owe the values only: a slice of a wider buffer may come back dense, so nothing
+    that was noted of its layout holds. A workspace is a vector of bytes, where places hold."""
+    if place is not None:
+        need = place[0] + 2 * rows * place[1]
+        if t.dtype != torch.uint8 or t.device != like.device or t.dim() != 1 or t.shape[0] < need:
+            raise RuntimeError(f"a saved workspace came back as {tuple(t.shape)} {t.dtype} on {t.device}")
+        t = t.contiguous()
+        return t, t.data_ptr() + place[0], place[1]
+    if t.dtype != dtype or t.device != like.device or t.shape != (rows, cols):
+        raise RuntimeError(f"a saved tensor of {[rows, cols]} {dtype} on {like.device} came back as {list(t.shape)} "
+                           f"{t.dtype} on {t.device}")
+    t = _rows(t)
+    return t, t.data_ptr(), _stride(t)
+
+
+def _gradients(grad, x, weight, places, preact, sizes, act, wanted):
+    tokens, inner, outer = sizes
+    dtype, dev = grad.dtype, grad.device
+    gx = torch.empty((tokens, inner), dtype=dtype, device=dev) if wanted[0] else None
+    gw = torch.empty((outer, inner), dtype=dtype, device=dev) if wanted[1] else None
+    gb = torch.empty((outer,), dtype=dtype, device=dev) if wanted[2] else None
     if tokens == 0:      # sums over nothing
         for g in (gw, gb):
             if g is not None:
                 g.zero_()
         return gx, gw, gb
     g = _rows(grad)
+    x, xp, xs = _saved(x, places[0], tokens, inner, grad, dtype)
+    weight, wp, ws = _saved(weight, places[1], outer, inner, grad, dtype)
+    zp = zs = 0
+    if preact is not None:
+        preact, zp, zs = _saved(preact, None, tokens, (outer + 3) // 4 * 4, grad, torch.float32)
     lib = _lib.load()
     a = _lib.FgLinearGradArgs(
-        g.data_ptr(), x_read.data_ptr() + places[0], w_read.data_ptr() + places[2], _ptr(preact), _ptr(gx), _ptr(gw),
-        _ptr(gb), None, 0, _DTYPES[x.dtype], tokens, inner, outer, act, 0, _stride(g), places[1], places[3],
-        _stride(preact), inner, inner)
+        g.data_ptr(), xp, wp, zp, _ptr(gx), _ptr(gw), _ptr(gb), None, 0, _DTYPES[dtype], tokens, inner, outer, act, 0,
+        _stride(g), xs, ws, zs, inner, inner)
     size = lib.fg_linear_grad_workspace_size(a)
     if size:
-        room = torch.empty(size, dtype=torch.uint8, device=x.device)
+        room = torch.empty(size, dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = room.data_ptr(), size
-    _call(x.device, lib.fg_linear_grad, a, "fg_linear_grad")
+    _call(dev, lib.fg_linear_grad, a, "fg_linear_grad")
     return gx, gw, gb
 
 

@@ -151,9 +151,10 @@ int fg_sample_min_p(const FgMinPArgs* m, void* stream) {
     if (a->vocab > (1 << 28) || a->batch > kMaxBatch) return FG_ENOTSUP;
     fg::minp::Params P{};
     if (a->hist_offsets != nullptr && a->hist_max_len < 0) return FG_EINVAL;
-    P.penalties = penalties(*a) && a->hist_max_len > 0;
+    P.penalties = penalties(*a);
     if (P.penalties) {
-        P.hist_max_len = a->hist_max_len;
+        // (a bound of 0 leaves room for a few ids, as in fg_sample: rows with more are marked)
+        P.hist_max_len = std::max(1, a->hist_max_len);
         P.wide_slots = slots_for(distinct(a->hist_max_len, a->vocab));
         P.slots = std::min(P.wide_slots, slots_for(fg::minp::HIST_CAP));
         P.tables = reinterpret_cast<uint2*>(reinterpret_cast<char*>(a->workspace) + marks_bytes(a->batch));

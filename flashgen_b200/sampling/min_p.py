@@ -92,9 +92,11 @@ def sample_min_p(logits: torch.Tensor, uniforms: torch.Tensor, min_p: torch.Tens
             raise ValueError(f"history ids must be one vector, got {list(ids.shape)}")
         ids = _vector(ids, torch.int32, ids.shape[0], dev, "history ids")
         offsets = _vector(offsets, torch.int64, B + 1, dev, "history offsets")
-        if longest == 0 or ids.numel() == 0:
+        if ids.numel() == 0:
             ids = offsets = None
             longest = 0
+        else:
+            longest = max(1, longest)
     lib = _lib.load()
     need = lib.fg_sample_min_p_workspace_size(B, V, longest)
     out = torch.empty(B, dtype=torch.int64, device=dev)

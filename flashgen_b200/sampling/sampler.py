@@ -159,7 +159,7 @@ def fused_sample(logits: torch.Tensor, packed: PackedParams, uniforms: torch.Ten
     a.out_probs = _ptr(probs)
     st = stream if stream is not None else torch.cuda.current_stream(logits.device)
     if packed.min_p is not None:
-        need = lib.fg_sample_min_p_workspace_size(B, V, a.hist_max_len if hist is not None else 0)
+        need = lib.fg_sample_min_p_workspace_size(B, V, max(1, a.hist_max_len) if hist is not None else 0)
         # of any content, unlike fg_sample's, whose counters stay zero between calls
         with torch.cuda.stream(st):
             own = torch.empty(need, dtype=torch.uint8, device=logits.device)

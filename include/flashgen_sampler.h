@@ -569,8 +569,8 @@ typedef struct FgMinPArgs {
 
 int fg_sample_min_p(const FgMinPArgs* args, void* stream);
 
-/* Bytes of workspace of fg_sample_min_p (hist_max_len 0 without penalties); 0 for an
- * invalid shape. Host-only. */
+/* Bytes of workspace of fg_sample_min_p (hist_max_len 0 without penalties, at least 1 with
+ * them); 0 for an invalid shape. Host-only. */
 size_t fg_sample_min_p_workspace_size(int32_t batch, int32_t vocab, int32_t hist_max_len);
 
 /* Human-readable name of a return code. */

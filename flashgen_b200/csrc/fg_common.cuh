@@ -42,8 +42,8 @@ __device__ __forceinline__ float div_rn(float x, float d, float r) {
     float q0 = x * r;
     float rem = __fmaf_rn(-q0, d, x);
     float q = __fmaf_rn(rem, r, q0);
-    float ax = fabsf(x);
-    if (!(ax >= 0x1p-100f && ax <= 0x1p100f)) q = __fdiv_rn(x, d);  // 0, tiny, huge, inf, NaN
+    // x of 0, tiny or NaN; a quotient that is huge (also of an ordinary x over a tiny d), inf or NaN
+    if (!(fabsf(x) >= 0x1p-100f && fabsf(q0) <= 0x1p100f)) q = __fdiv_rn(x, d);
     return q;
 }
 

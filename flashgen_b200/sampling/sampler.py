@@ -145,6 +145,8 @@ def fused_sample(logits: torch.Tensor, packed: PackedParams, uniforms: torch.Ten
     a.batch, a.vocab = B, V
     a.row_stride = logits.stride(0) if B > 1 else V
     a.vocab_offset, a.vocab_total = vocab_offset, vocab_total
+    if hist is not None and hist[0].numel() == 0:     # (an empty vector has no address)
+        hist = None
     if hist is not None:
         a.hist_ids, a.hist_offsets, a.hist_max_len = hist[0].data_ptr(), hist[1].data_ptr(), int(hist[2])
     f = packed.f32

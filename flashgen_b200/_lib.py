@@ -31,7 +31,7 @@ EXPORTED_SYMBOLS = ("fg_sample", "fg_sample_workspace_size", "fg_sample_candidat
                     "fg_apply_repetition_penalty", "fg_argmax", "fg_token_logprobs", "fg_token_logprobs_grad",
                     "fg_adapter_logits", "fg_adapter_set_wait", "fg_adapter_workspace_size",
                     "fg_clip_grad_norm", "fg_clip_workspace_size", "fg_linear", "fg_linear_workspace_size", "fg_linear_grad",
-                    "fg_linear_grad_workspace_size", "fg_sample_min_p", "fg_sample_min_p_workspace_size", "fg_strerror", "fg_version")
+                    "fg_linear_grad_workspace_size", "fg_sample_min_p", "fg_sample_min_p_rows", "fg_sample_min_p_workspace_size", "fg_strerror", "fg_version")
 
 
 class FgSampleArgs(ctypes.Structure):
@@ -286,8 +286,9 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
         lib.fg_adapter_set_wait.restype = ctypes.c_int
         lib.fg_adapter_workspace_size.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
         lib.fg_adapter_workspace_size.restype = ctypes.c_size_t
-        lib.fg_sample_min_p.argtypes = [ctypes.POINTER(FgMinPArgs), ctypes.c_void_p]
-        lib.fg_sample_min_p.restype = ctypes.c_int
+        for name in ("fg_sample_min_p", "fg_sample_min_p_rows"):
+            getattr(lib, name).argtypes = [ctypes.POINTER(FgMinPArgs), ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
         lib.fg_sample_min_p_workspace_size.argtypes = [ctypes.c_int32] * 3
         lib.fg_sample_min_p_workspace_size.restype = ctypes.c_size_t
         lib.fg_clip_grad_norm.argtypes = [ctypes.POINTER(FgClipArgs), ctypes.c_void_p]

@@ -128,6 +128,9 @@ int launch(fg::minp::Params P, DevInfo* d, cudaStream_t st) {
                         st, P);
 }
 
+// fg_sample_min_p; with `only` the rows that have min-p.
+int sample(const FgMinPArgs* m, bool only, void* stream);
+
 }  // namespace
 
 extern "C" {
@@ -137,8 +140,16 @@ size_t fg_sample_min_p_workspace_size(int32_t batch, int32_t vocab, int32_t hist
     return marks_bytes(batch) + (hist_max_len > 0 ? size_t(kMaxClusters) * slots_for(distinct(hist_max_len, vocab)) * 8 : 0);
 }
 
-int fg_sample_min_p(const FgMinPArgs* m, void* stream) {
-    if (m == nullptr) return FG_EINVAL;
+int fg_sample_min_p(const FgMinPArgs* m, void* stream) { return sample(m, false, stream); }
+
+int fg_sample_min_p_rows(const FgMinPArgs* m, void* stream) { return sample(m, true, stream); }
+
+}  // extern "C"
+
+namespace {
+
+int sample(const FgMinPArgs* m, bool only, void* stream) {
+    if (m == nullptr || (only && m->min_p == nullptr)) return FG_EINVAL;
     const FgSampleArgs* a = &m->sample;
     const int esz = elem_size(a->dtype);
     if (esz == 0 || a->logits == nullptr || a->batch < 0 || a->vocab < 1 || a->row_stride < a->vocab) return FG_EINVAL;
@@ -172,6 +183,7 @@ int fg_sample_min_p(const FgMinPArgs* m, void* stream) {
     P.greedy = a->greedy; P.uniforms = a->uniforms;
     P.out_ids = a->out_ids; P.out_status = a->out_status; P.out_probs = a->out_probs;
     P.out_logprobs = m->out_logprobs; P.out_kept = m->out_kept;
+    P.only = only;
     P.mass_shift = 62 - fg::host::bits_for(a->vocab);
     DevInfo* d = nullptr;
     const int rc = fg::host::device_info(&d);
@@ -184,4 +196,4 @@ int fg_sample_min_p(const FgMinPArgs* m, void* stream) {
     }
 }
 
-}  // extern "C"
+}  // namespace

@@ -67,6 +67,7 @@ struct Params {
     uint8_t* marks;            // [B]: rows handed to wide_kernel
     uint2* tables;             // wide_kernel's history tables, one per cluster
     int32_t penalties;         // histories and any of the three penalties are given
+    int32_t only;              // rows with min_p == 0 are left as they are
     int32_t hist_max_len;
     int32_t slots, wide_slots; // of a history table (powers of two)
     int32_t mass_shift;        // S
@@ -444,6 +445,10 @@ __global__ void __launch_bounds__(NT, 3) rows_kernel(const Params P, const int G
     auto hand_on = [&]() {
         if (rank == 0 && tid == 0) P.marks[r] = 1;
     };
+    if (P.only && row.min_p == 0.0f) {
+        copies_done<0>();
+        return;
+    }
     if (row.p.bad && !P.out_probs) {
         if (rank == 0 && tid == 0) write_error(P, r, row.p.bad);
         copies_done<0>();

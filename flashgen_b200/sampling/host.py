@@ -30,10 +30,12 @@ class _Staging:
         self.f32_h = torch.empty(7, batch, dtype=torch.float32).pin_memory()   # 5 params, uniforms, min_p
         self.i32_h = torch.empty(batch, dtype=torch.int32).pin_memory()
         self.u8_h = torch.empty(batch, dtype=torch.uint8).pin_memory()
+        self.other_h = torch.empty(batch, dtype=torch.uint8).pin_memory()      # greedy ones and those with min-p
         self.ids_h = torch.empty(batch, dtype=torch.int64).pin_memory()
         self.f32_d = torch.empty(7, batch, dtype=torch.float32, device=device)
         self.i32_d = torch.empty(batch, dtype=torch.int32, device=device)
         self.u8_d = torch.empty(batch, dtype=torch.uint8, device=device)
+        self.other_d = torch.empty(batch, dtype=torch.uint8, device=device)
         self.copied = None   # event after this set's last host-to-device copies
 
 
@@ -76,6 +78,12 @@ class HostBatchSampler:
         s.i32_d.copy_(s.i32_h, non_blocking=True)
         s.u8_d.copy_(s.u8_h, non_blocking=True)
         h2d += s.f32_h.numel() * 4 + B * 4 + B
+        has = f[6] != 0.0
+        mixed = bool(np.any(has)) and not np.all(has)
+        if mixed:
+            s.other_h.numpy()[:] = s.u8_h.numpy().astype(bool) | has
+            s.other_d.copy_(s.other_h, non_blocking=True)
+            h2d += B
         hist = None
         if hist_ids_h is not None:
             n = hist_ids_h.numel()
@@ -90,8 +98,8 @@ class HostBatchSampler:
         packed.any_presence = bool(np.any(params.presence_penalty != 0.0))
         packed.any_frequency = bool(np.any(params.frequency_penalty != 0.0))
         packed.all_greedy = False
-        if min_p is not None and np.any(np.asarray(min_p) != 0.0):
-            packed.min_p = s.f32_d[6]
+        packed.min_p = s.f32_d[6] if np.any(has) else None
+        packed.without_min_p = s.other_d if mixed else None
         fused_sample(self.logits_d, packed, s.f32_d[5], hist, out=self.ids_d, status=self.status_d)
         s.ids_h.copy_(self.ids_d, non_blocking=True)
         ev = torch.cuda.Event()

@@ -86,6 +86,8 @@ class PackedParams:
     """Per-row parameters as device structure-of-arrays."""
 
     min_p: Optional[torch.Tensor] = None      # [B] float32; None where no row has it
+    # where some rows have min-p and some have not: [B] uint8, `greedy` and the rows that have it
+    without_min_p: Optional[torch.Tensor] = None
 
     def __init__(self, temperature, top_p, top_k, rep, presence, frequency, greedy, device, min_p=None):
         B = len(temperature)
@@ -98,8 +100,12 @@ class PackedParams:
         self.any_presence = bool(np.any(np.asarray(presence) != 0.0))
         self.any_frequency = bool(np.any(np.asarray(frequency) != 0.0))
         self.all_greedy = bool(np.all(np.asarray(greedy) | (np.asarray(temperature) == 0.0)))
-        if min_p is not None and np.any(np.asarray(min_p) != 0.0):
+        has = np.zeros(B, dtype=bool) if min_p is None else np.asarray(min_p, dtype=np.float32) != 0.0
+        if np.any(has):
             self.min_p = torch.from_numpy(np.asarray(min_p, dtype=np.float32).copy()).to(device, non_blocking=True)
+            if not np.all(has):
+                other = (np.asarray(greedy, dtype=bool) | has).astype(np.uint8)
+                self.without_min_p = torch.from_numpy(other).to(device, non_blocking=True)
 
     @staticmethod
     def from_params(params: Sequence[SamplingParams], device) -> "PackedParams":
@@ -133,8 +139,8 @@ def fused_sample(logits: torch.Tensor, packed: PackedParams, uniforms: torch.Ten
                  probs: Optional[torch.Tensor] = None, vocab_offset: int = 0, vocab_total: int = 0,
                  stream: Optional[torch.cuda.Stream] = None,
                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """One fg_sample call on device tensors (fg_sample_min_p where a row has min-p; no
-    checks beyond the C ABI's)."""
+    """One fg_sample call on device tensors (no checks beyond the C ABI's). Rows that have
+    min-p are fg_sample_min_p's; the others' results do not depend on them."""
     lib = _lib.load()
     B, V = logits.shape
     if out is None:
@@ -160,22 +166,27 @@ def fused_sample(logits: torch.Tensor, packed: PackedParams, uniforms: torch.Ten
     a.out_status = _ptr(status)
     a.out_probs = _ptr(probs)
     st = stream if stream is not None else torch.cuda.current_stream(logits.device)
+    if packed.min_p is None or packed.without_min_p is not None:
+        if packed.min_p is not None:
+            # The rows that have min-p are greedy ones here, the least work, and sampled below
+            a.greedy = _ptr(packed.without_min_p)
+        if workspace is None:
+            need = _lib.workspace_size(B, V, a.dtype, a.hist_max_len if hist is not None else 0)
+            workspace = workspace_for(logits.device, st, need)
+        _lib.set_workspace(a, workspace)
+        with torch.cuda.device(logits.device):
+            _lib.check(lib.fg_sample(a, st.cuda_stream), "fg_sample")
     if packed.min_p is not None:
+        a.greedy = _ptr(packed.greedy)
         need = lib.fg_sample_min_p_workspace_size(B, V, max(1, a.hist_max_len) if hist is not None else 0)
         # of any content, unlike fg_sample's, whose counters stay zero between calls
         with torch.cuda.stream(st):
             own = torch.empty(need, dtype=torch.uint8, device=logits.device)
         _lib.set_workspace(a, own)
+        mixed = packed.without_min_p is not None
         with torch.cuda.device(logits.device):
-            _lib.check(lib.fg_sample_min_p(_lib.FgMinPArgs(a, packed.min_p.data_ptr(), None, None), st.cuda_stream),
-                       "fg_sample_min_p")
-        return out
-    if workspace is None:
-        need = _lib.workspace_size(B, V, a.dtype, a.hist_max_len if hist is not None else 0)
-        workspace = workspace_for(logits.device, st, need)
-    _lib.set_workspace(a, workspace)
-    with torch.cuda.device(logits.device):
-        _lib.check(lib.fg_sample(a, st.cuda_stream), "fg_sample")
+            _lib.check((lib.fg_sample_min_p_rows if mixed else lib.fg_sample_min_p)(
+                _lib.FgMinPArgs(a, packed.min_p.data_ptr(), None, None), st.cuda_stream), "fg_sample_min_p")
     return out
 
 

@@ -569,6 +569,11 @@ typedef struct FgMinPArgs {
 
 int fg_sample_min_p(const FgMinPArgs* args, void* stream);
 
+/* The same for the rows that have min-p: of rows whose min_p is 0 nothing is read and nothing
+ * written. After fg_sample on the same arguments a batch of both kinds is complete, and a row
+ * without min-p has fg_sample's result whatever its neighbours ask for. min_p must be given. */
+int fg_sample_min_p_rows(const FgMinPArgs* args, void* stream);
+
 /* Bytes of workspace of fg_sample_min_p (hist_max_len 0 without penalties, at least 1 with
  * them); 0 for an invalid shape. Host-only. */
 size_t fg_sample_min_p_workspace_size(int32_t batch, int32_t vocab, int32_t hist_max_len);

@@ -74,7 +74,8 @@ def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], *, scale: floa
     """``scale * sqrt(sum of squares)`` over all elements of ``grads`` (a tensor or a
     list of them, float32, float16 and bfloat16 mixed as they come), as a float32
     scalar on their device. Summed in 64 bits; neither huge nor tiny gradients
-    overflow or vanish on the way."""
+    overflow or vanish on the way. A number for logs and for clipping: no gradient
+    flows through it."""
     grads = _list(grads, "grads")
     if not grads:
         raise ValueError("no gradients")

@@ -13,6 +13,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .sampler import _DTYPES, _call, _ptr
@@ -158,7 +159,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     "gelu_tanh" or "silu". Products are summed in fp32, and bias, activation and
     residual are applied to the fp32 sum, which is rounded once.
 
-    Differentiable with respect to all four (once: a second derivative raises).
+    Differentiable with respect to all four (once: a second derivative raises, and so
+    does a tangent of forward mode).
     For that the sums before the activation are kept in fp32, and their
     gradients enter the two products of the backward pass rounded to the
     operands' type.
@@ -193,6 +195,11 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
             raise TypeError(f"{what} must be {dtype} on {dev} like the weight, got {t.dtype} on {t.device}")
         if t.shape != want:
             raise ValueError(f"{what} must be {list(want)}, got {list(t.shape)}")
+    # (level below 0: no forward-mode pass is open, the usual case)
+    if forward_ad._current_level >= 0:
+        for t, what in ((x, "x"), (weight, "weight"), (bias, "bias"), (residual, "residual")):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"fused_linear has no forward-mode derivative; {what} carries a tangent")
     if not weight.is_cuda:
         raise RuntimeError(f"flashgen_b200 runs on the GPU only; the weight is on {dev}")
     flat = x.dim() == 2

@@ -55,7 +55,8 @@ def sample_min_p(logits: torch.Tensor, uniforms: torch.Tensor, min_p: torch.Tens
     greedy), then of the tokens with at least ``min_p`` ([B] in [0, 1]; 0: off) times the
     largest probability the ``top_k`` likeliest (ties kept; <= 0: off), and of those the
     ``top_p`` nucleus. Every parameter is a vector of one value a row. Nothing is copied to
-    the host; ``check_errors`` reads the status back and raises.
+    the host; ``check_errors`` reads the status back and raises. No gradient flows through
+    the log probabilities (``logprobs_and_entropy`` has one).
 
     >>> r = sample_min_p(logits, torch.rand(B, device="cuda"), min_p, temperature=temperature)
     >>> r.ids, r.logprobs

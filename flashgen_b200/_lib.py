@@ -31,6 +31,7 @@ EXPORTED_SYMBOLS = ("fg_sample", "fg_sample_workspace_size", "fg_sample_candidat
                     "fg_apply_repetition_penalty", "fg_argmax", "fg_token_logprobs", "fg_token_logprobs_grad",
                     "fg_adapter_logits", "fg_adapter_set_wait", "fg_adapter_workspace_size",
                     "fg_clip_grad_norm", "fg_clip_workspace_size", "fg_linear", "fg_linear_workspace_size", "fg_linear_grad",
+                    "fg_linear_set_wait",
                     "fg_linear_grad_workspace_size", "fg_sample_min_p", "fg_sample_min_p_rows", "fg_sample_min_p_workspace_size", "fg_strerror", "fg_version")
 
 
@@ -300,6 +301,8 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
             getattr(lib, name).restype = ctypes.c_int
             getattr(lib, name + "_workspace_size").argtypes = [ctypes.POINTER(args)]
             getattr(lib, name + "_workspace_size").restype = ctypes.c_size_t
+        lib.fg_linear_set_wait.argtypes = [ctypes.c_int64, ctypes.c_int32]
+        lib.fg_linear_set_wait.restype = ctypes.c_int
         lib.fg_strerror.argtypes = [ctypes.c_int]
         lib.fg_strerror.restype = ctypes.c_char_p
         lib.fg_version.argtypes = []

@@ -19,6 +19,10 @@ using fg::lin::TILE_L;
 
 constexpr int32_t kMaxTokens = 1 << 20, kMaxInner = 1 << 20, kMaxOuter = 1 << 28;
 
+// fg_linear_set_wait
+std::atomic<int64_t> g_wait_ns{fg::lin::DEFAULT_WAIT_NS};
+std::atomic<int32_t> g_withhold{-1};
+
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
@@ -150,7 +154,8 @@ int product(Params P, int dtype, const Matrix& a, bool a_mn, const Matrix& b, bo
     P.accs = std::min(fg::lin::MAX_ACC, 512 / P.nt);
     P.tmem_cols = 32;
     while (P.tmem_cols < P.accs * P.nt) P.tmem_cols *= 2;
-    P.wait_ns = 1000000000;
+    P.wait_ns = uint64_t(g_wait_ns.load(std::memory_order_relaxed));
+    P.withhold = g_withhold.load(std::memory_order_relaxed);
     CUtensorMap amap, bmap;
     if (!fg::host::encode_rows(&amap, dtype, a.p, a.rows, a.dim, a.stride, a_mn ? 64 : TILE_L) ||
         !fg::host::encode_rows(&bmap, dtype, b.p, b.rows, b.dim, b.stride, b_mn ? 64 : cut.nt / cut.cg))
@@ -221,6 +226,14 @@ int launch_slope(const fg::lin::SlopeParams& S, int act, void* grad_bias, cudaSt
 }  // namespace
 
 extern "C" {
+
+int fg_linear_set_wait(int64_t limit_ns, int32_t withhold) {
+    if (limit_ns < 0 || limit_ns > fg::lin::DEFAULT_WAIT_NS || withhold < -1 || withhold >= fg::lin::MAX_ACC)
+        return FG_EINVAL;
+    g_wait_ns.store(limit_ns > 0 ? limit_ns : fg::lin::DEFAULT_WAIT_NS, std::memory_order_relaxed);
+    g_withhold.store(withhold, std::memory_order_relaxed);
+    return FG_OK;
+}
 
 size_t fg_linear_workspace_size(const FgLinearArgs* a) {
     if (a == nullptr || !shape_ok(a->dtype, a->tokens, a->inner, a->outer, a->activation)) return 0;

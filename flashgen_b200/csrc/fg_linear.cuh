@@ -109,7 +109,6 @@ constexpr int A_BYTES = TILE_L * TILE_K * 2;
 constexpr int BLOCK_BYTES = 64 * TILE_K * 2;       // an MN-major box: 64 elements by 64 steps of K
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
-constexpr int MAX_ACC = 4;
 template <int DT> struct Pieces { static constexpr int STEPS = DT == FG_DTYPE_BF16 ? 256 : 64; };   // of K, one accumulation
 
 struct Control {
@@ -291,7 +290,7 @@ product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__
             mbar_init(&C.empty[s], 1);
         }
         for (int i = 0; i < P.accs; ++i) {
-            mbar_init(&C.acc_full[i], 1);
+            mbar_init(&C.acc_full[i], i == P.withhold ? 2 : 1);
             mbar_init(&C.acc_empty[i], CG * EPI_WARPS);
         }
         mbar_init(&C.drain, 1);

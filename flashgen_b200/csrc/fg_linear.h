@@ -13,6 +13,8 @@ constexpr int TILE_L = 128, TILE_K = 64;   // accumulator lanes of a CTA; elemen
 constexpr int MAX_NT = 256;                // columns of a tile
 constexpr int MAX_STAGES = 12;
 constexpr int MAX_SPLITS = 8;
+constexpr int MAX_ACC = 4;                 // accumulators that take turns
+constexpr int64_t DEFAULT_WAIT_NS = 1000000000;   // limit of a wait: 1 s, far above any legitimate one
 
 // One product: out[c, l] = act(sum_k A[l, k] B[c, k] + bias[l]) + residual[c, l], l being the
 // contiguous dimension of out.
@@ -29,6 +31,7 @@ struct Params {
     int32_t stages, accs, tmem_cols;
     int32_t splits;           // CTAs (a cluster) that share a tile's sum over K
     uint64_t wait_ns;         // limit of each wait
+    int32_t withhold;         // accumulator whose products are never reported (for tests); -1: none
 };
 
 }  // namespace lin

@@ -451,7 +451,7 @@ size_t fg_clip_workspace_size(int32_t count);
  * FG_EINVAL.
  *
  * Every wait in the kernel is bounded (1 s); where one runs out, what was not computed is
- * NaN.
+ * NaN, which is all that says so: there is no status.
  *
  * Workspace: fg_linear_workspace_size(args) bytes (0 for aligned x and weight), 256-byte
  * aligned, written and read within the call. Calls that may run concurrently need separate
@@ -532,6 +532,10 @@ int fg_linear_grad(const FgLinearGradArgs* args, void* stream);
 
 /* Bytes of workspace of fg_linear_grad for these arguments. Host-only. */
 size_t fg_linear_grad_workspace_size(const FgLinearGradArgs* args);
+
+/* For tests of waits that run out, of fg_linear and fg_linear_grad: as fg_adapter_set_wait, with
+ * accumulators 0 .. 3. */
+int fg_linear_set_wait(int64_t limit_ns, int32_t withhold);
 
 /*
  * Sampling with min-p. The chain of fg_sample with one more filter: per row, y being the

@@ -63,11 +63,12 @@ def _norm(grads: List[torch.Tensor], out: Optional[List[torch.Tensor]], max_norm
     need = lib.fg_clip_workspace_size(n)
     if need == 0:
         raise ValueError(f"too many tensors: {n}")
-    room = torch.empty(need // 4 + 2, dtype=torch.float32, device=dev)   # the norm, then the workspace
-    at = room.data_ptr()
-    a = _lib.FgClipArgs(table.buffer_info()[0], n, 0, max_norm, scale, at, at + 8, need)
+    # (the norm is not a part of the workspace: a caller that keeps it would keep all of that)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    room = torch.empty(need, dtype=torch.uint8, device=dev)
+    a = _lib.FgClipArgs(table.buffer_info()[0], n, 0, max_norm, scale, norm.data_ptr(), room.data_ptr(), need)
     _call(dev, lib.fg_clip_grad_norm, a, "fg_clip_grad_norm")
-    return room[0]
+    return norm
 
 
 def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], *, scale: float = 1.0) -> torch.Tensor:

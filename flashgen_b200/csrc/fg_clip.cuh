@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(THREADS, 6) scale_kernel(const __grid_constant
     sum = block_sum(sum);
     const float norm = float(sqrt(sum) * double(scale));
     if (blockIdx.x == 0 && threadIdx.x == 0 && out_norm) *out_norm = norm;
-    const float ratio = __fdiv_rn(max_norm, norm + 1e-6f);
+    // (without a limit nothing is clipped, whatever the norm: infinity over infinity is no ratio)
+    const float ratio = max_norm < INFINITY || norm != norm ? __fdiv_rn(max_norm, norm + 1e-6f) : 1.0f;
     const float c = scale * (ratio < 1.0f || ratio != ratio ? ratio : 1.0f);
     int t = 0;
     uint32_t top = L.chunks;   // chunks from here on are done

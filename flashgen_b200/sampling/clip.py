@@ -97,8 +97,10 @@ def clip_grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm:
     In place, or into ``out``: tensors of the gradients' shapes, any of the three
     types each, that share no memory with the list. A list that names a tensor
     (or a part of it) twice is refused where it would be written twice. With a
-    norm that is NaN every gradient becomes NaN; with an infinite one finite
-    gradients become 0. ``check_errors`` reads the norm back and raises for both.
+    norm that is NaN every gradient becomes NaN; with an infinite one (of an infinite
+    gradient, or above the largest float32) finite gradients become 0, unless
+    ``max_norm`` is infinite too: then nothing is clipped. ``check_errors`` reads the
+    norm back and raises for both.
 
     >>> norm = clip_grad_norm([p.grad for p in params if p.grad is not None], 1.0)
     """

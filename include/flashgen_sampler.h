@@ -405,8 +405,9 @@ size_t fg_adapter_workspace_size(int32_t batch, int32_t dim, int32_t rank, int32
  * memory that meets no other tensor's gradients or results and no other part of its
  * own (FG_EINVAL otherwise). The squares are summed in 64 bits whatever the type, in
  * an order that does not depend on timing; products are rounded once to the result's
- * type. A NaN norm makes every result NaN; an infinite one makes the finite ones 0.
- * max_norm >= 0 (infinity: no clipping), scale positive and finite.
+ * type. A NaN norm makes every result NaN; an infinite one makes the finite ones 0 (a
+ * norm above the largest float is infinite). max_norm >= 0 (infinity: no clipping, with
+ * whatever norm that is a number), scale positive and finite.
  *
  * Workspace: fg_clip_workspace_size bytes, 8-byte aligned, written and read within the
  * call (no initial value). Calls that may run concurrently need separate workspaces.

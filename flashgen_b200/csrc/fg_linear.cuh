@@ -253,7 +253,9 @@ __device__ __forceinline__ void add_parts(const Params& P, const Lane<DT>& out, 
 // The tensor core truncates when it accumulates (about 0.05 n units of 2^-23 over n
 // elements of one sign), so the sum is taken in pieces, which the epilogue adds with
 // rounding: of 4096 for float16 (an eighth of half a unit of the result at most), of 16384
-// for bfloat16 (a twentieth).
+// for bfloat16 (a twentieth). bfloat16 with pieces of 4096 instead: 4096 tokens, 16384 x 4096
+// 397 us against 384, a training step of 16384 tokens, 4096 x 4096, 1276 against 1257; sums of
+// 8192 no difference.
 //
 // Bound: the weight's bytes for a few tokens (1 token, 4096 x 4096, bf16: 10 us with its 33.6 MB,
 // floor 5.1; the launch, the ring's fill and the parts' exchange are the rest), the tensor pipe

@@ -26,9 +26,9 @@ size_t marks_bytes(int64_t batch) { return size_t(std::max<int64_t>(batch, 1) + 
 // Distinct columns of a row's history at most.
 int64_t distinct(int32_t hist_max_len, int32_t vocab) { return std::max(1, std::min(hist_max_len, vocab)); }
 
-// CTAs a row: a power of two of which the batch fills no more than three an SM, with half a round
-// of copies for each. Kernels alone: one row of 256000 fp32 with 1, 2, 4, 8 CTAs 41.6, 30, 25, 22
-// us; 1024 rows of 128256 bf16 182, 207, 254, 340 us.
+// CTAs a row: a power of two of which the batch fills no more than three an SM (what fits
+// without histories), with half a round of copies for each. Kernels alone: one row of 256000
+// fp32 with 1, 2, 4, 8 CTAs 41.6, 30, 25, 22 us; 1024 rows of 128256 bf16 182, 207, 254, 340 us.
 int ctas_per_row(int32_t batch, int vocab, int elem, const DevInfo* d) {
     const int64_t chunks = int64_t(vocab) * elem / 16;
     int G = 1;

@@ -15,9 +15,10 @@
 // min-p and no small top-k, or flat rows) go to wide_kernel, which does the same over whole
 // rows, a cluster each.
 //
-// Measured (one B200, kernels alone, inputs rotated): 1 x 256000 fp32 18.7 us; 256 x 32000 bf16
-// masked, mixed parameters 61; 1024 x 128256 bf16 153; 512 x 128256 bf16, mixed, with histories
-// 237. A sort of every row's candidates, 64-bit exponentials and loads to registers together
+// Measured (one B200, kernels alone, inputs rotated, one draw of rows and parameters each; other
+// draws have other shares of flat and unbounded rows: the last two 130 to 150 and 170 to 245 as
+// whole calls): 1 x 256000 fp32 18.7 us; 256 x 32000 bf16 masked, mixed parameters 61; 1024 x
+// 128256 bf16 153; 512 x 128256 bf16, mixed, with histories 237. A sort of every row's candidates, 64-bit exponentials and loads to registers together
 // took 1036 us for the 1024 rows, the step that replaced the three 460.
 #pragma once
 
@@ -292,8 +293,10 @@ __device__ __forceinline__ uint32_t count_history(const Params& P, const Row& ro
 // the starts and ends of rows that no copy covers and the last flat rows. A
 // 16-byte chunk costs a packed maximum and one comparison; the chunks that reach the bound, a
 // few hundred of a row, are looked at element by element. The copies go through a ring in shared
-// memory: the candidates leave loads to registers little L1. Three CTAs an SM (two with
-// histories).
+// memory: the candidates leave loads to registers little L1. Three CTAs an SM. With histories
+// two, and one where the caller's longest is above 2048 ids: the table is sized by that bound,
+// whatever the rows have. 1024 x 128256 bf16, histories of 64 ids: 127 us a call with a bound of
+// 64, 142 with 2048, 244 with 4096 (no histories: 89).
 // ---------------------------------------------------------------------------
 struct Shared {
     uint32_t top;        // key of the largest (penalised) logit seen

@@ -500,7 +500,8 @@ size_t fg_linear_workspace_size(const FgLinearArgs* args);
  *   grad_x = dz weight      grad_weight = dz^T x      grad_bias = sum over tokens of dz
  *
  * (the residual's gradient is grad_out). Each of the three may be NULL. dz is rounded to
- * the operands' type for the two products, and summed for the bias before that; sums are
+ * the operands' type for the two products (float16: above 65504 it becomes infinite, so
+ * scale the loss for that), and summed for the bias before that; sums are
  * fp32, in an order that does not depend on timing. preact is read with activations other
  * than FG_ACT_NONE, weight for grad_x, x for grad_weight. Strides, alignment, waits and
  * workspace as in fg_linear. With no tokens the sums over them are 0.
@@ -549,8 +550,9 @@ int fg_linear_set_wait(int64_t limit_ns, int32_t withhold);
  *   draw    the first token, in that order, whose inclusive mass exceeds u times the
  *           kept mass
  *
- * (min_p == 0 keeps everything but -inf: the result is then fg_sample's.) Probabilities
- * are compared in 64 bits. Greedy rows take the first argmax of the penalised logits.
+ * (min_p == 0 keeps everything but -inf: the filters are then fg_sample's, whose masses are
+ * 32-bit exponentials, so that a draw within 1e-6 of a border between two tokens may
+ * differ.) Probabilities are compared in 64 bits. Greedy rows take the first argmax of the penalised logits.
  *
  * `sample` is read as in fg_sample, with these differences: temperature, top_p, top_k
  * (and min_p) may be NULL (1, 1, 0 and 0); there is no vocabulary sharding (vocab_offset 0,

@@ -40,3 +40,18 @@ def test_hooks(cuda_device, kind, dtype, act, size, lo):
     got = torch.autograd.grad(out, leaves, gy)
     assert all(torch.equal(a, c) for a, c in zip(got, want))
     assert not any(g.isnan().any() for g in got)
+
+
+@pytest.mark.parametrize("inner", [72, 77])
+def test_recomputed(cuda_device, inner):
+    # a block that is computed again in the backward pass instead of being kept
+    from torch.utils.checkpoint import checkpoint
+    x, w, b, r, gy = tensors(50, inner, 88, BF16, seed=22)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+
+    def block(x, w, b):
+        return fused_linear(x * 2, w, b, r, activation="gelu")
+
+    want = torch.autograd.grad(block(*leaves), leaves, gy)
+    got = torch.autograd.grad(checkpoint(block, *leaves, use_reentrant=False), leaves, gy)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))

@@ -88,7 +88,7 @@ class _FusedLinear(torch.autograd.Function):
             # (the inputs themselves as well: a change of them before the backward pass is noticed)
             ctx.save_for_backward(x, weight, None if x_read[0] is x else x_read[0],
                                   None if w_read[0] is weight else w_read[0], preact)
-            ctx.places, ctx.sizes = (x_read[1], w_read[1]), (x.shape[0], x.shape[1], weight.shape[0])
+            ctx.places, ctx.sizes = (x_read[1], w_read[1]), (*x.shape, weight.shape[0])
         ctx.act = act
         return out
 
@@ -105,19 +105,18 @@ class _FusedLinear(torch.autograd.Function):
         return gx, gw, gb, grad if wanted[3] else None, None
 
 
-def _saved(t: torch.Tensor, place, rows: int, cols: int, like: torch.Tensor, dtype: torch.dtype):
+def _saved(t: torch.Tensor, place, rows: int, cols: int, dev: int, dtype: torch.dtype):
     """What forward saved, as it came back, with its address and row stride. Hooks on saved tensors
     (offloading) owe the values only: a slice of a wider buffer may come back dense, so nothing
     that was noted of its layout holds. A workspace is a vector of bytes, where places hold."""
+    shape = t.shape
     if place is not None:
-        need = place[0] + 2 * rows * place[1]
-        if t.dtype != torch.uint8 or t.device != like.device or t.dim() != 1 or t.shape[0] < need:
-            raise RuntimeError(f"a saved workspace came back as {tuple(t.shape)} {t.dtype} on {t.device}")
+        if t.dtype is not torch.uint8 or t.get_device() != dev or len(shape) != 1 or shape[0] < place[0] + 2 * rows * place[1]:
+            raise RuntimeError(f"a saved workspace came back as {list(shape)} {t.dtype} on {t.device}")
         t = t.contiguous()
         return t, t.data_ptr() + place[0], place[1]
-    if t.dtype != dtype or t.device != like.device or t.shape != (rows, cols):
-        raise RuntimeError(f"a saved tensor of {[rows, cols]} {dtype} on {like.device} came back as {list(t.shape)} "
-                           f"{t.dtype} on {t.device}")
+    if t.dtype is not dtype or t.get_device() != dev or shape != (rows, cols):
+        raise RuntimeError(f"a saved tensor of {[rows, cols]} {dtype} came back as {list(shape)} {t.dtype} on {t.device}")
     t = _rows(t)
     return t, t.data_ptr(), _stride(t)
 
@@ -133,12 +132,12 @@ def _gradients(grad, x, weight, places, preact, sizes, act, wanted):
             if g is not None:
                 g.zero_()
         return gx, gw, gb
-    g = _rows(grad)
-    x, xp, xs = _saved(x, places[0], tokens, inner, grad, dtype)
-    weight, wp, ws = _saved(weight, places[1], outer, inner, grad, dtype)
+    g, on = _rows(grad), grad.get_device()
+    x, xp, xs = _saved(x, places[0], tokens, inner, on, dtype)
+    weight, wp, ws = _saved(weight, places[1], outer, inner, on, dtype)
     zp = zs = 0
     if preact is not None:
-        preact, zp, zs = _saved(preact, None, tokens, (outer + 3) // 4 * 4, grad, torch.float32)
+        preact, zp, zs = _saved(preact, None, tokens, (outer + 3) // 4 * 4, on, torch.float32)
     lib = _lib.load()
     a = _lib.FgLinearGradArgs(
         g.data_ptr(), xp, wp, zp, _ptr(gx), _ptr(gw), _ptr(gb), None, 0, _DTYPES[dtype], tokens, inner, outer, act, 0,

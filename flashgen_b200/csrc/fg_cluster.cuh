@@ -990,12 +990,11 @@ __global__ void __launch_bounds__(NT, 1) cluster_kernel(const __grid_constant__ 
             out = (M != M) ? (int64_t)gnan : (int64_t)gbc;
         } else if (M != M) {
             status |= FG_ROW_NAN;
-        } else if (M == INFINITY) {
+        } else if ((My = ydiv(p, M)) == INFINITY) {   // (also finite logits over a small temperature)
             status |= FG_ROW_POS_INF;
-        } else if (M == -INFINITY) {
+        } else if (My == -INFINITY) {
             status |= FG_ROW_ALL_MASKED;
         } else {
-            My = ydiv(p, M);
             const uint32_t rlo = gkmin, rhi = fkey(My);
             const uint32_t c_lo = (uint32_t)sl.c_lo;
             // ---- top-k threshold: the K-th largest key by count ----

@@ -1298,9 +1298,9 @@ __global__ void __launch_bounds__(NCT, 5) decide_kernel(const __grid_constant__ 
             defer = false;
         } else if (Mf != Mf) {
             status |= FG_ROW_NAN; defer = false;
-        } else if (Mf == INFINITY) {
+        } else if (ydiv(p, Mf) == INFINITY) {    // (also finite logits over a small temperature)
             status |= FG_ROW_POS_INF; defer = false;
-        } else if (Mf == -INFINITY) {
+        } else if (ydiv(p, Mf) == -INFINITY) {
             status |= FG_ROW_ALL_MASKED; defer = false;
         } else if (!defer) {
             // the decision set: the candidates (non-history, raw = final) and the
